@@ -341,6 +341,95 @@ int nott_attention_bwd(nott_ctx ctx, const nott_attn_desc* d, nott_dtype dtype,
                        const void* q, const void* k, const void* v, const void* o,
                        const void* dO, const float* lse, void* dq, void* dk, void* dv);
 
+/* ---- queries and keys: norm of each head, rotation by position --------------
+ * What decoder attention does between the packed projection and the attention
+ * core, in one pass over q and k.  For head vector x of dh elements:
+ *   z = x·r·gamma, r = 1/sqrt(mean(x²) + eps)          (norm = 1; z = x with norm = 0)
+ *   (y_a, y_b) = (z_a·cos θ − z_b·sin θ, z_a·sin θ + z_b·cos θ)  for each of the
+ *   rot/2 pairs (a, b) of the first rot elements: (i, i + rot/2), or with
+ *   interleaved = 1 (2i, 2i + 1); elements from rot on are z.
+ * The angle of pair i is θ = positions[axis][token] · inv_freq[i], formed in
+ * 64 bits: pairs 0 .. section[0]−1 take axis 0 (text: the only axis; video:
+ * time), the next section[1] axis 1 (height), and so on.
+ * q [b, t, hq, dh], k [b, t, hk, dh] (hk may differ from hq, and may be 0) with
+ * strides in elements for batch, token and head, the elements of a head side by
+ * side; three zeros = contiguous.  So q and k may be views of a packed
+ * projection, and the outputs head-major (strides {h·t·dh, dh, t·dh}).  Outputs
+ * of a call must not overlap themselves; each may be the input it comes from
+ * (same address and strides), else it must not overlap any input.
+ * gamma_q, gamma_k [dh] (dtype; null = ones; null when norm = 0); positions
+ * int64 [axes, b·t]; inv_freq double [rot/2] (both unread when rot = 0). */
+typedef struct nott_qk_rope_desc {
+    int64_t b, t, hq, hk, dh;   /* dh <= 512 */
+    int64_t rot;                /* rotated elements: even, 0 .. dh */
+    int64_t section[4];         /* pairs of each axis; their sum is rot/2 */
+    int64_t q_stride[3], k_stride[3];     /* q, k */
+    int64_t yq_stride[3], yk_stride[3];   /* yq, yk and their gradients */
+    int64_t dq_stride[3], dk_stride[3];   /* dq, dk (backward) */
+    int32_t axes;               /* 1 .. 4 */
+    int32_t interleaved;
+    int32_t norm;
+    int32_t reserved;
+    double eps;
+} nott_qk_rope_desc;
+int nott_qk_norm_rope_fwd(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype dtype,
+                          const void* q, const void* k, const void* gamma_q, const void* gamma_k,
+                          const int64_t* positions, const double* inv_freq, void* yq, void* yk);
+/* From the gradients dyq, dyk of the outputs and the inputs q, k (unread with
+ * norm = 0): dq, dk, and dgamma_q, dgamma_k fp32 [dh] (nullable), summed over
+ * tokens and heads.  dq may be q or dyq, dk may be k or dyk. */
+int nott_qk_norm_rope_bwd(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype dtype,
+                          const void* dyq, const void* dyk, const void* q, const void* k,
+                          const void* gamma_q, const void* gamma_k,
+                          const int64_t* positions, const double* inv_freq,
+                          void* dq, void* dk, float* dgamma_q, float* dgamma_k, int accumulate);
+
+/* ---- gated linear (gated feed-forward) ---------------------------------------
+ * A feed-forward layer's first half with a gate: both projections, the
+ * activation and the product.  w [2·f, d] (dtype) is packed, gate rows first,
+ * then up rows; b [2·f] fp32 nullable:
+ *   [g | u] = x·wᵀ + b,  h = act(g)·u        x [m, d], h [m, f]
+ * gu [m, 2·f] (dtype, nullable) receives [g | u] for the backward. */
+enum {
+    NOTT_ACT_SILU = 0,       /* g·sigmoid(g) */
+    NOTT_ACT_GELU = 1,       /* g·Φ(g) */
+    NOTT_ACT_GELU_TANH = 2,  /* its tanh form, g·sigmoid(2·sqrt(2/π)·(g + 0.044715·g³)) */
+    NOTT_ACT_RELU = 3,
+    NOTT_ACT_SIGMOID = 4
+};
+int nott_gated_linear_fwd(nott_ctx ctx, nott_dtype dtype, int64_t m, int64_t d, int64_t f, int act,
+                          const void* x, const void* w, const float* b, void* h, void* gu);
+/* From dh [m, f], x, w and the forward's gu:
+ *   dg = dh·u·act'(g), du = dh·act(g);  dx = [dg|du]·w,  dw = [dg|du]ᵀ·x, db = Σ_rows [dg|du]
+ * dx [m, d] (dtype), dw [2·f, d] and db [2·f] (fp32); each nullable (x is read
+ * for dw, w for dx).  The workspace holds [dg|du]. */
+int nott_gated_linear_bwd(nott_ctx ctx, nott_dtype dtype, int64_t m, int64_t d, int64_t f, int act,
+                          const void* dh, const void* x, const void* w, const void* gu,
+                          void* dx, float* dw, float* db, int accumulate);
+
+/* ---- log probabilities of given tokens ----------------------------------------
+ * What scoring, distillation and policy-gradient losses take from logits [n, c]
+ * (dtype) beside the mean cross-entropy above.  With z = scale·logits (scale > 0,
+ * an inverse temperature), per row, all outputs fp32 but the indices:
+ *   lse = log Σ exp(z),  logprob = z[label] − lse,  entropy = −Σ p·log p, p = exp(z − lse)
+ * and, with top > 0, the `top` largest logits, largest first (equal ones: lowest
+ * column first; NaN counts as largest): top_logprob, top_index [n, top].
+ * labels int64 [n]: −100 gives logprob 0 (the row's other outputs are unchanged),
+ * any other label outside [0, c) too, and is counted in nott_device_errors.
+ * Masked tokens (z below −1e30: logits of −inf, or of the type's lowest value)
+ * have p = 0, log p = −inf and add nothing; a row of nothing else has lse = −inf
+ * and entropy 0.  entropy and lse nullable.
+ * 0 <= top <= min(c, 64). */
+int nott_token_logprob_fwd(nott_ctx ctx, nott_dtype dtype, int64_t n, int64_t c, const void* logits,
+                           const int64_t* labels, double scale, int64_t top, float* logprob, float* entropy,
+                           float* lse, float* top_logprob, int64_t* top_index);
+/* dlogits = scale·(dlogprob·([j = label] − p) − dentropy·p·(log p + entropy)), from
+ * the forward's lse (and entropy with dentropy, which is nullable).  dlogits may
+ * be logits.  Rows with every token masked get zeros. */
+int nott_token_logprob_bwd(nott_ctx ctx, nott_dtype dtype, int64_t n, int64_t c, const void* logits,
+                           const int64_t* labels, double scale, const float* lse, const float* entropy,
+                           const float* dlogprob, const float* dentropy, void* dlogits);
+
 /* ---- Adam / AdamW --------------------------------------------------------
  * Replaces torch::optim::Adam::step / AdamW::step inherited by
  * Nott::Optimizer::Details::Adam / AdamW (optimizer/details/adam.hpp:63-154,

@@ -50,6 +50,15 @@ class AttnDesc(C.Structure):
                [("causal", C.c_int32), ("layout", C.c_int32), ("scale", f64), ("ld_qkv", i64), ("ld_o", i64)]
 
 
+class QkRopeDesc(C.Structure):
+    _fields_ = [(n, i64) for n in ("b", "t", "hq", "hk", "dh", "rot")] + [("section", i64 * 4)] + \
+               [(n, i64 * 3) for n in ("q_stride", "k_stride", "yq_stride", "yk_stride", "dq_stride", "dk_stride")] + \
+               [(n, C.c_int32) for n in ("axes", "interleaved", "norm", "reserved")] + [("eps", f64)]
+
+
+NOTT_ACT_SILU, NOTT_ACT_GELU, NOTT_ACT_GELU_TANH, NOTT_ACT_RELU, NOTT_ACT_SIGMOID = range(5)
+
+
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 SIGNATURES: dict[str, list] = {
     "nott_create": [i32, C.POINTER(vp)],
@@ -95,6 +104,12 @@ SIGNATURES: dict[str, list] = {
     "nott_softmax_xent_bwd": [vp, i32, i64, i64, vp, vp, f64, f64, vp, fp],
     "nott_attention_fwd": [vp, C.POINTER(AttnDesc), i32, vp, vp, vp, vp, fp],
     "nott_attention_bwd": [vp, C.POINTER(AttnDesc), i32, vp, vp, vp, vp, vp, fp, vp, vp, vp],
+    "nott_qk_norm_rope_fwd": [vp, C.POINTER(QkRopeDesc), i32, vp, vp, vp, vp, vp, vp, vp, vp],
+    "nott_qk_norm_rope_bwd": [vp, C.POINTER(QkRopeDesc), i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, fp, fp, i32],
+    "nott_gated_linear_fwd": [vp, i32, i64, i64, i64, i32, vp, vp, fp, vp, vp],
+    "nott_gated_linear_bwd": [vp, i32, i64, i64, i64, i32, vp, vp, vp, vp, vp, fp, fp, i32],
+    "nott_token_logprob_fwd": [vp, i32, i64, i64, vp, vp, f64, i64, fp, fp, fp, fp, vp],
+    "nott_token_logprob_bwd": [vp, i32, i64, i64, vp, vp, f64, fp, fp, fp, fp, vp],
     "nott_adam_step": [vp, i32, i64, vp, i32, vp, i32, fp, fp, f64, f64, f64, f64, f64, i64, i32],
     "nott_adam_step_graph": [vp, i32, i64, vp, i32, vp, i32, fp, fp, vp, vp, i32, i32],
     "nott_loss_accumulate": [vp, fp, f64, vp],

@@ -18,6 +18,7 @@ struct nott_ctx_s {
     hipStream_t stream = nullptr;
     void* ws = nullptr;            // current device workspace
     size_t ws_bytes = 0;
+    size_t ws_held = 0;            // its first bytes, taken by a WorkspaceHold
     std::vector<void*> retired;    // earlier, smaller workspaces: kept until nott_destroy
     size_t retired_bytes = 0;      // their total size
     size_t refused_bytes = 0;      // the last optional workspace that could not be allocated,
@@ -59,6 +60,21 @@ void* workspace(nott_ctx ctx, size_t bytes);
 // (an allocation would end the capture), and for some calls after a failed
 // allocation of this size or less.
 void* optional_workspace(nott_ctx ctx, size_t bytes);
+// Workspace that a call keeps while it makes others that take some themselves (a
+// composite of products): until the hold ends, workspace() hands out what lies
+// behind it.  A nested call that makes the arena grow leaves `p` in the retired
+// one, where it stays valid.  `p` is null on failure (error set).
+class WorkspaceHold {
+public:
+    WorkspaceHold(nott_ctx c, size_t bytes);
+    ~WorkspaceHold() { ctx_->ws_held = before_; }
+    WorkspaceHold(const WorkspaceHold&) = delete;
+    WorkspaceHold& operator=(const WorkspaceHold&) = delete;
+    char* p;
+private:
+    nott_ctx ctx_;
+    size_t before_;
+};
 // Looks up this device's static LayerNorm scratch (layernorm.hip).
 int layernorm_scratch_setup(nott_ctx ctx);
 // Checks the last launch and records an error message.

@@ -19,7 +19,8 @@ int hip_fail(nott_ctx ctx, hipError_t e, const char* what) {
 
 void* workspace(nott_ctx ctx, size_t bytes) {
     if (bytes == 0) bytes = 256;
-    if (bytes <= ctx->ws_bytes) return ctx->ws;
+    bytes += ctx->ws_held;
+    if (bytes <= ctx->ws_bytes) return static_cast<char*>(ctx->ws) + ctx->ws_held;
     // Geometric growth bounds the retired total by the current arena's size.
     size_t want = (bytes + (1u << 20) - 1) & ~size_t((1u << 20) - 1);
     want = std::max(want, 2 * ctx->ws_bytes);
@@ -37,12 +38,17 @@ void* workspace(nott_ctx ctx, size_t bytes) {
     }
     ctx->ws = fresh;
     ctx->ws_bytes = want;
-    return ctx->ws;
+    return static_cast<char*>(ctx->ws) + ctx->ws_held;
+}
+
+WorkspaceHold::WorkspaceHold(nott_ctx c, size_t bytes)
+    : p(static_cast<char*>(workspace(c, bytes))), ctx_(c), before_(c->ws_held) {
+    if (p) c->ws_held += (bytes + 255) & ~size_t(255);
 }
 
 void* optional_workspace(nott_ctx ctx, size_t bytes) {
     constexpr int kCallsBetweenTries = 64;   // a failing hipMalloc may go through the driver, and memory may come free
-    if (bytes <= ctx->ws_bytes && ctx->ws) return ctx->ws;
+    if (ctx->ws && bytes + ctx->ws_held <= ctx->ws_bytes) return static_cast<char*>(ctx->ws) + ctx->ws_held;
     if (ctx->stream) {
         hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
         if (hipStreamIsCapturing(ctx->stream, &status) != hipSuccess) {

@@ -1,0 +1,324 @@
+// Queries and keys between the packed projection and attention: root-mean-square
+// norm of every head, its weight, and the rotation by position, one pass.
+//
+//   forward : z = x·r·γ, r = 1/sqrt(mean x² + eps);  y = R(θ)·z
+//   backward: dz = R(θ)ᵀ·dy;  x̂ = x·r
+//             dx = r·(γ·dz − x̂·mean(γ·dz·x̂)),  dγ = Σ_{tokens, heads} dz·x̂
+// R turns the pairs (a, b) of the first `rot` elements by θ = position·inv_freq.
+// All arithmetic is fp32 on values rounded once, at the store; the angle is
+// taken in 64 bits as a fraction of a turn and reduced to [-1/2, 1/2] before it
+// is rounded, so that far positions (θ of 1e5 and more) keep their last bits.
+#include "common.hpp"
+
+namespace {
+
+using nott::ceil_div;
+
+constexpr int kMaxHead = 512;
+constexpr int kMaxAxes = 4;
+
+// Positions and frequencies; pair i belongs to the axis whose `first` is the last <= i.
+struct Turns {
+    const int64_t* positions;
+    const double* inv_freq;
+    int64_t tokens;
+    int32_t first[kMaxAxes];   // past the axes: rot/2
+    int32_t half;              // rot/2
+    int32_t interleaved;
+    __device__ __forceinline__ int64_t position(int64_t token, int pair) const {
+        int axis = 0;
+#pragma unroll
+        for (int a = 1; a < kMaxAxes; ++a) axis += pair >= first[a] ? 1 : 0;
+        return positions[axis * tokens + token];
+    }
+    __device__ __forceinline__ void turn(int64_t token, int pair, float& c, float& s) const {
+        // 1/(2π) in two parts: the second keeps what is left of a turn right past
+        // angles of 2^29, where the first's rounding reaches fp32
+        constexpr double kTurn = 0x1.45f306dc9c883p-3, kTurnLow = -0x1.6b01ec5417056p-57;
+        const double angle = (double)position(token, pair) * inv_freq[pair];
+        const double r = fma(angle, kTurn, -rint(angle * kTurn)) + angle * kTurnLow;
+        sincospif(2.f * (float)r, &s, &c);
+    }
+};
+
+// One of the two tensors: its heads, input x, output gradient dy (backward),
+// output, and their strides {batch, token, head}.
+template <typename T>
+struct Heads {
+    const T* x;
+    const T* dy;
+    T* out;
+    const T* gamma;
+    int64_t xs[3], ys[3], os[3];
+    int32_t n;
+};
+
+template <typename T>
+struct RopeArgs {
+    Heads<T> q, k;
+    Turns turns;
+    int32_t t, dh, norm;
+    float eps;
+    int64_t items;      // tokens · (hq + hk)
+    FastDiv by_heads, by_t;
+    float* partial;     // backward: [grid][2·dh] sums of dz·x̂, q then k; null: not asked for
+};
+
+__device__ __forceinline__ int64_t at(const int64_t (&s)[3], uint32_t b, uint32_t t, uint32_t h) {
+    return b * s[0] + t * s[1] + h * s[2];
+}
+
+// Any head size and alignment: a wave per head, element e = 64·v + lane.
+// Every load of a head comes before its stores (the stores wait for the loaded
+// values), so an output may be its input.
+template <typename T, bool BWD>
+__global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs<T> a) {
+    constexpr int V = kMaxHead / 64;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int half = a.turns.half;
+    float dgq[V], dgk[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) dgq[v] = dgk[v] = 0.f;
+    for (int64_t item = (int64_t)blockIdx.x * 4 + wid; item < a.items; item += (int64_t)gridDim.x * 4) {
+        uint32_t token, head, bi, ti;
+        a.by_heads.divmod((uint32_t)item, token, head);
+        a.by_t.divmod(token, bi, ti);
+        const bool is_q = head < (uint32_t)a.q.n;
+        const Heads<T>& h = is_q ? a.q : a.k;
+        if (!is_q) head -= a.q.n;
+        const T* x = h.x + at(h.xs, bi, ti, head);
+        const T* dy = BWD ? h.dy + at(h.ys, bi, ti, head) : nullptr;
+        T* out = BWD ? h.out + at(h.os, bi, ti, head) : h.out + at(h.ys, bi, ti, head);
+        const bool has_x = !BWD || a.norm;
+        float xv[V], ov[V];
+        float ss = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int e = 64 * v + lane;
+            xv[v] = has_x && e < a.dh ? Io<T>::ld(x, e) : 0.f;
+            ss = fmaf(xv[v], xv[v], ss);
+        }
+        float r = 1.f;
+        if (a.norm) r = rsqrtf(wave_sum(ss) / (float)a.dh + a.eps);
+        float dot = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int e = 64 * v + lane;
+            if (e >= a.dh) {
+                ov[v] = 0.f;
+                continue;
+            }
+            const float g = h.gamma ? Io<T>::ld(h.gamma, e) : 1.f;
+            // the other element of e's pair (e itself past the rotated ones)
+            const bool rotated = e < 2 * half;
+            const bool second = a.turns.interleaved ? (e & 1) : e >= half;
+            const int other = !rotated ? e : a.turns.interleaved ? e ^ 1 : second ? e - half : e + half;
+            float c = 1.f, s = 0.f;
+            if (rotated) a.turns.turn(token, a.turns.interleaved ? e >> 1 : second ? e - half : e, c, s);
+            if constexpr (!BWD) {
+                const float z = xv[v] * r * g;
+                const float zo = Io<T>::ld(x, other) * r * (h.gamma ? Io<T>::ld(h.gamma, other) : 1.f);
+                ov[v] = second ? fmaf(zo, s, z * c) : fmaf(-zo, s, z * c);
+            } else {
+                const float d = Io<T>::ld(dy, e), od = Io<T>::ld(dy, other);
+                const float dz = second ? fmaf(-od, s, d * c) : fmaf(od, s, d * c);
+                const float xh = xv[v] * r;
+                if (is_q) dgq[v] = fmaf(dz, xh, dgq[v]);
+                else dgk[v] = fmaf(dz, xh, dgk[v]);
+                ov[v] = dz * g;
+                dot = fmaf(ov[v], xh, dot);
+            }
+        }
+        if constexpr (BWD) {
+            if (a.norm) {
+                dot = wave_sum(dot) / (float)a.dh;
+#pragma unroll
+                for (int v = 0; v < V; ++v) ov[v] = r * (ov[v] - xv[v] * r * dot);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int e = 64 * v + lane;
+            if (e < a.dh) Io<T>::st(out, e, ov[v]);
+        }
+    }
+    if constexpr (BWD) {
+        if (!a.partial) return;
+        __shared__ float red[2][kMaxHead];
+        for (int w = 0; w < 4; ++w) {
+            if (wid == w) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    red[0][64 * v + lane] = w ? red[0][64 * v + lane] + dgq[v] : dgq[v];
+                    red[1][64 * v + lane] = w ? red[1][64 * v + lane] + dgk[v] : dgk[v];
+                }
+            }
+            __syncthreads();
+        }
+        float* p = a.partial + (int64_t)blockIdx.x * 2 * a.dh;
+        for (int e = threadIdx.x; e < a.dh; e += 256) {
+            p[e] = red[0][e];
+            p[a.dh + e] = red[1][e];
+        }
+    }
+}
+
+// dγ (+)= Σ_blocks partial[block], in an order that the grid alone fixes: a
+// workgroup has 16 columns, 16 threads of each taking every 16th block.
+__global__ __launch_bounds__(256) void rope_dgamma_kernel(const float* __restrict__ partial, int blocks, int dh,
+                                                          float* __restrict__ dgq, float* __restrict__ dgk,
+                                                          int accumulate) {
+    __shared__ float red[16][17];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+    const int col = blockIdx.x * 16 + c;
+    float s = 0.f;
+    if (col < 2 * dh) {
+#pragma unroll 8
+        for (int b = r; b < blocks; b += 16) s += partial[(int64_t)b * 2 * dh + col];
+    }
+    red[r][c] = s;
+    __syncthreads();
+    if (r != 0 || col >= 2 * dh) return;
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += red[i][c];
+    float* out = col < dh ? dgq : dgk;
+    if (!out) return;
+    const int e = col < dh ? col : col - dh;
+    out[e] = accumulate ? out[e] + t : t;
+}
+
+// `given`, or the strides of a contiguous [b, t, h, dh] where they are all 0.
+void strides(const int64_t (&given)[3], int64_t t, int64_t h, int64_t dh, int64_t (&s)[3]) {
+    const bool dense = given[0] == 0 && given[1] == 0 && given[2] == 0;
+    s[0] = dense ? t * h * dh : given[0];
+    s[1] = dense ? h * dh : given[1];
+    s[2] = dense ? dh : given[2];
+}
+
+int check(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype dtype, const char* who) {
+    auto bad = [&](const char* what) { return nott::fail(ctx, NOTT_ERR_INVALID_ARG, std::string(who) + ": " + what); };
+    if (!d) return bad("null descriptor");
+    if (!nott::valid_dtype(dtype)) return bad("bad dtype");
+    if (d->b < 0 || d->t < 0 || d->hq < 0 || d->hk < 0) return bad("negative size");
+    if (d->dh < 1 || d->dh > kMaxHead) return bad("head size must be 1 to 512");
+    if (d->rot < 0 || d->rot > d->dh || d->rot % 2) return bad("rot must be even, 0 to the head size");
+    if (d->axes < 1 || d->axes > kMaxAxes) return bad("axes must be 1 to 4");
+    int64_t pairs = 0;
+    for (int i = 0; i < kMaxAxes; ++i) {
+        if (d->section[i] < 0 || d->section[i] > d->rot || (i >= d->axes && d->section[i] != 0)) return bad("bad section");
+        pairs += d->section[i];
+    }
+    if (pairs != d->rot / 2) return bad("sections must add up to rot/2");
+    if (d->norm != 0 && d->norm != 1) return bad("norm must be 0 or 1");
+    if (!(d->eps >= 0.0)) return bad("eps must not be negative");
+    if (d->hq > 65535 || d->hk > 65535) return bad("too many heads");
+    const int64_t most = (int64_t(1) << 31) - 1;
+    if (d->b > most || d->t > most || (d->t && d->b > most / d->t) ||
+        (d->hq + d->hk && d->b * d->t > most / (d->hq + d->hk)))
+        return bad("too many tokens times heads");
+    return NOTT_OK;
+}
+
+template <typename T>
+RopeArgs<T> make_args(const nott_qk_rope_desc& d, const void* q, const void* k, const void* dyq, const void* dyk,
+                      const void* gq, const void* gk, const int64_t* positions, const double* inv_freq, void* oq,
+                      void* ok) {
+    RopeArgs<T> a{};
+    auto side = [&](Heads<T>& h, const void* x, const void* dy, void* out, const void* g, int64_t n,
+                    const int64_t (&xs)[3], const int64_t (&ys)[3], const int64_t (&os)[3]) {
+        h.x = static_cast<const T*>(x);
+        h.dy = static_cast<const T*>(dy);
+        h.out = static_cast<T*>(out);
+        h.gamma = static_cast<const T*>(g);
+        h.n = (int32_t)n;
+        strides(xs, d.t, n, d.dh, h.xs);
+        strides(ys, d.t, n, d.dh, h.ys);
+        strides(os, d.t, n, d.dh, h.os);
+    };
+    side(a.q, q, dyq, oq, gq, d.hq, d.q_stride, d.yq_stride, d.dq_stride);
+    side(a.k, k, dyk, ok, gk, d.hk, d.k_stride, d.yk_stride, d.dk_stride);
+    a.turns.positions = positions;
+    a.turns.inv_freq = inv_freq;
+    a.turns.tokens = d.b * d.t;
+    a.turns.half = (int32_t)(d.rot / 2);
+    a.turns.interleaved = d.interleaved != 0;
+    int64_t first = 0;
+    for (int i = 0; i < kMaxAxes; ++i) {
+        a.turns.first[i] = i < d.axes ? (int32_t)first : a.turns.half;
+        first += d.section[i];
+    }
+    a.t = (int32_t)d.t;
+    a.dh = (int32_t)d.dh;
+    a.norm = d.norm;
+    a.eps = (float)d.eps;
+    a.items = d.b * d.t * (d.hq + d.hk);
+    a.by_heads = FastDiv((uint32_t)(d.hq + d.hk));
+    a.by_t = FastDiv((uint32_t)d.t);
+    return a;
+}
+
+template <typename T>
+int forward(nott_ctx ctx, const RopeArgs<T>& a) {
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.items, 4), 32 * (int64_t)ctx->num_cu);
+    hipLaunchKernelGGL((rope_any_kernel<T, false>), dim3(grid), dim3(256), 0, ctx->stream, a);
+    return nott::launch_status(ctx, "qk_norm_rope");
+}
+
+template <typename T>
+int backward(nott_ctx ctx, RopeArgs<T> a, float* dgq, float* dgk, int accumulate) {
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.items, 4), 8 * (int64_t)ctx->num_cu);
+    if (a.norm && (dgq || dgk)) {
+        a.partial = static_cast<float*>(nott::workspace(ctx, sizeof(float) * 2 * (size_t)a.dh * grid));
+        if (!a.partial) return NOTT_ERR_ALLOC;
+    }
+    hipLaunchKernelGGL((rope_any_kernel<T, true>), dim3(grid), dim3(256), 0, ctx->stream, a);
+    if (a.partial)
+        hipLaunchKernelGGL(rope_dgamma_kernel, dim3((unsigned)ceil_div(2 * a.dh, 16)), dim3(256), 0, ctx->stream,
+                           a.partial, (int)grid, a.dh, dgq, dgk, accumulate);
+    return nott::launch_status(ctx, "qk_norm_rope backward");
+}
+
+}  // namespace
+
+extern "C" int nott_qk_norm_rope_fwd(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype dtype, const void* q,
+                                     const void* k, const void* gamma_q, const void* gamma_k, const int64_t* positions,
+                                     const double* inv_freq, void* yq, void* yk) {
+    NOTT_CHECK_CTX(ctx);
+    const int st = check(ctx, d, dtype, "nott_qk_norm_rope_fwd");
+    if (st != NOTT_OK) return st;
+    if (d->b * d->t * (d->hq + d->hk) == 0) return NOTT_OK;
+    NOTT_REQUIRE(ctx, (d->hq == 0 || (q && yq)) && (d->hk == 0 || (k && yk)), "nott_qk_norm_rope_fwd: null buffer");
+    NOTT_REQUIRE(ctx, d->rot == 0 || (positions && inv_freq), "nott_qk_norm_rope_fwd: null positions or inv_freq");
+    NOTT_REQUIRE(ctx, d->norm || (!gamma_q && !gamma_k), "nott_qk_norm_rope_fwd: a weight needs the norm");
+    nott::DeviceScope scope(ctx->device);
+    if (dtype == NOTT_F32)
+        return forward(ctx, make_args<float>(*d, q, k, nullptr, nullptr, gamma_q, gamma_k, positions, inv_freq, yq, yk));
+    return forward(ctx, make_args<bf16_t>(*d, q, k, nullptr, nullptr, gamma_q, gamma_k, positions, inv_freq, yq, yk));
+}
+
+extern "C" int nott_qk_norm_rope_bwd(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype dtype, const void* dyq,
+                                     const void* dyk, const void* q, const void* k, const void* gamma_q,
+                                     const void* gamma_k, const int64_t* positions, const double* inv_freq, void* dq,
+                                     void* dk, float* dgamma_q, float* dgamma_k, int accumulate) {
+    NOTT_CHECK_CTX(ctx);
+    const int st = check(ctx, d, dtype, "nott_qk_norm_rope_bwd");
+    if (st != NOTT_OK) return st;
+    NOTT_REQUIRE(ctx, d->norm || (!gamma_q && !gamma_k && !dgamma_q && !dgamma_k),
+                 "nott_qk_norm_rope_bwd: a weight needs the norm");
+    nott::DeviceScope scope(ctx->device);
+    if (d->b * d->t * (d->hq + d->hk) == 0) {
+        // no token: the weights' gradients sum over nothing
+        for (float* g : {dgamma_q, dgamma_k})
+            if (g && !accumulate && nott_zero(ctx, (int64_t)sizeof(float) * d->dh, g) != NOTT_OK) return NOTT_ERR_HIP;
+        return NOTT_OK;
+    }
+    NOTT_REQUIRE(ctx, (d->hq == 0 || (dyq && dq)) && (d->hk == 0 || (dyk && dk)), "nott_qk_norm_rope_bwd: null buffer");
+    NOTT_REQUIRE(ctx, !d->norm || ((d->hq == 0 || q) && (d->hk == 0 || k)), "nott_qk_norm_rope_bwd: the norm needs q and k");
+    NOTT_REQUIRE(ctx, d->rot == 0 || (positions && inv_freq), "nott_qk_norm_rope_bwd: null positions or inv_freq");
+    if (dtype == NOTT_F32)
+        return backward(ctx, make_args<float>(*d, q, k, dyq, dyk, gamma_q, gamma_k, positions, inv_freq, dq, dk), dgamma_q,
+                        dgamma_k, accumulate);
+    return backward(ctx, make_args<bf16_t>(*d, q, k, dyq, dyk, gamma_q, gamma_k, positions, inv_freq, dq, dk), dgamma_q,
+                    dgamma_k, accumulate);
+}

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _abi
-from ._abi import AttnDesc, Conv2dDesc, Pool2dDesc
+from ._abi import AttnDesc, Conv2dDesc, Pool2dDesc, QkRopeDesc
 
 _DTYPES = {torch.float32: _abi.NOTT_F32, torch.bfloat16: _abi.NOTT_BF16}
 
@@ -594,3 +594,256 @@ def attention_bwd(q, k, v, o, dO, lse, d: AttnDesc, out=None):
     _ctx_for(q).call("nott_attention_bwd", C.byref(d), nott_dtype(q.dtype), _ptr(q), _ptr(k), _ptr(v), _ptr(o),
                      _ptr(dO), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv))
     return dq, dk, dv
+
+
+# ------------------------------------------------- queries and keys: norm, rotation
+def rope_frequencies(rot: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
+    """inv_freq[i] = theta^(-2i/rot), i < rot/2, in float64: radians per position of each rotated pair."""
+    if rot < 0 or rot % 2 or not theta > 0:
+        raise ValueError("rot must be even and not negative, theta positive")
+    i = torch.arange(rot // 2, dtype=torch.float64, device=device)
+    return float(theta) ** (i * (-2.0 / max(rot, 1)))
+
+
+def _head_strides(t: Optional[torch.Tensor], name: str, shape, like: torch.Tensor) -> tuple:
+    """(batch, token, head) strides of a [b, t, h, dh] tensor whose heads are contiguous."""
+    if t is None:
+        return (0, 0, 0)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise TypeError(f"{name} must have the dtype and device of q")
+    if t.numel() and t.shape[3] > 1 and t.stride(3) != 1:
+        raise ValueError(f"the elements of a head of {name} must be contiguous")
+    st = tuple(t.stride()[:3])
+    if st == (0, 0, 0) and t.numel() > t.shape[3]:   # three zeros mean contiguous to the entry point
+        raise ValueError(f"{name} repeats one head (strides {t.stride()}); make it contiguous")
+    return st
+
+
+def _check_out(t: Optional[torch.Tensor], name: str):
+    """An output's elements must be apart from each other (no expanded dimension)."""
+    if t is None or t.numel() == 0:
+        return
+    reach = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st < reach:
+            raise ValueError(f"{name} overlaps itself (strides {t.stride()})")
+        reach = st * (n - 1) + reach
+
+
+class _QkRope:
+    """The checked arguments of a qk_norm_rope call."""
+
+    def __init__(self, q, k, positions, inv_freq, gamma_q, gamma_k, norm, eps, sections, interleaved):
+        if not isinstance(q, torch.Tensor) or q.dim() != 4 or (k is not None and k.dim() != 4):
+            raise ValueError("q and k must be [b, t, heads, dh]")
+        b, t, hq, dh = q.shape
+        hk = 0 if k is None else k.shape[2]
+        nott_dtype(q.dtype)
+        self.q_shape, self.k_shape = (b, t, hq, dh), (b, t, hk, dh)
+        if dh < 1 or dh > 512:
+            raise ValueError("head size must be 1 to 512")
+        if not eps >= 0:
+            raise ValueError("eps must not be negative")
+        if not norm and (gamma_q is not None or gamma_k is not None):
+            raise ValueError("a weight needs the norm")
+        rot, axes = 0, 1
+        if inv_freq is not None:
+            rot = 2 * inv_freq.numel()
+            if inv_freq.dim() != 1 or rot > dh:
+                raise ValueError(f"inv_freq must be [rot/2] with rot at most the head size {dh}")
+            if positions is None:
+                raise ValueError("inv_freq needs positions")
+            if positions.dim() == 2:
+                positions = positions[None]
+            if positions.dim() != 3 or tuple(positions.shape[1:]) != (b, t) or not 1 <= positions.shape[0] <= 4:
+                raise ValueError(f"positions must be [b, t] or [axes, b, t] with 1 to 4 axes for b = {b}, t = {t}")
+            axes = positions.shape[0]
+        elif positions is not None:
+            raise ValueError("positions need inv_freq")
+        sections = [rot // 2] if sections is None and axes == 1 else sections
+        if sections is None or len(sections) != axes or min(sections) < 0 or sum(sections) != rot // 2:
+            raise ValueError(f"sections must be {axes} pair counts that add up to {rot // 2}")
+        self.d = QkRopeDesc(b, t, hq, hk, dh, rot, (C.c_int64 * 4)(*sections))
+        self.d.axes, self.d.interleaved, self.d.norm, self.d.eps = axes, int(interleaved), int(norm), float(eps)
+        self.d.q_stride[:] = _head_strides(q, "q", self.q_shape, q)
+        self.d.k_stride[:] = _head_strides(k, "k", self.k_shape, q)
+        if rot:
+            _check(inv_freq, "inv_freq", dtype=torch.float64, device=q.device)
+            _check(positions, "positions", dtype=torch.int64, device=q.device)
+        for g, nm in ((gamma_q, "gamma_q"), (gamma_k, "gamma_k")):
+            if g is not None:
+                _check(g, nm, shape=(dh,), dtype=q.dtype, device=q.device)
+        if not q.is_cuda:
+            raise ValueError("q must be a device tensor")
+        self.positions, self.inv_freq = (positions, inv_freq) if rot else (None, None)
+
+
+def qk_norm_rope_fwd(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[torch.Tensor],
+                     inv_freq: Optional[torch.Tensor], gamma_q: Optional[torch.Tensor] = None,
+                     gamma_k: Optional[torch.Tensor] = None, *, norm: bool = True, eps: float = 1e-6, sections=None,
+                     interleaved: bool = False, out=None):
+    """Root-mean-square norm of each head of q [b, t, hq, dh] and k [b, t, hk, dh]
+    (views of a packed projection, any strides but the last) with its weight,
+    then the rotation of its first 2·len(inv_freq) elements by position:
+    positions int64 [b, t], or [axes, b, t] with `sections` pairs of each axis;
+    inv_freq float64 (rope_frequencies).  norm=False: the rotation alone;
+    positions and inv_freq None: the norm alone.  `out` = (yq, yk) to write into
+    (q and k themselves are fine).  Returns (yq, yk) (nott_qk_norm_rope_fwd)."""
+    a = _QkRope(q, k, positions, inv_freq, gamma_q, gamma_k, norm, eps, sections, interleaved)
+    yq, yk = out if out is not None else (torch.empty(a.q_shape, dtype=q.dtype, device=q.device),
+                                          None if k is None else torch.empty(a.k_shape, dtype=q.dtype, device=q.device))
+    for t, nm, shape, st in ((yq, "yq", a.q_shape, a.d.yq_stride), (yk, "yk", a.k_shape, a.d.yk_stride)):
+        if t is None and nm == "yk" and k is None:
+            continue
+        st[:] = _head_strides(t, nm, shape, q)
+        _check_out(t, nm)
+    _ctx_for(q).call("nott_qk_norm_rope_fwd", C.byref(a.d), nott_dtype(q.dtype), _ptr(q), _ptr(k), _ptr(gamma_q),
+                     _ptr(gamma_k), _ptr(a.positions), _ptr(a.inv_freq), _ptr(yq), _ptr(yk))
+    return yq, yk
+
+
+def qk_norm_rope_bwd(dyq: torch.Tensor, dyk: Optional[torch.Tensor], q: torch.Tensor, k: Optional[torch.Tensor],
+                     positions: Optional[torch.Tensor], inv_freq: Optional[torch.Tensor],
+                     gamma_q: Optional[torch.Tensor] = None, gamma_k: Optional[torch.Tensor] = None, *,
+                     norm: bool = True, eps: float = 1e-6, sections=None, interleaved: bool = False,
+                     dgamma_q: Optional[torch.Tensor] = None, dgamma_k: Optional[torch.Tensor] = None,
+                     accumulate: bool = False, out=None):
+    """Gradients of qk_norm_rope_fwd from those of its outputs and its inputs:
+    (dq, dk, dgamma_q, dgamma_k), the weights' in fp32 (None without weights).
+    `out` = (dq, dk) to write into, e.g. views of a packed gradient
+    (nott_qk_norm_rope_bwd)."""
+    a = _QkRope(q, k, positions, inv_freq, gamma_q, gamma_k, norm, eps, sections, interleaved)
+    if (k is None) != (dyk is None):
+        raise ValueError("dyk goes with k")
+    dq, dk = out if out is not None else (torch.empty(a.q_shape, dtype=q.dtype, device=q.device),
+                                          None if k is None else torch.empty(a.k_shape, dtype=q.dtype, device=q.device))
+    for t, nm, shape, st in ((dyq, "dyq", a.q_shape, a.d.yq_stride), (dyk, "dyk", a.k_shape, a.d.yk_stride),
+                             (dq, "dq", a.q_shape, a.d.dq_stride), (dk, "dk", a.k_shape, a.d.dk_stride)):
+        if t is None and k is None and nm in ("dyk", "dk"):
+            continue
+        st[:] = _head_strides(t, nm, shape, q)
+        if nm in ("dq", "dk"):
+            _check_out(t, nm)
+    dh = q.shape[3]
+    if gamma_q is not None and dgamma_q is None:
+        dgamma_q = torch.empty(dh, dtype=torch.float32, device=q.device)
+    if gamma_k is not None and dgamma_k is None:
+        dgamma_k = torch.empty(dh, dtype=torch.float32, device=q.device)
+    for g, nm in ((dgamma_q, "dgamma_q"), (dgamma_k, "dgamma_k")):
+        if g is not None:
+            _check(g, nm, shape=(dh,), dtype=torch.float32, device=q.device)
+    _ctx_for(q).call("nott_qk_norm_rope_bwd", C.byref(a.d), nott_dtype(q.dtype), _ptr(dyq), _ptr(dyk), _ptr(q), _ptr(k),
+                     _ptr(gamma_q), _ptr(gamma_k), _ptr(a.positions), _ptr(a.inv_freq), _ptr(dq), _ptr(dk),
+                     _ptr(dgamma_q), _ptr(dgamma_k), int(accumulate))
+    return dq, dk, dgamma_q, dgamma_k
+
+
+# ---------------------------------------------------------------- gated linear
+_ACTS = {"silu": _abi.NOTT_ACT_SILU, "gelu": _abi.NOTT_ACT_GELU, "gelu_tanh": _abi.NOTT_ACT_GELU_TANH,
+         "relu": _abi.NOTT_ACT_RELU, "sigmoid": _abi.NOTT_ACT_SIGMOID}
+
+
+def _gated_shapes(x: torch.Tensor, w: torch.Tensor, act: str):
+    if act not in _ACTS:
+        raise ValueError(f"unknown activation {act!r}; expected one of {', '.join(_ACTS)}")
+    if x.dim() < 1 or w.dim() != 2 or w.shape[0] == 0 or w.shape[0] % 2 or w.shape[1] == 0 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"w must be [2·f, d] (gate rows, then up rows) for x [..., d]: got {tuple(w.shape)} and "
+                         f"{tuple(x.shape)}")
+    d, f = w.shape[1], w.shape[0] // 2
+    nott_dtype(x.dtype)
+    _check(x, "x")
+    _check(w, "w", dtype=x.dtype, device=x.device)
+    return x.numel() // d, d, f
+
+
+def gated_linear_fwd(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None, *, act: str = "silu",
+                     save: bool = False):
+    """h = act(g)·u with [g | u] = x·wᵀ + b, w [2·f, d] packed gate rows first, b
+    fp32.  act: silu, gelu, gelu_tanh, relu, sigmoid.  Returns (h, gu): gu
+    [..., 2·f] is what the backward needs, None unless save
+    (nott_gated_linear_fwd)."""
+    m, d, f = _gated_shapes(x, w, act)
+    if b is not None:
+        _check(b, "b", shape=(2 * f,), dtype=torch.float32, device=x.device)
+    h = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=x.device)
+    gu = torch.empty((*x.shape[:-1], 2 * f), dtype=x.dtype, device=x.device) if save else None
+    _ctx_for(x).call("nott_gated_linear_fwd", nott_dtype(x.dtype), m, d, f, _ACTS[act], _ptr(x), _ptr(w), _ptr(b), _ptr(h),
+                     _ptr(gu))
+    return h, gu
+
+
+def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w: torch.Tensor, gu: torch.Tensor, *, act: str = "silu",
+                     need_dx: bool = True, need_dw: bool = True, need_db: bool = True,
+                     dx: Optional[torch.Tensor] = None, dw: Optional[torch.Tensor] = None,
+                     db: Optional[torch.Tensor] = None, accumulate: bool = False):
+    """(dx, dw, db) of gated_linear_fwd from dh and its gu; dw and db fp32
+    (nott_gated_linear_bwd)."""
+    m, d, f = _gated_shapes(x, w, act)
+    _check(dh, "dh", shape=(*x.shape[:-1], f), dtype=x.dtype, device=x.device)
+    _check(gu, "gu", shape=(*x.shape[:-1], 2 * f), dtype=x.dtype, device=x.device)
+    if need_dx:
+        dx = torch.empty_like(x) if dx is None else dx
+        _check(dx, "dx", shape=tuple(x.shape), dtype=x.dtype, device=x.device)
+    if need_dw:
+        dw = torch.empty((2 * f, d), dtype=torch.float32, device=x.device) if dw is None else dw
+        _check(dw, "dw", shape=(2 * f, d), dtype=torch.float32, device=x.device)
+    if need_db:
+        db = torch.empty((2 * f,), dtype=torch.float32, device=x.device) if db is None else db
+        _check(db, "db", shape=(2 * f,), dtype=torch.float32, device=x.device)
+    dx, dw, db = (t if need else None for t, need in ((dx, need_dx), (dw, need_dw), (db, need_db)))
+    _ctx_for(x).call("nott_gated_linear_bwd", nott_dtype(x.dtype), m, d, f, _ACTS[act], _ptr(dh), _ptr(x), _ptr(w),
+                     _ptr(gu), _ptr(dx), _ptr(dw), _ptr(db), int(accumulate))
+    return dx, dw, db
+
+
+# ------------------------------------------------- log probabilities of given tokens
+def token_logprob_fwd(logits: torch.Tensor, labels: torch.Tensor, *, scale: float = 1.0, top: int = 0):
+    """(logprob, entropy, lse, top_logprob, top_index) of the rows of logits [n, c]
+    under softmax(scale·logits): the log probability of each label (0 where it is
+    -100), the row's entropy and log-sum-exp (fp32 [n]), and its `top` most
+    likely columns with their log probabilities ([n, top], largest first, equal
+    ones lowest column first; None with top = 0) (nott_token_logprob_fwd)."""
+    n, c = _logprob_shapes(logits, labels, scale)
+    if not 0 <= top <= min(c, 64):
+        raise ValueError(f"top must be 0 to min(c, 64) = {min(c, 64)}")
+    _check(logits, "logits")
+    _check(labels, "labels", shape=(n,), dtype=torch.int64, device=logits.device)
+    lp, ent, lse = (torch.empty(n, dtype=torch.float32, device=logits.device) for _ in range(3))
+    tv = torch.empty((n, top), dtype=torch.float32, device=logits.device) if top else None
+    ti = torch.empty((n, top), dtype=torch.int64, device=logits.device) if top else None
+    _ctx_for(logits).call("nott_token_logprob_fwd", nott_dtype(logits.dtype), n, c, _ptr(logits), _ptr(labels),
+                          float(scale), int(top), _ptr(lp), _ptr(ent), _ptr(lse), _ptr(tv), _ptr(ti))
+    return lp, ent, lse, tv, ti
+
+
+def _logprob_shapes(logits: torch.Tensor, labels: torch.Tensor, scale: float):
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError("logits must be [n, c] with c > 0")
+    if tuple(labels.shape) != (logits.shape[0],):
+        raise ValueError(f"labels has shape {tuple(labels.shape)}, expected {(logits.shape[0],)}")
+    if not 0 < scale < 1e30:
+        raise ValueError("scale must be positive and finite")
+    return logits.shape
+
+
+def token_logprob_bwd(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, dlogprob: torch.Tensor, *,
+                      entropy: Optional[torch.Tensor] = None, dentropy: Optional[torch.Tensor] = None,
+                      scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dlogits of token_logprob_fwd's logprob (and, with dentropy and the forward's
+    entropy, of the entropy) from the forward's lse; out may be logits
+    (nott_token_logprob_bwd)."""
+    n, c = _logprob_shapes(logits, labels, scale)
+    if dentropy is not None and entropy is None:
+        raise ValueError("dentropy needs entropy")
+    _check(logits, "logits")
+    _check(labels, "labels", shape=(n,), dtype=torch.int64, device=logits.device)
+    for t, nm in ((lse, "lse"), (dlogprob, "dlogprob"), (entropy, "entropy"), (dentropy, "dentropy")):
+        if t is not None:
+            _check(t, nm, shape=(n,), dtype=torch.float32, device=logits.device)
+    dl = torch.empty_like(logits) if out is None else out
+    _check(dl, "out", shape=logits.shape, dtype=logits.dtype, device=logits.device)
+    _ctx_for(logits).call("nott_token_logprob_bwd", nott_dtype(logits.dtype), n, c, _ptr(logits), _ptr(labels),
+                          float(scale), _ptr(lse), _ptr(entropy), _ptr(dlogprob), _ptr(dentropy), _ptr(dl))
+    return dl
