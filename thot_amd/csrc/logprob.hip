@@ -3,8 +3,13 @@
 //   m = max z, S = Σ exp(z − m), T = Σ exp(z − m)·(z − m)
 //   lse = m + log S, logprob = (z_y − m) − log S, entropy = log S − T/S
 //   dlogit_j = scale·(dlp·([j = y] − p_j) − dH·p_j·(log p_j + H)), p = exp(z − lse)
-// m, S and T are carried together over one read of the row: with a new maximum m'
-// and a = exp(m − m'), S' = a·S and T' = a·(T + S·(m − m')).
+// Forward: one read of the row.  m, S and T are carried together: with a new
+// maximum m' and a = exp(m − m'), S' = a·S and T' = a·(T + S·(m − m')).  The same
+// running maxima give the top tokens: the top-th largest of 64 maxima over 64
+// disjoint shares of the row is a bound that at least `top` elements reach and
+// few more do (24 of any number for 20), and only threads whose own maximum
+// reaches it read their elements again.
+// Backward: one read and one write.
 #include "common.hpp"
 
 namespace {
@@ -13,7 +18,14 @@ using nott::ceil_div;
 
 constexpr int64_t kIgnoreIndex = -100;
 constexpr int kMaxTop = 64;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kUnroll = 4;          // 16-byte groups in flight per thread
+constexpr int kMaxSplits = 64;      // a merging wave has a lane for each
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718f;
+// Logits of −inf or the type's lowest value mask a token: below this (times scale)
+// there is nothing.  As the maximum's first value it keeps −inf − (−inf) out.
+constexpr float kNothing = -1e30f;
+// Exponents (base 2) are not taken below this: 0·(−inf) is no part of a sum.
+constexpr float kLeast = -300.f;
 
 // e^x for x <= 0: what the rounding of x·log2 e leaves (2^-19 of the result at
 // x = −30) is taken into the result.  Below −200 (masked logits: −inf and the
@@ -23,58 +35,69 @@ __device__ __forceinline__ float exp_neg(float x) {
     const float t = x * kLog2e;
     const float r = fmaf(x, kLog2e, -t);
     const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, r * 0.69314718f, e);
+    return fmaf(e, r * kLn2, e);
 }
 
-// Logits of −inf or the type's lowest value mask a token: below this there is
-// nothing.  As the maximum's first value it keeps −inf − (−inf) out of everything.
-constexpr float kNothing = -1e30f;
+// z = scale·logit; to_log2 = scale·log2 e; first: the maximum of no live logit.
+struct Scale {
+    float scale, to_log2, first;
+};
 
-// The running statistics of a part of a row.  A NaN stays in s and t.
+// The running statistics of a part of a row: the largest logit m, s = Σ 2^w and
+// t = Σ w·2^w with w = (logit − m)·to_log2.  A NaN stays in s.
 struct Stats {
     float m, s, t;
-    __device__ __forceinline__ void add(float z) {
-        if (z > m) {
-            const float d = m - z, a = exp_neg(d);
-            t = a * fmaf(s, fmaxf(d, -200.f), t);
-            s *= a;
-            m = z;
-        }
-        const float d = z - m, e = exp_neg(d);
-        s += e;
-        t = fmaf(e, fmaxf(d, -200.f), t);
-    }
-    __device__ __forceinline__ void merge(const Stats& o) {
-        const float n = fmaxf(m, o.m);
-        const float da = m - n, db = o.m - n;
-        const float a = exp_neg(da), b = exp_neg(db);
-        t = a * fmaf(s, fmaxf(da, -200.f), t) + b * fmaf(o.s, fmaxf(db, -200.f), o.t);
-        s = a * s + b * o.s;
+    // Carries s and t over to the maximum n >= m.
+    __device__ __forceinline__ void raise(float n, const Scale& sc) {
+        const float d = fmaxf((m - n) * sc.to_log2, kLeast);
+        const float a = __builtin_amdgcn_exp2f(d);
+        t = a * fmaf(s, d, t);
+        s *= a;
         m = n;
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&v)[N], const Scale& sc) {
+        float n = m;
+#pragma unroll
+        for (int e = 0; e < N; ++e) n = fmaxf(n, v[e]);
+        raise(n, sc);
+        const float off = -n * sc.to_log2;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float w = fmaf(v[e], sc.to_log2, off);
+            const float p = __builtin_amdgcn_exp2f(w);
+            s += p;
+            t = fmaf(p, fmaxf(w, kLeast), t);
+        }
+    }
+    __device__ __forceinline__ void merge(Stats o, const Scale& sc) {
+        const float n = fmaxf(m, o.m);
+        raise(n, sc);
+        o.raise(n, sc);
+        s += o.s;
+        t += o.t;
+    }
+    __device__ __forceinline__ void merge_wave(const Scale& sc) {
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) merge(Stats{__shfl_xor(m, i), __shfl_xor(s, i), __shfl_xor(t, i)}, sc);
     }
 };
 
 // Order of the most likely tokens as one whole number: the value in an order that
-// integers keep (−0 as +0, NaN above all), then the lower column.
+// integers keep (−0 as +0, NaN above all), then the lower column.  0 is no key.
 __device__ __forceinline__ uint64_t top_key(float z, uint32_t col) {
     uint32_t u = __builtin_bit_cast(uint32_t, z + 0.f);
     u = z != z ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
     return ((uint64_t)u << 32) | (uint32_t)~col;
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int mask) {
-    const uint32_t lo = __shfl_xor((uint32_t)v, mask), hi = __shfl_xor((uint32_t)(v >> 32), mask);
-    return ((uint64_t)hi << 32) | lo;
-}
-
-__device__ __forceinline__ uint64_t block_max64(uint64_t v, uint64_t* red) {
-    for (int s = 32; s; s >>= 1) v = max(v, shfl_xor64(v, s));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t r = red[0];
-    for (int i = 1; i < (int)blockDim.x / 64; ++i) r = max(r, red[i]);
-    __syncthreads();
-    return r;
+__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const uint32_t lo = __shfl_xor((uint32_t)v, s), hi = __shfl_xor((uint32_t)(v >> 32), s);
+        v = max(v, ((uint64_t)hi << 32) | lo);
+    }
+    return v;
 }
 
 struct FwdOut {
@@ -86,77 +109,333 @@ struct FwdOut {
     unsigned long long* err;
 };
 
-// log p of a logit z (scaled) in a row of statistics st.
-__device__ __forceinline__ float log_p(float z, const Stats& st, float logs) {
-    return st.s == 0.f || z < kNothing ? -INFINITY : (z - st.m) - logs;
+// log p of a logit in a row of statistics st, logs = log st.s.
+__device__ __forceinline__ float log_p(float x, const Stats& st, float logs, const Scale& sc) {
+    return st.s == 0.f || x * sc.scale < kNothing ? -INFINITY : (x - st.m) * sc.scale - logs;
 }
 
 // The row's outputs from its statistics.
 template <typename T>
-__device__ __forceinline__ void write_row(const FwdOut& o, int64_t row, int64_t y, int64_t c, const T* z, float scale,
+__device__ __forceinline__ void write_row(const FwdOut& o, int64_t row, int64_t y, int64_t c, const T* z, const Scale& sc,
                                           const Stats& st, float logs) {
     const bool empty = st.s == 0.f;   // every token masked
     float lp = 0.f;
-    if (y >= 0 && y < c) lp = log_p(Io<T>::ld(z, y) * scale, st, logs);
+    if (y >= 0 && y < c) lp = log_p(Io<T>::ld(z, y), st, logs, sc);
     else if (y != kIgnoreIndex) atomicAdd(o.err, 1ull);
     o.logprob[row] = lp;
-    if (o.lse) o.lse[row] = empty ? -INFINITY : st.m + logs;
-    if (o.entropy) o.entropy[row] = empty ? 0.f : logs - st.t / st.s;
+    if (o.lse) o.lse[row] = empty ? -INFINITY : fmaf(st.m, sc.scale, logs);
+    if (o.entropy) o.entropy[row] = empty ? 0.f : logs - st.t * kLn2 / st.s;
 }
 
-// Any row, a workgroup each; the top tokens one after the other, each by a scan
-// for the largest key below the last one.
 template <typename T>
-__global__ __launch_bounds__(256) void logprob_any_kernel(const T* __restrict__ logits,
-                                                          const int64_t* __restrict__ labels, int64_t c, float scale,
-                                                          int top, FwdOut o) {
-    __shared__ Stats part[4];
-    __shared__ uint64_t red[4];
+__device__ __forceinline__ void write_top(const FwdOut& o, int64_t at, uint64_t key, const T* z, const Stats& st,
+                                          float logs, const Scale& sc) {
+    const uint32_t col = ~(uint32_t)key;
+    o.top_index[at] = col;
+    o.top_logprob[at] = log_p(Io<T>::ld(z, col), st, logs, sc);
+}
+
+template <typename T>
+__device__ __forceinline__ typename Pack16<T>::Raw minus_inf() {
+    if constexpr (sizeof(T) == 2) return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+    else return f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+}
+
+// A part of a row of any alignment as its whole 16-byte groups (group i at base +
+// i·G) and the fewer than 2·G elements before and after them, one per thread.
+template <typename T>
+struct Span {
+    static constexpr int G = Pack16<T>::N;
+    const T* base;
+    int groups;
+    int single;   // this thread's single element from p, −1: none
+    __device__ __forceinline__ Span(const T* p, int len) {
+        const int s0 = min((int)((G - ((uintptr_t)p / sizeof(T)) % G) % G), len);
+        groups = (len - s0) / G;
+        base = p + s0;
+        const int tail = s0 + groups * G, tid = (int)threadIdx.x;
+        single = tid < s0 ? tid : tail + (tid - s0) < len ? tail + (tid - s0) : -1;
+    }
+};
+
+// A workgroup per row, or with splits > 1 per part of `chunk` columns, whose
+// statistics and top keys go to `stats` [row][split] and `keys` [row][split][top].
+// LDS holds `cap` candidates for the top tokens; a row in which more reach the
+// bound (many equal logits, or too few live ones for a bound) is scanned for each.
+// Bound by memory (one read of the logits), then by the exponential and four more
+// instructions an element.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void logprob_kernel(const T* __restrict__ logits, const int64_t* __restrict__ labels,
+                                                     int64_t c, int chunk, Scale sc, int top, int cap, FwdOut o,
+                                                     Stats* __restrict__ stats, uint64_t* __restrict__ keys) {
+    constexpr int G = Pack16<T>::N, W = NT / 64;
+    extern __shared__ uint64_t cand[];
+    __shared__ Stats part[W];
+    __shared__ float share[NT];
+    __shared__ float bound_s;
+    __shared__ int count;
+    __shared__ uint64_t red[W];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int64_t row = blockIdx.x;
     const T* z = logits + row * c;
-    Stats st{kNothing, 0.f, 0.f};
-    for (int64_t j = threadIdx.x; j < c; j += 256) st.add(Io<T>::ld(z, j) * scale);
-    for (int s = 32; s; s >>= 1) st.merge(Stats{__shfl_xor(st.m, s), __shfl_xor(st.s, s), __shfl_xor(st.t, s)});
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = st;
+    const int64_t j0 = (int64_t)blockIdx.y * chunk;
+    const int len = (int)min((int64_t)chunk, c - j0);
+    const Span<T> sp(z + j0, len);
+    Stats st{sc.first, 0.f, 0.f};
+    const int full = sp.groups / (NT * kUnroll);
+    for (int i = 0; i < full; ++i) {
+        typename Pack16<T>::Raw raw[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            raw[u] = Pack16<T>::template raw<true>(sp.base + (int64_t)((i * kUnroll + u) * NT + tid) * G);
+        float v[kUnroll * G];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) Pack16<T>::unpack(raw[u], reinterpret_cast<float(&)[G]>(v[u * G]));
+        st.add(v, sc);
+    }
+    for (int k = full * kUnroll * NT + tid; k < sp.groups; k += NT) {
+        float v[G];
+        Pack16<T>::template ld<true>(sp.base + (int64_t)k * G, v);
+        st.add(v, sc);
+    }
+    if (sp.single >= 0) {
+        const float v[1] = {Io<T>::ld(z + j0, sp.single)};
+        st.add(v, sc);
+    }
+    const float own = st.s != st.s ? INFINITY : st.m;   // a NaN is among the largest
+    if (tid == 0) count = 0;
+    share[tid] = own;
+    st.merge_wave(sc);
+    if (lane == 0) part[wid] = st;
     __syncthreads();
     st = part[0];
-    for (int i = 1; i < 4; ++i) st.merge(part[i]);
+#pragma unroll
+    for (int i = 1; i < W; ++i) st.merge(part[i], sc);
     const float logs = logf(st.s);
-    if (threadIdx.x == 0) write_row(o, row, labels[row], c, z, scale, st, logs);
+    const bool whole = gridDim.y == 1;
+    const int64_t at = row * gridDim.y + blockIdx.y;
+    if (tid == 0) {
+        if (whole) write_row(o, row, labels[row], c, z, sc, st, logs);
+        else stats[at] = st;
+    }
+    if (top == 0) return;
+    if (wid == 0) {
+        float v = share[lane];
+#pragma unroll
+        for (int i = 1; i < W; ++i) v = fmaxf(v, share[i * 64 + lane]);
+        int rank = 0;
+#pragma unroll
+        for (int j = 0; j < 64; ++j) {
+            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), j));
+            rank += w > v || (w == v && j < lane) ? 1 : 0;
+        }
+        if (rank == top - 1) bound_s = v;
+    }
+    __syncthreads();
+    // no bound among live logits: every element is a candidate
+    const float bound = bound_s > sc.first ? bound_s : -INFINITY;
+    auto offer = [&](float x, int64_t col) {
+        if (x < bound) return;
+        const int i = atomicAdd(&count, 1);
+        if (i < cap) cand[i] = top_key(x, (uint32_t)col);
+    };
+    if (!(own < bound) || bound == -INFINITY) {
+        const int64_t first = j0 + (sp.base - (z + j0));
+        for (int k = tid; k < sp.groups; k += NT * kUnroll) {
+            typename Pack16<T>::Raw raw[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+                raw[u] = Pack16<T>::template raw<false>(sp.base + (int64_t)min(k + u * NT, sp.groups - 1) * G);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                if (k + u * NT >= sp.groups) break;
+                float v[G];
+                Pack16<T>::unpack(raw[u], v);
+#pragma unroll
+                for (int e = 0; e < G; ++e) offer(v[e], first + (int64_t)(k + u * NT) * G + e);
+            }
+        }
+        if (sp.single >= 0) offer(Io<T>::ld(z + j0, sp.single), j0 + sp.single);
+    }
+    __syncthreads();
+    const int n = count;
+    auto put = [&](int i, uint64_t key) {
+        if (whole) write_top(o, row * top + i, key, z, st, logs, sc);
+        else keys[at * top + i] = key;
+    };
+    if (n <= cap) {
+        for (int i = tid; i < n; i += NT) {
+            const uint64_t key = cand[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += cand[j] > key ? 1 : 0;
+            if (rank < top) put(rank, key);
+        }
+        for (int i = n + tid; i < top; i += NT) put(i, 0);   // only in a part shorter than top
+        return;
+    }
     uint64_t last = ~uint64_t(0);
     for (int i = 0; i < top; ++i) {
         uint64_t best = 0;
-        for (int64_t j = threadIdx.x; j < c; j += 256) {
-            const uint64_t key = top_key(Io<T>::ld(z, j), (uint32_t)j);
+        for (int j = tid; j < len; j += NT) {
+            const uint64_t key = top_key(Io<T>::ld(z + j0, j), (uint32_t)(j0 + j));
             if (key < last && key > best) best = key;
         }
-        last = block_max64(best, red);
-        if (threadIdx.x == 0) {
-            const int64_t j = (uint32_t)~(uint32_t)last;
-            o.top_index[row * top + i] = j;
-            o.top_logprob[row * top + i] = log_p(Io<T>::ld(z, j) * scale, st, logs);
-        }
+        best = wave_max64(best);
+        if (lane == 0) red[wid] = best;
+        __syncthreads();
+        last = red[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) last = max(last, red[w]);
+        __syncthreads();
+        if (tid == 0) put(i, last);
     }
 }
 
+// The rows from their parts, a wave each: lane s has split s's statistics and its
+// sorted keys, of which the largest head is taken `top` times.
 template <typename T>
-__global__ __launch_bounds__(256) void logprob_bwd_any_kernel(const T* logits, const int64_t* __restrict__ labels,
-                                                              int64_t c, float scale, const float* __restrict__ lse,
-                                                              const float* __restrict__ entropy,
-                                                              const float* __restrict__ dlogprob,
-                                                              const float* __restrict__ dentropy, T* dlogits) {
+__global__ __launch_bounds__(64) void logprob_merge_kernel(const T* __restrict__ logits,
+                                                           const int64_t* __restrict__ labels, int64_t c, int splits,
+                                                           Scale sc, int top, FwdOut o, const Stats* __restrict__ stats,
+                                                           const uint64_t* __restrict__ keys) {
+    const int lane = (int)threadIdx.x;
     const int64_t row = blockIdx.x;
+    const bool mine = lane < splits;
+    const uint64_t* list = keys + (row * splits + lane) * top;
+    Stats st = mine ? stats[row * splits + lane] : Stats{sc.first, 0.f, 0.f};
+    int taken = 0;
+    uint64_t head = mine && top ? list[0] : 0;
+    st.merge_wave(sc);
+    const float logs = logf(st.s);
+    const T* z = logits + row * c;
+    if (lane == 0) write_row(o, row, labels[row], c, z, sc, st, logs);
+    uint64_t won = 0;   // lane i: the i-th
+    for (int i = 0; i < top; ++i) {
+        const uint64_t best = wave_max64(head);
+        if (lane == i) won = best;
+        if (head == best) {
+            ++taken;
+            head = taken < top ? list[taken] : 0;
+        }
+    }
+    if (lane < top) write_top(o, row * top + lane, won, z, st, logs, sc);
+}
+
+// The gradient of one part of a row: NT·kUnroll groups, part 0 with the single
+// elements.  A group's loads are all issued before its stores, so dlogits may be
+// logits.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void logprob_bwd_kernel(const T* logits, const int64_t* __restrict__ labels, int64_t c,
+                                                         uint32_t parts, FastDiv by_parts, float scale,
+                                                         const float* __restrict__ lse,
+                                                         const float* __restrict__ entropy,
+                                                         const float* __restrict__ dlogprob,
+                                                         const float* __restrict__ dentropy, T* dlogits) {
+    constexpr int G = Pack16<T>::N;
+    uint32_t r32, part;
+    by_parts.divmod(blockIdx.x, r32, part);
+    const int64_t row = r32;
+    const int tid = (int)threadIdx.x;
+    const T* z = logits + row * c;
+    T* dz = dlogits + row * c;
+    const Span<T> sp(z, (int)c);
+    const int k0 = (int)part * NT * kUnroll + tid;
+    typename Pack16<T>::Raw raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) raw[u] = minus_inf<T>();
+    if (sp.groups > 0) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            raw[u] = Pack16<T>::template raw<true>(sp.base + (int64_t)min(k0 + u * NT, sp.groups - 1) * G);
+    }
     const int64_t y = labels[row];
     const bool given = y >= 0 && y < c;
     const float l = lse[row], h = dentropy ? entropy[row] : 0.f;
     const float dl = given ? dlogprob[row] : 0.f, dh = dentropy ? dentropy[row] : 0.f;
-    for (int64_t j = threadIdx.x; j < c; j += 256) {
-        const float lp = Io<T>::ld(logits, row * c + j) * scale - l;
-        const float p = exp_neg(lp);
-        float g = -p * fmaf(dh, fmaxf(lp, -200.f) + h, dl);
-        if (j == y) g += dl;
-        Io<T>::st(dlogits, row * c + j, l == -INFINITY ? 0.f : g * scale);
+    const int first = (int)(sp.base - z);
+    auto grad = [&](float x, int col) {
+        const float lp = fmaf(x, scale, -l);
+        float g = -exp_neg(lp) * fmaf(dh, fmaxf(lp, -200.f) + h, dl);
+        if (col == (int)y) g += dl;
+        return l == -INFINITY ? 0.f : g * scale;
+    };
+    const bool vec = ((uintptr_t)(dz + first) % 16) == 0;
+    const float xs = part == 0 && sp.single >= 0 ? Io<T>::ld(z, sp.single) : 0.f;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const int k = k0 + u * NT;
+        if (k >= sp.groups) break;
+        const int col = first + k * G;
+        float v[G];
+        Pack16<T>::unpack(raw[u], v);
+#pragma unroll
+        for (int e = 0; e < G; ++e) v[e] = grad(v[e], col + e);
+        if (vec) {
+            Pack16<T>::template st<true>(dz + col, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < G; ++e) Io<T>::st(dz, col + e, v[e]);
+        }
     }
+    if (part == 0 && sp.single >= 0) Io<T>::st(dz, sp.single, grad(xs, sp.single));
+}
+
+// Up to this many columns a row is one wave's.
+constexpr int64_t kWaveColumns = 2048;
+
+template <typename T>
+int forward(nott_ctx ctx, int64_t n, int64_t c, const T* logits, const int64_t* labels, double scale, int top,
+            const FwdOut& o) {
+    const Scale sc{(float)scale, (float)(scale * 1.4426950408889634), (float)std::max(-1e30 / scale, -3e38)};
+    const int nt = c <= kWaveColumns ? 64 : 256;
+    // Fewer rows than fill the card are split, into parts of at least 4096 columns.
+    int64_t splits = 1;
+    if (n < 4 * ctx->num_cu)
+        splits = std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, 4 * (int64_t)ctx->num_cu / n, c / 4096}));
+    const int64_t chunk = splits == 1 ? c : ceil_div(ceil_div(c, splits), 64) * 64;
+    splits = ceil_div(c, chunk);
+    Stats* stats = nullptr;
+    uint64_t* keys = nullptr;
+    if (splits > 1) {
+        const size_t sb = (sizeof(Stats) * (size_t)(n * splits) + 255) & ~size_t(255);
+        char* ws = static_cast<char*>(nott::workspace(ctx, sb + sizeof(uint64_t) * (size_t)(n * splits * top)));
+        if (!ws) return NOTT_ERR_ALLOC;
+        stats = reinterpret_cast<Stats*>(ws);
+        keys = reinterpret_cast<uint64_t*>(ws + sb);
+    }
+    const int cap = top == 0 ? 0 : nt == 64 ? 256 : 1024;
+    const dim3 grid((unsigned)n, (unsigned)splits);
+    if (nt == 64)
+        hipLaunchKernelGGL((logprob_kernel<T, 64>), grid, dim3(64), sizeof(uint64_t) * cap, ctx->stream, logits, labels, c,
+                           (int)chunk, sc, top, cap, o, stats, keys);
+    else
+        hipLaunchKernelGGL((logprob_kernel<T, 256>), grid, dim3(256), sizeof(uint64_t) * cap, ctx->stream, logits, labels,
+                           c, (int)chunk, sc, top, cap, o, stats, keys);
+    if (splits > 1)
+        hipLaunchKernelGGL(logprob_merge_kernel<T>, dim3((unsigned)n), dim3(64), 0, ctx->stream, logits, labels, c,
+                           (int)splits, sc, top, o, stats, keys);
+    return nott::launch_status(ctx, "token_logprob");
+}
+
+template <typename T>
+int backward(nott_ctx ctx, int64_t n, int64_t c, const T* logits, const int64_t* labels, float scale, const float* lse,
+             const float* entropy, const float* dlogprob, const float* dentropy, T* dlogits) {
+    const int nt = c <= kWaveColumns ? 64 : 256;
+    const int64_t parts = std::max<int64_t>(1, ceil_div(c, (int64_t)nt * kUnroll * Pack16<T>::N));
+    // as many rows a launch as workgroups have numbers
+    const int64_t rows = std::max<int64_t>(1, ((int64_t(1) << 31) - 1) / parts);
+    for (int64_t r = 0; r < n; r += rows) {
+        const unsigned grid = (unsigned)(std::min(rows, n - r) * parts);
+        const FastDiv by((uint32_t)parts);
+        auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(grid), dim3(nt), 0, ctx->stream, logits + r * c, labels + r, c, (uint32_t)parts,
+                               by, scale, lse + r, entropy ? entropy + r : nullptr, dlogprob + r,
+                               dentropy ? dentropy + r : nullptr, dlogits + r * c);
+        };
+        if (nt == 64) launch(logprob_bwd_kernel<T, 64>);
+        else launch(logprob_bwd_kernel<T, 256>);
+    }
+    return nott::launch_status(ctx, "token_logprob backward");
 }
 
 }  // namespace
@@ -175,13 +454,8 @@ extern "C" int nott_token_logprob_fwd(nott_ctx ctx, nott_dtype dtype, int64_t n,
     NOTT_REQUIRE(ctx, top == 0 || (top_logprob && top_index), "nott_token_logprob_fwd: top needs top_logprob and top_index");
     nott::DeviceScope scope(ctx->device);
     const FwdOut o{logprob, entropy, lse, top_logprob, top_index, ctx->err_word};
-    if (dtype == NOTT_F32)
-        hipLaunchKernelGGL(logprob_any_kernel<float>, dim3((unsigned)n), dim3(256), 0, ctx->stream,
-                           static_cast<const float*>(logits), labels, c, (float)scale, (int)top, o);
-    else
-        hipLaunchKernelGGL(logprob_any_kernel<bf16_t>, dim3((unsigned)n), dim3(256), 0, ctx->stream,
-                           static_cast<const bf16_t*>(logits), labels, c, (float)scale, (int)top, o);
-    return nott::launch_status(ctx, "token_logprob");
+    if (dtype == NOTT_F32) return forward(ctx, n, c, static_cast<const float*>(logits), labels, scale, (int)top, o);
+    return forward(ctx, n, c, static_cast<const bf16_t*>(logits), labels, scale, (int)top, o);
 }
 
 extern "C" int nott_token_logprob_bwd(nott_ctx ctx, nott_dtype dtype, int64_t n, int64_t c, const void* logits,
@@ -197,12 +471,8 @@ extern "C" int nott_token_logprob_bwd(nott_ctx ctx, nott_dtype dtype, int64_t n,
     NOTT_REQUIRE(ctx, !dentropy || entropy, "nott_token_logprob_bwd: dentropy needs entropy");
     nott::DeviceScope scope(ctx->device);
     if (dtype == NOTT_F32)
-        hipLaunchKernelGGL(logprob_bwd_any_kernel<float>, dim3((unsigned)n), dim3(256), 0, ctx->stream,
-                           static_cast<const float*>(logits), labels, c, (float)scale, lse, entropy, dlogprob, dentropy,
-                           static_cast<float*>(dlogits));
-    else
-        hipLaunchKernelGGL(logprob_bwd_any_kernel<bf16_t>, dim3((unsigned)n), dim3(256), 0, ctx->stream,
-                           static_cast<const bf16_t*>(logits), labels, c, (float)scale, lse, entropy, dlogprob, dentropy,
-                           static_cast<bf16_t*>(dlogits));
-    return nott::launch_status(ctx, "token_logprob backward");
+        return backward(ctx, n, c, static_cast<const float*>(logits), labels, (float)scale, lse, entropy, dlogprob,
+                        dentropy, static_cast<float*>(dlogits));
+    return backward(ctx, n, c, static_cast<const bf16_t*>(logits), labels, (float)scale, lse, entropy, dlogprob, dentropy,
+                    static_cast<bf16_t*>(dlogits));
 }
