@@ -60,7 +60,7 @@ struct RopeArgs {
     int32_t t, dh, norm;
     float eps;
     int64_t items;      // tokens · (hq + hk)
-    FastDiv by_heads, by_t;
+    FastDiv by_heads, by_t, by_half;
     float* partial;     // backward: [grid][2·dh] sums of dz·x̂, q then k; null: not asked for
 };
 
@@ -163,6 +163,217 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs<T> a) {
     }
 }
 
+// Σ over the LPH lanes (a power of two) that share a head; all of them get it.
+template <int LPH>
+__device__ __forceinline__ float head_sum(float v) {
+    if constexpr (LPH >= 2) v += dpp_f32<0xB1>(v);    // quad_perm [1,0,3,2]
+    if constexpr (LPH >= 4) v += dpp_f32<0x4E>(v);    // quad_perm [2,3,0,1]
+    if constexpr (LPH >= 8) v += dpp_f32<0x141>(v);   // row_half_mirror
+    if constexpr (LPH >= 16) v += dpp_f32<0x140>(v);  // row_mirror
+    if constexpr (LPH >= 32) v += __shfl_xor(v, 16);
+    if constexpr (LPH >= 64) v += __shfl_xor(v, 32);
+    return v;
+}
+
+// Heads of whole aligned 16-byte chunks: LPH lanes a head, each with two chunks
+// that hold both elements of its pairs (chunks c and c + rot/2, or neighbours), so
+// a head's norm, weight and rotation need no exchange but the sum.  A workgroup
+// takes `tpb` tokens at a time: it issues the loads of its first heads, forms the
+// tokens' cosines and sines in LDS while they are on their way (once for all
+// heads), then runs over the heads, U in flight a lane.
+// Memory bound: one read and one write of q and k (and one more read backward).
+template <typename T, int LPH, bool BWD>
+__global__ __launch_bounds__(256) void rope_vec_kernel(RopeArgs<T> a, int tpb) {
+    constexpr int E = Pack16<T>::N, GPB = 256 / LPH, U = BWD ? 2 : 4;
+    typedef typename Pack16<T>::Raw Raw;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    f32x2* table = reinterpret_cast<f32x2*>(lds);   // [tpb][rot/2] {cos, sin}
+    const int tid = (int)threadIdx.x, slot = tid % LPH, group = tid / LPH;
+    const int half = a.turns.half, nc = a.dh / E, heads = a.q.n + a.k.n;
+    const bool inter = a.turns.interleaved;
+    // this lane's chunks; rotated: they are the two halves of pairs
+    const int hc = inter ? 0 : half / E;
+    const bool rotated = slot < hc;
+    const int c0 = rotated ? slot : 2 * hc + 2 * (slot - hc), c1 = rotated ? slot + hc : c0 + 1;
+    const bool has0 = c0 < nc, has1 = c1 < nc;
+    const int e0 = has0 ? c0 * E : 0, e1 = has1 ? c1 * E : 0;
+    const float inv_dh = 1.f / (float)a.dh;
+    Raw gq0, gq1, gk0, gk1;
+    if (a.q.gamma) gq0 = Pack16<T>::raw(a.q.gamma + e0), gq1 = Pack16<T>::raw(a.q.gamma + e1);
+    if (a.k.gamma) gk0 = Pack16<T>::raw(a.k.gamma + e0), gk1 = Pack16<T>::raw(a.k.gamma + e1);
+    float dg[BWD ? 4 : 1][E];   // dγ of this lane's chunks: q, q, k, k
+#pragma unroll
+    for (auto& d : dg)
+#pragma unroll
+        for (int e = 0; e < E; ++e) d[e] = 0.f;
+    for (int64_t t0 = (int64_t)blockIdx.x * tpb; t0 < a.turns.tokens; t0 += (int64_t)gridDim.x * tpb) {
+        const int nt = (int)min((int64_t)tpb, a.turns.tokens - t0);
+        const int items = nt * heads;
+        for (int base = 0; base < items; base += GPB * U) {
+            Raw rx[U][2], rd[BWD ? U : 1][2];
+            int64_t to[U];
+            uint32_t tok[U];
+            bool of_q[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                uint32_t head, bi, ti;
+                a.by_heads.divmod((uint32_t)min(base + u * GPB + group, items - 1), tok[u], head);
+                a.by_t.divmod((uint32_t)t0 + tok[u], bi, ti);
+                of_q[u] = head < (uint32_t)a.q.n;
+                if (!of_q[u]) head -= a.q.n;
+                const Heads<T>& h = of_q[u] ? a.q : a.k;
+                if (!BWD || a.norm) {
+                    const T* x = h.x + at(h.xs, bi, ti, head);
+                    rx[u][0] = Pack16<T>::raw(x + e0);
+                    rx[u][1] = Pack16<T>::raw(x + e1);
+                }
+                if constexpr (BWD) {
+                    const T* dy = h.dy + at(h.ys, bi, ti, head);
+                    rd[u][0] = Pack16<T>::raw(dy + e0);
+                    rd[u][1] = Pack16<T>::raw(dy + e1);
+                }
+                to[u] = BWD ? at(h.os, bi, ti, head) : at(h.ys, bi, ti, head);
+            }
+            if (base == 0 && half > 0) {
+                __syncthreads();   // the last tokens' readers are done
+                for (int i = tid; i < nt * half; i += 256) {
+                    uint32_t t, pair;
+                    a.by_half.divmod((uint32_t)i, t, pair);
+                    float c, s;
+                    a.turns.turn(t0 + t, (int)pair, c, s);
+                    table[i] = f32x2{c, s};
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                // y0, y1: turned from / to z0, z1 (BWD: dy turned back)
+                float v0[E], v1[E];
+                const f32x2* tab = table + (int)tok[u] * half;
+                auto turn = [&](float (&p)[E], float (&q)[E]) {
+                    if (!inter) {
+                        if (rotated) {
+#pragma unroll
+                            for (int e = 0; e < E; ++e) {
+                                const f32x2 cs = tab[c0 * E + e];
+                                const float s = BWD ? -cs.y : cs.y, b = q[e];
+                                q[e] = fmaf(p[e], s, b * cs.x);
+                                p[e] = fmaf(-b, s, p[e] * cs.x);
+                            }
+                        }
+                        return;
+                    }
+                    auto neighbours = [&](float (&w)[E], int pair) {
+#pragma unroll
+                        for (int e = 0; e < E; e += 2) {
+                            if (pair + e / 2 >= half) continue;
+                            const f32x2 cs = tab[pair + e / 2];
+                            const float s = BWD ? -cs.y : cs.y, b = w[e + 1];
+                            w[e + 1] = fmaf(w[e], s, b * cs.x);
+                            w[e] = fmaf(-b, s, w[e] * cs.x);
+                        }
+                    };
+                    neighbours(p, e0 / 2);
+                    neighbours(q, e1 / 2);
+                };
+                float x0[E], x1[E], r = 1.f;
+                if (!BWD || a.norm) {
+                    Pack16<T>::unpack(rx[u][0], x0);
+                    Pack16<T>::unpack(rx[u][1], x1);
+                    float ss = 0.f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        x0[e] = has0 ? x0[e] : 0.f;
+                        x1[e] = has1 ? x1[e] : 0.f;
+                        ss = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], ss));
+                    }
+                    if (a.norm) r = rsqrtf(fmaf(head_sum<LPH>(ss), inv_dh, a.eps));
+                }
+                const bool weighted = (of_q[u] ? a.q.gamma : a.k.gamma) != nullptr;
+                float g0[E], g1[E];
+                Pack16<T>::unpack(of_q[u] ? gq0 : gk0, g0);
+                Pack16<T>::unpack(of_q[u] ? gq1 : gk1, g1);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    g0[e] = weighted ? g0[e] : 1.f;
+                    g1[e] = weighted ? g1[e] : 1.f;
+                }
+                if constexpr (!BWD) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        v0[e] = a.norm ? x0[e] * r * g0[e] : x0[e];
+                        v1[e] = a.norm ? x1[e] * r * g1[e] : x1[e];
+                    }
+                    turn(v0, v1);
+                } else {
+                    Pack16<T>::unpack(rd[u][0], v0);
+                    Pack16<T>::unpack(rd[u][1], v1);
+                    turn(v0, v1);
+                    if (a.norm) {
+                        // an item past the last adds nothing to dγ
+                        const bool counts = base + u * GPB + group < items;
+                        float dot = 0.f;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            x0[e] *= r;
+                            x1[e] *= r;
+                        }
+                        if (counts && of_q[u]) {
+#pragma unroll
+                            for (int e = 0; e < E; ++e) {
+                                dg[0][e] = fmaf(v0[e], x0[e], dg[0][e]);
+                                dg[1][e] = fmaf(v1[e], x1[e], dg[1][e]);
+                            }
+                        } else if (counts) {
+#pragma unroll
+                            for (int e = 0; e < E; ++e) {
+                                dg[2][e] = fmaf(v0[e], x0[e], dg[2][e]);
+                                dg[3][e] = fmaf(v1[e], x1[e], dg[3][e]);
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            v0[e] *= g0[e];
+                            v1[e] *= g1[e];
+                            dot = fmaf(has0 ? v0[e] : 0.f, x0[e], fmaf(has1 ? v1[e] : 0.f, x1[e], dot));
+                        }
+                        dot = head_sum<LPH>(dot) * inv_dh;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            v0[e] = r * fmaf(-x0[e], dot, v0[e]);
+                            v1[e] = r * fmaf(-x1[e], dot, v1[e]);
+                        }
+                    }
+                }
+                if (base + u * GPB + group < items) {
+                    T* out = (of_q[u] ? a.q.out : a.k.out) + to[u];
+                    if (has0) Pack16<T>::st(out + e0, v0);
+                    if (has1) Pack16<T>::st(out + e1, v1);
+                }
+            }
+        }
+    }
+    if constexpr (BWD) {
+        if (!a.partial) return;
+        // over the wave's heads, then the four waves in order
+        __syncthreads();
+        const int lane = tid & 63, wid = tid >> 6;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+#pragma unroll
+                for (int s = LPH; s < 64; s <<= 1) dg[i][e] += __shfl_xor(dg[i][e], s);
+                if (lane < LPH && ((i & 1) ? has1 : has0))
+                    lds[(wid * 2 + (i >> 1)) * a.dh + ((i & 1) ? e1 : e0) + e] = dg[i][e];
+            }
+        __syncthreads();
+        float* p = a.partial + (int64_t)blockIdx.x * 2 * a.dh;
+        for (int j = tid; j < 2 * a.dh; j += 256)
+            p[j] = (lds[j] + lds[2 * a.dh + j]) + (lds[4 * a.dh + j] + lds[6 * a.dh + j]);
+    }
+}
+
 // dγ (+)= Σ_blocks partial[block], in an order that the grid alone fixes: a
 // workgroup has 16 columns, 16 threads of each taking every 16th block.
 __global__ __launch_bounds__(256) void rope_dgamma_kernel(const float* __restrict__ partial, int blocks, int dh,
@@ -255,27 +466,91 @@ RopeArgs<T> make_args(const nott_qk_rope_desc& d, const void* q, const void* k, 
     a.items = d.b * d.t * (d.hq + d.hk);
     a.by_heads = FastDiv((uint32_t)(d.hq + d.hk));
     a.by_t = FastDiv((uint32_t)d.t);
+    a.by_half = FastDiv((uint32_t)std::max<int64_t>(1, d.rot / 2));
     return a;
+}
+
+// Whether the heads are whole 16-byte chunks wherever they lie, and no chunk holds
+// both rotated halves.
+template <typename T>
+bool in_chunks(const RopeArgs<T>& a, bool bwd) {
+    constexpr int E = Pack16<T>::N;
+    if (a.dh % E || (!a.turns.interleaved && a.turns.half % E)) return false;
+    for (const Heads<T>* h : {&a.q, &a.k}) {
+        if (h->n == 0) continue;
+        const bool x = !bwd || a.norm;
+        for (const void* p : {(const void*)(x ? h->x : nullptr), (const void*)h->dy, (const void*)h->out, (const void*)h->gamma})
+            if ((uintptr_t)p % 16) return false;
+        for (int i = 0; i < 3; ++i)
+            if ((x && h->xs[i] % E) || h->ys[i] % E || (bwd && h->os[i] % E)) return false;
+    }
+    return true;
+}
+
+struct Launch {
+    unsigned grid;
+    int lph, tpb;
+    size_t lds;
+};
+// Tokens of a workgroup: as many as fill its lanes' loads once (one token's heads
+// more often), fewer where there are too few for every CU, with at most 16 KiB of
+// cosines and sines.  Backward the workgroups take turns, so that there are few
+// partial sums of dγ.
+template <typename T>
+Launch plan(nott_ctx ctx, const RopeArgs<T>& a, bool bwd) {
+    constexpr int E = Pack16<T>::N;
+    Launch l{};
+    const int slots = (a.dh / E + 1) / 2;
+    for (l.lph = 2; l.lph < slots;) l.lph *= 2;
+    const int heads = a.q.n + a.k.n;
+    int64_t tpb = (int64_t)(256 / l.lph) * (bwd ? 2 : 4) / heads;
+    if (a.turns.half) tpb = std::min<int64_t>(tpb, 2048 / a.turns.half);
+    tpb = std::min<int64_t>(tpb, a.turns.tokens / ctx->num_cu);
+    l.tpb = (int)std::max<int64_t>(tpb, 1);
+    l.grid = (unsigned)std::min<int64_t>(ceil_div(a.turns.tokens, l.tpb), bwd ? 8 * (int64_t)ctx->num_cu : 0x7fffffff);
+    l.lds = std::max(sizeof(f32x2) * (size_t)l.tpb * a.turns.half, bwd ? sizeof(float) * 8 * (size_t)a.dh : 0);
+    return l;
+}
+
+template <typename T, bool BWD>
+void launch_vec(nott_ctx ctx, const Launch& l, const RopeArgs<T>& a) {
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(l.grid), dim3(256), l.lds, ctx->stream, a, l.tpb); };
+    switch (l.lph) {
+        case 2: return go(rope_vec_kernel<T, 2, BWD>);
+        case 4: return go(rope_vec_kernel<T, 4, BWD>);
+        case 8: return go(rope_vec_kernel<T, 8, BWD>);
+        case 16: return go(rope_vec_kernel<T, 16, BWD>);
+        case 32: return go(rope_vec_kernel<T, 32, BWD>);
+        default:   // fp32 heads past 256
+            if constexpr (sizeof(T) == 4) return go(rope_vec_kernel<T, 64, BWD>);
+    }
 }
 
 template <typename T>
 int forward(nott_ctx ctx, const RopeArgs<T>& a) {
-    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.items, 4), 32 * (int64_t)ctx->num_cu);
-    hipLaunchKernelGGL((rope_any_kernel<T, false>), dim3(grid), dim3(256), 0, ctx->stream, a);
+    if (in_chunks(a, false)) {
+        launch_vec<T, false>(ctx, plan(ctx, a, false), a);
+    } else {
+        const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.items, 4), 32 * (int64_t)ctx->num_cu);
+        hipLaunchKernelGGL((rope_any_kernel<T, false>), dim3(grid), dim3(256), 0, ctx->stream, a);
+    }
     return nott::launch_status(ctx, "qk_norm_rope");
 }
 
 template <typename T>
 int backward(nott_ctx ctx, RopeArgs<T> a, float* dgq, float* dgk, int accumulate) {
-    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.items, 4), 8 * (int64_t)ctx->num_cu);
+    const bool vec = in_chunks(a, true);
+    Launch l = vec ? plan(ctx, a, true) : Launch{};
+    if (!vec) l.grid = (unsigned)std::min<int64_t>(ceil_div(a.items, 4), 8 * (int64_t)ctx->num_cu);
     if (a.norm && (dgq || dgk)) {
-        a.partial = static_cast<float*>(nott::workspace(ctx, sizeof(float) * 2 * (size_t)a.dh * grid));
+        a.partial = static_cast<float*>(nott::workspace(ctx, sizeof(float) * 2 * (size_t)a.dh * l.grid));
         if (!a.partial) return NOTT_ERR_ALLOC;
     }
-    hipLaunchKernelGGL((rope_any_kernel<T, true>), dim3(grid), dim3(256), 0, ctx->stream, a);
+    if (vec) launch_vec<T, true>(ctx, l, a);
+    else hipLaunchKernelGGL((rope_any_kernel<T, true>), dim3(l.grid), dim3(256), 0, ctx->stream, a);
     if (a.partial)
         hipLaunchKernelGGL(rope_dgamma_kernel, dim3((unsigned)ceil_div(2 * a.dh, 16)), dim3(256), 0, ctx->stream,
-                           a.partial, (int)grid, a.dh, dgq, dgk, accumulate);
+                           a.partial, (int)l.grid, a.dh, dgq, dgk, accumulate);
     return nott::launch_status(ctx, "qk_norm_rope backward");
 }
 
