@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -23,6 +24,10 @@ def nott_dtype(t: torch.dtype) -> int:
     if t not in _DTYPES:
         raise TypeError(f"unsupported dtype {t}; expected float32 or bfloat16")
     return _DTYPES[t]
+
+
+# The current stream's handle without a Stream object around it (1.1 us a call).
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 class Context:
@@ -45,7 +50,7 @@ class Context:
             pass
 
     def call(self, name: str, *args):
-        self.lib.nott_set_stream(self.handle, C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream))
+        self.lib.nott_set_stream(self.handle, _raw_stream(self.device))
         rc = getattr(self.lib, name)(self.handle, *args)
         if rc != 0:
             msg = self.lib.nott_last_error(self.handle).decode()
@@ -76,7 +81,7 @@ def context(device: Optional[int] = None) -> Context:
 
 
 def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else C.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _check(t: torch.Tensor, name: str, shape=None, dtype=None, device=None):
@@ -608,22 +613,22 @@ def rope_frequencies(rot: int, theta: float = 10000.0, device="cuda") -> torch.T
 def _head_strides(t: Optional[torch.Tensor], name: str, shape, like: torch.Tensor) -> tuple:
     """(batch, token, head) strides of a [b, t, h, dh] tensor whose heads are contiguous."""
     if t is None:
-        return (0, 0, 0)
-    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} is missing")
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != like.dtype or t.device != like.device:
         raise TypeError(f"{name} must have the dtype and device of q")
-    if t.numel() and t.shape[3] > 1 and t.stride(3) != 1:
+    sb, st, sh, one = t.stride()
+    if one != 1 and t.numel() and shape[3] > 1:
         raise ValueError(f"the elements of a head of {name} must be contiguous")
-    st = tuple(t.stride()[:3])
-    if st == (0, 0, 0) and t.numel() > t.shape[3]:   # three zeros mean contiguous to the entry point
+    if sb == st == sh == 0 and t.numel() > shape[3]:   # three zeros mean contiguous to the entry point
         raise ValueError(f"{name} repeats one head (strides {t.stride()}); make it contiguous")
-    return st
+    return sb, st, sh
 
 
-def _check_out(t: Optional[torch.Tensor], name: str):
+def _check_out(t: torch.Tensor, name: str):
     """An output's elements must be apart from each other (no expanded dimension)."""
-    if t is None or t.numel() == 0:
+    if t.is_contiguous() or t.numel() == 0:
         return
     reach = 1
     for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
@@ -632,52 +637,67 @@ def _check_out(t: Optional[torch.Tensor], name: str):
         reach = st * (n - 1) + reach
 
 
-class _QkRope:
-    """The checked arguments of a qk_norm_rope call."""
+_DENSE = (0, 0, 0)
+# QkRopeDesc's fields in order (a fifth of the time of its constructor, 4 us)
+_QK_ROPE = struct.Struct("=28q4id")
+assert _QK_ROPE.size == C.sizeof(QkRopeDesc)
 
-    def __init__(self, q, k, positions, inv_freq, gamma_q, gamma_k, norm, eps, sections, interleaved):
-        if not isinstance(q, torch.Tensor) or q.dim() != 4 or (k is not None and k.dim() != 4):
-            raise ValueError("q and k must be [b, t, heads, dh]")
-        b, t, hq, dh = q.shape
-        hk = 0 if k is None else k.shape[2]
-        nott_dtype(q.dtype)
-        self.q_shape, self.k_shape = (b, t, hq, dh), (b, t, hk, dh)
-        if dh < 1 or dh > 512:
-            raise ValueError("head size must be 1 to 512")
-        if not eps >= 0:
-            raise ValueError("eps must not be negative")
-        if not norm and (gamma_q is not None or gamma_k is not None):
-            raise ValueError("a weight needs the norm")
-        rot, axes = 0, 1
-        if inv_freq is not None:
-            rot = 2 * inv_freq.numel()
-            if inv_freq.dim() != 1 or rot > dh:
-                raise ValueError(f"inv_freq must be [rot/2] with rot at most the head size {dh}")
-            if positions is None:
-                raise ValueError("inv_freq needs positions")
-            if positions.dim() == 2:
-                positions = positions[None]
-            if positions.dim() != 3 or tuple(positions.shape[1:]) != (b, t) or not 1 <= positions.shape[0] <= 4:
-                raise ValueError(f"positions must be [b, t] or [axes, b, t] with 1 to 4 axes for b = {b}, t = {t}")
-            axes = positions.shape[0]
-        elif positions is not None:
-            raise ValueError("positions need inv_freq")
-        sections = [rot // 2] if sections is None and axes == 1 else sections
-        if sections is None or len(sections) != axes or min(sections) < 0 or sum(sections) != rot // 2:
-            raise ValueError(f"sections must be {axes} pair counts that add up to {rot // 2}")
-        self.d = QkRopeDesc(b, t, hq, hk, dh, rot, (C.c_int64 * 4)(*sections))
-        self.d.axes, self.d.interleaved, self.d.norm, self.d.eps = axes, int(interleaved), int(norm), float(eps)
-        self.d.q_stride[:] = _head_strides(q, "q", self.q_shape, q)
-        self.d.k_stride[:] = _head_strides(k, "k", self.k_shape, q)
-        if rot:
-            _check(inv_freq, "inv_freq", dtype=torch.float64, device=q.device)
-            _check(positions, "positions", dtype=torch.int64, device=q.device)
-        for g, nm in ((gamma_q, "gamma_q"), (gamma_k, "gamma_k")):
-            if g is not None:
-                _check(g, nm, shape=(dh,), dtype=q.dtype, device=q.device)
-        if not q.is_cuda:
-            raise ValueError("q must be a device tensor")
-        self.positions, self.inv_freq = (positions, inv_freq) if rot else (None, None)
+
+def _out_strides(t: Optional[torch.Tensor], name: str, shape, like: torch.Tensor) -> tuple:
+    st = _head_strides(t, name, shape, like)
+    _check_out(t, name)
+    return st
+
+
+def _qk_rope_desc(q, k, positions, inv_freq, gamma_q, gamma_k, norm, eps, sections, interleaved):
+    """Checks the arguments that qk_norm_rope's two directions share: the descriptor
+    (strides of q and k filled in), positions, the output shapes."""
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("q and k must be [b, t, heads, dh]")
+    b, t, hq, dh = q.shape
+    hk = 0 if k is None else k.shape[2]
+    nott_dtype(q.dtype)
+    if dh < 1 or dh > 512:
+        raise ValueError("head size must be 1 to 512")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    if not norm and (gamma_q is not None or gamma_k is not None):
+        raise ValueError("a weight needs the norm")
+    rot, axes = 0, 1
+    if inv_freq is not None:
+        rot = 2 * inv_freq.numel()
+        if inv_freq.dim() != 1 or rot > dh:
+            raise ValueError(f"inv_freq must be [rot/2] with rot at most the head size {dh}")
+        if positions is None:
+            raise ValueError("inv_freq needs positions")
+        if positions.dim() == 2:
+            positions = positions[None]
+        if positions.dim() != 3 or not 1 <= positions.shape[0] <= 4 or positions.shape[1:] != (b, t):
+            raise ValueError(f"positions must be [b, t] or [axes, b, t] with 1 to 4 axes for b = {b}, t = {t}")
+        axes = positions.shape[0]
+    elif positions is not None:
+        raise ValueError("positions need inv_freq")
+    if sections is None and axes == 1:
+        sections = (rot // 2,)
+    elif sections is None or len(sections) != axes or min(sections) < 0 or sum(sections) != rot // 2:
+        raise ValueError(f"sections must be {axes} pair counts that add up to {rot // 2}")
+    dev = q.device
+    q_st = _head_strides(q, "q", q.shape, q)
+    k_shape = torch.Size((b, t, hk, dh))
+    k_st = _DENSE if k is None else _head_strides(k, "k", k_shape, q)
+    if rot:
+        _check(inv_freq, "inv_freq", dtype=torch.float64, device=dev)
+        _check(positions, "positions", dtype=torch.int64, device=dev)
+    if gamma_q is not None:
+        _check(gamma_q, "gamma_q", shape=(dh,), dtype=q.dtype, device=dev)
+    if gamma_k is not None:
+        _check(gamma_k, "gamma_k", shape=(dh,), dtype=q.dtype, device=dev)
+    if not q.is_cuda:
+        raise ValueError("q must be a device tensor")
+    d = QkRopeDesc.from_buffer_copy(_QK_ROPE.pack(b, t, hq, hk, dh, rot, *sections, *(0, 0, 0, 0)[axes:], *q_st, *k_st,
+                                                  *_DENSE, *_DENSE, *_DENSE, *_DENSE, axes, bool(interleaved), bool(norm),
+                                                  0, eps))
+    return d, (positions if rot else None), k_shape
 
 
 def qk_norm_rope_fwd(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[torch.Tensor],
@@ -691,16 +711,16 @@ def qk_norm_rope_fwd(q: torch.Tensor, k: Optional[torch.Tensor], positions: Opti
     inv_freq float64 (rope_frequencies).  norm=False: the rotation alone;
     positions and inv_freq None: the norm alone.  `out` = (yq, yk) to write into
     (q and k themselves are fine).  Returns (yq, yk) (nott_qk_norm_rope_fwd)."""
-    a = _QkRope(q, k, positions, inv_freq, gamma_q, gamma_k, norm, eps, sections, interleaved)
-    yq, yk = out if out is not None else (torch.empty(a.q_shape, dtype=q.dtype, device=q.device),
-                                          None if k is None else torch.empty(a.k_shape, dtype=q.dtype, device=q.device))
-    for t, nm, shape, st in ((yq, "yq", a.q_shape, a.d.yq_stride), (yk, "yk", a.k_shape, a.d.yk_stride)):
-        if t is None and nm == "yk" and k is None:
-            continue
-        st[:] = _head_strides(t, nm, shape, q)
-        _check_out(t, nm)
-    _ctx_for(q).call("nott_qk_norm_rope_fwd", C.byref(a.d), nott_dtype(q.dtype), _ptr(q), _ptr(k), _ptr(gamma_q),
-                     _ptr(gamma_k), _ptr(a.positions), _ptr(a.inv_freq), _ptr(yq), _ptr(yk))
+    d, positions, k_shape = _qk_rope_desc(q, k, positions, inv_freq, gamma_q, gamma_k, norm, eps, sections, interleaved)
+    if out is None:
+        yq, yk = q.new_empty(q.shape), None if k is None else k.new_empty(k_shape)
+    else:
+        yq, yk = out
+        d.yq_stride[:] = _out_strides(yq, "yq", q.shape, q)
+        if k is not None:
+            d.yk_stride[:] = _out_strides(yk, "yk", k_shape, q)
+    _ctx_for(q).call("nott_qk_norm_rope_fwd", C.byref(d), _DTYPES[q.dtype], _ptr(q), _ptr(k), _ptr(gamma_q),
+                     _ptr(gamma_k), _ptr(positions), _ptr(inv_freq), _ptr(yq), None if k is None else _ptr(yk))
     return yq, yk
 
 
@@ -714,29 +734,30 @@ def qk_norm_rope_bwd(dyq: torch.Tensor, dyk: Optional[torch.Tensor], q: torch.Te
     (dq, dk, dgamma_q, dgamma_k), the weights' in fp32 (None without weights).
     `out` = (dq, dk) to write into, e.g. views of a packed gradient
     (nott_qk_norm_rope_bwd)."""
-    a = _QkRope(q, k, positions, inv_freq, gamma_q, gamma_k, norm, eps, sections, interleaved)
+    d, positions, k_shape = _qk_rope_desc(q, k, positions, inv_freq, gamma_q, gamma_k, norm, eps, sections, interleaved)
     if (k is None) != (dyk is None):
         raise ValueError("dyk goes with k")
-    dq, dk = out if out is not None else (torch.empty(a.q_shape, dtype=q.dtype, device=q.device),
-                                          None if k is None else torch.empty(a.k_shape, dtype=q.dtype, device=q.device))
-    for t, nm, shape, st in ((dyq, "dyq", a.q_shape, a.d.yq_stride), (dyk, "dyk", a.k_shape, a.d.yk_stride),
-                             (dq, "dq", a.q_shape, a.d.dq_stride), (dk, "dk", a.k_shape, a.d.dk_stride)):
-        if t is None and k is None and nm in ("dyk", "dk"):
-            continue
-        st[:] = _head_strides(t, nm, shape, q)
-        if nm in ("dq", "dk"):
-            _check_out(t, nm)
+    d.yq_stride[:] = _head_strides(dyq, "dyq", q.shape, q)
+    if k is not None:
+        d.yk_stride[:] = _head_strides(dyk, "dyk", k_shape, q)
+    if out is None:
+        dq, dk = q.new_empty(q.shape), None if k is None else k.new_empty(k_shape)
+    else:
+        dq, dk = out
+        d.dq_stride[:] = _out_strides(dq, "dq", q.shape, q)
+        if k is not None:
+            d.dk_stride[:] = _out_strides(dk, "dk", k_shape, q)
     dh = q.shape[3]
     if gamma_q is not None and dgamma_q is None:
-        dgamma_q = torch.empty(dh, dtype=torch.float32, device=q.device)
+        dgamma_q = q.new_empty(dh, dtype=torch.float32)
     if gamma_k is not None and dgamma_k is None:
-        dgamma_k = torch.empty(dh, dtype=torch.float32, device=q.device)
+        dgamma_k = q.new_empty(dh, dtype=torch.float32)
     for g, nm in ((dgamma_q, "dgamma_q"), (dgamma_k, "dgamma_k")):
         if g is not None:
             _check(g, nm, shape=(dh,), dtype=torch.float32, device=q.device)
-    _ctx_for(q).call("nott_qk_norm_rope_bwd", C.byref(a.d), nott_dtype(q.dtype), _ptr(dyq), _ptr(dyk), _ptr(q), _ptr(k),
-                     _ptr(gamma_q), _ptr(gamma_k), _ptr(a.positions), _ptr(a.inv_freq), _ptr(dq), _ptr(dk),
-                     _ptr(dgamma_q), _ptr(dgamma_k), int(accumulate))
+    _ctx_for(q).call("nott_qk_norm_rope_bwd", C.byref(d), _DTYPES[q.dtype], _ptr(dyq), _ptr(dyk), _ptr(q), _ptr(k),
+                     _ptr(gamma_q), _ptr(gamma_k), _ptr(positions), _ptr(inv_freq), _ptr(dq),
+                     None if k is None else _ptr(dk), _ptr(dgamma_q), _ptr(dgamma_k), int(accumulate))
     return dq, dk, dgamma_q, dgamma_k
 
 
@@ -810,9 +831,9 @@ def token_logprob_fwd(logits: torch.Tensor, labels: torch.Tensor, *, scale: floa
         raise ValueError(f"top must be 0 to min(c, 64) = {min(c, 64)}")
     _check(logits, "logits")
     _check(labels, "labels", shape=(n,), dtype=torch.int64, device=logits.device)
-    lp, ent, lse = (torch.empty(n, dtype=torch.float32, device=logits.device) for _ in range(3))
-    tv = torch.empty((n, top), dtype=torch.float32, device=logits.device) if top else None
-    ti = torch.empty((n, top), dtype=torch.int64, device=logits.device) if top else None
+    lp, ent, lse = logits.new_empty((3, n), dtype=torch.float32).unbind(0)
+    tv = logits.new_empty((n, top), dtype=torch.float32) if top else None
+    ti = logits.new_empty((n, top), dtype=torch.int64) if top else None
     _ctx_for(logits).call("nott_token_logprob_fwd", nott_dtype(logits.dtype), n, c, _ptr(logits), _ptr(labels),
                           float(scale), int(top), _ptr(lp), _ptr(ent), _ptr(lse), _ptr(tv), _ptr(ti))
     return lp, ent, lse, tv, ti
