@@ -22,16 +22,20 @@ __device__ __forceinline__ float exp_near(float x) {
     const float e = __builtin_amdgcn_exp2f(t);
     return fmaf(e, r * 0.69314718f, e);
 }
+// FAST (bf16 results): the exponent's rounding, |x|·2^-24 of the result, stays in;
+// no clamp is needed then (exp2 ends in 0 or infinity, 1/infinity is 0).
+template <bool FAST>
 __device__ __forceinline__ float sigmoid(float x) {
+    if constexpr (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.4426950f));
     const float e = exp_near(__builtin_amdgcn_fmed3f(-x, -80.f, 80.f));
     return x != x ? x : __builtin_amdgcn_rcpf(1.f + e);
 }
 
 // The activation (a) and its derivative (da).
-template <int ACT>
+template <int ACT, bool FAST>
 __device__ __forceinline__ void activate(float g, float& a, float& da) {
     if constexpr (ACT == NOTT_ACT_SILU) {
-        const float e = sigmoid(g);
+        const float e = sigmoid<FAST>(g);
         a = g * e;
         da = fmaf(a, 1.f - e, e);
     } else if constexpr (ACT == NOTT_ACT_GELU) {
@@ -39,20 +43,20 @@ __device__ __forceinline__ void activate(float g, float& a, float& da) {
         a = g * cdf;
         da = fmaf(g * 0.39894228f, exp_near(fmaxf(-0.5f * g * g, -120.f)), cdf);
     } else if constexpr (ACT == NOTT_ACT_GELU_TANH) {
-        const float e = sigmoid(1.5957691f * fmaf(0.044715f * g, g * g, g));
+        const float e = sigmoid<FAST>(1.5957691f * fmaf(0.044715f * g, g * g, g));
         a = g * e;
         da = fmaf(a * (1.f - e), 1.5957691f * fmaf(0.134145f * g, g, 1.f), e);
     } else if constexpr (ACT == NOTT_ACT_RELU) {
         a = relu_out(g);
         da = g > 0.f ? 1.f : g != g ? g : 0.f;
     } else {
-        a = sigmoid(g);
+        a = sigmoid<FAST>(g);
         da = a * (1.f - a);
     }
 }
 
 template <class F>
-int with_act(int act, F f) {
+__host__ __device__ __forceinline__ auto with_act(int act, F f) {
     switch (act) {
         case NOTT_ACT_SILU: return f(std::integral_constant<int, NOTT_ACT_SILU>());
         case NOTT_ACT_GELU: return f(std::integral_constant<int, NOTT_ACT_GELU>());
@@ -61,6 +65,110 @@ int with_act(int act, F f) {
         default: return f(std::integral_constant<int, NOTT_ACT_SIGMOID>());
     }
 }
+
+// The forward's epilogue on the direct-to-LDS engine: a wave's TM×32 block of g
+// and u (lane l: row l % 32, columns 8q + 4·(l/32) + e in register 4q + e of each
+// 32×32 block) becomes h and, where asked for, [g | u], each staged through LDS
+// as [row][32] with the 16-byte chunk at chunk ^ (row/2 % 4) and its halves
+// exchanged on rows with bit 3 set, and stored as whole 64-byte row pieces.
+struct GatedStore {
+    bf16_t* h;
+    bf16_t* gu;
+    const float* bias;
+    int64_t m, f;
+    int32_t act;
+    bool vec;   // 16-byte stores fit every row
+    template <int TM>
+    __device__ __forceinline__ void flush(const char NOTT_LDS* buf, bf16_t* dst, int64_t ld, int64_t m0, int64_t c0,
+                                          int lane) const {
+        if (vec) {
+            const int c = lane & 3;
+#pragma unroll
+            for (int it = 0; it < TM / 16; ++it) {
+                const int row = 16 * it + (lane >> 2);
+                u32x4 w = *reinterpret_cast<const u32x4 NOTT_LDS*>(buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+                if ((row >> 3) & 1) w = u32x4{w.z, w.w, w.x, w.y};
+                if (m0 + row < m && c0 + 8 * c < f) *reinterpret_cast<u32x4*>(dst + (m0 + row) * ld + c0 + 8 * c) = w;
+            }
+        } else {
+            const int c = lane & 31;
+            for (int it = 0; it < TM / 2; ++it) {
+                const int row = 2 * it + (lane >> 5);
+                const bf16_t v = *reinterpret_cast<const bf16_t NOTT_LDS*>(
+                    buf + row * 64 + (((c >> 3) ^ ((row >> 1) & 3)) << 4) + ((((c >> 2) & 1) ^ ((row >> 3) & 1)) << 3) +
+                    (c & 3) * 2);
+                if (m0 + row < m && c0 + c < f) dst[(m0 + row) * ld + c0 + c] = v;
+            }
+        }
+    }
+    template <int TM, int FM>
+    __device__ __forceinline__ void store_pair(f32x16 (&acc)[FM][2], char NOTT_LDS* buf, int64_t m0, int64_t c0,
+                                               int lane) const {
+        const int r = lane & 31, hf = lane >> 5;
+        auto put = [&](int row, int q, const float (&v)[4]) {
+            const u32x2 w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+            *reinterpret_cast<u32x2 NOTT_LDS*>(buf + row * 64 + ((q ^ ((row >> 1) & 3)) << 4) +
+                                               ((hf ^ ((row >> 3) & 1)) << 3)) = w;
+        };
+        auto stage = [&](int which) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[i][which][4 * q + e];
+                    put(32 * i + r, q, v);
+                }
+        };
+        if (bias) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                float b[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int64_t c = c0 + 8 * (e >> 2) + 4 * hf + (e & 3);
+                    b[e] = bias[(c < f ? c : f - 1) + w * f];
+                }
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[i][w][e] += b[e];
+            }
+        }
+        if (gu) {
+            stage(0);
+            flush<TM>(buf, gu, 2 * f, m0, c0, lane);
+            stage(1);
+            flush<TM>(buf, gu + f, 2 * f, m0, c0, lane);
+        }
+        with_act(act, [&](auto A) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float a, da;
+                        activate<decltype(A)::value, true>(acc[i][0][4 * q + e], a, da);
+                        v[e] = a * acc[i][1][4 * q + e];
+                    }
+                    put(32 * i + r, q, v);
+                }
+        });
+        flush<TM>(buf, h, f, m0, c0, lane);
+    }
+};
+
+}  // namespace
+
+template <>
+struct nott::gemm::dma::IsPaired<GatedStore> {
+    static constexpr bool value = true;
+};
+
+namespace {
 
 // h (and gu) from the fp32 products pre [m, 2f] and the bias.
 template <typename T, int ACT>
@@ -72,7 +180,7 @@ __global__ __launch_bounds__(256) void gated_act_kernel(const float* __restrict_
     for (int64_t r = blockIdx.y; r < m; r += gridDim.y) {
         const float g = pre[r * 2 * f + c] + bg, u = pre[r * 2 * f + f + c] + bu;
         float a, da;
-        activate<ACT>(g, a, da);
+        activate<ACT, sizeof(T) == 2>(g, a, da);
         Io<T>::st(h, r * f + c, a * u);
         if (gu) {
             Io<T>::st(gu, r * 2 * f + c, g);
@@ -81,13 +189,14 @@ __global__ __launch_bounds__(256) void gated_act_kernel(const float* __restrict_
     }
 }
 
-// [dg|du] [m, 2f] as T, in bf16 also what its rounding leaves (lo).  A workgroup
+// [dg|du] in rows of ld elements as T, in bf16 also what its rounding leaves (lo),
+// and zeros past 2f.  A workgroup
 // takes 64 columns and every gridDim.y-th group of 4 rows; partial (null: no db)
 // [gridDim.y][2f] receives its column sums of the unrounded values.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void gated_dact_kernel(const T* __restrict__ dh, const T* __restrict__ gu, int64_t m,
-                                                         int64_t f, T* __restrict__ hi, T* __restrict__ lo,
-                                                         float* __restrict__ partial) {
+                                                         int64_t f, int64_t ld, T* __restrict__ hi,
+                                                         T* __restrict__ lo, float* __restrict__ partial) {
     __shared__ float red[2][4][64];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     const int64_t c = (int64_t)blockIdx.x * 64 + lane;
@@ -97,16 +206,20 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const T* __restrict__ d
             const float g = Io<T>::ld(gu, r * 2 * f + c), u = Io<T>::ld(gu, r * 2 * f + f + c);
             const float d = Io<T>::ld(dh, r * f + c);
             float a, da;
-            activate<ACT>(g, a, da);
+            activate<ACT, sizeof(T) == 2>(g, a, da);
             const float dg = d * u * da, du = d * a;
             sg += dg;
             su += du;
-            Io<T>::st(hi, r * 2 * f + c, dg);
-            Io<T>::st(hi, r * 2 * f + f + c, du);
+            Io<T>::st(hi, r * ld + c, dg);
+            Io<T>::st(hi, r * ld + f + c, du);
             if constexpr (sizeof(T) == 2) {
                 if (lo) {
-                    lo[r * 2 * f + c] = f32_to_bf16(dg - bf16_to_f32(f32_to_bf16(dg)));
-                    lo[r * 2 * f + f + c] = f32_to_bf16(du - bf16_to_f32(f32_to_bf16(du)));
+                    lo[r * ld + c] = f32_to_bf16(dg - bf16_to_f32(f32_to_bf16(dg)));
+                    lo[r * ld + f + c] = f32_to_bf16(du - bf16_to_f32(f32_to_bf16(du)));
+                }
+                for (int64_t j = 2 * f + c; j < ld; j += f) {
+                    hi[r * ld + j] = 0;
+                    if (lo) lo[r * ld + j] = 0;
                 }
             }
         }
@@ -142,15 +255,172 @@ struct AccStore {
         *p = accumulate ? *p + v : v;
     }
 };
+// The same, and its split-K partials, for the product of both pieces of [dg|du]
+// (stacked along k) with x twice.
+struct PiecesStore : AccStore {
+    int64_t wrap;
+};
+struct PiecesPartial : dma::PartialRowStore {
+    int64_t wrap;
+};
+__device__ __forceinline__ PiecesPartial at_split(const PiecesPartial& ep, int z) { return {ep.at(z), ep.wrap}; }
 
-// C = A·B, operands as in gemm_dma.hpp, on whichever engine takes them.
+}  // namespace
+
+template <> struct nott::gemm::dma::IsWrapped<PiecesStore> { static constexpr bool value = true; };
+template <> struct nott::gemm::dma::IsWrapped<PiecesPartial> { static constexpr bool value = true; };
+
+namespace {
+
+bool ok16(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+int64_t up8(int64_t n) { return (n + 7) & ~int64_t(7); }
+
+// A copy of src [rows, cols] with zeros up to [prows, pcols], for tensors whose rows
+// no 16-byte load fits (the copy is small beside the product it is for).
+__global__ __launch_bounds__(256) void pad_kernel(const bf16_t* __restrict__ src, int64_t rows, int64_t cols,
+                                                  bf16_t* __restrict__ dst, int64_t prows, int64_t pcols) {
+    const int64_t n = prows * pcols / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i * 8 / pcols, c = i * 8 - r * pcols;
+        bf16_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = r < rows && c + e < cols ? src[r * cols + c + e] : bf16_t(0);
+        *reinterpret_cast<u32x4*>(dst + i * 8) = Pack<bf16_t>::make(v);
+    }
+}
+void pad(nott_ctx ctx, const bf16_t* src, int64_t rows, int64_t cols, bf16_t* dst, int64_t prows, int64_t pcols) {
+    hipLaunchKernelGGL(pad_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(prows * pcols, 2048), 8192)), dim3(256), 0,
+                       ctx->stream, src, rows, cols, dst, prows, pcols);
+}
+
+// 16 bytes from any element's address.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+// Few rows (single tokens of some sequences): the weights are streamed once, 16
+// gate rows and the matching 16 up rows a workgroup, its 8 waves dealing out 64
+// k's at a time; x's rows are the other MFMA operand (16·MT of them), both straight
+// from memory into registers in the operand layout (lane l: row l % 16, k =
+// 8·(l/16) + 0..7 of each 32).  The waves' sums meet in LDS.  Rows may start at any
+// address; TAIL: d >= 8 is no multiple of 8, and the last chunk of a row is the
+// row's last 8 elements, moved down.
+// 1 row of 1024 → 4096 4.9 us, 8 rows 5.4 (the 16.8 MB of weights take 3.4 at the
+// copy rate), of 4096 → 11008 31 and 33 us.
+template <int MT, bool TAIL>
+__global__ __launch_bounds__(512) void gated_rows_kernel(const bf16_t* __restrict__ x, const bf16_t* __restrict__ w,
+                                                         const float* __restrict__ bias, int64_t m, int64_t d, int64_t f,
+                                                         int act, bf16_t* __restrict__ h, bf16_t* __restrict__ gu) {
+    constexpr int NW = 8;
+    __shared__ float red[NW][2][MT][256];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int r = lane & 15, kq = lane >> 4;
+    const int64_t c0 = (int64_t)blockIdx.x * 16;
+    const int64_t row = c0 + r < f ? c0 + r : f - 1;
+    const bf16_t* wg = w + row * d;
+    const bf16_t* wu = wg + f * d;
+    const bf16_t* xr[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xr[t] = x + (16 * t + r < m ? 16 * t + r : m - 1) * d;
+    auto chunk = [&](const bf16_t* p, int64_t k) {
+        const int64_t at = k + 8 <= d ? k : d - 8;
+        u32x4 v = *reinterpret_cast<const u32x4_any*>(p + at);
+        if constexpr (TAIL) {
+            unsigned __int128 b = __builtin_bit_cast(unsigned __int128, v);
+            v = __builtin_bit_cast(u32x4, b >> (16 * ((int)(k - at) & 7)));
+        }
+        return k < d ? v : u32x4{0, 0, 0, 0};
+    };
+    f32x4 acc[2][MT];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 g[2][2], u[2][2], b[2][2][MT];
+    auto load = [&](int p, int64_t unit) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int64_t k = 64 * unit + 32 * s + 8 * kq;
+            g[p][s] = chunk(wg, k);
+            u[p][s] = chunk(wu, k);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) b[p][s][t] = chunk(xr[t], k);
+        }
+    };
+    auto mma = [&](int p) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const bf16x8 xv = __builtin_bit_cast(bf16x8, b[p][s][t]);
+                acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, g[p][s]), xv, acc[0][t], 0, 0, 0);
+                acc[1][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u[p][s]), xv, acc[1][t], 0, 0, 0);
+            }
+    };
+    const int64_t units = (d + 63) / 64;
+    for (int64_t i = wid; i < units; i += 2 * NW) {   // two units of 64 k in flight
+        load(0, i);
+        const bool two = i + NW < units;
+        if (two) load(1, i + NW);
+        mma(0);
+        if (two) mma(1);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) *reinterpret_cast<f32x4*>(&red[wid][i][t][lane * 4]) = acc[i][t];
+    __syncthreads();
+    // lane l's register e: token l % 16, column 4·(l/16) + e
+    for (int p = threadIdx.x; p < MT * 256; p += 512) {
+        const int c = p & 15, tok = p >> 4;
+        const int at = ((c >> 2) * 16 + (tok & 15)) * 4 + (c & 3);
+        const int64_t col = c0 + c;
+        if (col >= f || tok >= m) continue;
+        float g = bias ? bias[col] : 0.f, u = bias ? bias[f + col] : 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            g += red[i][0][tok >> 4][at];
+            u += red[i][1][tok >> 4][at];
+        }
+        const float a = with_act(act, [&](auto A) {
+            float a, da;
+            activate<decltype(A)::value, true>(g, a, da);
+            return a;
+        });
+        Io<bf16_t>::st(h, tok * f + col, a * u);
+        if (gu) {
+            Io<bf16_t>::st(gu, tok * 2 * f + col, g);
+            Io<bf16_t>::st(gu, tok * 2 * f + f + col, u);
+        }
+    }
+}
+
+int forward_rows(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* x, const bf16_t* w,
+                 const float* b, bf16_t* h, bf16_t* gu) {
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(f, 16)), dim3(512), 0, ctx->stream, x, w, b, m, d, f, act, h, gu);
+    };
+    const bool tail = d % 8 != 0;
+    if (m <= 16) tail ? go(gated_rows_kernel<1, true>) : go(gated_rows_kernel<1, false>);
+    else if (m <= 32) tail ? go(gated_rows_kernel<2, true>) : go(gated_rows_kernel<2, false>);
+    else tail ? go(gated_rows_kernel<4, true>) : go(gated_rows_kernel<4, false>);
+    return launch_status(ctx, "gated_linear");
+}
+
+// Whether gated_rows_kernel beats 128×128 tiles: it reads the weights at the copy
+// rate for up to 16 rows and slower as x's operands join them, the tiles take
+// 0.55 us for each 64 of d (and a copy of operands that lie badly).  1024 → 4096:
+// 32 rows 7.1 us against 12.0, 64 rows 9.6 against 12.1; 4096 → 11008: 16 rows 37.0
+// and 37.2, 32 rows 48 against 37, 64 rows 72 against 37.
+bool takes_rows(nott_ctx ctx, int64_t m, int64_t d, int64_t f, bool padded) {
+    if (m <= 16 || m > 64) return m <= 16;
+    const double weights = 4.0 * (double)f * (double)d / 4.9e6;
+    const double rounds = (double)ceil_div(ceil_div(f, 64), ctx->num_cu);
+    return weights * (m <= 32 ? 1.35 : 2.0) <= rounds * (double)ceil_div(d, 64) * 0.55 + (padded ? 2 * weights + 2 : 0);
+}
+
+// C = A·B on the generic engine; AT, BT as in gemm_dma.hpp.
 template <typename T, bool AT, bool BT, class EP>
 int product(nott_ctx ctx, const T* A, int64_t lda, const T* B, int64_t ldb, const EP& ep, int64_t M, int64_t N,
             int64_t K) {
-    if constexpr (sizeof(T) == 2) {
-        const int st = dma::run<AT, BT>(ctx, A, lda, B, ldb, ep, M, N, K);
-        if (st != NOTT_ERR_UNSUPPORTED) return st;
-    }
     auto go = [&](const auto& la, const auto& lb) {
         return small_grid(ctx, M, N) ? run_small<T>(ctx, la, lb, ep, M, N, K) : run<T>(ctx, la, lb, ep, M, N, K);
     };
@@ -160,16 +430,36 @@ int product(nott_ctx ctx, const T* A, int64_t lda, const T* B, int64_t ldb, cons
     else return go(RowKLoader<T>{A, lda, M, K, vec(A, lda)}, RowKLoader<T>{B, ldb, N, K, vec(B, ldb)});
 }
 
-template <typename T>
-int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const T* x, const T* w, const float* b, T* h, T* gu) {
+int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* x, const bf16_t* w, const float* b,
+        bf16_t* h, bf16_t* gu) {
+    const int64_t dp = up8(d);
+    const bool rows = takes_rows(ctx, m, d, f, !ok16(w, d));
+    if (rows && d >= 8) return forward_rows(ctx, m, d, f, act, x, w, b, h, gu);
+    NOTT_REQUIRE(ctx, ceil_div(m, 128) * ceil_div(f, 64) < (int64_t)1 << 26, "nott_gated_linear_fwd: too large");
+    const bool pad_x = !ok16(x, d), pad_w = !ok16(w, d);
+    WorkspaceHold ws(ctx, sizeof(bf16_t) * (size_t)(((pad_x ? m : 0) + (pad_w ? 2 * f : 0)) * dp));
+    if (!ws.p) return NOTT_ERR_ALLOC;
+    bf16_t* xp = reinterpret_cast<bf16_t*>(ws.p);
+    bf16_t* wp = xp + (pad_x ? m * dp : 0);
+    if (pad_x) pad(ctx, x, m, d, xp, m, dp);
+    if (pad_w) pad(ctx, w, 2 * f, d, wp, 2 * f, dp);
+    if (rows) return forward_rows(ctx, m, dp, f, act, pad_x ? xp : x, pad_w ? wp : w, b, h, gu);
+    const GatedStore ep{h, gu, b, m, f, act, ok16(h, f) && ok16(gu, f)};
+    const dma::Plan p = dma::plan(ctx, m, 2 * f, dp, false, false, 1);
+    return dma::launch_shape<false, false, false>(ctx, p.shape, pad_x ? xp : x, dp, pad_w ? wp : w, dp, ep, m, 2 * f, dp, 1,
+                                                  dp);
+}
+
+int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* x, const float* w, const float* b, float* h,
+        float* gu) {
     WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * 2 * f));
     if (!ws.p) return NOTT_ERR_ALLOC;
     float* pre = reinterpret_cast<float*>(ws.p);
     RowMajorStore<float> ep{pre, 2 * f, m, 2 * f, nullptr};
-    const int st = product<T, false, false>(ctx, x, d, w, d, ep, m, 2 * f, d);
+    const int st = product<float, false, false>(ctx, x, d, w, d, ep, m, 2 * f, d);
     if (st != NOTT_OK) return st;
     return with_act(act, [&](auto a) {
-        hipLaunchKernelGGL((gated_act_kernel<T, decltype(a)::value>),
+        hipLaunchKernelGGL((gated_act_kernel<float, decltype(a)::value>),
                            dim3((unsigned)ceil_div(f, 256), (unsigned)std::min<int64_t>(m, 65535)), dim3(256), 0,
                            ctx->stream, pre, b, m, f, h, gu);
         return launch_status(ctx, "gated_linear");
@@ -178,38 +468,81 @@ int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const T* x, cons
 
 constexpr int kSlabs = 64;
 
+// [dg|du] in rows of ld elements (zeros past 2·f) to hi, and lo (bf16, nullable); db.
 template <typename T>
-int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const T* dh, const T* x, const T* w, const T* gu, T* dx,
-        float* dw, float* db, int accumulate) {
-    const size_t body = (sizeof(T) * (size_t)(m * 2 * f) + 255) & ~size_t(255);
-    const bool two = sizeof(T) == 2 && dw;
-    WorkspaceHold ws(ctx, body * (two ? 2 : 1) + (db ? sizeof(float) * kSlabs * 2 * (size_t)f : 0));
-    if (!ws.p) return NOTT_ERR_ALLOC;
-    T* hi = reinterpret_cast<T*>(ws.p);
-    T* lo = two ? reinterpret_cast<T*>(ws.p + body) : nullptr;
-    float* partial = db ? reinterpret_cast<float*>(ws.p + body * (two ? 2 : 1)) : nullptr;
-    int st = with_act(act, [&](auto a) {
-        hipLaunchKernelGGL((gated_dact_kernel<T, decltype(a)::value>), dim3((unsigned)ceil_div(f, 64), kSlabs), dim3(256),
-                           0, ctx->stream, dh, gu, m, f, hi, lo, partial);
-        return launch_status(ctx, "gated_linear backward");
-    });
-    if (st != NOTT_OK) return st;
+int activation_bwd(nott_ctx ctx, int64_t m, int64_t f, int64_t ld, int act, const T* dh, const T* gu, T* hi, T* lo,
+                   float* db, int accumulate) {
+    float* partial = nullptr;
     if (db) {
+        partial = static_cast<float*>(nott::workspace(ctx, sizeof(float) * kSlabs * 2 * (size_t)f));
+        if (!partial) return NOTT_ERR_ALLOC;
+    }
+    with_act(act, [&](auto a) {
+        hipLaunchKernelGGL((gated_dact_kernel<T, decltype(a)::value>), dim3((unsigned)ceil_div(f, 64), kSlabs), dim3(256),
+                           0, ctx->stream, dh, gu, m, f, ld, hi, lo, partial);
+    });
+    if (db)
         hipLaunchKernelGGL(gated_db_kernel, dim3((unsigned)ceil_div(2 * f, 256)), dim3(256), 0, ctx->stream, partial,
                            kSlabs, 2 * f, db, accumulate);
-        st = launch_status(ctx, "gated_linear db");
-        if (st != NOTT_OK) return st;
-    }
+    return launch_status(ctx, "gated_linear backward");
+}
+
+int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* dh, const bf16_t* x, const bf16_t* w,
+        const bf16_t* gu, bf16_t* dx, float* dw, float* db, int accumulate) {
+    const int64_t dp = up8(d), fp = up8(2 * f);
+    // the direct-to-LDS engine, where a product has its 128 rows and columns
+    const bool dma_dx = dx && m >= 128 && d >= 128, dma_dw = dw && 2 * f >= 128 && d >= 128;
+    const bool pad_x = dma_dw && !ok16(x, d), pad_w = dma_dx && (!ok16(w, d) || fp != 2 * f);
+    const size_t piece = sizeof(bf16_t) * (size_t)(m * fp);
+    WorkspaceHold ws(ctx, piece * (dw ? 2 : 1) + sizeof(bf16_t) * (size_t)(((pad_x ? m : 0) + (pad_w ? fp : 0)) * dp));
+    if (!ws.p) return NOTT_ERR_ALLOC;
+    bf16_t* hi = reinterpret_cast<bf16_t*>(ws.p);
+    bf16_t* lo = dw ? hi + m * fp : nullptr;
+    int st = activation_bwd(ctx, m, f, fp, act, dh, gu, hi, lo, db, accumulate);
+    if (st != NOTT_OK) return st;
+    bf16_t* xp = hi + m * fp * (dw ? 2 : 1);
+    bf16_t* wp = xp + (pad_x ? m * dp : 0);
+    if (pad_x) pad(ctx, x, m, d, xp, m, dp);
+    if (pad_w) pad(ctx, w, 2 * f, d, wp, fp, dp);
     if (dx) {
-        RowMajorStore<T> ep{dx, d, m, d, nullptr};
-        st = product<T, false, true>(ctx, hi, 2 * f, w, d, ep, m, d, 2 * f);
+        const RowMajorStore<bf16_t> ep{dx, d, m, d, nullptr};
+        st = dma_dx ? dma::run<false, true>(ctx, hi, fp, pad_w ? wp : w, dp, ep, m, dp, fp)
+                    : product<bf16_t, false, true>(ctx, hi, fp, w, d, ep, m, d, 2 * f);
         if (st != NOTT_OK) return st;
     }
-    if (dw) {
-        st = product<T, true, true>(ctx, hi, 2 * f, x, d, AccStore{dw, 2 * f, d, accumulate}, 2 * f, d, m);
+    if (!dw) return st;
+    if (!dma_dw) {
+        st = product<bf16_t, true, true>(ctx, hi, fp, x, d, AccStore{dw, 2 * f, d, accumulate}, 2 * f, d, m);
         if (st != NOTT_OK) return st;
-        if (two) st = product<T, true, true>(ctx, lo, 2 * f, x, d, AccStore{dw, 2 * f, d, 1}, 2 * f, d, m);
+        return product<bf16_t, true, true>(ctx, lo, fp, x, d, AccStore{dw, 2 * f, d, 1}, 2 * f, d, m);
     }
+    // one product over both pieces, 2·m deep
+    const bf16_t* X = pad_x ? xp : x;
+    dma::Plan p = dma::plan(ctx, fp, dp, 2 * m, true, false, 0);
+    float* part = nullptr;
+    if (p.splits > 1) {
+        part = static_cast<float*>(nott::optional_workspace(ctx, sizeof(float) * (size_t)(p.splits * fp * dp)));
+        if (!part) p = dma::plan(ctx, fp, dp, 2 * m, true, false, 1);
+    }
+    const PiecesStore ep{{dw, 2 * f, d, accumulate}, m};
+    if (!part) return dma::launch_shape<true, true, false>(ctx, p.shape, hi, fp, X, dp, ep, fp, dp, 2 * m, 1, p.kps);
+    st = dma::launch_shape<true, true, false>(ctx, p.shape, hi, fp, X, dp, PiecesPartial{{part, nullptr, fp, dp}, m}, fp, dp,
+                                              2 * m, p.splits, p.kps);
+    if (st != NOTT_OK) return st;
+    launch_splitk_reduce(ctx, part, p.splits, fp, dp, static_cast<const AccStore&>(ep));
+    return launch_status(ctx, "gated_linear dw");
+}
+
+int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* dh, const float* x, const float* w,
+        const float* gu, float* dx, float* dw, float* db, int accumulate) {
+    WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * 2 * f));
+    if (!ws.p) return NOTT_ERR_ALLOC;
+    float* dgu = reinterpret_cast<float*>(ws.p);
+    int st = activation_bwd<float>(ctx, m, f, 2 * f, act, dh, gu, dgu, nullptr, db, accumulate);
+    if (st == NOTT_OK && dx)
+        st = product<float, false, true>(ctx, dgu, 2 * f, w, d, RowMajorStore<float>{dx, d, m, d, nullptr}, m, d, 2 * f);
+    if (st == NOTT_OK && dw)
+        st = product<float, true, true>(ctx, dgu, 2 * f, x, d, AccStore{dw, 2 * f, d, accumulate}, 2 * f, d, m);
     return st;
 }
 
@@ -225,9 +558,9 @@ extern "C" int nott_gated_linear_fwd(nott_ctx ctx, nott_dtype dtype, int64_t m, 
     NOTT_REQUIRE(ctx, x && w && h, "nott_gated_linear_fwd: null buffer");
     nott::DeviceScope scope(ctx->device);
     if (dtype == NOTT_F32)
-        return fwd<float>(ctx, m, d, f, act, static_cast<const float*>(x), static_cast<const float*>(w), b,
+        return fwd(ctx, m, d, f, act, static_cast<const float*>(x), static_cast<const float*>(w), b,
                           static_cast<float*>(h), static_cast<float*>(gu));
-    return fwd<bf16_t>(ctx, m, d, f, act, static_cast<const bf16_t*>(x), static_cast<const bf16_t*>(w), b,
+    return fwd(ctx, m, d, f, act, static_cast<const bf16_t*>(x), static_cast<const bf16_t*>(w), b,
                        static_cast<bf16_t*>(h), static_cast<bf16_t*>(gu));
 }
 
@@ -252,10 +585,10 @@ extern "C" int nott_gated_linear_bwd(nott_ctx ctx, nott_dtype dtype, int64_t m, 
     NOTT_REQUIRE(ctx, !dx || w, "nott_gated_linear_bwd: dx needs w");
     NOTT_REQUIRE(ctx, !dw || x, "nott_gated_linear_bwd: dw needs x");
     if (dtype == NOTT_F32)
-        return bwd<float>(ctx, m, d, f, act, static_cast<const float*>(dh), static_cast<const float*>(x),
+        return bwd(ctx, m, d, f, act, static_cast<const float*>(dh), static_cast<const float*>(x),
                           static_cast<const float*>(w), static_cast<const float*>(gu), static_cast<float*>(dx), dw, db,
                           accumulate);
-    return bwd<bf16_t>(ctx, m, d, f, act, static_cast<const bf16_t*>(dh), static_cast<const bf16_t*>(x),
+    return bwd(ctx, m, d, f, act, static_cast<const bf16_t*>(dh), static_cast<const bf16_t*>(x),
                        static_cast<const bf16_t*>(w), static_cast<const bf16_t*>(gu), static_cast<bf16_t*>(dx), dw, db,
                        accumulate);
 }

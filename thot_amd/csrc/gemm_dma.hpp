@@ -63,10 +63,14 @@ using lds::wait_vm_lgkm0;
 // a multiple of 8) are filled with zeros.
 static __device__ u32x4 zero_chunk;
 
-template <bool TR, int R, int NW, bool TAIL>
+//
+// PAIR (k-contiguous): the operand is two stacked halves of rows/2 rows, and the
+// tile takes 32 rows of the first, the same 32 of the second, the next 32, ...
+// wrap (row-contiguous, nonzero): the operand's k-rows from `wrap` on are those from 0 on.
+template <bool TR, int R, int NW, bool TAIL, bool PAIR = false>
 __device__ __forceinline__ void fill_block(int qq, const bf16_t* __restrict__ p, int64_t ld, int64_t row0,
                                            int64_t rows, int64_t k0, int64_t K, char NOTT_LDS* dst, int wid,
-                                           int lane) {
+                                           int lane, int64_t wrap = 0) {
     constexpr int NB = R / 8;
     static_assert(NB % NW == 0, "tile blocks must split evenly over the waves");
     const int q = qq * NW + wid;
@@ -74,8 +78,15 @@ __device__ __forceinline__ void fill_block(int qq, const bf16_t* __restrict__ p,
     if constexpr (!TR) {
         const int r = 8 * q + (lane >> 3);
         const int c = (lane & 7) ^ ((r >> 1) & 7);
-        int64_t gr = row0 + r;
-        gr = gr < rows ? gr : rows - 1;
+        int64_t gr;
+        if constexpr (PAIR) {
+            const int64_t half = rows >> 1;
+            gr = (row0 >> 1) + 32 * (r >> 6) + (r & 31);
+            gr = (gr < half ? gr : half - 1) + ((r & 32) ? half : 0);
+        } else {
+            gr = row0 + r;
+            gr = gr < rows ? gr : rows - 1;
+        }
         src = p + gr * ld + k0 + 8 * c;
         if (TAIL && k0 + 8 * c >= K) src = reinterpret_cast<const bf16_t*>(&zero_chunk);
     } else {
@@ -86,7 +97,7 @@ __device__ __forceinline__ void fill_block(int qq, const bf16_t* __restrict__ p,
         const int cr = ((b % (2 * R)) >> 4) ^ ((k & 3) << 2);
         int64_t gc = row0 + 8 * cr;
         gc = gc <= rows - 8 ? gc : rows - 8;
-        src = p + (k0 + k) * ld + gc;
+        src = p + (k0 + k - (k0 + k >= wrap ? wrap : 0)) * ld + gc;
         if (TAIL && k0 + k >= K) src = reinterpret_cast<const bf16_t*>(&zero_chunk);
     }
     dma16(src, lds_addr(dst) + 1024 * q);
@@ -217,6 +228,19 @@ __device__ __forceinline__ void add_frag(float& s, const Frag<true>& f) {
     add_bf16x2(s, w.w);
 }
 
+// An epilogue for products whose B is two stacked halves (see fill_block): a wave
+// has 32 columns of the first half in acc[i][0] and the same of the second in
+// acc[i][1], and hands both, transposed as for store_tile, to
+// ep.store_pair<TM, FM>(acc, buf, m0, column, lane) with TM·64 bytes of LDS.
+template <class EP> struct IsPaired { static constexpr bool value = false; };
+// An epilogue of products whose A is two pieces of one operand stacked along k, so
+// that B's k-rows repeat from ep.wrap on (fill_block).
+template <class EP> struct IsWrapped { static constexpr bool value = false; };
+template <class EP>
+__device__ __forceinline__ int64_t wrap_of(const EP& ep) {
+    if constexpr (IsWrapped<EP>::value) return ep.wrap;
+    else return 0;
+}
 template <class EP> struct IsBf16RowMajor { static constexpr bool value = false; };
 template <> struct IsBf16RowMajor<RowMajorStore<bf16_t>> { static constexpr bool value = true; };
 
@@ -313,7 +337,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const bf16_t* __rest
     static_assert(TM % 32 == 0 && TN % 32 == 0, "wave tiles are whole 32x32 blocks");
     static_assert(S >= 2 && (S - 2) * LOADS < 64, "ring depth");
     // bf16 results: transposed accumulators, stored through LDS (store_tile)
-    constexpr bool SWAP = IsBf16RowMajor<EP>::value && !ROWSUM;
+    constexpr bool PAIR = IsPaired<EP>::value;
+    constexpr bool SWAP = (IsBf16RowMajor<EP>::value || PAIR) && !ROWSUM;
     static_assert(!SWAP || (TN == 64 && NW * TM * 128 <= S * STAGE), "the staged output tile fits the ring");
     extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
     char NOTT_LDS* smem = (char NOTT_LDS*)smem_raw;
@@ -347,14 +372,14 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const bf16_t* __rest
             for (int i = 0; i < LOADS; ++i) {
                 if (i < from || i >= to) continue;
                 if (i < LA) fill_block<AT, BM, NW, false>(i, A, lda, m0, M, k0, K, st, wid, lane);
-                else fill_block<BT, BN, NW, false>(i - LA, B, ldb, n0, N, k0, K, st + A_BYTES, wid, lane);
+                else fill_block<BT, BN, NW, false, PAIR>(i - LA, B, ldb, n0, N, k0, K, st + A_BYTES, wid, lane, wrap_of(ep));
             }
         } else {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 if (i < from || i >= to) continue;
                 if (i < LA) fill_block<AT, BM, NW, true>(i, A, lda, m0, M, k0, K, st, wid, lane);
-                else fill_block<BT, BN, NW, true>(i - LA, B, ldb, n0, N, k0, K, st + A_BYTES, wid, lane);
+                else fill_block<BT, BN, NW, true, PAIR>(i - LA, B, ldb, n0, N, k0, K, st + A_BYTES, wid, lane, wrap_of(ep));
             }
         }
     };
@@ -439,23 +464,27 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const bf16_t* __rest
             if (lane < 32) ep.rowsum(m0 + wm * TM + 32 * i + lane, v);
         }
     }
-    if constexpr (SWAP) {
+    if constexpr (PAIR) {
+        wait_vm_lgkm0<0>();   // as in store_tile
+        barrier();
+        ep.template store_pair<TM, FM>(acc, smem + wid * (TM * 64), m0 + wm * TM, (n0 + wn * TN) / 2, lane);
+    } else if constexpr (SWAP) {
         store_tile<TM, FM, FN>(ep, acc, smem + wid * (TM * 128), m0 + wm * TM, n0 + wn * TN, lane);
-        return;
+    } else {
+        // Accumulator layout of a 32×32 block: lane l holds column l % 32 and,
+        // in register 4q + e, row 8q + 4·(l/32) + e.
+        const int col = lane & 31, rh = (lane >> 5) * 4;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        ColumnOf<EP>::store(ep, m0 + wm * TM + 32 * i + 8 * q + rh + e, n0 + wn * TN + 32 * j + col,
+                                            acc[i][j][4 * q + e], 0);
     }
-    // Accumulator layout of a 32×32 block: lane l holds column l % 32 and,
-    // in register 4q + e, row 8q + 4·(l/32) + e.
-    const int col = lane & 31, rh = (lane >> 5) * 4;
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    ColumnOf<EP>::store(ep, m0 + wm * TM + 32 * i + 8 * q + rh + e, n0 + wn * TN + 32 * j + col,
-                                        acc[i][j][4 * q + e], 0);
 }
 
 template <bool AT, bool BT, int BM, int BN, int WM, int WN, int S>
