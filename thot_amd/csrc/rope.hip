@@ -60,7 +60,7 @@ struct RopeArgs {
     int32_t t, dh, norm;
     float eps;
     int64_t items;      // tokens · (hq + hk)
-    FastDiv by_heads, by_t, by_half;
+    FastDiv by_heads, by_t, by_width;   // by_width: pairs of a token's table
     float* partial;     // backward: [grid][2·dh] sums of dz·x̂, q then k; null: not asked for
 };
 
@@ -175,6 +175,12 @@ __device__ __forceinline__ float head_sum(float v) {
     return v;
 }
 
+template <typename T>
+__device__ __forceinline__ typename Pack16<T>::Raw ones() {
+    if constexpr (sizeof(T) == 2) return u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    else return f32x4{1.f, 1.f, 1.f, 1.f};
+}
+
 // Heads of whole aligned 16-byte chunks: LPH lanes a head, each with two chunks
 // that hold both elements of its pairs (chunks c and c + rot/2, or neighbours), so
 // a head's norm, weight and rotation need no exchange but the sum.  A workgroup
@@ -186,8 +192,12 @@ template <typename T, int LPH, bool BWD>
 __global__ __launch_bounds__(256) void rope_vec_kernel(RopeArgs<T> a, int tpb) {
     constexpr int E = Pack16<T>::N, GPB = 256 / LPH, U = BWD ? 2 : 4;
     typedef typename Pack16<T>::Raw Raw;
+    // {cos, sin} of each token's pairs, two pairs (16 bytes) of every chunk side by
+    // side: [tpb][pairs of a chunk / 2][chunks], so that the lanes of a head read a
+    // run.  Half-split: a chunk of E pairs for each rotated lane; neighbours: a
+    // chunk's E/2 pairs, those past the rotated ones with the angle 0.
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    f32x2* table = reinterpret_cast<f32x2*>(lds);   // [tpb][rot/2] {cos, sin}
+    f32x4* table = reinterpret_cast<f32x4*>(lds);
     const int tid = (int)threadIdx.x, slot = tid % LPH, group = tid / LPH;
     const int half = a.turns.half, nc = a.dh / E, heads = a.q.n + a.k.n;
     const bool inter = a.turns.interleaved;
@@ -197,10 +207,11 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeArgs<T> a, int tpb) {
     const int c0 = rotated ? slot : 2 * hc + 2 * (slot - hc), c1 = rotated ? slot + hc : c0 + 1;
     const bool has0 = c0 < nc, has1 = c1 < nc;
     const int e0 = has0 ? c0 * E : 0, e1 = has1 ? c1 * E : 0;
+    const int ppc = inter ? E / 2 : E, chunks = inter ? nc : hc, width = ppc * chunks;   // of a token's table
     const float inv_dh = 1.f / (float)a.dh;
-    Raw gq0, gq1, gk0, gk1;
-    if (a.q.gamma) gq0 = Pack16<T>::raw(a.q.gamma + e0), gq1 = Pack16<T>::raw(a.q.gamma + e1);
-    if (a.k.gamma) gk0 = Pack16<T>::raw(a.k.gamma + e0), gk1 = Pack16<T>::raw(a.k.gamma + e1);
+    const Raw one = ones<T>();
+    const Raw gq0 = a.q.gamma ? Pack16<T>::raw(a.q.gamma + e0) : one, gq1 = a.q.gamma ? Pack16<T>::raw(a.q.gamma + e1) : one;
+    const Raw gk0 = a.k.gamma ? Pack16<T>::raw(a.k.gamma + e0) : one, gk1 = a.k.gamma ? Pack16<T>::raw(a.k.gamma + e1) : one;
     float dg[BWD ? 4 : 1][E];   // dγ of this lane's chunks: q, q, k, k
 #pragma unroll
     for (auto& d : dg)
@@ -236,68 +247,61 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeArgs<T> a, int tpb) {
             }
             if (base == 0 && half > 0) {
                 __syncthreads();   // the last tokens' readers are done
-                for (int i = tid; i < nt * half; i += 256) {
+                for (int i = tid; i < nt * width; i += 256) {
                     uint32_t t, pair;
-                    a.by_half.divmod((uint32_t)i, t, pair);
-                    float c, s;
-                    a.turns.turn(t0 + t, (int)pair, c, s);
-                    table[i] = f32x2{c, s};
+                    a.by_width.divmod((uint32_t)i, t, pair);
+                    float c = 1.f, s = 0.f;
+                    if ((int)pair < half) a.turns.turn(t0 + t, (int)pair, c, s);
+                    const int chunk = (int)pair / ppc, in = (int)pair % ppc;
+                    reinterpret_cast<f32x2*>(lds)[t * width + ((in >> 1) * chunks + chunk) * 2 + (in & 1)] = f32x2{c, s};
                 }
                 __syncthreads();
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                // y0, y1: turned from / to z0, z1 (BWD: dy turned back)
                 float v0[E], v1[E];
-                const f32x2* tab = table + (int)tok[u] * half;
+                const f32x4* tab = table + (int)tok[u] * (width / 2);
+                // turns the pair (a, b) by {cos, sin}, BWD: back
+                auto turn2 = [](float& a, float& b, float c, float s) {
+                    if (BWD) s = -s;
+                    const float y = fmaf(-b, s, a * c);
+                    b = fmaf(a, s, b * c);
+                    a = y;
+                };
                 auto turn = [&](float (&p)[E], float (&q)[E]) {
+                    if (half == 0) return;
                     if (!inter) {
-                        if (rotated) {
+                        if (!rotated) return;
 #pragma unroll
-                            for (int e = 0; e < E; ++e) {
-                                const f32x2 cs = tab[c0 * E + e];
-                                const float s = BWD ? -cs.y : cs.y, b = q[e];
-                                q[e] = fmaf(p[e], s, b * cs.x);
-                                p[e] = fmaf(-b, s, p[e] * cs.x);
-                            }
+                        for (int e = 0; e < E; e += 2) {
+                            const f32x4 cs = tab[e / 2 * chunks + c0];
+                            turn2(p[e], q[e], cs.x, cs.y);
+                            turn2(p[e + 1], q[e + 1], cs.z, cs.w);
                         }
                         return;
                     }
-                    auto neighbours = [&](float (&w)[E], int pair) {
 #pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            if (pair + e / 2 >= half) continue;
-                            const f32x2 cs = tab[pair + e / 2];
-                            const float s = BWD ? -cs.y : cs.y, b = w[e + 1];
-                            w[e + 1] = fmaf(w[e], s, b * cs.x);
-                            w[e] = fmaf(-b, s, w[e] * cs.x);
-                        }
-                    };
-                    neighbours(p, e0 / 2);
-                    neighbours(q, e1 / 2);
+                    for (int e = 0; e < E; e += 4) {
+                        const f32x4 cs = tab[e / 4 * chunks + (has0 ? c0 : 0)], ct = tab[e / 4 * chunks + (has1 ? c1 : 0)];
+                        turn2(p[e], p[e + 1], cs.x, cs.y);
+                        turn2(p[e + 2], p[e + 3], cs.z, cs.w);
+                        turn2(q[e], q[e + 1], ct.x, ct.y);
+                        turn2(q[e + 2], q[e + 3], ct.z, ct.w);
+                    }
                 };
                 float x0[E], x1[E], r = 1.f;
                 if (!BWD || a.norm) {
-                    Pack16<T>::unpack(rx[u][0], x0);
-                    Pack16<T>::unpack(rx[u][1], x1);
+                    // absent chunks are zero
+                    Pack16<T>::unpack(has0 ? rx[u][0] : Raw{}, x0);
+                    Pack16<T>::unpack(has1 ? rx[u][1] : Raw{}, x1);
                     float ss = 0.f;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        x0[e] = has0 ? x0[e] : 0.f;
-                        x1[e] = has1 ? x1[e] : 0.f;
-                        ss = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], ss));
-                    }
+                    for (int e = 0; e < E; ++e) ss = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], ss));
                     if (a.norm) r = rsqrtf(fmaf(head_sum<LPH>(ss), inv_dh, a.eps));
                 }
-                const bool weighted = (of_q[u] ? a.q.gamma : a.k.gamma) != nullptr;
                 float g0[E], g1[E];
                 Pack16<T>::unpack(of_q[u] ? gq0 : gk0, g0);
                 Pack16<T>::unpack(of_q[u] ? gq1 : gk1, g1);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    g0[e] = weighted ? g0[e] : 1.f;
-                    g1[e] = weighted ? g1[e] : 1.f;
-                }
                 if constexpr (!BWD) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
@@ -335,7 +339,7 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeArgs<T> a, int tpb) {
                         for (int e = 0; e < E; ++e) {
                             v0[e] *= g0[e];
                             v1[e] *= g1[e];
-                            dot = fmaf(has0 ? v0[e] : 0.f, x0[e], fmaf(has1 ? v1[e] : 0.f, x1[e], dot));
+                            dot = fmaf(v0[e], x0[e], fmaf(v1[e], x1[e], dot));
                         }
                         dot = head_sum<LPH>(dot) * inv_dh;
 #pragma unroll
@@ -375,24 +379,19 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(RopeArgs<T> a, int tpb) {
 }
 
 // dγ (+)= Σ_blocks partial[block], in an order that the grid alone fixes: a
-// workgroup has 16 columns, 16 threads of each taking every 16th block.
-__global__ __launch_bounds__(256) void rope_dgamma_kernel(const float* __restrict__ partial, int blocks, int dh,
-                                                          float* __restrict__ dgq, float* __restrict__ dgk,
-                                                          int accumulate) {
-    __shared__ float red[16][17];
+// workgroup has 16 columns, 64 threads of each taking every 64th block.
+__global__ __launch_bounds__(1024) void rope_dgamma_kernel(const float* __restrict__ partial, int blocks, int dh,
+                                                           float* __restrict__ dgq, float* __restrict__ dgk,
+                                                           int accumulate) {
+    __shared__ float red[64][17];
     const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
-    const int col = blockIdx.x * 16 + c;
-    float s = 0.f;
-    if (col < 2 * dh) {
-#pragma unroll 8
-        for (int b = r; b < blocks; b += 16) s += partial[(int64_t)b * 2 * dh + col];
-    }
-    red[r][c] = s;
+    const int col = blockIdx.x * 16 + c, at = col < 2 * dh ? col : 0;
+    red[r][c] = r < blocks ? ordered_sum1(partial + (int64_t)r * 2 * dh + at, (int64_t)64 * 2 * dh, (blocks - r + 63) / 64) : 0.f;
     __syncthreads();
     if (r != 0 || col >= 2 * dh) return;
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += red[i][c];
+    for (int i = 0; i < 64; ++i) t += red[i][c];
     float* out = col < dh ? dgq : dgk;
     if (!out) return;
     const int e = col < dh ? col : col - dh;
@@ -431,6 +430,12 @@ int check(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype dtype, const char
     return NOTT_OK;
 }
 
+// Pairs of a token's cosine and sine table: the head's where pairs are neighbours.
+template <typename T>
+int table_pairs(const RopeArgs<T>& a) {
+    return a.turns.half == 0 ? 0 : a.turns.interleaved ? a.dh / 2 : a.turns.half;
+}
+
 template <typename T>
 RopeArgs<T> make_args(const nott_qk_rope_desc& d, const void* q, const void* k, const void* dyq, const void* dyk,
                       const void* gq, const void* gk, const int64_t* positions, const double* inv_freq, void* oq,
@@ -466,7 +471,7 @@ RopeArgs<T> make_args(const nott_qk_rope_desc& d, const void* q, const void* k, 
     a.items = d.b * d.t * (d.hq + d.hk);
     a.by_heads = FastDiv((uint32_t)(d.hq + d.hk));
     a.by_t = FastDiv((uint32_t)d.t);
-    a.by_half = FastDiv((uint32_t)std::max<int64_t>(1, d.rot / 2));
+    a.by_width = FastDiv((uint32_t)std::max<int64_t>(1, table_pairs(a)));
     return a;
 }
 
@@ -492,23 +497,23 @@ struct Launch {
     int lph, tpb;
     size_t lds;
 };
-// Tokens of a workgroup: as many as fill its lanes' loads once (one token's heads
-// more often), fewer where there are too few for every CU, with at most 16 KiB of
-// cosines and sines.  Backward the workgroups take turns, so that there are few
-// partial sums of dγ.
+// Tokens that a workgroup takes at a time: forward as many as fill its lanes' loads
+// once; backward, where each workgroup leaves partial sums of dγ, its share of 4
+// workgroups a CU.  Fewer where there are too few for every CU, and with at most
+// 16 KiB of cosines and sines.
 template <typename T>
 Launch plan(nott_ctx ctx, const RopeArgs<T>& a, bool bwd) {
     constexpr int E = Pack16<T>::N;
     Launch l{};
-    const int slots = (a.dh / E + 1) / 2;
+    const int slots = (a.dh / E + 1) / 2, pairs = table_pairs(a);
     for (l.lph = 2; l.lph < slots;) l.lph *= 2;
-    const int heads = a.q.n + a.k.n;
-    int64_t tpb = (int64_t)(256 / l.lph) * (bwd ? 2 : 4) / heads;
-    if (a.turns.half) tpb = std::min<int64_t>(tpb, 2048 / a.turns.half);
-    tpb = std::min<int64_t>(tpb, a.turns.tokens / ctx->num_cu);
+    const int64_t tokens = a.turns.tokens, groups = 4 * (int64_t)ctx->num_cu;
+    int64_t tpb = bwd ? ceil_div(tokens, groups) : (int64_t)(256 / l.lph) * 4 / (a.q.n + a.k.n);
+    if (pairs) tpb = std::min<int64_t>(tpb, 2048 / pairs);
+    tpb = std::min<int64_t>(tpb, ceil_div(tokens, ctx->num_cu));
     l.tpb = (int)std::max<int64_t>(tpb, 1);
-    l.grid = (unsigned)std::min<int64_t>(ceil_div(a.turns.tokens, l.tpb), bwd ? 8 * (int64_t)ctx->num_cu : 0x7fffffff);
-    l.lds = std::max(sizeof(f32x2) * (size_t)l.tpb * a.turns.half, bwd ? sizeof(float) * 8 * (size_t)a.dh : 0);
+    l.grid = (unsigned)std::min<int64_t>(ceil_div(tokens, l.tpb), bwd ? groups : 0x7fffffff);
+    l.lds = std::max(sizeof(f32x2) * (size_t)l.tpb * pairs, bwd ? sizeof(float) * 8 * (size_t)a.dh : 0);
     return l;
 }
 
@@ -549,7 +554,7 @@ int backward(nott_ctx ctx, RopeArgs<T> a, float* dgq, float* dgk, int accumulate
     if (vec) launch_vec<T, true>(ctx, l, a);
     else hipLaunchKernelGGL((rope_any_kernel<T, true>), dim3(l.grid), dim3(256), 0, ctx->stream, a);
     if (a.partial)
-        hipLaunchKernelGGL(rope_dgamma_kernel, dim3((unsigned)ceil_div(2 * a.dh, 16)), dim3(256), 0, ctx->stream,
+        hipLaunchKernelGGL(rope_dgamma_kernel, dim3((unsigned)ceil_div(2 * a.dh, 16)), dim3(1024), 0, ctx->stream,
                            a.partial, (int)l.grid, a.dh, dgq, dgk, accumulate);
     return nott::launch_status(ctx, "qk_norm_rope backward");
 }

@@ -748,13 +748,16 @@ def qk_norm_rope_bwd(dyq: torch.Tensor, dyk: Optional[torch.Tensor], q: torch.Te
         if k is not None:
             d.dk_stride[:] = _out_strides(dk, "dk", k_shape, q)
     dh = q.shape[3]
-    if gamma_q is not None and dgamma_q is None:
-        dgamma_q = q.new_empty(dh, dtype=torch.float32)
-    if gamma_k is not None and dgamma_k is None:
-        dgamma_k = q.new_empty(dh, dtype=torch.float32)
-    for g, nm in ((dgamma_q, "dgamma_q"), (dgamma_k, "dgamma_k")):
-        if g is not None:
-            _check(g, nm, shape=(dh,), dtype=torch.float32, device=q.device)
+    if gamma_q is not None and gamma_k is not None and dgamma_q is None and dgamma_k is None:
+        dgamma_q, dgamma_k = q.new_empty((2, dh), dtype=torch.float32).unbind(0)
+    else:
+        if gamma_q is not None and dgamma_q is None:
+            dgamma_q = q.new_empty(dh, dtype=torch.float32)
+        if gamma_k is not None and dgamma_k is None:
+            dgamma_k = q.new_empty(dh, dtype=torch.float32)
+        for g, nm in ((dgamma_q, "dgamma_q"), (dgamma_k, "dgamma_k")):
+            if g is not None:
+                _check(g, nm, shape=(dh,), dtype=torch.float32, device=q.device)
     _ctx_for(q).call("nott_qk_norm_rope_bwd", C.byref(d), _DTYPES[q.dtype], _ptr(dyq), _ptr(dyk), _ptr(q), _ptr(k),
                      _ptr(gamma_q), _ptr(gamma_k), _ptr(positions), _ptr(inv_freq), _ptr(dq),
                      None if k is None else _ptr(dk), _ptr(dgamma_q), _ptr(dgamma_k), int(accumulate))
