@@ -752,6 +752,132 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     }
 };
 
+// --------------------------- norm and rotation of queries and keys
+// q [b, t, hq, dh], k [b, t, hk, dh] (views of a packed projection as they are) →
+// head-major yq [b, hq, t, dh], yk [b, hk, t, dh], as AttentionFn takes them
+// (nott_qk_norm_rope_fwd / _bwd).  positions int64 [axes, b, t], inv_freq double
+// [rot/2], sections: pairs of each axis.  gamma_q / gamma_k: fp32 masters, whose
+// gradients are accumulated; gamma_*c in the compute type; absent() for none.
+struct QkNormRopeFn : torch::autograd::Function<QkNormRopeFn> {
+    static Tensor heads(const Tensor& x) { return x.stride(-1) == 1 ? x : x.contiguous(); }
+    static void strides(int64_t (&s)[3], const Tensor& x, int64_t token, int64_t head) {
+        const bool one = x.numel() <= x.size(-1);   // three zeros would mean contiguous, which one head is
+        s[0] = one ? 0 : x.stride(0); s[1] = one ? 0 : x.stride(token); s[2] = one ? 0 : x.stride(head);
+        if (!one && s[0] == 0 && s[1] == 0 && s[2] == 0)
+            throw std::invalid_argument("Nott::HIP: q and k must not repeat one head");
+    }
+    static nott_qk_rope_desc desc(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
+                                  const std::vector<int64_t>& sections, bool interleaved, bool norm, double eps) {
+        if (q.dim() != 4 || k.dim() != 4 || k.size(0) != q.size(0) || k.size(1) != q.size(1) || k.size(3) != q.size(3))
+            throw std::invalid_argument("Nott::HIP: q and k must be [b, t, heads, dh] with the same b, t and dh");
+        nott_qk_rope_desc d{};
+        d.b = q.size(0); d.t = q.size(1); d.hq = q.size(2); d.hk = k.size(2); d.dh = q.size(3);
+        d.axes = 1;
+        if (present(inv_freq)) {
+            if (positions.dim() != 3 || positions.size(1) != d.b || positions.size(2) != d.t || positions.size(0) < 1 ||
+                positions.size(0) > 4 || positions.scalar_type() != torch::kInt64 || !positions.is_contiguous() ||
+                positions.device() != q.device())
+                throw std::invalid_argument("Nott::HIP: positions must be int64 [axes, b, t], 1 to 4 axes, on q's device");
+            if (inv_freq.scalar_type() != torch::kFloat64 || !inv_freq.is_contiguous() || inv_freq.device() != q.device())
+                throw std::invalid_argument("Nott::HIP: inv_freq must be a contiguous double tensor on q's device");
+            d.rot = 2 * inv_freq.numel();
+            d.axes = (int32_t)positions.size(0);
+            if (sections.empty() && d.axes == 1) d.section[0] = d.rot / 2;
+            else if ((int64_t)sections.size() != d.axes) throw std::invalid_argument("Nott::HIP: one section per axis");
+            for (size_t i = 0; i < sections.size(); ++i) d.section[i] = sections[i];
+        }
+        d.interleaved = interleaved; d.norm = norm; d.eps = eps;
+        strides(d.q_stride, q, 1, 2);
+        strides(d.k_stride, k, 1, 2);
+        return d;
+    }
+    static variable_list forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor gamma_q, Tensor gamma_k, Tensor gamma_qc,
+                                 Tensor gamma_kc, Tensor positions, Tensor inv_freq, std::vector<int64_t> sections,
+                                 bool interleaved, bool norm, double eps) {
+        q = heads(q); k = heads(k);
+        if (k.scalar_type() != q.scalar_type() || k.device() != q.device())
+            throw std::invalid_argument("Nott::HIP: k must have q's type and device");
+        nott_qk_rope_desc d = desc(q, k, positions, inv_freq, sections, interleaved, norm, eps);
+        for (const Tensor& g : {gamma_qc, gamma_kc})
+            if (present(g) && (g.numel() != d.dh || g.scalar_type() != q.scalar_type() || !g.is_contiguous()))
+                throw std::invalid_argument("Nott::HIP: a weight must be [dh] of q's type");
+        Tensor yq = torch::empty({d.b, d.hq, d.t, d.dh}, q.options()), yk = torch::empty({d.b, d.hk, d.t, d.dh}, q.options());
+        strides(d.yq_stride, yq, 2, 1);
+        strides(d.yk_stride, yk, 2, 1);
+        nott_ctx c = bind(q);
+        check(nott_qk_norm_rope_fwd(c, &d, dtype_of(q), ptr(q), ptr(k), ptr(gamma_qc), ptr(gamma_kc),
+                                    present(inv_freq) ? positions.data_ptr<int64_t>() : nullptr,
+                                    present(inv_freq) ? inv_freq.data_ptr<double>() : nullptr, ptr(yq), ptr(yk)),
+              c, "norm and rotation forward");
+        ctx->save_for_backward({q, k, gamma_q, gamma_k, gamma_qc, gamma_kc, positions, inv_freq});
+        ctx->saved_data["sections"] = sections;
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["norm"] = norm;
+        ctx->saved_data["eps"] = eps;
+        return {yq, yk};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        auto s = ctx->get_saved_variables();
+        Tensor q = s[0], k = s[1], positions = s[6], inv_freq = s[7];
+        nott_qk_rope_desc d = desc(q, k, positions, inv_freq, ctx->saved_data["sections"].toIntVector(),
+                                   ctx->saved_data["interleaved"].toBool(), ctx->saved_data["norm"].toBool(),
+                                   ctx->saved_data["eps"].toDouble());
+        // an output that nothing used has no gradient
+        auto grad = [&](const Tensor& g, int64_t h) {
+            return g.defined() ? heads(g) : torch::zeros({d.b, h, d.t, d.dh}, q.options());
+        };
+        Tensor dyq = grad(grads[0], d.hq), dyk = grad(grads[1], d.hk);
+        strides(d.yq_stride, dyq, 2, 1);
+        strides(d.yk_stride, dyk, 2, 1);
+        Tensor dq = torch::empty({d.b, d.t, d.hq, d.dh}, q.options()), dk = torch::empty({d.b, d.t, d.hk, d.dh}, q.options());
+        Tensor gq = grad_buffer(s[2]), gk = grad_buffer(s[3]);
+        nott_ctx c = bind(q);
+        check(nott_qk_norm_rope_bwd(c, &d, dtype_of(q), ptr(dyq), ptr(dyk), ptr(q), ptr(k), ptr(s[4]), ptr(s[5]),
+                                    present(inv_freq) ? positions.data_ptr<int64_t>() : nullptr,
+                                    present(inv_freq) ? inv_freq.data_ptr<double>() : nullptr, ptr(dq), ptr(dk), fptr(gq),
+                                    fptr(gk), 1),
+              c, "norm and rotation backward");
+        return {dq, dk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// ------------------------------------------------------------ gated linear
+// h = act(g)·u with [g | u] = x·wᵀ + b (nott_gated_linear_fwd / _bwd): w [2·f, d]
+// gate rows first, act a NOTT_ACT_* value.  [g | u] is kept only where a backward
+// may come.
+struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
+    static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w, Tensor wc, Tensor b, int64_t act, bool keep) {
+        x = contig(x);
+        if (wc.dim() != 2 || wc.size(0) % 2 || wc.size(0) == 0 || x.size(-1) != wc.size(1) || x.scalar_type() != wc.scalar_type())
+            throw std::invalid_argument("Nott::HIP: a gated linear layer's weight must be [2·f, d] for x [..., d], of x's type");
+        const int64_t d = x.size(-1), m = x.numel() / d, f = wc.size(0) / 2;
+        auto shape = x.sizes().vec();
+        shape.back() = f;
+        Tensor h = torch::empty(shape, x.options());
+        Tensor gu = keep ? torch::empty({m, 2 * f}, x.options()) : absent(x);
+        nott_ctx c = bind(x);
+        check(nott_gated_linear_fwd(c, dtype_of(x), m, d, f, (int)act, ptr(x), ptr(wc), fptr(b), ptr(h), ptr(gu)), c,
+              "gated linear forward");
+        ctx->save_for_backward({x, w, wc, b, gu});
+        ctx->saved_data["needs_dx"] = x.requires_grad();
+        ctx->saved_data["act"] = act;
+        return h;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        auto s = ctx->get_saved_variables();
+        Tensor x = s[0], w = s[1], wc = s[2], b = s[3], gu = s[4];
+        Tensor dh = contig(grads[0]);
+        const int64_t d = x.size(-1), m = x.numel() / d, f = wc.size(0) / 2;
+        Tensor dx = ctx->saved_data["needs_dx"].toBool() ? torch::empty_like(x) : Tensor();
+        Tensor gw = grad_buffer(w), gb = grad_buffer(b);
+        nott_ctx c = bind(dh);
+        check(nott_gated_linear_bwd(c, dtype_of(dh), m, d, f, (int)ctx->saved_data["act"].toInt(), ptr(dh), ptr(x), ptr(wc),
+                                    ptr(gu), ptr(dx), fptr(gw), fptr(gb), 1),
+              c, "gated linear backward");
+        return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
 // ------------------------------------------ scaled dot-product attention
 struct AttentionFn : torch::autograd::Function<AttentionFn> {
     static nott_attn_desc desc(const Tensor& q, const Tensor& k, bool causal, double scale) {
@@ -853,6 +979,39 @@ struct CrossEntropyFn : torch::autograd::Function<CrossEntropyFn> {
         Tensor out = torch::empty_like(dl);
         nott_ctx c = bind(dl);
         check(nott_scale(c, dtype_of(dl), dl.numel(), ptr(dl), g.data_ptr<float>(), ptr(out)), c, "cross-entropy bwd");
+        return {out, Tensor(), Tensor()};
+    }
+};
+
+// ---------------------------------------- log probabilities of given tokens
+// {logprob, entropy} (fp32 [n]) of the rows of logits under softmax(scale·logits)
+// (nott_token_logprob_fwd / _bwd); −100 labels give 0.
+struct TokenLogProbFn : torch::autograd::Function<TokenLogProbFn> {
+    static variable_list forward(AutogradContext* ctx, Tensor logits, Tensor labels, double scale) {
+        logits = contig(logits);
+        labels = contig(labels);
+        auto fo = logits.options().dtype(torch::kFloat32);
+        const int64_t n = logits.size(0), c = logits.size(1);
+        Tensor lp = torch::empty({n}, fo), ent = torch::empty({n}, fo), lse = torch::empty({n}, fo);
+        nott_ctx h = bind(logits);
+        check(nott_token_logprob_fwd(h, dtype_of(logits), n, c, ptr(logits), labels.data_ptr<int64_t>(), scale, 0, fptr(lp),
+                                     fptr(ent), fptr(lse), nullptr, nullptr),
+              h, "token log probability");
+        ctx->save_for_backward({logits, labels, lse, ent});
+        ctx->saved_data["scale"] = scale;
+        return {lp, ent};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        auto s = ctx->get_saved_variables();
+        Tensor logits = s[0], labels = s[1], lse = s[2], ent = s[3];
+        Tensor dlp = grads[0].defined() ? contig(grads[0]) : torch::zeros_like(lse);
+        Tensor dent = grads[1].defined() ? contig(grads[1]) : Tensor();
+        Tensor out = torch::empty_like(logits);
+        nott_ctx c = bind(logits);
+        check(nott_token_logprob_bwd(c, dtype_of(logits), logits.size(0), logits.size(1), ptr(logits),
+                                     labels.data_ptr<int64_t>(), ctx->saved_data["scale"].toDouble(), fptr(lse), fptr(ent),
+                                     fptr(dlp), fptr(dent), ptr(out)),
+              c, "token log probability backward");
         return {out, Tensor(), Tensor()};
     }
 };
@@ -1090,6 +1249,24 @@ public:
     BatchNorm2d bn1{nullptr}, bn3{nullptr};
 };
 TORCH_MODULE(ResidualBasicBlock);
+
+// h = act(g)·u of a gated linear layer (w the fp32 master, wc its working copy, b
+// fp32 or undefined); the pre-activations are kept only where a backward may come.
+inline Tensor gated_linear(const Tensor& x, const Tensor& w, const Tensor& wc, const Tensor& b, int64_t act) {
+    // (asked here: inside the function grad mode is off either way)
+    const bool keep = torch::GradMode::is_enabled() &&
+                      (x.requires_grad() || w.requires_grad() || (b.defined() && b.requires_grad()));
+    return GatedLinearFn::apply(x, w, wc, or_absent(b, w), act, keep);
+}
+
+// {logprob, entropy} of each row's label under softmax(scale·logits).
+inline std::pair<Tensor, Tensor> token_logprob(const Tensor& logits, const Tensor& labels, double scale = 1.0) {
+    if (logits.dim() != 2 || labels.dim() != 1 || labels.size(0) != logits.size(0) ||
+        labels.scalar_type() != torch::kInt64 || labels.device() != logits.device())
+        throw std::invalid_argument("Nott::HIP: logits must be [n, c], labels int64 [n] on the same device");
+    auto r = TokenLogProbFn::apply(logits, labels, scale);
+    return {r[0], r[1]};
+}
 
 inline Tensor cross_entropy(const Tensor& logits, const Tensor& labels, double label_smoothing = 0.0) {
     return CrossEntropyFn::apply(logits, labels, label_smoothing);

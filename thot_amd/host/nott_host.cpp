@@ -554,6 +554,39 @@ PYBIND11_MODULE(_nott_host, m) {
     m.doc() = "C++ host layer (Nott::HIP) over libnott_hip: configs[0] and configs[4] training steps";
     // Workspace held by the device's contexts (one per stream used).
     m.def("workspace_bytes", [](int device) { return NH::device_workspace_bytes(device); }, py::arg("device") = 0);
+    // The transformer nodes as differentiable functions of tensors (parameter
+    // gradients are accumulated into the masters' .grad, as in every layer).
+    using OptT = std::optional<Tensor>;
+    auto given = [](const OptT& t) { return t ? *t : Tensor(); };
+    auto compute = [](const OptT& c, const OptT& master, const Tensor& like) {
+        return c ? *c : master ? *master : NH::absent(like);
+    };
+    m.def("linear", [=](const Tensor& x, const Tensor& w, const OptT& b, const OptT& wc) {
+        return NH::LinearFn::apply(x, w, wc ? *wc : w, NH::or_absent(given(b), w), (int64_t)0);
+    }, py::arg("x"), py::arg("w"), py::arg("b") = py::none(), py::arg("w_compute") = py::none());
+    m.def("layer_norm", [=](const Tensor& x, const Tensor& g, const Tensor& b, const OptT& gc, const OptT& bc, double eps) {
+        return NH::LayerNormFn::apply(x, g, b, gc ? *gc : g, bc ? *bc : b, eps);
+    }, py::arg("x"), py::arg("gamma"), py::arg("beta"), py::arg("gamma_compute") = py::none(),
+          py::arg("beta_compute") = py::none(), py::arg("eps") = 1e-5);
+    m.def("attention", [](const Tensor& q, const Tensor& k, const Tensor& v, bool causal) {
+        return NH::AttentionFn::apply(q, k, v, causal, 1.0 / std::sqrt((double)q.size(-1)));
+    }, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("causal") = true);
+    m.def("qk_norm_rope", [=](const Tensor& q, const Tensor& k, const OptT& positions, const OptT& inv_freq, const OptT& gq,
+                              const OptT& gk, const OptT& gqc, const OptT& gkc, std::vector<int64_t> sections,
+                              bool interleaved, bool norm, double eps) {
+        auto r = NH::QkNormRopeFn::apply(q, k, NH::or_absent(given(gq), q), NH::or_absent(given(gk), q), compute(gqc, gq, q),
+                                         compute(gkc, gk, q), NH::or_absent(given(positions), q),
+                                         NH::or_absent(given(inv_freq), q), sections, interleaved, norm, eps);
+        return std::make_pair(r[0], r[1]);
+    }, py::arg("q"), py::arg("k"), py::arg("positions") = py::none(), py::arg("inv_freq") = py::none(),
+          py::arg("gamma_q") = py::none(), py::arg("gamma_k") = py::none(), py::arg("gamma_q_compute") = py::none(),
+          py::arg("gamma_k_compute") = py::none(), py::arg("sections") = std::vector<int64_t>{},
+          py::arg("interleaved") = false, py::arg("norm") = true, py::arg("eps") = 1e-6);
+    m.def("gated_linear", [=](const Tensor& x, const Tensor& w, const OptT& b, const OptT& wc, int64_t act) {
+        return NH::gated_linear(x, w, wc ? *wc : w, given(b), act);
+    }, py::arg("x"), py::arg("w"), py::arg("b") = py::none(), py::arg("w_compute") = py::none(), py::arg("act") = 0);
+    m.def("token_logprob", [](const Tensor& z, const Tensor& y, double scale) { return NH::token_logprob(z, y, scale); },
+          py::arg("logits"), py::arg("labels"), py::arg("scale") = 1.0);
     // Whether trainers run convolution weight gradients on the side stream
     // (on by default; the switch exists so tests can compare both orders).
     m.def("set_side_stream", [](bool on) { NH::set_side_stream_enabled(on); }, py::arg("on"));
