@@ -68,35 +68,50 @@ __host__ __device__ __forceinline__ auto with_act(int act, F f) {
 
 // The forward's epilogue on the direct-to-LDS engine: a wave's TM×32 block of g
 // and u (lane l: row l % 32, columns 8q + 4·(l/32) + e in register 4q + e of each
-// 32×32 block) becomes h and, where asked for, [g | u], each staged through LDS
-// as [row][32] with the 16-byte chunk at chunk ^ (row/2 % 4) and its halves
-// exchanged on rows with bit 3 set, and stored as whole 64-byte row pieces.
+// 32×32 block) becomes h and, where asked for, [g | u], each staged through LDS as
+// [row][32] and stored as whole row pieces of 64 (bf16) or 128 bytes.  bf16: the
+// 16-byte chunk at chunk ^ (row/2 % 4), its halves exchanged on rows with bit 3
+// set; fp32: at chunk ^ (row % 8).
+template <typename T>
 struct GatedStore {
-    bf16_t* h;
-    bf16_t* gu;
+    T* h;
+    T* gu;
     const float* bias;
     int64_t m, f;
     int32_t act;
     bool vec;   // 16-byte stores fit every row
+    static constexpr int E = 16 / (int)sizeof(T), C = 32 / E;   // a row's chunks
+    static __device__ __forceinline__ int at(int row, int chunk) {
+        return row * 32 * (int)sizeof(T) + ((chunk ^ (sizeof(T) == 2 ? (row >> 1) & 3 : row & 7)) << 4);
+    }
+    // Columns 8q + 4·hf + 0..3 of a row.
+    static __device__ __forceinline__ void put(char NOTT_LDS* buf, int row, int q, int hf, const float (&v)[4]) {
+        if constexpr (sizeof(T) == 2) {
+            const u32x2 w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+            *reinterpret_cast<u32x2 NOTT_LDS*>(buf + at(row, q) + ((hf ^ ((row >> 3) & 1)) << 3)) = w;
+        } else {
+            *reinterpret_cast<f32x4 NOTT_LDS*>(buf + at(row, 2 * q + hf)) = f32x4{v[0], v[1], v[2], v[3]};
+        }
+    }
     template <int TM>
-    __device__ __forceinline__ void flush(const char NOTT_LDS* buf, bf16_t* dst, int64_t ld, int64_t m0, int64_t c0,
+    __device__ __forceinline__ void flush(const char NOTT_LDS* buf, T* dst, int64_t ld, int64_t m0, int64_t c0,
                                           int lane) const {
         if (vec) {
-            const int c = lane & 3;
+            const int c = lane % C;
 #pragma unroll
-            for (int it = 0; it < TM / 16; ++it) {
-                const int row = 16 * it + (lane >> 2);
-                u32x4 w = *reinterpret_cast<const u32x4 NOTT_LDS*>(buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
-                if ((row >> 3) & 1) w = u32x4{w.z, w.w, w.x, w.y};
-                if (m0 + row < m && c0 + 8 * c < f) *reinterpret_cast<u32x4*>(dst + (m0 + row) * ld + c0 + 8 * c) = w;
+            for (int it = 0; it < TM * C / 64; ++it) {
+                const int row = 64 / C * it + lane / C;
+                u32x4 w = *reinterpret_cast<const u32x4 NOTT_LDS*>(buf + at(row, c));
+                if (sizeof(T) == 2 && ((row >> 3) & 1)) w = u32x4{w.z, w.w, w.x, w.y};
+                if (m0 + row < m && c0 + E * c < f) *reinterpret_cast<u32x4*>(dst + (m0 + row) * ld + c0 + E * c) = w;
             }
         } else {
             const int c = lane & 31;
             for (int it = 0; it < TM / 2; ++it) {
                 const int row = 2 * it + (lane >> 5);
-                const bf16_t v = *reinterpret_cast<const bf16_t NOTT_LDS*>(
-                    buf + row * 64 + (((c >> 3) ^ ((row >> 1) & 3)) << 4) + ((((c >> 2) & 1) ^ ((row >> 3) & 1)) << 3) +
-                    (c & 3) * 2);
+                const int b = sizeof(T) == 2 ? at(row, c >> 3) + ((((c >> 2) & 1) ^ ((row >> 3) & 1)) << 3) + (c & 3) * 2
+                                             : at(row, c >> 2) + (c & 3) * 4;
+                const T v = *reinterpret_cast<const T NOTT_LDS*>(buf + b);
                 if (m0 + row < m && c0 + c < f) dst[(m0 + row) * ld + c0 + c] = v;
             }
         }
@@ -105,11 +120,6 @@ struct GatedStore {
     __device__ __forceinline__ void store_pair(f32x16 (&acc)[FM][2], char NOTT_LDS* buf, int64_t m0, int64_t c0,
                                                int lane) const {
         const int r = lane & 31, hf = lane >> 5;
-        auto put = [&](int row, int q, const float (&v)[4]) {
-            const u32x2 w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-            *reinterpret_cast<u32x2 NOTT_LDS*>(buf + row * 64 + ((q ^ ((row >> 1) & 3)) << 4) +
-                                               ((hf ^ ((row >> 3) & 1)) << 3)) = w;
-        };
         auto stage = [&](int which) {
 #pragma unroll
             for (int i = 0; i < FM; ++i)
@@ -118,7 +128,7 @@ struct GatedStore {
                     float v[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = acc[i][which][4 * q + e];
-                    put(32 * i + r, q, v);
+                    put(buf, 32 * i + r, q, hf, v);
                 }
         };
         if (bias) {
@@ -151,10 +161,10 @@ struct GatedStore {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float a, da;
-                        activate<decltype(A)::value, true>(acc[i][0][4 * q + e], a, da);
+                        activate<decltype(A)::value, sizeof(T) == 2>(acc[i][0][4 * q + e], a, da);
                         v[e] = a * acc[i][1][4 * q + e];
                     }
-                    put(32 * i + r, q, v);
+                    put(buf, 32 * i + r, q, hf, v);
                 }
         });
         flush<TM>(buf, h, f, m0, c0, lane);
@@ -163,28 +173,29 @@ struct GatedStore {
 
 }  // namespace
 
-template <>
-struct nott::gemm::dma::IsPaired<GatedStore> {
+template <typename T>
+struct nott::gemm::dma::IsPaired<GatedStore<T>> {
     static constexpr bool value = true;
 };
 
 namespace {
 
 // h (and gu) from the fp32 products pre [m, 2f] and the bias.
-template <typename T, int ACT>
+template <int ACT>
 __global__ __launch_bounds__(256) void gated_act_kernel(const float* __restrict__ pre, const float* __restrict__ b,
-                                                        int64_t m, int64_t f, T* __restrict__ h, T* __restrict__ gu) {
+                                                        int64_t m, int64_t f, float* __restrict__ h,
+                                                        float* __restrict__ gu) {
     const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= f) return;
     const float bg = b ? b[c] : 0.f, bu = b ? b[f + c] : 0.f;
     for (int64_t r = blockIdx.y; r < m; r += gridDim.y) {
         const float g = pre[r * 2 * f + c] + bg, u = pre[r * 2 * f + f + c] + bu;
         float a, da;
-        activate<ACT, sizeof(T) == 2>(g, a, da);
-        Io<T>::st(h, r * f + c, a * u);
+        activate<ACT, false>(g, a, da);
+        h[r * f + c] = a * u;
         if (gu) {
-            Io<T>::st(gu, r * 2 * f + c, g);
-            Io<T>::st(gu, r * 2 * f + f + c, u);
+            gu[r * 2 * f + c] = g;
+            gu[r * 2 * f + f + c] = u;
         }
     }
 }
@@ -217,10 +228,10 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const T* __restrict__ d
                     lo[r * ld + c] = f32_to_bf16(dg - bf16_to_f32(f32_to_bf16(dg)));
                     lo[r * ld + f + c] = f32_to_bf16(du - bf16_to_f32(f32_to_bf16(du)));
                 }
-                for (int64_t j = 2 * f + c; j < ld; j += f) {
-                    hi[r * ld + j] = 0;
-                    if (lo) lo[r * ld + j] = 0;
-                }
+            }
+            for (int64_t j = 2 * f + c; j < ld; j += f) {
+                hi[r * ld + j] = T(0);
+                if (lo) lo[r * ld + j] = T(0);
             }
         }
     }
@@ -272,24 +283,36 @@ template <> struct nott::gemm::dma::IsWrapped<PiecesPartial> { static constexpr 
 
 namespace {
 
-bool ok16(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
-int64_t up8(int64_t n) { return (n + 7) & ~int64_t(7); }
+// Rows of ld elements that all start on a 16-byte address.
+template <typename T>
+bool ok16(const T* p, int64_t ld) {
+    return (uintptr_t)p % 16 == 0 && ld * (int64_t)sizeof(T) % 16 == 0;
+}
+// n rounded up to whole 16-byte chunks.
+template <typename T>
+int64_t chunks_up(int64_t n) {
+    constexpr int64_t E = 16 / (int64_t)sizeof(T);
+    return (n + E - 1) / E * E;
+}
 
 // A copy of src [rows, cols] with zeros up to [prows, pcols], for tensors whose rows
 // no 16-byte load fits (the copy is small beside the product it is for).
-__global__ __launch_bounds__(256) void pad_kernel(const bf16_t* __restrict__ src, int64_t rows, int64_t cols,
-                                                  bf16_t* __restrict__ dst, int64_t prows, int64_t pcols) {
-    const int64_t n = prows * pcols / 8;
+template <typename T>
+__global__ __launch_bounds__(256) void pad_kernel(const T* __restrict__ src, int64_t rows, int64_t cols,
+                                                  T* __restrict__ dst, int64_t prows, int64_t pcols) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int64_t n = prows * pcols / E;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i * 8 / pcols, c = i * 8 - r * pcols;
-        bf16_t v[8];
+        const int64_t r = i * E / pcols, c = i * E - r * pcols;
+        T v[E];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = r < rows && c + e < cols ? src[r * cols + c + e] : bf16_t(0);
-        *reinterpret_cast<u32x4*>(dst + i * 8) = Pack<bf16_t>::make(v);
+        for (int e = 0; e < E; ++e) v[e] = r < rows && c + e < cols ? src[r * cols + c + e] : T(0);
+        *reinterpret_cast<u32x4*>(dst + i * E) = Pack<T>::make(v);
     }
 }
-void pad(nott_ctx ctx, const bf16_t* src, int64_t rows, int64_t cols, bf16_t* dst, int64_t prows, int64_t pcols) {
-    hipLaunchKernelGGL(pad_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(prows * pcols, 2048), 8192)), dim3(256), 0,
+template <typename T>
+void pad(nott_ctx ctx, const T* src, int64_t rows, int64_t cols, T* dst, int64_t prows, int64_t pcols) {
+    hipLaunchKernelGGL(pad_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(prows * pcols, 2048), 8192)), dim3(256), 0,
                        ctx->stream, src, rows, cols, dst, prows, pcols);
 }
 
@@ -430,40 +453,88 @@ int product(nott_ctx ctx, const T* A, int64_t lda, const T* B, int64_t ldb, cons
     else return go(RowKLoader<T>{A, lda, M, K, vec(A, lda)}, RowKLoader<T>{B, ldb, N, K, vec(B, ldb)});
 }
 
-int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* x, const bf16_t* w, const float* b,
-        bf16_t* h, bf16_t* gu) {
-    const int64_t dp = up8(d);
-    const bool rows = takes_rows(ctx, m, d, f, !ok16(w, d));
-    if (rows && d >= 8) return forward_rows(ctx, m, d, f, act, x, w, b, h, gu);
-    NOTT_REQUIRE(ctx, ceil_div(m, 128) * ceil_div(f, 64) < (int64_t)1 << 26, "nott_gated_linear_fwd: too large");
-    const bool pad_x = !ok16(x, d), pad_w = !ok16(w, d);
-    WorkspaceHold ws(ctx, sizeof(bf16_t) * (size_t)(((pad_x ? m : 0) + (pad_w ? 2 * f : 0)) * dp));
-    if (!ws.p) return NOTT_ERR_ALLOC;
-    bf16_t* xp = reinterpret_cast<bf16_t*>(ws.p);
-    bf16_t* wp = xp + (pad_x ? m * dp : 0);
-    if (pad_x) pad(ctx, x, m, d, xp, m, dp);
-    if (pad_w) pad(ctx, w, 2 * f, d, wp, 2 * f, dp);
-    if (rows) return forward_rows(ctx, m, dp, f, act, pad_x ? xp : x, pad_w ? wp : w, b, h, gu);
-    const GatedStore ep{h, gu, b, m, f, act, ok16(h, f) && ok16(gu, f)};
-    const dma::Plan p = dma::plan(ctx, m, 2 * f, dp, false, false, 1);
-    return dma::launch_shape<false, false, false>(ctx, p.shape, pad_x ? xp : x, dp, pad_w ? wp : w, dp, ep, m, 2 * f, dp, 1,
-                                                  dp);
+// The fp32 engines' estimated times (us).  Direct-to-LDS tiles: their MFMA time at
+// the rate they reach, in whole rounds of the CUs' tiles, splits' partials included;
+// the generic engine: its rate with any split.
+struct Plan32 {
+    int bm;   // tiles of 128×128, two workgroups a CU, or 256×128, one
+    int64_t splits, kps;
+    double us;
+};
+Plan32 plan32(nott_ctx ctx, int64_t M, int64_t N, int64_t K, bool split) {
+    constexpr double kFlopUs = 0.75 * 157.3e6 / 256;   // a CU's, reached
+    const int64_t stages = ceil_div(K, dma::kStageK<float>);
+    Plan32 best{128, 1, K, 0};
+    for (const int bm : {128, 256}) {
+        const int64_t tiles = ceil_div(M, bm) * ceil_div(N, 128);
+        for (int64_t n = 1; n <= (split ? 16 : 1) && (n == 1 || stages / n >= 4); n *= 2) {
+            const int64_t per = ceil_div(stages, n), splits = ceil_div(stages, per);
+            double us = 3 + (double)ceil_div(tiles * splits, ctx->num_cu) * (double)per * (bm * 128 * 64.0) / kFlopUs;
+            if (splits > 1) us += 2 + 8.0 * (double)(splits * M * N) / 5.9e6;
+            if (best.us == 0 || us < best.us)
+                best = {bm, splits, splits > 1 ? per * dma::kStageK<float> : K, us};
+        }
+    }
+    return best;
+}
+template <bool AT, bool BT, class EP>
+int launch32(nott_ctx ctx, const Plan32& p, const float* A, int64_t lda, const float* B, int64_t ldb, const EP& ep,
+             int64_t M, int64_t N, int64_t K) {
+    if (p.bm == 256)
+        return dma::launch<dma::Config<AT, BT, 256, 128, 4, 2, 3>, false>(ctx, A, lda, B, ldb, ep, M, N, K, p.splits, p.kps);
+    return dma::launch<dma::Config<AT, BT, 128, 128, 2, 2, 2>, false>(ctx, A, lda, B, ldb, ep, M, N, K, p.splits, p.kps);
+}
+// Whether an fp32 product goes to the generic engine, which spreads few tiles over
+// the CUs by splitting k and runs at `rate` TFLOP/s.  1576 rows of 768 → 2048: forward
+// 118 us on the direct-to-LDS tiles against 163, dx 143 against 168, dw 145 against
+// 139; 512 rows of 1024 → 2048: forward 73 against 50.
+bool generic32(double us, int64_t M, int64_t N, int64_t K, double rate) {
+    return 6 + 2.0 * (double)M * (double)N * (double)K / (rate * 1e6) < us;
 }
 
-int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* x, const float* w, const float* b, float* h,
-        float* gu) {
-    WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * 2 * f));
+template <typename T>
+int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const T* x, const T* w, const float* b, T* h, T* gu) {
+    const int64_t dp = chunks_up<T>(d);
+    typename std::conditional<sizeof(T) == 2, dma::Plan, Plan32>::type p;
+    bool rows = false;
+    if constexpr (sizeof(T) == 2) {
+        rows = takes_rows(ctx, m, d, f, !ok16(w, d));
+        if (rows && d >= 8) return forward_rows(ctx, m, d, f, act, x, w, b, h, gu);
+        p = dma::plan(ctx, m, 2 * f, dp, false, false, 1);
+    } else {
+        p = plan32(ctx, m, 2 * f, dp, false);
+        if (generic32(p.us, m, 2 * f, d, 70)) {
+            WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * 2 * f));
+            if (!ws.p) return NOTT_ERR_ALLOC;
+            float* pre = reinterpret_cast<float*>(ws.p);
+            const RowMajorStore<float> ep{pre, 2 * f, m, 2 * f, nullptr};
+            const int st = product<float, false, false>(ctx, x, d, w, d, ep, m, 2 * f, d);
+            if (st != NOTT_OK) return st;
+            with_act(act, [&](auto a) {
+                hipLaunchKernelGGL((gated_act_kernel<decltype(a)::value>),
+                                   dim3((unsigned)ceil_div(f, 256), (unsigned)std::min<int64_t>(m, 65535)), dim3(256), 0,
+                                   ctx->stream, pre, b, m, f, h, gu);
+            });
+            return launch_status(ctx, "gated_linear");
+        }
+    }
+    NOTT_REQUIRE(ctx, ceil_div(m, 128) * ceil_div(f, 64) < (int64_t)1 << 26, "nott_gated_linear_fwd: too large");
+    const bool pad_x = !ok16(x, d), pad_w = !ok16(w, d);
+    WorkspaceHold ws(ctx, sizeof(T) * (size_t)(((pad_x ? m : 0) + (pad_w ? 2 * f : 0)) * dp));
     if (!ws.p) return NOTT_ERR_ALLOC;
-    float* pre = reinterpret_cast<float*>(ws.p);
-    RowMajorStore<float> ep{pre, 2 * f, m, 2 * f, nullptr};
-    const int st = product<float, false, false>(ctx, x, d, w, d, ep, m, 2 * f, d);
-    if (st != NOTT_OK) return st;
-    return with_act(act, [&](auto a) {
-        hipLaunchKernelGGL((gated_act_kernel<float, decltype(a)::value>),
-                           dim3((unsigned)ceil_div(f, 256), (unsigned)std::min<int64_t>(m, 65535)), dim3(256), 0,
-                           ctx->stream, pre, b, m, f, h, gu);
-        return launch_status(ctx, "gated_linear");
-    });
+    T* xp = reinterpret_cast<T*>(ws.p);
+    T* wp = xp + (pad_x ? m * dp : 0);
+    if (pad_x) pad(ctx, x, m, d, xp, m, dp);
+    if (pad_w) pad(ctx, w, 2 * f, d, wp, 2 * f, dp);
+    const T* X = pad_x ? xp : x;
+    const T* W = pad_w ? wp : w;
+    if constexpr (sizeof(T) == 2)
+        if (rows) return forward_rows(ctx, m, dp, f, act, X, W, b, h, gu);
+    const GatedStore<T> ep{h, gu, b, m, f, act, ok16(h, f) && ok16(gu, f)};
+    if constexpr (sizeof(T) == 2)
+        return dma::launch_shape<false, false, false>(ctx, p.shape, X, dp, W, dp, ep, m, 2 * f, dp, 1, dp);
+    else
+        return launch32<false, false>(ctx, p, X, dp, W, dp, ep, m, 2 * f, dp);
 }
 
 constexpr int kSlabs = 64;
@@ -489,7 +560,7 @@ int activation_bwd(nott_ctx ctx, int64_t m, int64_t f, int64_t ld, int act, cons
 
 int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* dh, const bf16_t* x, const bf16_t* w,
         const bf16_t* gu, bf16_t* dx, float* dw, float* db, int accumulate) {
-    const int64_t dp = up8(d), fp = up8(2 * f);
+    const int64_t dp = chunks_up<bf16_t>(d), fp = chunks_up<bf16_t>(2 * f);
     // the direct-to-LDS engine, where a product has its 128 rows and columns
     const bool dma_dx = dx && m >= 128 && d >= 128, dma_dw = dw && 2 * f >= 128 && d >= 128;
     const bool pad_x = dma_dw && !ok16(x, d), pad_w = dma_dx && (!ok16(w, d) || fp != 2 * f);
@@ -533,16 +604,48 @@ int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* dh
     return launch_status(ctx, "gated_linear dw");
 }
 
+// C = A·B in fp32 on the direct-to-LDS engine, as planned.
+template <bool AT, bool BT, class EP>
+int product32(nott_ctx ctx, Plan32 p, const float* A, int64_t lda, const float* B, int64_t ldb, const EP& ep, int64_t M,
+              int64_t N, int64_t K) {
+    float* part = nullptr;
+    if (p.splits > 1) {
+        part = static_cast<float*>(nott::optional_workspace(ctx, sizeof(float) * (size_t)(p.splits * M * N)));
+        if (!part) p = plan32(ctx, M, N, K, false);
+    }
+    if (!part) return launch32<AT, BT>(ctx, p, A, lda, B, ldb, ep, M, N, K);
+    const int st = launch32<AT, BT>(ctx, p, A, lda, B, ldb, dma::PartialRowStore{part, nullptr, M, N}, M, N, K);
+    if (st != NOTT_OK) return st;
+    launch_splitk_reduce(ctx, part, p.splits, M, N, ep);
+    return launch_status(ctx, "gated_linear splits");
+}
+
 int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* dh, const float* x, const float* w,
         const float* gu, float* dx, float* dw, float* db, int accumulate) {
-    WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * 2 * f));
+    const int64_t dp = chunks_up<float>(d), fp = chunks_up<float>(2 * f);
+    const Plan32 px = plan32(ctx, m, dp, fp, true), pw = plan32(ctx, fp, dp, m, true);
+    const bool dma_dx = dx && !generic32(px.us, m, d, 2 * f, 65), dma_dw = dw && !generic32(pw.us, 2 * f, d, m, 85);
+    const bool pad_x = dma_dw && !ok16(x, d), pad_w = dma_dx && (!ok16(w, d) || fp != 2 * f);
+    WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * fp + ((pad_x ? m : 0) + (pad_w ? fp : 0)) * dp));
     if (!ws.p) return NOTT_ERR_ALLOC;
     float* dgu = reinterpret_cast<float*>(ws.p);
-    int st = activation_bwd<float>(ctx, m, f, 2 * f, act, dh, gu, dgu, nullptr, db, accumulate);
-    if (st == NOTT_OK && dx)
-        st = product<float, false, true>(ctx, dgu, 2 * f, w, d, RowMajorStore<float>{dx, d, m, d, nullptr}, m, d, 2 * f);
-    if (st == NOTT_OK && dw)
-        st = product<float, true, true>(ctx, dgu, 2 * f, x, d, AccStore{dw, 2 * f, d, accumulate}, 2 * f, d, m);
+    float* xp = dgu + m * fp;
+    float* wp = xp + (pad_x ? m * dp : 0);
+    int st = activation_bwd<float>(ctx, m, f, fp, act, dh, gu, dgu, nullptr, db, accumulate);
+    if (st != NOTT_OK) return st;
+    if (pad_x) pad(ctx, x, m, d, xp, m, dp);
+    if (pad_w) pad(ctx, w, 2 * f, d, wp, fp, dp);
+    if (dx) {
+        const AccStore ep{dx, m, d, 0};
+        st = dma_dx ? product32<false, true>(ctx, px, dgu, fp, pad_w ? wp : w, dp, ep, m, dp, fp)
+                    : product<float, false, true>(ctx, dgu, fp, w, d, ep, m, d, 2 * f);
+        if (st != NOTT_OK) return st;
+    }
+    if (dw) {
+        const AccStore ep{dw, 2 * f, d, accumulate};
+        st = dma_dw ? product32<true, true>(ctx, pw, dgu, fp, pad_x ? xp : x, dp, ep, fp, dp, m)
+                    : product<float, true, true>(ctx, dgu, fp, x, d, ep, 2 * f, d, m);
+    }
     return st;
 }
 
@@ -558,9 +661,9 @@ extern "C" int nott_gated_linear_fwd(nott_ctx ctx, nott_dtype dtype, int64_t m, 
     NOTT_REQUIRE(ctx, x && w && h, "nott_gated_linear_fwd: null buffer");
     nott::DeviceScope scope(ctx->device);
     if (dtype == NOTT_F32)
-        return fwd(ctx, m, d, f, act, static_cast<const float*>(x), static_cast<const float*>(w), b,
+        return fwd<float>(ctx, m, d, f, act, static_cast<const float*>(x), static_cast<const float*>(w), b,
                           static_cast<float*>(h), static_cast<float*>(gu));
-    return fwd(ctx, m, d, f, act, static_cast<const bf16_t*>(x), static_cast<const bf16_t*>(w), b,
+    return fwd<bf16_t>(ctx, m, d, f, act, static_cast<const bf16_t*>(x), static_cast<const bf16_t*>(w), b,
                        static_cast<bf16_t*>(h), static_cast<bf16_t*>(gu));
 }
 
