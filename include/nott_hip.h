@@ -389,7 +389,8 @@ int nott_qk_norm_rope_bwd(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype d
  * activation and the product.  w [2·f, d] (dtype) is packed, gate rows first,
  * then up rows; b [2·f] fp32 nullable:
  *   [g | u] = x·wᵀ + b,  h = act(g)·u        x [m, d], h [m, f]
- * gu [m, 2·f] (dtype, nullable) receives [g | u] for the backward. */
+ * gu [m, 2·f] (dtype, nullable) receives [g | u] for the backward.  No output may
+ * overlap an input. */
 enum {
     NOTT_ACT_SILU = 0,       /* g·sigmoid(g) */
     NOTT_ACT_GELU = 1,       /* g·Φ(g) */

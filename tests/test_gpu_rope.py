@@ -230,8 +230,10 @@ def test_accumulate_queries_alone_and_empty():
     none = torch.empty((1, 0, 4), device="cuda", dtype=torch.int64)
     acc.fill_(3.0)
     assert ops.qk_norm_rope_fwd(e, e, none, freq, gq, gk)[0].shape == e.shape
-    ops.qk_norm_rope_bwd(e, e, e, e, none, freq, gq, gk, dgamma_q=acc, accumulate=True)
+    ops.qk_norm_rope_bwd(e, e, e, e, none, freq, gq, gk, dgamma_q=acc, dgamma_k=acc.clone(), accumulate=True)
     assert bool((acc == 3).all())
+    with pytest.raises(ValueError, match="accumulate needs"):
+        ops.qk_norm_rope_bwd(e, e, e, e, none, freq, gq, gk, dgamma_q=acc, accumulate=True)
     ops.qk_norm_rope_bwd(e, e, e, e, none, freq, gq, gk, dgamma_q=acc)
     assert bool((acc == 0).all())
 

@@ -75,6 +75,14 @@ def test_gated(x, w, act, match):
         ops.gated_linear_fwd(torch.zeros(x), torch.zeros(w), act=act)
 
 
+def test_accumulation_without_gradients():
+    x, w, gu = torch.zeros(3, 8), torch.zeros(10, 8), torch.zeros(3, 10)
+    with pytest.raises(ValueError, match="accumulate needs"):
+        ops.gated_linear_bwd(torch.zeros(3, 5), x, w, gu, need_db=False, accumulate=True)
+    with pytest.raises(ValueError, match="accumulate needs"):
+        ops.gated_linear_bwd(torch.zeros(3, 5), x, w, gu, dw=w, accumulate=True)
+
+
 def test_gated_types():
     with pytest.raises(TypeError):
         ops.gated_linear_fwd(torch.zeros((3, 8), dtype=torch.float16), torch.zeros((10, 8), dtype=torch.float16))

@@ -63,17 +63,18 @@ void* optional_workspace(nott_ctx ctx, size_t bytes);
 // Workspace that a call keeps while it makes others that take some themselves (a
 // composite of products): until the hold ends, workspace() hands out what lies
 // behind it.  A nested call that makes the arena grow leaves `p` in the retired
-// one, where it stays valid.  `p` is null on failure (error set).
+// one, where it stays valid.  No bytes take nothing.  failed(): error set.
 class WorkspaceHold {
 public:
     WorkspaceHold(nott_ctx c, size_t bytes);
     ~WorkspaceHold() { ctx_->ws_held = before_; }
     WorkspaceHold(const WorkspaceHold&) = delete;
     WorkspaceHold& operator=(const WorkspaceHold&) = delete;
+    bool failed() const { return !p && bytes_; }
     char* p;
 private:
     nott_ctx ctx_;
-    size_t before_;
+    size_t bytes_, before_;
 };
 // Looks up this device's static LayerNorm scratch (layernorm.hip).
 int layernorm_scratch_setup(nott_ctx ctx);

@@ -42,7 +42,7 @@ void* workspace(nott_ctx ctx, size_t bytes) {
 }
 
 WorkspaceHold::WorkspaceHold(nott_ctx c, size_t bytes)
-    : p(static_cast<char*>(workspace(c, bytes))), ctx_(c), before_(c->ws_held) {
+    : p(bytes ? static_cast<char*>(workspace(c, bytes)) : nullptr), ctx_(c), bytes_(bytes), before_(c->ws_held) {
     if (p) c->ws_held += (bytes + 255) & ~size_t(255);
 }
 

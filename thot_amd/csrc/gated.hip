@@ -505,7 +505,7 @@ int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const T* x, cons
         p = plan32(ctx, m, 2 * f, dp, false);
         if (generic32(p.us, m, 2 * f, d, 70)) {
             WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * 2 * f));
-            if (!ws.p) return NOTT_ERR_ALLOC;
+            if (ws.failed()) return NOTT_ERR_ALLOC;
             float* pre = reinterpret_cast<float*>(ws.p);
             const RowMajorStore<float> ep{pre, 2 * f, m, 2 * f, nullptr};
             const int st = product<float, false, false>(ctx, x, d, w, d, ep, m, 2 * f, d);
@@ -521,7 +521,7 @@ int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const T* x, cons
     NOTT_REQUIRE(ctx, ceil_div(m, 128) * ceil_div(f, 64) < (int64_t)1 << 26, "nott_gated_linear_fwd: too large");
     const bool pad_x = !ok16(x, d), pad_w = !ok16(w, d);
     WorkspaceHold ws(ctx, sizeof(T) * (size_t)(((pad_x ? m : 0) + (pad_w ? 2 * f : 0)) * dp));
-    if (!ws.p) return NOTT_ERR_ALLOC;
+    if (ws.failed()) return NOTT_ERR_ALLOC;
     T* xp = reinterpret_cast<T*>(ws.p);
     T* wp = xp + (pad_x ? m * dp : 0);
     if (pad_x) pad(ctx, x, m, d, xp, m, dp);
@@ -566,7 +566,7 @@ int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* dh
     const bool pad_x = dma_dw && !ok16(x, d), pad_w = dma_dx && (!ok16(w, d) || fp != 2 * f);
     const size_t piece = sizeof(bf16_t) * (size_t)(m * fp);
     WorkspaceHold ws(ctx, piece * (dw ? 2 : 1) + sizeof(bf16_t) * (size_t)(((pad_x ? m : 0) + (pad_w ? fp : 0)) * dp));
-    if (!ws.p) return NOTT_ERR_ALLOC;
+    if (ws.failed()) return NOTT_ERR_ALLOC;
     bf16_t* hi = reinterpret_cast<bf16_t*>(ws.p);
     bf16_t* lo = dw ? hi + m * fp : nullptr;
     int st = activation_bwd(ctx, m, f, fp, act, dh, gu, hi, lo, db, accumulate);
@@ -627,7 +627,7 @@ int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* dh,
     const bool dma_dx = dx && !generic32(px.us, m, d, 2 * f, 65), dma_dw = dw && !generic32(pw.us, 2 * f, d, m, 85);
     const bool pad_x = dma_dw && !ok16(x, d), pad_w = dma_dx && (!ok16(w, d) || fp != 2 * f);
     WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * fp + ((pad_x ? m : 0) + (pad_w ? fp : 0)) * dp));
-    if (!ws.p) return NOTT_ERR_ALLOC;
+    if (ws.failed()) return NOTT_ERR_ALLOC;
     float* dgu = reinterpret_cast<float*>(ws.p);
     float* xp = dgu + m * fp;
     float* wp = xp + (pad_x ? m * dp : 0);

@@ -380,6 +380,8 @@ __global__ __launch_bounds__(NT) void logprob_bwd_kernel(const T* logits, const 
     if (part == 0 && sp.single >= 0) Io<T>::st(dz, sp.single, grad(xs, sp.single));
 }
 
+// Workgroups of a launch: its threads are counted in 32 bits.
+constexpr int64_t kMaxGrid = int64_t(1) << 23;
 // Up to this many columns a row is one wave's.
 constexpr int64_t kWaveColumns = 2048;
 
@@ -392,25 +394,29 @@ int forward(nott_ctx ctx, int64_t n, int64_t c, const T* logits, const int64_t* 
     int64_t splits = 1;
     if (n < 4 * ctx->num_cu)
         splits = std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, 4 * (int64_t)ctx->num_cu / n, c / 4096}));
-    const int64_t chunk = splits == 1 ? c : ceil_div(ceil_div(c, splits), 64) * 64;
+    int64_t chunk = splits == 1 ? c : ceil_div(ceil_div(c, splits), 64) * 64;
     splits = ceil_div(c, chunk);
     Stats* stats = nullptr;
     uint64_t* keys = nullptr;
     if (splits > 1) {
         const size_t sb = (sizeof(Stats) * (size_t)(n * splits) + 255) & ~size_t(255);
-        char* ws = static_cast<char*>(nott::workspace(ctx, sb + sizeof(uint64_t) * (size_t)(n * splits * top)));
-        if (!ws) return NOTT_ERR_ALLOC;
+        char* ws = static_cast<char*>(nott::optional_workspace(ctx, sb + sizeof(uint64_t) * (size_t)(n * splits * top)));
         stats = reinterpret_cast<Stats*>(ws);
         keys = reinterpret_cast<uint64_t*>(ws + sb);
+        if (!ws) splits = 1, chunk = c;
     }
     const int cap = top == 0 ? 0 : nt == 64 ? 256 : 1024;
-    const dim3 grid((unsigned)n, (unsigned)splits);
-    if (nt == 64)
-        hipLaunchKernelGGL((logprob_kernel<T, 64>), grid, dim3(64), sizeof(uint64_t) * cap, ctx->stream, logits, labels, c,
-                           (int)chunk, sc, top, cap, o, stats, keys);
-    else
-        hipLaunchKernelGGL((logprob_kernel<T, 256>), grid, dim3(256), sizeof(uint64_t) * cap, ctx->stream, logits, labels,
-                           c, (int)chunk, sc, top, cap, o, stats, keys);
+    for (int64_t r = 0; r < n; r += kMaxGrid) {   // more than one only for rows that are not split
+        const dim3 grid((unsigned)std::min(kMaxGrid, n - r), (unsigned)splits);
+        const FwdOut at{o.logprob + r, o.entropy ? o.entropy + r : nullptr, o.lse ? o.lse + r : nullptr,
+                        top ? o.top_logprob + r * top : nullptr, top ? o.top_index + r * top : nullptr, o.err};
+        auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, grid, dim3(nt), sizeof(uint64_t) * cap, ctx->stream, logits + r * c, labels + r, c,
+                               (int)chunk, sc, top, cap, at, stats, keys);
+        };
+        if (nt == 64) launch(logprob_kernel<T, 64>);
+        else launch(logprob_kernel<T, 256>);
+    }
     if (splits > 1)
         hipLaunchKernelGGL(logprob_merge_kernel<T>, dim3((unsigned)n), dim3(64), 0, ctx->stream, logits, labels, c,
                            (int)splits, sc, top, o, stats, keys);
@@ -422,8 +428,7 @@ int backward(nott_ctx ctx, int64_t n, int64_t c, const T* logits, const int64_t*
              const float* entropy, const float* dlogprob, const float* dentropy, T* dlogits) {
     const int nt = c <= kWaveColumns ? 64 : 256;
     const int64_t parts = std::max<int64_t>(1, ceil_div(c, (int64_t)nt * kUnroll * Pack16<T>::N));
-    // as many rows a launch as workgroups have numbers
-    const int64_t rows = std::max<int64_t>(1, ((int64_t(1) << 31) - 1) / parts);
+    const int64_t rows = std::max<int64_t>(1, kMaxGrid / parts);
     for (int64_t r = 0; r < n; r += rows) {
         const unsigned grid = (unsigned)(std::min(rows, n - r) * parts);
         const FastDiv by((uint32_t)parts);

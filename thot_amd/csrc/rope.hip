@@ -517,7 +517,7 @@ Launch plan(nott_ctx ctx, const RopeArgs<T>& a, bool bwd) {
     if (pairs) tpb = std::min<int64_t>(tpb, 2048 / pairs);
     tpb = std::min<int64_t>(tpb, ceil_div(tokens, ctx->num_cu));
     l.tpb = (int)std::max<int64_t>(tpb, 1);
-    l.grid = (unsigned)std::min<int64_t>(ceil_div(tokens, l.tpb), bwd ? groups : 0x7fffffff);
+    l.grid = (unsigned)std::min<int64_t>(ceil_div(tokens, l.tpb), bwd ? groups : 1 << 23);   // a launch's threads in 32 bits
     l.lds = std::max(sizeof(f32x2) * (size_t)l.tpb * pairs, bwd ? sizeof(float) * 8 * (size_t)a.dh : 0);
     return l;
 }

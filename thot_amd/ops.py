@@ -737,6 +737,8 @@ def qk_norm_rope_bwd(dyq: torch.Tensor, dyk: Optional[torch.Tensor], q: torch.Te
     d, positions, k_shape = _qk_rope_desc(q, k, positions, inv_freq, gamma_q, gamma_k, norm, eps, sections, interleaved)
     if (k is None) != (dyk is None):
         raise ValueError("dyk goes with k")
+    if accumulate and ((gamma_q is not None and dgamma_q is None) or (gamma_k is not None and dgamma_k is None)):
+        raise ValueError("accumulate needs the gradients to add to")
     d.yq_stride[:] = _head_strides(dyq, "dyq", q.shape, q)
     if k is not None:
         d.yk_stride[:] = _head_strides(dyk, "dyk", k_shape, q)
@@ -804,6 +806,8 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w: torch.Tensor, gu: tor
                      db: Optional[torch.Tensor] = None, accumulate: bool = False):
     """(dx, dw, db) of gated_linear_fwd from dh and its gu; dw and db fp32
     (nott_gated_linear_bwd)."""
+    if accumulate and ((need_dw and dw is None) or (need_db and db is None)):
+        raise ValueError("accumulate needs the gradients to add to")
     m, d, f = _gated_shapes(x, w, act)
     _check(dh, "dh", shape=(*x.shape[:-1], f), dtype=x.dtype, device=x.device)
     _check(gu, "gu", shape=(*x.shape[:-1], 2 * f), dtype=x.dtype, device=x.device)
