@@ -7,8 +7,8 @@
 // maximum m' and a = exp(m − m'), S' = a·S and T' = a·(T + S·(m − m')).  The same
 // running maxima give the top tokens: the top-th largest of 64 maxima over 64
 // disjoint shares of the row is a bound that at least `top` elements reach and
-// few more do (24 of any number for 20), and only threads whose own maximum
-// reaches it read their elements again.
+// few more do (24 of any number for 20); what the few threads whose own maximum
+// reaches it have read is read again, by all threads together.
 // Backward: one read and one write.
 #include "common.hpp"
 
@@ -91,13 +91,47 @@ __device__ __forceinline__ uint64_t top_key(float z, uint32_t col) {
     return ((uint64_t)u << 32) | (uint32_t)~col;
 }
 
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_max64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, 0xf, 0xf, false);
+    return max(v, ((uint64_t)hi << 32) | lo);
+}
+template <int L>
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, L), hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), L);
+    return ((uint64_t)hi << 32) | lo;
+}
+// The largest of the wave's keys, as wave_max (a shuffled one takes 0.4 us).
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const uint32_t lo = __shfl_xor((uint32_t)v, s), hi = __shfl_xor((uint32_t)(v >> 32), s);
-        v = max(v, ((uint64_t)hi << 32) | lo);
+    v = dpp_max64<0xB1>(v);
+    v = dpp_max64<0x4E>(v);
+    v = dpp_max64<0x141>(v);
+    v = dpp_max64<0x140>(v);
+    return max(max(lane_u64<0>(v), lane_u64<16>(v)), max(lane_u64<32>(v), lane_u64<48>(v)));
+}
+
+// The top-th largest of the wave's 64 values (none a NaN): up to 16 by taking the
+// largest away one after the other, past that by every lane's rank.
+__device__ __forceinline__ float wave_nth(float v, int top) {
+    const int lane = (int)threadIdx.x & 63;
+    if (top <= 16) {
+        float m = wave_max(v);
+        for (int i = 1; i < top; ++i) {
+            const uint64_t hit = __ballot(v == m);
+            if (lane == __ffsll((unsigned long long)hit) - 1) v = -INFINITY;
+            m = wave_max(v);
+        }
+        return m;
     }
-    return v;
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < 64; ++j) {
+        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), j));
+        rank += w > v || (w == v && j < lane) ? 1 : 0;
+    }
+    const uint64_t hit = __ballot(rank == top - 1);
+    return __shfl(v, __ffsll((unsigned long long)hit) - 1);
 }
 
 struct FwdOut {
@@ -173,7 +207,8 @@ __global__ __launch_bounds__(NT) void logprob_kernel(const T* __restrict__ logit
     __shared__ Stats part[W];
     __shared__ float share[NT];
     __shared__ float bound_s;
-    __shared__ int count;
+    __shared__ int count, hot_count;
+    __shared__ int hot[NT];
     __shared__ uint64_t red[W];
     const int tid = (int)threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int64_t row = blockIdx.x;
@@ -193,17 +228,26 @@ __global__ __launch_bounds__(NT) void logprob_kernel(const T* __restrict__ logit
         for (int u = 0; u < kUnroll; ++u) Pack16<T>::unpack(raw[u], reinterpret_cast<float(&)[G]>(v[u * G]));
         st.add(v, sc);
     }
-    for (int k = full * kUnroll * NT + tid; k < sp.groups; k += NT) {
-        float v[G];
-        Pack16<T>::template ld<true>(sp.base + (int64_t)k * G, v);
-        st.add(v, sc);
+    if (full * kUnroll * NT < sp.groups) {   // the rest, its loads in flight together
+        const int k = full * kUnroll * NT + tid;
+        typename Pack16<T>::Raw raw[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            raw[u] = Pack16<T>::template raw<true>(sp.base + (int64_t)min(k + u * NT, sp.groups - 1) * G);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            if (full * kUnroll * NT + u * NT >= sp.groups) break;
+            float v[G];
+            Pack16<T>::unpack(k + u * NT < sp.groups ? raw[u] : minus_inf<T>(), v);
+            st.add(v, sc);
+        }
     }
     if (sp.single >= 0) {
         const float v[1] = {Io<T>::ld(z + j0, sp.single)};
         st.add(v, sc);
     }
     const float own = st.s != st.s ? INFINITY : st.m;   // a NaN is among the largest
-    if (tid == 0) count = 0;
+    if (tid == 0) count = hot_count = 0;
     share[tid] = own;
     st.merge_wave(sc);
     if (lane == 0) part[wid] = st;
@@ -223,13 +267,8 @@ __global__ __launch_bounds__(NT) void logprob_kernel(const T* __restrict__ logit
         float v = share[lane];
 #pragma unroll
         for (int i = 1; i < W; ++i) v = fmaxf(v, share[i * 64 + lane]);
-        int rank = 0;
-#pragma unroll
-        for (int j = 0; j < 64; ++j) {
-            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), j));
-            rank += w > v || (w == v && j < lane) ? 1 : 0;
-        }
-        if (rank == top - 1) bound_s = v;
+        v = wave_nth(v, top);
+        if (lane == 0) bound_s = v;
     }
     __syncthreads();
     // no bound among live logits: every element is a candidate
@@ -239,23 +278,31 @@ __global__ __launch_bounds__(NT) void logprob_kernel(const T* __restrict__ logit
         const int i = atomicAdd(&count, 1);
         if (i < cap) cand[i] = top_key(x, (uint32_t)col);
     };
-    if (!(own < bound) || bound == -INFINITY) {
-        const int64_t first = j0 + (sp.base - (z + j0));
-        for (int k = tid; k < sp.groups; k += NT * kUnroll) {
-            typename Pack16<T>::Raw raw[kUnroll];
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                raw[u] = Pack16<T>::template raw<false>(sp.base + (int64_t)min(k + u * NT, sp.groups - 1) * G);
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                if (k + u * NT >= sp.groups) break;
-                float v[G];
-                Pack16<T>::unpack(raw[u], v);
-#pragma unroll
-                for (int e = 0; e < G; ++e) offer(v[e], first + (int64_t)(k + u * NT) * G + e);
-            }
-        }
+    if (!(own < bound)) {
+        hot[atomicAdd(&hot_count, 1)] = tid;
         if (sp.single >= 0) offer(Io<T>::ld(z + j0, sp.single), j0 + sp.single);
+    }
+    __syncthreads();
+    // groups tid, tid + NT, ... of the hot threads
+    const int64_t first = j0 + (sp.base - (z + j0));
+    const int nh = hot_count, all = nh * ((sp.groups + NT - 1) / NT);
+    for (int i = tid; i < all; i += NT * 2) {
+        int k[2];
+        typename Pack16<T>::Raw raw[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int w = min(i + u * NT, all - 1), turn = w / nh;
+            k[u] = hot[w - turn * nh] + turn * NT;
+            raw[u] = Pack16<T>::template raw<false>(sp.base + (int64_t)min(k[u], sp.groups - 1) * G);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (i + u * NT >= all || k[u] >= sp.groups) continue;
+            float v[G];
+            Pack16<T>::unpack(raw[u], v);
+#pragma unroll
+            for (int e = 0; e < G; ++e) offer(v[e], first + (int64_t)k[u] * G + e);
+        }
     }
     __syncthreads();
     const int n = count;
@@ -382,14 +429,17 @@ __global__ __launch_bounds__(NT) void logprob_bwd_kernel(const T* logits, const 
 
 // Workgroups of a launch: its threads are counted in 32 bits.
 constexpr int64_t kMaxGrid = int64_t(1) << 23;
-// Up to this many columns a row is one wave's.
-constexpr int64_t kWaveColumns = 2048;
+// Threads of a row: one wave up to 2048 columns, and up to 4096 where there are rows
+// for every SIMD.
+int row_threads(nott_ctx ctx, int64_t n, int64_t c) {
+    return c <= 2048 || (c <= 4096 && n >= 8 * (int64_t)ctx->num_cu) ? 64 : 256;
+}
 
 template <typename T>
 int forward(nott_ctx ctx, int64_t n, int64_t c, const T* logits, const int64_t* labels, double scale, int top,
             const FwdOut& o) {
     const Scale sc{(float)scale, (float)(scale * 1.4426950408889634), (float)std::max(-1e30 / scale, -3e38)};
-    const int nt = c <= kWaveColumns ? 64 : 256;
+    const int nt = row_threads(ctx, n, c);
     // Fewer rows than fill the card are split, into parts of at least 4096 columns.
     int64_t splits = 1;
     if (n < 4 * ctx->num_cu)
@@ -426,7 +476,7 @@ int forward(nott_ctx ctx, int64_t n, int64_t c, const T* logits, const int64_t* 
 template <typename T>
 int backward(nott_ctx ctx, int64_t n, int64_t c, const T* logits, const int64_t* labels, float scale, const float* lse,
              const float* entropy, const float* dlogprob, const float* dentropy, T* dlogits) {
-    const int nt = c <= kWaveColumns ? 64 : 256;
+    const int nt = c <= 2048 ? 64 : 256;
     const int64_t parts = std::max<int64_t>(1, ceil_div(c, (int64_t)nt * kUnroll * Pack16<T>::N));
     const int64_t rows = std::max<int64_t>(1, kMaxGrid / parts);
     for (int64_t r = 0; r < n; r += rows) {
