@@ -220,3 +220,42 @@ def test_captured_and_other_stream(m):
         torch.cuda.synchronize()
         for p, q in zip(got, step()):
             assert torch.equal(p, q), i
+
+
+# fp32 products that are taken from bf16 pieces of their operands: each term keeps all
+# but 4.01 u (the two parts that are left out, 2^-16·2^-8 each, and what three pieces
+# leave of each operand, 2^-24), and only hi·hi sums at full size: k/4 additions and 5
+# times as many of less than 2^-7.
+@pytest.mark.parametrize("m,d,f,spread", [(2150, 605, 1237, 0), (1600, 768, 1024, 20), (700, 1500, 2500, 0),
+                                          (130, 2048, 4096, 20), (6001, 640, 200, 20)])
+def test_large_in_fp32(m, d, f, spread):
+    x, w, b, dh = make(m, d, f, torch.float32, True, seed=m)
+    g = torch.Generator(device="cuda").manual_seed(m + 1)
+    if spread:   # rows of very different magnitudes
+        for t in (x, dh):
+            t.mul_(torch.exp2(torch.randint(-spread, 2, (m, 1), generator=g, device="cuda").float()))
+
+    def err(k, mag):
+        return (0.26 * k + 22) * U * mag
+    gu64 = x.double() @ w.double().t() + b.double()
+    tol = err(d, x.double().abs() @ w.double().abs().t() + b.double().abs())
+    h, gu = ops.gated_linear_fwd(x, w, b, save=True)
+    torch.cuda.synchronize()
+    near(gu, gu64, tol, "gu")
+    a, da = act64("silu", gu64[:, :f])
+    u, eg, eu = gu64[:, f:], tol[:, :f], tol[:, f:]
+    near(h, a * u, (18 + 2 * gu64[:, :f].square()) * U * (a * u).abs() + (1.13 + eg) * eg * u.abs() + a.abs() * eu +
+         1.13 * eg * eu + 2e-5 * U * u.abs(), "h")
+    gate, up = gu.double().chunk(2, -1)
+    a, da = act64("silu", gate)
+    v = torch.cat((dh.double() * up * da, dh.double() * a), 1)
+    rel = (16 + 2 * gate * gate) * U
+    ev = torch.cat((rel * (dh.double() * up).abs() * (da.abs() + 0.3), rel * (dh.double() * (a.abs() + 1e-6)).abs()), 1)
+    dx, dw, db = ops.gated_linear_bwd(dh, x, w, gu)
+    torch.cuda.synchronize()
+    near(dx, v @ w.double(), ev @ w.double().abs() + err(2 * f, v.abs() @ w.double().abs()), "dx")
+    near(dw, v.t() @ x.double(), ev.t() @ x.double().abs() + err(m, v.abs().t() @ x.double().abs()), "dw")
+    near(db, v.sum(0), ev.sum(0) + (m / 64 + 96) * U * v.abs().sum(0), "db")
+    dw2 = torch.full_like(dw, 2.0)
+    ops.gated_linear_bwd(dh, x, w, gu, dw=dw2, need_dx=False, need_db=False, accumulate=True)
+    near(dw2, dw.double() + 2, 2 * U * (dw.double().abs() + 2), "dw accumulated")

@@ -4,7 +4,17 @@
 //             dx = [dg|du]·w, dw = [dg|du]ᵀ·x, db = Σ_rows [dg|du]
 // h is rounded once from fp32 pre-activations.  [dg|du] is rounded to bf16 for
 // dx (a bf16 output); dw is fp32, so there [dg|du] goes in as two bf16 pieces,
-// hi = bf16(v) and lo = bf16(v − hi) (2^-18 of v is lost, where one piece loses 2^-9).
+// hi = bf16(v) and lo = bf16(v − hi) (up to 2^-16 of v is lost, 2.7e-6 in the mean,
+// where one piece loses 2^-8 and 1.7e-3).
+//
+// fp32 layers take the bf16 matrix cores as well, wherever the products are large:
+// v = hi + mid + lo holds all 24 bits, and the six products of pieces that reach
+// 2^-23 of the whole (hi·hi, hi·mid, mid·hi, mid·mid, hi·lo, lo·hi) are summed in
+// fp32, the small ones first: six products, where the fp32 matrix instructions take
+// the time of sixteen, and no further from 64 bits than those (8192 rows of 1024 ->
+// 2048 422 us, 554 with fp32 instructions on tiles of the same engine; gradients 460
+// and 462 against 557 and 600).  An infinity comes out as NaN, and from 3.39e38 a value
+// counts as one.
 #include "gemm_dma.hpp"
 
 namespace {
@@ -81,8 +91,9 @@ struct GatedStore {
     int32_t act;
     bool vec;   // 16-byte stores fit every row
     static constexpr int E = 16 / (int)sizeof(T), C = 32 / E;   // a row's chunks
+    static constexpr int kRowBytes = 32 * (int)sizeof(T);
     static __device__ __forceinline__ int at(int row, int chunk) {
-        return row * 32 * (int)sizeof(T) + ((chunk ^ (sizeof(T) == 2 ? (row >> 1) & 3 : row & 7)) << 4);
+        return row * kRowBytes + ((chunk ^ (sizeof(T) == 2 ? (row >> 1) & 3 : row & 7)) << 4);
     }
     // Columns 8q + 4·hf + 0..3 of a row.
     static __device__ __forceinline__ void put(char NOTT_LDS* buf, int row, int q, int hf, const float (&v)[4]) {
@@ -171,12 +182,16 @@ struct GatedStore {
     }
 };
 
+// fp32, from bf16 pieces of x and w.
+struct GatedPieces : GatedStore<float> {
+    dma::Pieces pieces;
+};
+
 }  // namespace
 
-template <typename T>
-struct nott::gemm::dma::IsPaired<GatedStore<T>> {
-    static constexpr bool value = true;
-};
+template <> struct nott::gemm::dma::IsPaired<GatedStore<bf16_t>> { static constexpr bool value = true; };
+template <> struct nott::gemm::dma::IsPaired<GatedPieces> { static constexpr bool value = true; };
+template <> struct nott::gemm::dma::IsPieces<GatedPieces> { static constexpr bool value = true; };
 
 namespace {
 
@@ -200,16 +215,26 @@ __global__ __launch_bounds__(256) void gated_act_kernel(const float* __restrict_
     }
 }
 
-// [dg|du] in rows of ld elements as T, in bf16 also what its rounding leaves (lo),
-// and zeros past 2f.  A workgroup takes 64·E columns (E = 1, or whole 16-byte chunks
-// where all rows fit them and ld is 2f) and every gridDim.y-th group of 4 rows;
-// partial (null: no db) [gridDim.y][2f] receives its column sums of the unrounded
+// E fp32 values as bf16 (E = 1, 4 or 8; aligned to E elements).
+template <int E>
+__device__ __forceinline__ void store_piece(bf16_t* p, const float (&v)[E]) {
+    if constexpr (E == 8) Pack16<bf16_t>::st(p, v);
+    else if constexpr (E == 4) Vec4<bf16_t>::st(p, f32x4{v[0], v[1], v[2], v[3]});
+    else *p = f32_to_bf16(v[0]);
+}
+
+// [dg|du] in rows of ld elements with zeros past 2f: as fp32 (whole, the generic
+// engine's operand) and as bf16 pieces, each `stride` elements behind the one before
+// and the rounding of what that leaves.  A workgroup takes 64·E columns (E = 1, or
+// whole 16-byte chunks where all rows fit them and ld is 2f) and every gridDim.y-th
+// group of 4 rows; partial (null: no db) [gridDim.y][2f] receives its column sums of the unrounded
 // values.  Bound by memory: 8192 x 4096 bf16 with both pieces, 470 MB, 74 us (6.3 TB/s;
 // 94 an element at a time).
 template <typename T, int ACT, int E>
 __global__ __launch_bounds__(256) void gated_dact_kernel(const T* __restrict__ dh, const T* __restrict__ gu, int64_t m,
-                                                         int64_t f, int64_t ld, T* __restrict__ hi,
-                                                         T* __restrict__ lo, float* __restrict__ partial) {
+                                                         int64_t f, int64_t ld, float* __restrict__ whole,
+                                                         bf16_t* __restrict__ out, int pieces, int64_t stride,
+                                                         float* __restrict__ partial) {
     __shared__ float red[2][4][64 * E];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * E;
@@ -220,9 +245,16 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const T* __restrict__ d
         if constexpr (E == 1) v[0] = Io<T>::ld(p, 0);
         else Pack16<T>::ld(p, v);
     };
-    auto store = [](T* p, const float (&v)[E]) {
-        if constexpr (E == 1) Io<T>::st(p, 0, v[0]);
-        else Pack16<T>::st(p, v);
+    auto store = [&](int64_t at, float (&v)[E]) {
+        if (whole) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) whole[at + e] = v[e];
+        }
+        for (int p = 0; p < pieces; ++p) {
+            store_piece<E>(out + p * stride + at, v);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] -= bf16_to_f32(f32_to_bf16(v[e]));
+        }
     };
     if (c < f) {
         for (int64_t r = (int64_t)blockIdx.y * 4 + wid; r < m; r += (int64_t)gridDim.y * 4) {
@@ -239,23 +271,12 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const T* __restrict__ d
                 sg[e] += dg[e];
                 su[e] += du[e];
             }
-            store(hi + r * ld + c, dg);
-            store(hi + r * ld + f + c, du);
-            if constexpr (sizeof(T) == 2) {
-                if (lo) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        dg[e] -= bf16_to_f32(f32_to_bf16(dg[e]));
-                        du[e] -= bf16_to_f32(f32_to_bf16(du[e]));
-                    }
-                    store(lo + r * ld + c, dg);
-                    store(lo + r * ld + f + c, du);
-                }
-            }
+            store(r * ld + c, dg);
+            store(r * ld + f + c, du);
             if constexpr (E == 1) {
                 for (int64_t j = 2 * f + c; j < ld; j += f) {
-                    hi[r * ld + j] = T(0);
-                    if (lo) lo[r * ld + j] = T(0);
+                    float none[1] = {0.f};
+                    store(r * ld + j, none);
                 }
             }
         }
@@ -302,20 +323,19 @@ struct AccStore {
         *p = accumulate ? *p + v : v;
     }
 };
-// The same, and its split-K partials, for the product of both pieces of [dg|du]
-// (stacked along k) with x twice.
+// The same, and its split-K partials, for products of pieces.
 struct PiecesStore : AccStore {
-    int64_t wrap;
+    dma::Pieces pieces;
 };
 struct PiecesPartial : dma::PartialRowStore {
-    int64_t wrap;
+    dma::Pieces pieces;
 };
-__device__ __forceinline__ PiecesPartial at_split(const PiecesPartial& ep, int z) { return {ep.at(z), ep.wrap}; }
+__device__ __forceinline__ PiecesPartial at_split(const PiecesPartial& ep, int z) { return {ep.at(z), ep.pieces}; }
 
 }  // namespace
 
-template <> struct nott::gemm::dma::IsWrapped<PiecesStore> { static constexpr bool value = true; };
-template <> struct nott::gemm::dma::IsWrapped<PiecesPartial> { static constexpr bool value = true; };
+template <> struct nott::gemm::dma::IsPieces<PiecesStore> { static constexpr bool value = true; };
+template <> struct nott::gemm::dma::IsPieces<PiecesPartial> { static constexpr bool value = true; };
 
 namespace {
 
@@ -324,32 +344,33 @@ template <typename T>
 bool ok16(const T* p, int64_t ld) {
     return (uintptr_t)p % 16 == 0 && ld * (int64_t)sizeof(T) % 16 == 0;
 }
-// n rounded up to whole 16-byte chunks.
-template <typename T>
-int64_t chunks_up(int64_t n) {
-    constexpr int64_t E = 16 / (int64_t)sizeof(T);
-    return (n + E - 1) / E * E;
-}
+// n rounded up to whole 16-byte chunks of bf16.
+int64_t up8(int64_t n) { return (n + 7) & ~int64_t(7); }
 
-// A copy of src [rows, cols] with zeros up to [prows, pcols], for tensors whose rows
-// no 16-byte load fits (the copy is small beside the product it is for).
+// src [rows, cols] as `pieces` bf16 pieces [prows, pcols] with zeros past it, each the
+// rounding of what the ones before leave: the copy of a bf16 tensor whose rows no
+// 16-byte load fits, and an fp32 tensor for the bf16 engine.
 template <typename T>
-__global__ __launch_bounds__(256) void pad_kernel(const T* __restrict__ src, int64_t rows, int64_t cols,
-                                                  T* __restrict__ dst, int64_t prows, int64_t pcols) {
-    constexpr int E = 16 / (int)sizeof(T);
-    const int64_t n = prows * pcols / E;
+__global__ __launch_bounds__(256) void pieces_kernel(const T* __restrict__ src, int64_t rows, int64_t cols,
+                                                     bf16_t* __restrict__ dst, int64_t prows, int64_t pcols, int pieces) {
+    const int64_t n = prows * pcols / 8;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i * E / pcols, c = i * E - r * pcols;
-        T v[E];
+        const int64_t r = i * 8 / pcols, c = i * 8 - r * pcols;
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = r < rows && c + e < cols ? src[r * cols + c + e] : T(0);
-        *reinterpret_cast<u32x4*>(dst + i * E) = Pack<T>::make(v);
+        for (int e = 0; e < 8; ++e) v[e] = r < rows && c + e < cols ? Io<T>::ld(src, r * cols + c + e) : 0.f;
+        for (int p = 0; p < pieces; ++p) {
+            Pack16<bf16_t>::st(dst + p * prows * pcols + i * 8, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] -= bf16_to_f32(f32_to_bf16(v[e]));
+        }
     }
 }
 template <typename T>
-void pad(nott_ctx ctx, const T* src, int64_t rows, int64_t cols, T* dst, int64_t prows, int64_t pcols) {
-    hipLaunchKernelGGL(pad_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(prows * pcols, 2048), 8192)), dim3(256), 0,
-                       ctx->stream, src, rows, cols, dst, prows, pcols);
+void to_pieces(nott_ctx ctx, const T* src, int64_t rows, int64_t cols, bf16_t* dst, int64_t prows, int64_t pcols,
+               int pieces) {
+    hipLaunchKernelGGL(pieces_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(prows * pcols, 2048), 8192)), dim3(256),
+                       0, ctx->stream, src, rows, cols, dst, prows, pcols, pieces);
 }
 
 // 16 bytes from any element's address.
@@ -489,96 +510,80 @@ int product(nott_ctx ctx, const T* A, int64_t lda, const T* B, int64_t ldb, cons
     else return go(RowKLoader<T>{A, lda, M, K, vec(A, lda)}, RowKLoader<T>{B, ldb, N, K, vec(B, ldb)});
 }
 
-// The fp32 engines' estimated times (us).  Direct-to-LDS tiles: their MFMA time at
-// the rate they reach, in whole rounds of the CUs' tiles, splits' partials included;
-// the generic engine: its rate with any split.
-struct Plan32 {
-    int bm;   // tiles of 128×128, two workgroups a CU, or 256×128, one
-    int64_t splits, kps;
-    double us;
-};
-Plan32 plan32(nott_ctx ctx, int64_t M, int64_t N, int64_t K, bool split) {
-    constexpr double kFlopUs = 0.75 * 157.3e6 / 256;   // a CU's, reached
-    const int64_t stages = ceil_div(K, dma::kStageK<float>);
-    Plan32 best{128, 1, K, 0};
-    for (const int bm : {128, 256}) {
-        const int64_t tiles = ceil_div(M, bm) * ceil_div(N, 128);
-        for (int64_t n = 1; n <= (split ? 16 : 1) && (n == 1 || stages / n >= 4); n *= 2) {
-            const int64_t per = ceil_div(stages, n), splits = ceil_div(stages, per);
-            double us = 3 + (double)ceil_div(tiles * splits, ctx->num_cu) * (double)per * (bm * 128 * 64.0) / kFlopUs;
-            if (splits > 1) us += 2 + 8.0 * (double)(splits * M * N) / 5.9e6;
-            if (best.us == 0 || us <= best.us)   // of equals the larger tile: 116 us against 123 at 1576 x 768 -> 2048
-                best = {bm, splits, splits > 1 ? per * dma::kStageK<float> : K, us};
-        }
-    }
-    return best;
-}
-template <bool AT, bool BT, class EP>
-int launch32(nott_ctx ctx, const Plan32& p, const float* A, int64_t lda, const float* B, int64_t ldb, const EP& ep,
-             int64_t M, int64_t N, int64_t K) {
-    if (p.bm == 256)
-        return dma::launch<dma::Config<AT, BT, 256, 128, 4, 2, 3>, false>(ctx, A, lda, B, ldb, ep, M, N, K, p.splits, p.kps);
-    return dma::launch<dma::Config<AT, BT, 128, 128, 2, 2, 2>, false>(ctx, A, lda, B, ldb, ep, M, N, K, p.splits, p.kps);
-}
-// Whether an fp32 product goes to the generic engine, which spreads few tiles over
-// the CUs by splitting k and runs at `rate` TFLOP/s.  1576 rows of 768 → 2048: forward
-// 118 us on the direct-to-LDS tiles against 163, dx 143 against 168, dw 145 against
-// 139; 512 rows of 1024 → 2048: forward 73 against 50.
-bool generic32(double us, int64_t M, int64_t N, int64_t K, double rate) {
-    return 6 + 2.0 * (double)M * (double)N * (double)K / (rate * 1e6) < us;
+// The six products of fp32 pieces (hi 0, mid 1, lo 2), first factor and second.
+constexpr uint32_t kPairs = 6, kFirst = 0x001102, kSecond = 0x010120;
+
+// Whether an fp32 product of M×N×K, with so many elements to split into pieces, goes to
+// the direct-to-LDS engine: its plan's time and the split's, a quarter more than in
+// bf16 layers (every bit of the pieces is busy), against the generic engine's 75
+// TFLOP/s, which spreads few tiles over the CUs by splitting k.  In us, generic and
+// pieces (forward; dx and dw with the activation gradient): 1576 rows of 768 -> 2048 163
+// and 98, 170 and 103, 139 and 109; 1024 of 768 -> 1024 45 and 65, 64 and 52, 60 and 50;
+// 256 of 512 -> 1024 19 and 43, 22 and 31, 24 and 31.  On 20 sizes of 100 to 16384 rows
+// the choice is the better one or within 15% of it.
+bool takes_pieces(nott_ctx ctx, int64_t M, int64_t N, int64_t K, bool both_tr, bool split, int64_t elements) {
+    const double us = dma::plan(ctx, M, N, kPairs * ceil_div(K, dma::BK) * dma::BK, both_tr, false, split ? 0 : 1).us;
+    return 1.25 * (us + 4 + (double)elements / 5e5) < 6 + 2.0 * (double)M * (double)N * (double)K / 75e6 &&
+           ceil_div(M, 128) * ceil_div(N, 64) < (int64_t)1 << 23;
 }
 
-template <typename T>
-int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const T* x, const T* w, const float* b, T* h, T* gu) {
-    const int64_t dp = chunks_up<T>(d);
-    typename std::conditional<sizeof(T) == 2, dma::Plan, Plan32>::type p;
-    bool rows = false;
-    if constexpr (sizeof(T) == 2) {
-        rows = takes_rows(ctx, m, d, f, !ok16(w, d));
-        if (rows && d >= 8) return forward_rows(ctx, m, d, f, act, x, w, b, h, gu);
-        p = dma::plan(ctx, m, 2 * f, dp, false, false, 1);
-    } else {
-        p = plan32(ctx, m, 2 * f, dp, false);
-        if (generic32(p.us, m, 2 * f, d, 70)) {
-            WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * 2 * f));
-            if (ws.failed()) return NOTT_ERR_ALLOC;
-            float* pre = reinterpret_cast<float*>(ws.p);
-            const RowMajorStore<float> ep{pre, 2 * f, m, 2 * f, nullptr};
-            const int st = product<float, false, false>(ctx, x, d, w, d, ep, m, 2 * f, d);
-            if (st != NOTT_OK) return st;
-            with_act(act, [&](auto a) {
-                hipLaunchKernelGGL((gated_act_kernel<decltype(a)::value>),
-                                   dim3((unsigned)ceil_div(f, 256), (unsigned)std::min<int64_t>(m, 65535)), dim3(256), 0,
-                                   ctx->stream, pre, b, m, f, h, gu);
-            });
-            return launch_status(ctx, "gated_linear");
-        }
-    }
+int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* x, const bf16_t* w, const float* b,
+        bf16_t* h, bf16_t* gu) {
+    const int64_t dp = up8(d);
+    const bool rows = takes_rows(ctx, m, d, f, !ok16(w, d));
+    if (rows && d >= 8) return forward_rows(ctx, m, d, f, act, x, w, b, h, gu);
     NOTT_REQUIRE(ctx, ceil_div(m, 128) * ceil_div(f, 64) < (int64_t)1 << 26, "nott_gated_linear_fwd: too large");
     const bool pad_x = !ok16(x, d), pad_w = !ok16(w, d);
-    WorkspaceHold ws(ctx, sizeof(T) * (size_t)(((pad_x ? m : 0) + (pad_w ? 2 * f : 0)) * dp));
+    WorkspaceHold ws(ctx, sizeof(bf16_t) * (size_t)(((pad_x ? m : 0) + (pad_w ? 2 * f : 0)) * dp));
     if (ws.failed()) return NOTT_ERR_ALLOC;
-    T* xp = reinterpret_cast<T*>(ws.p);
-    T* wp = xp + (pad_x ? m * dp : 0);
-    if (pad_x) pad(ctx, x, m, d, xp, m, dp);
-    if (pad_w) pad(ctx, w, 2 * f, d, wp, 2 * f, dp);
-    const T* X = pad_x ? xp : x;
-    const T* W = pad_w ? wp : w;
-    if constexpr (sizeof(T) == 2)
-        if (rows) return forward_rows(ctx, m, dp, f, act, X, W, b, h, gu);
-    const GatedStore<T> ep{h, gu, b, m, f, act, ok16(h, f) && ok16(gu, f)};
-    if constexpr (sizeof(T) == 2)
-        return dma::launch_shape<false, false, false>(ctx, p.shape, X, dp, W, dp, ep, m, 2 * f, dp, 1, dp);
-    else
-        return launch32<false, false>(ctx, p, X, dp, W, dp, ep, m, 2 * f, dp);
+    bf16_t* xp = reinterpret_cast<bf16_t*>(ws.p);
+    bf16_t* wp = xp + (pad_x ? m * dp : 0);
+    if (pad_x) to_pieces(ctx, x, m, d, xp, m, dp, 1);
+    if (pad_w) to_pieces(ctx, w, 2 * f, d, wp, 2 * f, dp, 1);
+    const bf16_t* X = pad_x ? xp : x;
+    const bf16_t* W = pad_w ? wp : w;
+    if (rows) return forward_rows(ctx, m, dp, f, act, X, W, b, h, gu);
+    const GatedStore<bf16_t> ep{h, gu, b, m, f, act, ok16(h, f) && ok16(gu, f)};
+    const dma::Plan p = dma::plan(ctx, m, 2 * f, dp, false, false, 1);
+    return dma::launch_shape<false, false, false>(ctx, p.shape, X, dp, W, dp, ep, m, 2 * f, dp, 1, dp);
 }
 
-// [dg|du] in rows of ld elements (zeros past 2·f) to hi, and lo (bf16, nullable); db.
+int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* x, const float* w, const float* b, float* h,
+        float* gu) {
+    const int64_t dp = up8(d);
+    if (!takes_pieces(ctx, m, 2 * f, dp, false, false, (m + 2 * f) * dp)) {
+        WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * 2 * f));
+        if (ws.failed()) return NOTT_ERR_ALLOC;
+        float* pre = reinterpret_cast<float*>(ws.p);
+        const RowMajorStore<float> ep{pre, 2 * f, m, 2 * f, nullptr};
+        const int st = product<float, false, false>(ctx, x, d, w, d, ep, m, 2 * f, d);
+        if (st != NOTT_OK) return st;
+        with_act(act, [&](auto a) {
+            hipLaunchKernelGGL((gated_act_kernel<decltype(a)::value>),
+                               dim3((unsigned)ceil_div(f, 256), (unsigned)std::min<int64_t>(m, 65535)), dim3(256), 0,
+                               ctx->stream, pre, b, m, f, h, gu);
+        });
+        return launch_status(ctx, "gated_linear");
+    }
+    WorkspaceHold ws(ctx, 3 * sizeof(bf16_t) * (size_t)((m + 2 * f) * dp));
+    if (ws.failed()) return NOTT_ERR_ALLOC;
+    bf16_t* xp = reinterpret_cast<bf16_t*>(ws.p);
+    bf16_t* wp = xp + 3 * m * dp;
+    to_pieces(ctx, x, m, d, xp, m, dp, 3);
+    to_pieces(ctx, w, 2 * f, d, wp, 2 * f, dp, 3);
+    const int64_t deep = kPairs * ceil_div(dp, dma::BK) * dma::BK;
+    const dma::Plan p = dma::plan(ctx, m, 2 * f, deep, false, false, 1);
+    const GatedPieces ep{{h, gu, b, m, f, act, ok16(h, f) && ok16(gu, f)},
+                         dma::pieces(kPairs, kFirst, kSecond, m * dp, 2 * f * dp, dp)};
+    return dma::launch_shape<false, false, false>(ctx, p.shape, xp, dp, wp, dp, ep, m, 2 * f, dp, 1, deep);
+}
+
+// [dg|du] in rows of ld elements (zeros past 2·f), whole or as pieces (gated_dact_kernel); db.
 template <typename T>
-int activation_bwd(nott_ctx ctx, int64_t m, int64_t f, int64_t ld, int act, const T* dh, const T* gu, T* hi, T* lo,
-                   float* db, int accumulate) {
+int activation_bwd(nott_ctx ctx, int64_t m, int64_t f, int64_t ld, int act, const T* dh, const T* gu, float* whole,
+                   bf16_t* out, int pieces, float* db, int accumulate) {
     constexpr int E = 16 / (int)sizeof(T);
-    const bool vec = ld == 2 * f && f >= 64 * E && ok16(dh, f) && ok16(gu, f) && ok16(hi, f) && ok16(lo, f);
+    const bool vec = ld == 2 * f && f >= 64 * E && ok16(dh, f) && ok16(gu, f);
     // about eight workgroups a CU, of at least 4 rows; fewer where each leaves sums for db
     const int64_t columns = ceil_div(f, 64 * (vec ? E : 1));
     const int64_t slabs = std::max<int64_t>(1, std::min<int64_t>({ceil_div(8 * (int64_t)ctx->num_cu, columns), ceil_div(m, 4),
@@ -592,7 +597,7 @@ int activation_bwd(nott_ctx ctx, int64_t m, int64_t f, int64_t ld, int act, cons
         constexpr int A = decltype(a)::value;
         auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)columns, (unsigned)slabs), dim3(256), 0, ctx->stream, dh, gu, m, f, ld,
-                               hi, lo, partial);
+                               whole, out, pieces, m * ld, partial);
         };
         if (vec) go(gated_dact_kernel<T, A, E>);
         else go(gated_dact_kernel<T, A, 1>);
@@ -603,23 +608,43 @@ int activation_bwd(nott_ctx ctx, int64_t m, int64_t f, int64_t ld, int act, cons
     return launch_status(ctx, "gated_linear backward");
 }
 
+// ep's M×N = Σ over the pairs of pieces, K deep each, rows and columns of A and B in
+// whole chunks.
+template <bool AT, bool BT>
+int pieces_product(nott_ctx ctx, const bf16_t* A, int64_t lda, const bf16_t* B, int64_t ldb, const AccStore& ep,
+                   const dma::Pieces& pc, int64_t M, int64_t N, int64_t K) {
+    const int64_t deep = pc.count * ceil_div(K, dma::BK) * dma::BK;
+    dma::Plan p = dma::plan(ctx, M, N, deep, AT && BT, false, 0);
+    float* part = nullptr;
+    if (p.splits > 1) {
+        part = static_cast<float*>(nott::optional_workspace(ctx, sizeof(float) * (size_t)(p.splits * M * N)));
+        if (!part) p = dma::plan(ctx, M, N, deep, AT && BT, false, 1);
+    }
+    if (!part)
+        return dma::launch_shape<AT, BT, false>(ctx, p.shape, A, lda, B, ldb, PiecesStore{ep, pc}, M, N, K, 1, deep);
+    const int st = dma::launch_shape<AT, BT, false>(ctx, p.shape, A, lda, B, ldb,
+                                                    PiecesPartial{{part, nullptr, M, N}, pc}, M, N, K, p.splits, p.kps);
+    if (st != NOTT_OK) return st;
+    launch_splitk_reduce(ctx, part, p.splits, M, N, ep);
+    return launch_status(ctx, "gated_linear splits");
+}
+
 int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* dh, const bf16_t* x, const bf16_t* w,
         const bf16_t* gu, bf16_t* dx, float* dw, float* db, int accumulate) {
-    const int64_t dp = chunks_up<bf16_t>(d), fp = chunks_up<bf16_t>(2 * f);
+    const int64_t dp = up8(d), fp = up8(2 * f);
     // the direct-to-LDS engine, where a product has its 128 rows and columns
     const bool dma_dx = dx && m >= 128 && d >= 128, dma_dw = dw && 2 * f >= 128 && d >= 128;
     const bool pad_x = dma_dw && !ok16(x, d), pad_w = dma_dx && (!ok16(w, d) || fp != 2 * f);
-    const size_t piece = sizeof(bf16_t) * (size_t)(m * fp);
-    WorkspaceHold ws(ctx, piece * (dw ? 2 : 1) + sizeof(bf16_t) * (size_t)(((pad_x ? m : 0) + (pad_w ? fp : 0)) * dp));
+    WorkspaceHold ws(ctx, sizeof(bf16_t) * (size_t)(m * fp * (dw ? 2 : 1) + ((pad_x ? m : 0) + (pad_w ? fp : 0)) * dp));
     if (ws.failed()) return NOTT_ERR_ALLOC;
     bf16_t* hi = reinterpret_cast<bf16_t*>(ws.p);
-    bf16_t* lo = dw ? hi + m * fp : nullptr;
-    int st = activation_bwd(ctx, m, f, fp, act, dh, gu, hi, lo, db, accumulate);
-    if (st != NOTT_OK) return st;
+    bf16_t* lo = hi + m * fp;
     bf16_t* xp = hi + m * fp * (dw ? 2 : 1);
     bf16_t* wp = xp + (pad_x ? m * dp : 0);
-    if (pad_x) pad(ctx, x, m, d, xp, m, dp);
-    if (pad_w) pad(ctx, w, 2 * f, d, wp, fp, dp);
+    int st = activation_bwd(ctx, m, f, fp, act, dh, gu, nullptr, hi, dw ? 2 : 1, db, accumulate);
+    if (st != NOTT_OK) return st;
+    if (pad_x) to_pieces(ctx, x, m, d, xp, m, dp, 1);
+    if (pad_w) to_pieces(ctx, w, 2 * f, d, wp, fp, dp, 1);
     if (dx) {
         const RowMajorStore<bf16_t> ep{dx, d, m, d, nullptr};
         st = dma_dx ? dma::run<false, true>(ctx, hi, fp, pad_w ? wp : w, dp, ep, m, dp, fp)
@@ -632,66 +657,40 @@ int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* dh
         if (st != NOTT_OK) return st;
         return product<bf16_t, true, true>(ctx, lo, fp, x, d, AccStore{dw, 2 * f, d, 1}, 2 * f, d, m);
     }
-    // one product over both pieces, 2·m deep
-    const bf16_t* X = pad_x ? xp : x;
-    dma::Plan p = dma::plan(ctx, fp, dp, 2 * m, true, false, 0);
-    float* part = nullptr;
-    if (p.splits > 1) {
-        part = static_cast<float*>(nott::optional_workspace(ctx, sizeof(float) * (size_t)(p.splits * fp * dp)));
-        if (!part) p = dma::plan(ctx, fp, dp, 2 * m, true, false, 1);
-    }
-    const PiecesStore ep{{dw, 2 * f, d, accumulate}, m};
-    if (!part) return dma::launch_shape<true, true, false>(ctx, p.shape, hi, fp, X, dp, ep, fp, dp, 2 * m, 1, p.kps);
-    st = dma::launch_shape<true, true, false>(ctx, p.shape, hi, fp, X, dp, PiecesPartial{{part, nullptr, fp, dp}, m}, fp, dp,
-                                              2 * m, p.splits, p.kps);
-    if (st != NOTT_OK) return st;
-    launch_splitk_reduce(ctx, part, p.splits, fp, dp, static_cast<const AccStore&>(ep));
-    return launch_status(ctx, "gated_linear dw");
-}
-
-// C = A·B in fp32 on the direct-to-LDS engine, as planned.
-template <bool AT, bool BT, class EP>
-int product32(nott_ctx ctx, Plan32 p, const float* A, int64_t lda, const float* B, int64_t ldb, const EP& ep, int64_t M,
-              int64_t N, int64_t K) {
-    float* part = nullptr;
-    if (p.splits > 1) {
-        part = static_cast<float*>(nott::optional_workspace(ctx, sizeof(float) * (size_t)(p.splits * M * N)));
-        if (!part) p = plan32(ctx, M, N, K, false);
-    }
-    if (!part) return launch32<AT, BT>(ctx, p, A, lda, B, ldb, ep, M, N, K);
-    const int st = launch32<AT, BT>(ctx, p, A, lda, B, ldb, dma::PartialRowStore{part, nullptr, M, N}, M, N, K);
-    if (st != NOTT_OK) return st;
-    launch_splitk_reduce(ctx, part, p.splits, M, N, ep);
-    return launch_status(ctx, "gated_linear splits");
+    // lo·x, then hi·x
+    return pieces_product<true, true>(ctx, hi, fp, pad_x ? xp : x, dp, AccStore{dw, 2 * f, d, accumulate},
+                                      dma::pieces(2, 0x01, 0x00, m * fp, 0, m), fp, dp, m);
 }
 
 int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* dh, const float* x, const float* w,
         const float* gu, float* dx, float* dw, float* db, int accumulate) {
-    const int64_t dp = chunks_up<float>(d), fp = chunks_up<float>(2 * f);
-    const Plan32 px = plan32(ctx, m, dp, fp, true), pw = plan32(ctx, fp, dp, m, true);
-    const bool dma_dx = dx && !generic32(px.us, m, d, 2 * f, 65), dma_dw = dw && !generic32(pw.us, 2 * f, d, m, 85);
-    const bool pad_x = dma_dw && !ok16(x, d), pad_w = dma_dx && (!ok16(w, d) || fp != 2 * f);
-    WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * fp + ((pad_x ? m : 0) + (pad_w ? fp : 0)) * dp));
+    const int64_t dp = up8(d), fp = up8(2 * f);
+    const bool pieces_dx = dx && takes_pieces(ctx, m, dp, fp, false, true, fp * dp);
+    const bool pieces_dw = dw && takes_pieces(ctx, fp, dp, m, true, true, m * dp);
+    const bool pieces = pieces_dx || pieces_dw, whole = (dx && !pieces_dx) || (dw && !pieces_dw);
+    const int64_t ld = pieces ? fp : 2 * f;
+    WorkspaceHold ws(ctx, sizeof(float) * (size_t)(whole ? m * ld : 0) +
+                              3 * sizeof(bf16_t) * (size_t)((pieces ? m * fp : 0) + ((pieces_dw ? m : 0) + (pieces_dx ? fp : 0)) * dp));
     if (ws.failed()) return NOTT_ERR_ALLOC;
-    float* dgu = reinterpret_cast<float*>(ws.p);
-    float* xp = dgu + m * fp;
-    float* wp = xp + (pad_x ? m * dp : 0);
-    int st = activation_bwd<float>(ctx, m, f, fp, act, dh, gu, dgu, nullptr, db, accumulate);
+    bf16_t* dgu = reinterpret_cast<bf16_t*>(ws.p);
+    bf16_t* xp = dgu + (pieces ? 3 * m * fp : 0);
+    bf16_t* wp = xp + (pieces_dw ? 3 * m * dp : 0);
+    float* all = reinterpret_cast<float*>(wp + (pieces_dx ? 3 * fp * dp : 0));
+    int st = activation_bwd(ctx, m, f, ld, act, dh, gu, whole ? all : nullptr, dgu, pieces ? 3 : 0, db, accumulate);
     if (st != NOTT_OK) return st;
-    if (pad_x) pad(ctx, x, m, d, xp, m, dp);
-    if (pad_w) pad(ctx, w, 2 * f, d, wp, fp, dp);
-    if (dx) {
-        const AccStore ep{dx, m, d, 0};
-        st = dma_dx ? product32<false, true>(ctx, px, dgu, fp, pad_w ? wp : w, dp, ep, m, dp, fp)
-                    : product<float, false, true>(ctx, dgu, fp, w, d, ep, m, d, 2 * f);
-        if (st != NOTT_OK) return st;
+    const AccStore to_dx{dx, m, d, 0}, to_dw{dw, 2 * f, d, accumulate};
+    if (pieces_dx) {
+        to_pieces(ctx, w, 2 * f, d, wp, fp, dp, 3);
+        st = pieces_product<false, true>(ctx, dgu, fp, wp, dp, to_dx, dma::pieces(kPairs, kFirst, kSecond, m * fp, fp * dp, fp),
+                                         m, dp, fp);
+    } else if (dx) {
+        st = product<float, false, true>(ctx, all, ld, w, d, to_dx, m, d, 2 * f);
     }
-    if (dw) {
-        const AccStore ep{dw, 2 * f, d, accumulate};
-        st = dma_dw ? product32<true, true>(ctx, pw, dgu, fp, pad_x ? xp : x, dp, ep, fp, dp, m)
-                    : product<float, true, true>(ctx, dgu, fp, x, d, ep, 2 * f, d, m);
-    }
-    return st;
+    if (st != NOTT_OK || !dw) return st;
+    if (!pieces_dw) return product<float, true, true>(ctx, all, ld, x, d, to_dw, 2 * f, d, m);
+    to_pieces(ctx, x, m, d, xp, m, dp, 3);
+    return pieces_product<true, true>(ctx, dgu, fp, xp, dp, to_dw, dma::pieces(kPairs, kFirst, kSecond, m * fp, m * dp, m), fp,
+                                      dp, m);
 }
 
 }  // namespace
@@ -706,9 +705,9 @@ extern "C" int nott_gated_linear_fwd(nott_ctx ctx, nott_dtype dtype, int64_t m, 
     NOTT_REQUIRE(ctx, x && w && h, "nott_gated_linear_fwd: null buffer");
     nott::DeviceScope scope(ctx->device);
     if (dtype == NOTT_F32)
-        return fwd<float>(ctx, m, d, f, act, static_cast<const float*>(x), static_cast<const float*>(w), b,
+        return fwd(ctx, m, d, f, act, static_cast<const float*>(x), static_cast<const float*>(w), b,
                           static_cast<float*>(h), static_cast<float*>(gu));
-    return fwd<bf16_t>(ctx, m, d, f, act, static_cast<const bf16_t*>(x), static_cast<const bf16_t*>(w), b,
+    return fwd(ctx, m, d, f, act, static_cast<const bf16_t*>(x), static_cast<const bf16_t*>(w), b,
                        static_cast<bf16_t*>(h), static_cast<bf16_t*>(gu));
 }
 

@@ -1,7 +1,6 @@
-// MFMA GEMM with direct-to-LDS operand fills (gfx950), for bf16 operands and (the
-// gated linear layer's) fp32 ones.
+// bf16 MFMA GEMM with direct-to-LDS operand fills (gfx950).
 //
-//   C[M×N] = Σ_k A(m, k)·B(n, k),  fp32 accumulate:
+//   C[M×N] = Σ_k A(m, k)·B(n, k),  fp32 accumulate, bf16 operands:
 //   A(m, k) = A[m·lda + k]  (AT = false)   or   A[k·lda + m]  (AT = true)
 //   B(n, k) = B[n·ldb + k]  (BT = false)   or   B[k·ldb + n]  (BT = true)
 //
@@ -23,11 +22,6 @@
 //     operands are read with ds_read_b64_tr_b16, which hands lane i of each
 //     16-lane group the 4 k-consecutive values of row i from a [k][row]
 //     block, i.e. the MFMA operand layout, so no transpose is ever stored.
-// fp32: the same stages of 128 bytes of k per row (32 k's, v_mfma_f32_32x32x2_f32).
-// A slice is 8 k's: lanes 0..31 hold k = 0..3 of their row, lanes 32..63 k = 4..7, for
-// the slice's four MFMAs one after the other (both operands alike); a
-// row-contiguous operand is read element by element, 32 rows side by side, and
-// needs no swizzle.
 // Stages form an S-deep ring: the loads of stage t+S-1 go into the slot of
 // stage t-1 once every wave has passed the barrier that follows its last read
 // of it, so S-1 stages are in flight while one is multiplied.  A 3-deep ring
@@ -54,8 +48,7 @@ namespace nott {
 namespace gemm {
 namespace dma {
 
-constexpr int BK = 64;   // k's of a stage, bf16
-template <typename T> constexpr int kStageK = 128 / (int)sizeof(T);
+constexpr int BK = 64;
 
 using lds::barrier;
 using lds::dma16;
@@ -65,23 +58,22 @@ using lds::wait_vm_lgkm0;
 // Issues block qq of this wave's share of one operand tile (R rows × 64 k, its
 // NB = R/8 1 KB blocks dealt to the NW waves in turn) of stage k0.  Rows past
 // `rows` are clamped to the last row (their results are never stored);
-// row-contiguous operands need rows in whole 16-byte chunks, one at least.  TAIL: the
-// stage may reach past K; its 16-byte chunks from K on (a k-contiguous operand's K is
-// whole chunks) are filled with zeros.
+// row-contiguous operands need rows % 8 == 0 and rows >= 8.  TAIL: the stage
+// may reach past K; its 16-byte chunks from K on (a k-contiguous operand's K is
+// a multiple of 8) are filled with zeros.
 static __device__ u32x4 zero_chunk;
 
 //
 // PAIR (k-contiguous): the operand is two stacked halves of rows/2 rows, and the
 // tile takes 32 rows of the first, the same 32 of the second, the next 32, ...
-// wrap (row-contiguous, nonzero): the operand's k-rows from `wrap` on are those from 0 on.
-template <bool TR, int R, int NW, bool TAIL, bool PAIR = false, typename T>
-__device__ __forceinline__ void fill_block(int qq, const T* __restrict__ p, int64_t ld, int64_t row0,
+template <bool TR, int R, int NW, bool TAIL, bool PAIR = false>
+__device__ __forceinline__ void fill_block(int qq, const bf16_t* __restrict__ p, int64_t ld, int64_t row0,
                                            int64_t rows, int64_t k0, int64_t K, char NOTT_LDS* dst, int wid,
-                                           int lane, int64_t wrap = 0) {
-    constexpr int NB = R / 8, E = 16 / (int)sizeof(T);
+                                           int lane) {
+    constexpr int NB = R / 8;
     static_assert(NB % NW == 0, "tile blocks must split evenly over the waves");
     const int q = qq * NW + wid;
-    const T* src;
+    const bf16_t* src;
     if constexpr (!TR) {
         const int r = 8 * q + (lane >> 3);
         const int c = (lane & 7) ^ ((r >> 1) & 7);
@@ -94,19 +86,18 @@ __device__ __forceinline__ void fill_block(int qq, const T* __restrict__ p, int6
             gr = row0 + r;
             gr = gr < rows ? gr : rows - 1;
         }
-        src = p + gr * ld + k0 + E * c;
-        if (TAIL && k0 + E * c >= K) src = reinterpret_cast<const T*>(&zero_chunk);
+        src = p + gr * ld + k0 + 8 * c;
+        if (TAIL && k0 + 8 * c >= K) src = reinterpret_cast<const bf16_t*>(&zero_chunk);
     } else {
-        constexpr int RB = R * (int)sizeof(T);   // bytes of a k-row
-        static_assert(RB >= 256 && RB <= 1024, "a block holds whole k-rows of at least 256 bytes");
-        constexpr int KPB = 1024 / RB;   // k-rows per block
+        static_assert(R >= 128, "row-contiguous tiles need at least 128 rows");
+        constexpr int KPB = 1024 / (2 * R);   // k-rows per block
         const int b = 16 * lane;
-        const int k = q * KPB + b / RB;
-        const int cr = ((b % RB) >> 4) ^ (sizeof(T) == 2 ? (k & 3) << 2 : 0);
-        int64_t gc = row0 + E * cr;
-        gc = gc <= rows - E ? gc : rows - E;
-        src = p + (k0 + k - (k0 + k >= wrap ? wrap : 0)) * ld + gc;
-        if (TAIL && k0 + k >= K) src = reinterpret_cast<const T*>(&zero_chunk);
+        const int k = q * KPB + b / (2 * R);
+        const int cr = ((b % (2 * R)) >> 4) ^ ((k & 3) << 2);
+        int64_t gc = row0 + 8 * cr;
+        gc = gc <= rows - 8 ? gc : rows - 8;
+        src = p + (k0 + k) * ld + gc;
+        if (TAIL && k0 + k >= K) src = reinterpret_cast<const bf16_t*>(&zero_chunk);
     }
     dma16(src, lds_addr(dst) + 1024 * q);
 }
@@ -115,13 +106,13 @@ __device__ __forceinline__ void fill_block(int qq, const T* __restrict__ p, int6
 // 16-byte read from a [row][k] tile, or two transposing 8-byte reads from a
 // [k][row] tile.
 typedef short v4i16 __attribute__((ext_vector_type(4)));
-template <bool TR, typename T = bf16_t> struct Frag;
-template <> struct Frag<false, bf16_t> {
+template <bool TR> struct Frag;
+template <> struct Frag<false> {
     u32x4 v;
     __device__ __forceinline__ bf16x8 get() const { return __builtin_bit_cast(bf16x8, v); }
     __device__ __forceinline__ void ld(const char NOTT_LDS* p) { v = *reinterpret_cast<const u32x4 NOTT_LDS*>(p); }
 };
-template <> struct Frag<true, bf16_t> {
+template <> struct Frag<true> {
     v4i16 lo, hi;
     __device__ __forceinline__ bf16x8 get() const {
         const v4i16 w[2] = {lo, hi};
@@ -132,31 +123,6 @@ template <> struct Frag<true, bf16_t> {
         hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4i16 NOTT_LDS*)(p + hi_off));
     }
 };
-template <> struct Frag<false, float> {
-    f32x4 v;
-    __device__ __forceinline__ f32x4 get() const { return v; }
-    __device__ __forceinline__ void ld(const char NOTT_LDS* p) { v = *reinterpret_cast<const f32x4 NOTT_LDS*>(p); }
-};
-template <> struct Frag<true, float> {
-    f32x4 v;
-    __device__ __forceinline__ f32x4 get() const { return v; }
-    __device__ __forceinline__ void ld(const char NOTT_LDS* p, int k_bytes) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float NOTT_LDS*>(p + e * k_bytes);
-    }
-};
-
-// acc += the product of step E of a slice of two fragments, the first's rows as rows
-// of the result (one MFMA a slice in bf16, four in fp32).
-template <typename T> constexpr int kSteps = sizeof(T) == 2 ? 1 : 4;
-template <int E>
-__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 acc) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
-}
-template <int E>
-__device__ __forceinline__ f32x16 mma32(f32x4 a, f32x4 b, f32x16 acc) {
-    return __builtin_amdgcn_mfma_f32_32x32x2f32(a[E], b[E], acc, 0, 0, 0);
-}
 
 // Per-lane LDS byte offsets of one operand's fragments inside a stage tile
 // (R rows; this wave's rows start at w0; F fragments of 32 rows).
@@ -166,43 +132,36 @@ __device__ __forceinline__ f32x16 mma32(f32x4 a, f32x4 b, f32x16 acc) {
 //   [k][row] tile: fragment f, slice s, half h at off[f] + (16s + 4h)·2R, where
 //     off[f] = k·2R + (((r>>3) ^ 4·(k&3))·16) + (r&7)·2 with
 //     r = w0 + 32f + 16·((l>>4)&1) + 4·(l&3), k = 8·(l/32) + ((l&15)>>2).
-//   fp32 [k][row] tile: fragment f, slice s, k's 8s + 4·(l/32) + 0..3 of row
-//     w0 + 32f + l%32: off[f] + 8s·4R, and 4R bytes from k to k.
-template <bool TR, int R, int F, typename T = bf16_t>
+template <bool TR, int R, int F>
 struct FragAddr {
-    static constexpr int RB = R * (int)sizeof(T);
     uint32_t off[TR ? F : 4];
     __device__ __forceinline__ void init(int w0, int lane) {
         if constexpr (!TR) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
                 off[s] = (uint32_t)((w0 + (lane & 31)) * 128 + ((((2 * s) | (lane >> 5)) ^ ((lane >> 1) & 7)) << 4));
-        } else if constexpr (sizeof(T) == 2) {
+        } else {
             const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
 #pragma unroll
             for (int f = 0; f < F; ++f) {
                 const int r = w0 + 32 * f + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                off[f] = (uint32_t)(k * RB + (((r >> 3) ^ ((k & 3) << 2)) << 4) + (r & 7) * 2);
+                off[f] = (uint32_t)(k * (2 * R) + (((r >> 3) ^ ((k & 3) << 2)) << 4) + (r & 7) * 2);
             }
-        } else {
-#pragma unroll
-            for (int f = 0; f < F; ++f) off[f] = (uint32_t)(4 * (lane >> 5) * RB + (w0 + 32 * f + (lane & 31)) * 4);
         }
     }
     // Reads fragment FI of slice S of the tile at `base`.
     template <int S, int FI>
-    __device__ __forceinline__ void read(Frag<TR, T>& d, const char NOTT_LDS* base) const {
+    __device__ __forceinline__ void read(Frag<TR>& d, const char NOTT_LDS* base) const {
         if constexpr (!TR) d.ld(base + off[S] + 4096 * FI);
-        else if constexpr (sizeof(T) == 2) d.ld(base + off[FI] + 16 * S * RB, 4 * RB);
-        else d.ld(base + off[FI] + 8 * S * RB, RB);
+        else d.ld(base + off[FI] + 16 * S * 2 * R, 4 * 2 * R);
     }
 };
 
-template <int S, bool TR, int R, int F, typename T, int I = 0>
-__device__ __forceinline__ void read_all(Frag<TR, T> (&d)[F], const FragAddr<TR, R, F, T>& a, const char NOTT_LDS* base) {
+template <int S, bool TR, int R, int F, int I = 0>
+__device__ __forceinline__ void read_all(Frag<TR> (&d)[F], const FragAddr<TR, R, F>& a, const char NOTT_LDS* base) {
     if constexpr (I < F) {
         a.template read<S, I>(d[I], base);
-        read_all<S, TR, R, F, T, I + 1>(d, a, base);
+        read_all<S, TR, R, F, I + 1>(d, a, base);
     }
 }
 
@@ -271,16 +230,22 @@ __device__ __forceinline__ void add_frag(float& s, const Frag<true>& f) {
 // An epilogue for products whose B is two stacked halves (see fill_block): a wave
 // has 32 columns of the first half in acc[i][0] and the same of the second in
 // acc[i][1], and hands both, transposed as for store_tile, to
-// ep.store_pair<TM, FM>(acc, buf, m0, column, lane) with LDS for TM·32 of T.
+// ep.store_pair<TM, FM>(acc, buf, m0, column, lane) with TM·EP::kRowBytes of LDS.
 template <class EP> struct IsPaired { static constexpr bool value = false; };
-// An epilogue of products whose A is two pieces of one operand stacked along k, so
-// that B's k-rows repeat from ep.wrap on (fill_block).
-template <class EP> struct IsWrapped { static constexpr bool value = false; };
-template <class EP>
-__device__ __forceinline__ int64_t wrap_of(const EP& ep) {
-    if constexpr (IsWrapped<EP>::value) return ep.wrap;
-    else return 0;
+// Operands held as sums of bf16 pieces (each stride_a or stride_b elements behind the
+// one before): C = Σ_p A_{i(p)}·B_{j(p)} over `count` pairs of pieces, one after the
+// other along k.  Every pair takes the same stages of the pieces' K, the last one
+// filled up with zeros; i and j are the pair's digits (4 bits each) of a and b.
+struct Pieces {
+    uint32_t count, a, b;
+    int64_t stride_a, stride_b;
+    FastDiv stages;   // of a pair
+};
+inline Pieces pieces(uint32_t count, uint32_t a, uint32_t b, int64_t stride_a, int64_t stride_b, int64_t K) {
+    return {count, a, b, stride_a, stride_b, FastDiv((uint32_t)ceil_div(K, BK))};
 }
+// An epilogue that has them as ep.pieces; its products' splits count pairs·stages.
+template <class EP> struct IsPieces { static constexpr bool value = false; };
 template <class EP> struct IsBf16RowMajor { static constexpr bool value = false; };
 template <> struct IsBf16RowMajor<RowMajorStore<bf16_t>> { static constexpr bool value = true; };
 
@@ -364,12 +329,12 @@ __device__ __forceinline__ void store_tile(const EP& ep, const f32x16 (&acc)[FM]
 // there fragment f's sum is kept by wave column f % WN, so each row is
 // summed once; the two k-halves of a row are held by lanes l and l+32 and
 // combined at the end; the epilogue receives it via ep.rowsum(m, v).
-template <bool AT, bool BT, int BM, int BN, int WM, int WN, int S, bool ROWSUM, bool TAIL, class EP, typename T>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const T* __restrict__ A, int64_t lda,
-                                                             const T* __restrict__ B, int64_t ldb, EP ep0,
+template <bool AT, bool BT, int BM, int BN, int WM, int WN, int S, bool ROWSUM, bool TAIL, class EP>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const bf16_t* __restrict__ A, int64_t lda,
+                                                             const bf16_t* __restrict__ B, int64_t ldb, EP ep0,
                                                              int64_t M, int64_t N, int64_t K, int64_t kps, int splits,
                                                              int gm, int by_tile) {
-    constexpr int NW = WM * WN, BK = kStageK<T>;
+    constexpr int NW = WM * WN;
     constexpr int TM = BM / WM, TN = BN / WN;
     constexpr int FM = TM / 32, FN = TN / 32;
     constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
@@ -389,7 +354,13 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const T* __restrict_
     const EP ep = at_split(ep0, z);
     const int64_t m0 = (int64_t)pm * BM, n0 = (int64_t)pn * BN;
     const int64_t kb = (int64_t)z * kps;
-    const int64_t ke = kb + kps < K ? kb + kps : K;
+    int64_t ke;
+    if constexpr (IsPieces<EP>::value) {   // whole stages of every pair
+        const int64_t all = (int64_t)ep0.pieces.count * ep0.pieces.stages.d * BK;
+        ke = kb + kps < all ? kb + kps : all;
+    } else {
+        ke = kb + kps < K ? kb + kps : K;
+    }
     const int nk = ke > kb ? (int)((ke - kb + BK - 1) / BK) : 0;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wid / WN, wn = wid % WN;
@@ -402,34 +373,53 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const T* __restrict_
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-    // Issues loads [from, to) of this wave's LOADS for stage t.
+    // Issues loads [from, to) of this wave's LOADS for stage t.  The stages come in
+    // order: of pieces, the pair and its stage are carried along.
     constexpr int LA = BM / 8 / NW;
+    uint32_t pair = 0, stage = 0;
+    const bf16_t *Ap = A, *Bp = B;
+    auto take_pair = [&] {
+        if constexpr (IsPieces<EP>::value) {
+            Ap = A + ((ep0.pieces.a >> (4 * pair)) & 15) * ep0.pieces.stride_a;
+            Bp = B + ((ep0.pieces.b >> (4 * pair)) & 15) * ep0.pieces.stride_b;
+        }
+    };
+    if constexpr (IsPieces<EP>::value) {
+        ep0.pieces.stages.divmod((uint32_t)(kb / BK), pair, stage);
+        pair = __builtin_amdgcn_readfirstlane(pair);
+        stage = __builtin_amdgcn_readfirstlane(stage);
+        take_pair();
+    }
     auto issue = [&](int t, int slot, int from, int to) {
         char NOTT_LDS* st = smem + slot * STAGE;
-        const int64_t k0 = kb + (int64_t)t * BK;
+        int64_t k0 = kb + (int64_t)t * BK;
+        if constexpr (IsPieces<EP>::value) k0 = (int64_t)stage * BK;
         if (!TAIL || k0 + BK <= K) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 if (i < from || i >= to) continue;
-                if (i < LA) fill_block<AT, BM, NW, false>(i, A, lda, m0, M, k0, K, st, wid, lane);
-                else fill_block<BT, BN, NW, false, PAIR>(i - LA, B, ldb, n0, N, k0, K, st + A_BYTES, wid, lane, wrap_of(ep));
+                if (i < LA) fill_block<AT, BM, NW, false>(i, Ap, lda, m0, M, k0, K, st, wid, lane);
+                else fill_block<BT, BN, NW, false, PAIR>(i - LA, Bp, ldb, n0, N, k0, K, st + A_BYTES, wid, lane);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 if (i < from || i >= to) continue;
-                if (i < LA) fill_block<AT, BM, NW, true>(i, A, lda, m0, M, k0, K, st, wid, lane);
-                else fill_block<BT, BN, NW, true, PAIR>(i - LA, B, ldb, n0, N, k0, K, st + A_BYTES, wid, lane, wrap_of(ep));
+                if (i < LA) fill_block<AT, BM, NW, true>(i, Ap, lda, m0, M, k0, K, st, wid, lane);
+                else fill_block<BT, BN, NW, true, PAIR>(i - LA, Bp, ldb, n0, N, k0, K, st + A_BYTES, wid, lane);
             }
         }
+        if constexpr (IsPieces<EP>::value) {
+            if (from < LOADS && to == LOADS && ++stage == ep0.pieces.stages.d) stage = 0, ++pair, take_pair();
+        }
     };
-    FragAddr<AT, BM, FM, T> fa;
-    FragAddr<BT, BN, FN, T> fb;
+    FragAddr<AT, BM, FM> fa;
+    FragAddr<BT, BN, FN> fb;
     fa.init(wm * TM, lane);
     fb.init(wn * TN, lane);
 
-    Frag<AT, T> a[2][FM];
-    Frag<BT, T> b[2][FN];
+    Frag<AT> a[2][FM];
+    Frag<BT> b[2][FN];
     float rs[FM];
 #pragma unroll
     for (int i = 0; i < FM; ++i) rs[i] = 0.f;
@@ -441,21 +431,12 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const T* __restrict_
                     if (i % WN == wn) add_frag(rs[i], a[p][i]);
             }
         }
-        auto step = [&](auto e) {   // the same accumulator again only FM·FN products later
-            constexpr int E = decltype(e)::value;
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = SWAP ? mma32<E>(b[p][j].get(), a[p][i].get(), acc[i][j])
-                                     : mma32<E>(a[p][i].get(), b[p][j].get(), acc[i][j]);
-        };
-        step(std::integral_constant<int, 0>());
-        if constexpr (kSteps<T> == 4) {
-            step(std::integral_constant<int, 1>());
-            step(std::integral_constant<int, 2>());
-            step(std::integral_constant<int, 3>());
-        }
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = SWAP ? __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[p][j].get(), a[p][i].get(), acc[i][j], 0, 0, 0)
+                                 : __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[p][i].get(), b[p][j].get(), acc[i][j], 0, 0, 0);
     };
 
     // Stages 0..S-2 are in flight before the loop.  The loads of stage t+S
@@ -516,7 +497,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const T* __restrict_
     if constexpr (PAIR) {
         wait_vm_lgkm0<0>();   // as in store_tile
         barrier();
-        ep.template store_pair<TM, FM>(acc, smem + wid * (TM * 32 * (int)sizeof(T)), m0 + wm * TM, (n0 + wn * TN) / 2, lane);
+        ep.template store_pair<TM, FM>(acc, smem + wid * (TM * EP::kRowBytes), m0 + wm * TM, (n0 + wn * TN) / 2, lane);
     } else if constexpr (SWAP) {
         store_tile<TM, FM, FN>(ep, acc, smem + wid * (TM * 128), m0 + wm * TM, n0 + wn * TN, lane);
     } else {
@@ -553,6 +534,7 @@ enum class Shape { T256x256, T256x128, T128x128, T128x128x2 };
 struct Plan {
     Shape shape;
     int64_t splits, kps;
+    float us;   // estimated
 };
 
 // Picks the tile shape and the split-K count with the least estimated time:
@@ -584,8 +566,7 @@ inline Plan plan(nott_ctx ctx, int64_t M, int64_t N, int64_t K, bool both_tr, bo
     constexpr float kSplitUs = 1.8f, kUnevenUs = 1.4f, kPartialUs = 0.04f, kPartialRowsUs = 0.21f;
     constexpr float kPartialBytesPerUs = 5.9e6f;
     const int64_t nkb = ceil_div(K, BK);
-    Plan best{Shape::T128x128, 1, K};
-    float best_us = 0.f;
+    Plan best{Shape::T128x128, 1, K, 0.f};
     for (const Cost& c : kCosts) {
         const int64_t tiles = ceil_div(M, c.bm) * ceil_div(N, c.bn), slots = (int64_t)ctx->num_cu * c.per_cu;
         const float idle = c.idle + (rowsum ? c.rows : 0.f), load = both_tr ? c.load_tr : c.load;
@@ -600,10 +581,7 @@ inline Plan plan(nott_ctx ctx, int64_t M, int64_t N, int64_t K, bool both_tr, bo
             if (n > 1)
                 us += kSplitUs + (n % 8 && n != 2 && n != 4 ? kUnevenUs : 0.f) + (float)n * (rowsum ? kPartialRowsUs : kPartialUs) +
                       8.f * (float)(n * M * N) / kPartialBytesPerUs;
-            if (best_us == 0.f || us < best_us) {
-                best_us = us;
-                best = Plan{c.shape, n, n > 1 ? stages * BK : K};
-            }
+            if (best.us == 0.f || us < best.us) best = Plan{c.shape, n, n > 1 ? stages * BK : K, us};
             if (splits > 0) break;
         }
     }
@@ -623,10 +601,10 @@ inline bool applies(const bf16_t* A, int64_t lda, const bf16_t* B, int64_t ldb, 
     return ceil_div(M, 128) * ceil_div(N, 128) < (int64_t)1 << 26;   // tiles times splits in an int
 }
 
-template <class Cfg, bool ROWSUM, bool TAIL, class EP, typename T>
-int launch_as(nott_ctx ctx, const T* A, int64_t lda, const T* B, int64_t ldb, const EP& ep, int64_t M,
+template <class Cfg, bool ROWSUM, bool TAIL, class EP>
+int launch_as(nott_ctx ctx, const bf16_t* A, int64_t lda, const bf16_t* B, int64_t ldb, const EP& ep, int64_t M,
            int64_t N, int64_t K, int64_t splits, int64_t kps) {
-    auto fn = gemm_kernel<Cfg::kAT, Cfg::kBT, Cfg::kBM, Cfg::kBN, Cfg::kWM, Cfg::kWN, Cfg::kS, ROWSUM, TAIL, EP, T>;
+    auto fn = gemm_kernel<Cfg::kAT, Cfg::kBT, Cfg::kBM, Cfg::kBN, Cfg::kWM, Cfg::kWN, Cfg::kS, ROWSUM, TAIL, EP>;
     static bool attr = false;   // one setting per kernel instantiation
     if (!attr) {
         if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -635,22 +613,22 @@ int launch_as(nott_ctx ctx, const T* A, int64_t lda, const T* B, int64_t ldb, co
         attr = true;
     }
     const int64_t tiles = ceil_div(M, Cfg::kBM) * ceil_div(N, Cfg::kBN);
-    const int64_t bytes = (int64_t)sizeof(T) * (M + N) * K;
+    const int64_t bytes = 2 * (M + N) * K;
     const int by_tile = splits > 1 && tiles % 8 == 0 && bytes >= 5000000 && bytes < 22000000;
     hipLaunchKernelGGL(fn, dim3((unsigned)(tiles * splits)), dim3(Cfg::kThreads), Cfg::kLds, ctx->stream, A, lda, B,
                        ldb, ep, M, N, K, kps, (int)splits, 4, by_tile);
     return launch_status(ctx, "gemm_dma");
 }
 
-template <class Cfg, bool ROWSUM, class EP, typename T>
-int launch(nott_ctx ctx, const T* A, int64_t lda, const T* B, int64_t ldb, const EP& ep, int64_t M,
+template <class Cfg, bool ROWSUM, class EP>
+int launch(nott_ctx ctx, const bf16_t* A, int64_t lda, const bf16_t* B, int64_t ldb, const EP& ep, int64_t M,
            int64_t N, int64_t K, int64_t splits, int64_t kps) {
-    return K % kStageK<T> ? launch_as<Cfg, ROWSUM, true>(ctx, A, lda, B, ldb, ep, M, N, K, splits, kps)
+    return K % BK ? launch_as<Cfg, ROWSUM, true>(ctx, A, lda, B, ldb, ep, M, N, K, splits, kps)
                   : launch_as<Cfg, ROWSUM, false>(ctx, A, lda, B, ldb, ep, M, N, K, splits, kps);
 }
 
-template <bool AT, bool BT, bool ROWSUM, class EP, typename T>
-int launch_shape(nott_ctx ctx, Shape sh, const T* A, int64_t lda, const T* B, int64_t ldb, const EP& ep,
+template <bool AT, bool BT, bool ROWSUM, class EP>
+int launch_shape(nott_ctx ctx, Shape sh, const bf16_t* A, int64_t lda, const bf16_t* B, int64_t ldb, const EP& ep,
                  int64_t M, int64_t N, int64_t K, int64_t splits, int64_t kps) {
     switch (sh) {
         case Shape::T256x128:
