@@ -347,34 +347,60 @@ bool ok16(const T* p, int64_t ld) {
 // n rounded up to whole 16-byte chunks of bf16.
 int64_t up8(int64_t n) { return (n + 7) & ~int64_t(7); }
 
-// src [rows, cols] as `pieces` bf16 pieces [prows, pcols] with zeros past it, each the
-// rounding of what the ones before leave: the copy of a bf16 tensor whose rows no
-// 16-byte load fits, and an fp32 tensor for the bf16 engine.
+// 16 bytes from any element's address.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+// src [rows, cols] to bf16 pieces [prows, pcols] at dst, one behind the other, zeros
+// past src's rows and columns.  No rows: nothing.
 template <typename T>
-__global__ __launch_bounds__(256) void pieces_kernel(const T* __restrict__ src, int64_t rows, int64_t cols,
-                                                     bf16_t* __restrict__ dst, int64_t prows, int64_t pcols, int pieces) {
-    const int64_t n = prows * pcols / 8;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i * 8 / pcols, c = i * 8 - r * pcols;
+struct PieceJob {
+    const T* src = nullptr;
+    int64_t rows = 0, cols = 0;
+    bf16_t* dst = nullptr;
+    int64_t chunks = 0;   // of 8 elements
+    FastDiv row;          // chunks of a row
+    PieceJob() = default;
+    PieceJob(const T* s, int64_t r, int64_t c, bf16_t* d, int64_t prows, int64_t pcols)
+        : src(s), rows(r), cols(c), dst(d), chunks(prows * pcols / 8), row((uint32_t)(pcols / 8)) {}
+};
+// Two jobs in one launch, `pieces` pieces of each, every one the rounding of what the
+// ones before leave: the copy of a bf16 tensor whose rows no 16-byte load fits, and
+// fp32 tensors for the bf16 engine.  A thread has 8 elements.
+template <typename T>
+__global__ __launch_bounds__(256) void pieces_kernel(PieceJob<T> a, PieceJob<T> b, int pieces) {
+    const PieceJob<T> j = blockIdx.y ? b : a;
+    const bool small = j.chunks < (int64_t)1 << 32;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < j.chunks; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = small ? j.row.div((uint32_t)i) : i / j.row.d, c = (i - r * j.row.d) * 8;
+        const T* p = j.src + r * j.cols + c;
         float v[8];
+        if (r < j.rows && c + 8 <= j.cols) {
+            if constexpr (sizeof(T) == 2) {
+                Pack16<bf16_t>::unpack(*reinterpret_cast<const u32x4_any*>(p), v);
+            } else {
+                const f32x4 lo = reinterpret_cast<const f32x4_any*>(p)[0], hi = reinterpret_cast<const f32x4_any*>(p)[1];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = r < rows && c + e < cols ? Io<T>::ld(src, r * cols + c + e) : 0.f;
-        for (int p = 0; p < pieces; ++p) {
-            Pack16<bf16_t>::st(dst + p * prows * pcols + i * 8, v);
+                for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = r < j.rows && c + e < j.cols ? Io<T>::ld(p, e) : 0.f;
+        }
+        for (int k = 0; k < pieces; ++k) {
+            Pack16<bf16_t>::st(j.dst + (k * j.chunks + i) * 8, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] -= bf16_to_f32(f32_to_bf16(v[e]));
         }
     }
 }
 template <typename T>
-void to_pieces(nott_ctx ctx, const T* src, int64_t rows, int64_t cols, bf16_t* dst, int64_t prows, int64_t pcols,
-               int pieces) {
-    hipLaunchKernelGGL(pieces_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(prows * pcols, 2048), 8192)), dim3(256),
-                       0, ctx->stream, src, rows, cols, dst, prows, pcols, pieces);
+void to_pieces(nott_ctx ctx, int pieces, const PieceJob<T>& a, const PieceJob<T>& b = {}) {
+    const int64_t most = std::max(a.chunks, b.chunks);
+    if (most == 0) return;
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(most, 256), 8192);
+    hipLaunchKernelGGL(pieces_kernel<T>, dim3(blocks, b.chunks ? 2 : 1), dim3(256), 0, ctx->stream, a, b, pieces);
 }
-
-// 16 bytes from any element's address.
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 // Few rows (single tokens of some sequences): the weights are streamed once, 16
 // gate rows and the matching 16 up rows a workgroup, its 8 waves dealing out 64
@@ -538,8 +564,8 @@ int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* x,
     if (ws.failed()) return NOTT_ERR_ALLOC;
     bf16_t* xp = reinterpret_cast<bf16_t*>(ws.p);
     bf16_t* wp = xp + (pad_x ? m * dp : 0);
-    if (pad_x) to_pieces(ctx, x, m, d, xp, m, dp, 1);
-    if (pad_w) to_pieces(ctx, w, 2 * f, d, wp, 2 * f, dp, 1);
+    using Job = PieceJob<bf16_t>;
+    to_pieces(ctx, 1, pad_x ? Job(x, m, d, xp, m, dp) : Job(), pad_w ? Job(w, 2 * f, d, wp, 2 * f, dp) : Job());
     const bf16_t* X = pad_x ? xp : x;
     const bf16_t* W = pad_w ? wp : w;
     if (rows) return forward_rows(ctx, m, dp, f, act, X, W, b, h, gu);
@@ -569,8 +595,7 @@ int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* x, 
     if (ws.failed()) return NOTT_ERR_ALLOC;
     bf16_t* xp = reinterpret_cast<bf16_t*>(ws.p);
     bf16_t* wp = xp + 3 * m * dp;
-    to_pieces(ctx, x, m, d, xp, m, dp, 3);
-    to_pieces(ctx, w, 2 * f, d, wp, 2 * f, dp, 3);
+    to_pieces(ctx, 3, PieceJob<float>(x, m, d, xp, m, dp), PieceJob<float>(w, 2 * f, d, wp, 2 * f, dp));
     const int64_t deep = kPairs * ceil_div(dp, dma::BK) * dma::BK;
     const dma::Plan p = dma::plan(ctx, m, 2 * f, deep, false, false, 1);
     const GatedPieces ep{{h, gu, b, m, f, act, ok16(h, f) && ok16(gu, f)},
@@ -643,8 +668,8 @@ int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* dh
     bf16_t* wp = xp + (pad_x ? m * dp : 0);
     int st = activation_bwd(ctx, m, f, fp, act, dh, gu, nullptr, hi, dw ? 2 : 1, db, accumulate);
     if (st != NOTT_OK) return st;
-    if (pad_x) to_pieces(ctx, x, m, d, xp, m, dp, 1);
-    if (pad_w) to_pieces(ctx, w, 2 * f, d, wp, fp, dp, 1);
+    using Job = PieceJob<bf16_t>;
+    to_pieces(ctx, 1, pad_x ? Job(x, m, d, xp, m, dp) : Job(), pad_w ? Job(w, 2 * f, d, wp, fp, dp) : Job());
     if (dx) {
         const RowMajorStore<bf16_t> ep{dx, d, m, d, nullptr};
         st = dma_dx ? dma::run<false, true>(ctx, hi, fp, pad_w ? wp : w, dp, ep, m, dp, fp)
@@ -678,9 +703,10 @@ int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* dh,
     float* all = reinterpret_cast<float*>(wp + (pieces_dx ? 3 * fp * dp : 0));
     int st = activation_bwd(ctx, m, f, ld, act, dh, gu, whole ? all : nullptr, dgu, pieces ? 3 : 0, db, accumulate);
     if (st != NOTT_OK) return st;
+    using Job = PieceJob<float>;
+    to_pieces(ctx, 3, pieces_dx ? Job(w, 2 * f, d, wp, fp, dp) : Job(), pieces_dw ? Job(x, m, d, xp, m, dp) : Job());
     const AccStore to_dx{dx, m, d, 0}, to_dw{dw, 2 * f, d, accumulate};
     if (pieces_dx) {
-        to_pieces(ctx, w, 2 * f, d, wp, fp, dp, 3);
         st = pieces_product<false, true>(ctx, dgu, fp, wp, dp, to_dx, dma::pieces(kPairs, kFirst, kSecond, m * fp, fp * dp, fp),
                                          m, dp, fp);
     } else if (dx) {
@@ -688,7 +714,6 @@ int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* dh,
     }
     if (st != NOTT_OK || !dw) return st;
     if (!pieces_dw) return product<float, true, true>(ctx, all, ld, x, d, to_dw, 2 * f, d, m);
-    to_pieces(ctx, x, m, d, xp, m, dp, 3);
     return pieces_product<true, true>(ctx, dgu, fp, xp, dp, to_dw, dma::pieces(kPairs, kFirst, kSecond, m * fp, m * dp, m), fp,
                                       dp, m);
 }
