@@ -12,8 +12,8 @@
 // 2^-23 of the whole (hi·hi, hi·mid, mid·hi, mid·mid, hi·lo, lo·hi) are summed in
 // fp32, the small ones first: six products, where the fp32 matrix instructions take
 // the time of sixteen, and no further from 64 bits than those (8192 rows of 1024 ->
-// 2048 422 us, 554 with fp32 instructions on tiles of the same engine; gradients 460
-// and 462 against 557 and 600).  An infinity comes out as NaN, and from 3.39e38 a value
+// 2048 408 us, 554 with fp32 instructions on tiles of the same engine; gradients 456
+// and 459 against 557 and 600).  An infinity comes out as NaN, and from 3.39e38 a value
 // counts as one.
 #include "gemm_dma.hpp"
 
@@ -540,16 +540,16 @@ int product(nott_ctx ctx, const T* A, int64_t lda, const T* B, int64_t ldb, cons
 constexpr uint32_t kPairs = 6, kFirst = 0x001102, kSecond = 0x010120;
 
 // Whether an fp32 product of M×N×K, with so many elements to split into pieces, goes to
-// the direct-to-LDS engine: its plan's time and the split's, a quarter more than in
-// bf16 layers (every bit of the pieces is busy), against the generic engine's 75
-// TFLOP/s, which spreads few tiles over the CUs by splitting k.  In us, generic and
-// pieces (forward; dx and dw with the activation gradient): 1576 rows of 768 -> 2048 163
-// and 98, 170 and 103, 139 and 109; 1024 of 768 -> 1024 45 and 65, 64 and 52, 60 and 50;
-// 256 of 512 -> 1024 19 and 43, 22 and 31, 24 and 31.  On 20 sizes of 100 to 16384 rows
-// the choice is the better one or within 15% of it.
+// the direct-to-LDS engine: its plan's time and the split's against the generic engine's
+// 70 TFLOP/s, which spreads few tiles over the CUs by splitting k.  In us, generic and
+// pieces (forward; dx and dw with the activation gradient): 1576 rows of 768 -> 2048 162
+// and 88, 171 and 95, 140 and 102; 1024 of 768 -> 1024 43 and 57, 62 and 46, 58 and 45;
+// 256 of 512 -> 1024 19 and 38, 22 and 29, 24 and 29.  On 25 sizes of 128 to 16384 rows
+// the choice costs 1.4% over the better one in the mean (most where a forward of odd
+// width has its loads element by element: 53 against 42).
 bool takes_pieces(nott_ctx ctx, int64_t M, int64_t N, int64_t K, bool both_tr, bool split, int64_t elements) {
     const double us = dma::plan(ctx, M, N, kPairs * ceil_div(K, dma::BK) * dma::BK, both_tr, false, split ? 0 : 1).us;
-    return 1.25 * (us + 4 + (double)elements / 5e5) < 6 + 2.0 * (double)M * (double)N * (double)K / 75e6 &&
+    return us + 4 + (double)elements / 5e5 < 6 + 2.0 * (double)M * (double)N * (double)K / 70e6 &&
            ceil_div(M, 128) * ceil_div(N, 64) < (int64_t)1 << 23;
 }
 
