@@ -259,3 +259,53 @@ def test_large_in_fp32(m, d, f, spread):
     dw2 = torch.full_like(dw, 2.0)
     ops.gated_linear_bwd(dh, x, w, gu, dw=dw2, need_dx=False, need_db=False, accumulate=True)
     near(dw2, dw.double() + 2, 2 * U * (dw.double().abs() + 2), "dw accumulated")
+
+
+def test_large_in_fp32_captured():
+    """Split operands live in the workspace: replays between eager calls of other sizes, and another stream."""
+    m, d, f = 1100, 700, 1300
+    x, w, b, dh = make(m, d, f, torch.float32, True)
+    small = make(200, d, f, torch.float32, True)
+
+    def step(x, dh):
+        h, gu = ops.gated_linear_fwd(x, w, b, save=True)
+        return (h, gu, *ops.gated_linear_bwd(dh, x, w, gu))
+    want = step(x, dh)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        other = step(x, dh)
+    s.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(other, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x, dh)
+    for i in range(3):
+        x.copy_(torch.randn_like(x))
+        step(small[0], small[3])
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(got, step(x, dh)):
+            assert torch.equal(p, q), i
+
+
+def test_large_in_fp32_keeps_nan():
+    """NaN and infinity spread to what they reach and to nothing else."""
+    m, d, f = 1100, 700, 1300
+    x, w, b, dh = make(m, d, f, torch.float32, False)
+    clean = ops.gated_linear_fwd(x, w)[0]
+    x[7, 3], x[900, 699] = float("nan"), float("inf")
+    h, gu = ops.gated_linear_fwd(x, w, save=True)
+    rows = torch.ones(m, dtype=torch.bool, device="cuda")
+    rows[7] = rows[900] = False
+    assert torch.equal(h[rows], clean[rows])
+    assert bool(gu[7].isnan().all()) and not bool(gu[900].isfinite().any())
+    dh[5, 9] = float("nan")
+    x.nan_to_num_(0, 0, 0)
+    gu = ops.gated_linear_fwd(x, w, save=True)[1]
+    dx, dw, db = ops.gated_linear_bwd(dh, x, w, gu)
+    assert bool(dx[5].isnan().all()) and bool(dx[torch.arange(m, device="cuda") != 5].isfinite().all())
+    hit = torch.zeros(2 * f, dtype=torch.bool, device="cuda")
+    hit[9] = hit[f + 9] = True
+    assert bool(dw[hit].isnan().all()) and bool(dw[~hit].isfinite().all())
+    assert torch.equal(db.isnan(), hit)
