@@ -225,3 +225,16 @@ def test_captured_and_other_stream():
         torch.cuda.synchronize()
         for a, b in zip(got, step()):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("n,c", [(3, 700), (2, 5000), (600, 3000), (2, 100000)])
+def test_nan_in_the_first_column_leads(n, c, dt):
+    """NaN counts as largest wherever it stands, among so many equal logits that the row is scanned for each."""
+    z = torch.zeros((n, c), device="cuda", dtype=DT[dt])
+    z[:, 0] = z[:, c // 2] = math.nan
+    z[:, 5] = 1.0
+    top = ops.token_logprob_fwd(z, torch.zeros(n, device="cuda", dtype=torch.int64), top=5)[4]
+    torch.cuda.synchronize()
+    want = torch.tensor([0, c // 2, 5, 1, 2], device="cuda").expand(n, 5)
+    assert torch.equal(top, want)

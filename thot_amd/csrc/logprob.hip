@@ -84,10 +84,11 @@ struct Stats {
 };
 
 // Order of the most likely tokens as one whole number: the value in an order that
-// integers keep (−0 as +0, NaN above all), then the lower column.  0 is no key.
+// integers keep (−0 as +0, NaN above all), then the lower column.  0 and all ones
+// are no keys.
 __device__ __forceinline__ uint64_t top_key(float z, uint32_t col) {
     uint32_t u = __builtin_bit_cast(uint32_t, z + 0.f);
-    u = z != z ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    u = z != z ? 0xfffffffeu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
     return ((uint64_t)u << 32) | (uint32_t)~col;
 }
 
