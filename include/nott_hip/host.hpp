@@ -224,6 +224,10 @@ inline nott_dtype dtype_of(const Tensor& t) {
 inline bool present(const Tensor& t) { return t.defined() && t.numel() > 0; }
 inline Tensor absent(const Tensor& like) { return torch::empty({0}, like.options().dtype(torch::kFloat32)); }
 inline Tensor or_absent(const Tensor& t, const Tensor& like) { return t.defined() ? t : absent(like); }
+// Whether t is n elements of a type, side by side, where x lies.
+inline bool operand(const Tensor& t, const Tensor& x, torch::ScalarType type, int64_t n) {
+    return t.scalar_type() == type && t.numel() == n && t.is_contiguous() && t.device() == x.device();
+}
 
 inline void* ptr(const Tensor& t) { return present(t) ? t.data_ptr() : nullptr; }
 inline float* fptr(const Tensor& t) { return present(t) ? t.data_ptr<float>() : nullptr; }
@@ -799,8 +803,11 @@ struct QkNormRopeFn : torch::autograd::Function<QkNormRopeFn> {
             throw std::invalid_argument("Nott::HIP: k must have q's type and device");
         nott_qk_rope_desc d = desc(q, k, positions, inv_freq, sections, interleaved, norm, eps);
         for (const Tensor& g : {gamma_qc, gamma_kc})
-            if (present(g) && (g.numel() != d.dh || g.scalar_type() != q.scalar_type() || !g.is_contiguous()))
+            if (present(g) && !operand(g, q, q.scalar_type(), d.dh))
                 throw std::invalid_argument("Nott::HIP: a weight must be [dh] of q's type");
+        for (const Tensor& g : {gamma_q, gamma_k})
+            if (present(g) && !operand(g, q, g.scalar_type(), d.dh))
+                throw std::invalid_argument("Nott::HIP: a weight must be [dh] on q's device");
         Tensor yq = torch::empty({d.b, d.hq, d.t, d.dh}, q.options()), yk = torch::empty({d.b, d.hk, d.t, d.dh}, q.options());
         strides(d.yq_stride, yq, 2, 1);
         strides(d.yk_stride, yk, 2, 1);
@@ -848,8 +855,13 @@ struct QkNormRopeFn : torch::autograd::Function<QkNormRopeFn> {
 struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w, Tensor wc, Tensor b, int64_t act, bool keep) {
         x = contig(x);
-        if (wc.dim() != 2 || wc.size(0) % 2 || wc.size(0) == 0 || x.size(-1) != wc.size(1) || x.scalar_type() != wc.scalar_type())
+        if (x.dim() < 1 || wc.dim() != 2 || wc.size(0) % 2 || wc.numel() == 0 || x.size(-1) != wc.size(1) ||
+            !operand(wc, x, x.scalar_type(), wc.numel()))
             throw std::invalid_argument("Nott::HIP: a gated linear layer's weight must be [2·f, d] for x [..., d], of x's type");
+        if (!operand(w, x, w.scalar_type(), wc.numel()))
+            throw std::invalid_argument("Nott::HIP: a gated linear layer's weight and its working copy differ");
+        if (present(b) && !operand(b, x, torch::kFloat32, wc.size(0)))
+            throw std::invalid_argument("Nott::HIP: a gated linear layer's bias must be [2·f] in fp32");
         const int64_t d = x.size(-1), m = x.numel() / d, f = wc.size(0) / 2;
         auto shape = x.sizes().vec();
         shape.back() = f;

@@ -1,9 +1,14 @@
 """Arguments that the language-model operators refuse, before anything reaches a
-device: the checks of thot_amd.ops on host tensors."""
+device: the checks of thot_amd.ops and of the host layer on host tensors."""
 import pytest
 import torch
 
 from thot_amd import ops
+
+
+@pytest.fixture(scope="module")
+def host():
+    return pytest.importorskip("thot_amd._nott_host")
 
 
 def heads(b=2, t=3, h=4, dh=8, dtype=torch.float32):
@@ -111,3 +116,35 @@ def test_logprob_shapes():
     one = torch.zeros(3)
     with pytest.raises(ValueError, match="needs entropy"):
         ops.token_logprob_bwd(torch.zeros(3, 5), y, one, one, dentropy=one)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(w=torch.zeros(0, 8)), "weight must be"),
+    (dict(x=torch.zeros(3, 0), w=torch.zeros(4, 0)), "weight must be"),
+    (dict(w=torch.zeros(8, 4).t()), "weight must be"),
+    (dict(w=torch.zeros(6, 8), w_compute=torch.zeros(4, 8)), "working copy"),
+    (dict(b=torch.zeros(3)), "bias must be"),
+    (dict(b=torch.zeros(8)[::2]), "bias must be"),
+    (dict(b=torch.zeros(4, dtype=torch.float64)), "bias must be"),
+    (dict(), "HIP device"),
+])
+def test_host_gated_linear(host, kw, match):
+    a = dict(x=torch.zeros(3, 8), w=torch.zeros(4, 8))
+    a.update(kw)
+    with pytest.raises(ValueError, match=match):
+        host.gated_linear(**a)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(gamma_q=torch.ones(7)), "weight must be"),
+    (dict(gamma_k=torch.ones(16)[::2]), "weight must be"),
+    (dict(gamma_q=torch.ones(6), gamma_q_compute=torch.ones(8)), "weight must be"),
+    (dict(k=torch.zeros(2, 3, 4, 8, dtype=torch.bfloat16)), "q's type"),
+    (dict(), "HIP device"),
+])
+def test_host_qk_norm_rope(host, kw, match):
+    q = torch.zeros(2, 3, 4, 8)
+    a = dict(q=q, k=q)
+    a.update(kw)
+    with pytest.raises(ValueError, match=match):
+        host.qk_norm_rope(**a)

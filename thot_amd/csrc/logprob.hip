@@ -199,6 +199,8 @@ struct Span {
 // bound (many equal logits, or too few live ones for a bound) is scanned for each.
 // Bound by memory (one read of the logits), then by the exponential and four more
 // instructions an element.
+// 16384x32000 bf16, top 5, 187 us (5.6 TB/s; 222 in the mean of twenty in a row);
+// 8x128256 bf16, top 8, in parts of 4096 columns and more 6.9 us and 4.7 to join them.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void logprob_kernel(const T* __restrict__ logits, const int64_t* __restrict__ labels,
                                                      int64_t c, int chunk, Scale sc, int top, int cap, FwdOut o,
@@ -371,7 +373,7 @@ __global__ __launch_bounds__(64) void logprob_merge_kernel(const T* __restrict__
 
 // The gradient of one part of a row: NT·kUnroll groups, part 0 with the single
 // elements.  A group's loads are all issued before its stores, so dlogits may be
-// logits.
+// logits.  Bound by memory: 4096x50257 fp32 with entropies 284 us (5.8 TB/s).
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void logprob_bwd_kernel(const T* logits, const int64_t* __restrict__ labels, int64_t c,
                                                          uint32_t parts, FastDiv by_parts, float scale,
