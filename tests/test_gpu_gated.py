@@ -309,3 +309,16 @@ def test_large_in_fp32_keeps_nan():
     hit[9] = hit[f + 9] = True
     assert bool(dw[hit].isnan().all()) and bool(dw[~hit].isfinite().all())
     assert torch.equal(db.isnan(), hit)
+
+
+@pytest.mark.parametrize("e", [-105, 100])
+def test_large_in_fp32_far_from_one(e):
+    """x of 2^e: a power of two changes no rounding down to 2^-105, where the pieces of every value above 2^-110 are
+    whole; a smaller one (1 of 40) is off by 2^-134 at most."""
+    m, d, f = 1100, 700, 1300
+    x, w, _, _ = make(m, d, f, torch.float32, False)
+    xs = torch.ldexp(x, torch.tensor(e, device="cuda"))
+    got = ops.gated_linear_fwd(xs, w, save=True)[1]
+    mag = xs.double().abs() @ w.double().abs().t()
+    tol = (0.26 * d + 22) * U * mag + 2.0 ** -134 * w.double().abs().sum(1)
+    near(got, xs.double() @ w.double().t(), tol, "gu")

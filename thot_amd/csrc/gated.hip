@@ -14,7 +14,9 @@
 // the time of sixteen, and no further from 64 bits than those (8192 rows of 1024 ->
 // 2048 408 us, 554 with fp32 instructions on tiles of the same engine; gradients 456
 // and 459 against 557 and 600).  An infinity comes out as NaN, and from 3.39e38 a value
-// counts as one.
+// counts as one; the last piece ends at bf16's least number, so that values below
+// 2^-110 keep 2^-134 rather than their own last bit (inputs of 2^-110 come out with an
+// error of 1.5e-7 in the norm as all others, of 2^-115 with 1.1e-6).
 #include "gemm_dma.hpp"
 
 namespace {
