@@ -2,10 +2,10 @@
 //
 //   backward: dg = dh·u·act'(g), du = dh·act(g)
 //             dx = [dg|du]·w, dw = [dg|du]ᵀ·x, db = Σ_rows [dg|du]
-// h is rounded once from fp32 pre-activations.  [dg|du] is rounded to bf16 for
-// dx (a bf16 output); dw is fp32, so there [dg|du] goes in as two bf16 pieces,
-// hi = bf16(v) and lo = bf16(v − hi) (up to 2^-16 of v is lost, 2.7e-6 in the mean,
-// where one piece loses 2^-8 and 1.7e-3).
+// h is rounded once from fp32 pre-activations.  In bf16 layers [dg|du] goes into the
+// products as bf16 pieces cut toward zero: three for the fp32 dw (all 24 bits), two
+// for dx, of which the second ends at 2^-15 of a value where dx itself is rounded to
+// 2^-8 (one piece put as much into dx as its rounding: 2.3e-3 in the norm for 1.7e-3).
 //
 // fp32 layers take the bf16 matrix cores as well, wherever the products are large:
 // v = hi + mid + lo holds all 24 bits, and the six products of pieces that reach
@@ -228,9 +228,36 @@ __device__ __forceinline__ void store_piece(bf16_t* p, const float (&v)[E]) {
     else *p = f32_to_bf16(v[0]);
 }
 
+// v cut to bf16 toward zero; NaN stays.
+__device__ __forceinline__ float toward_zero(float v) {
+    return v != v ? v : __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);
+}
+// v as bf16 pieces `stride` elements apart, each cut toward zero from what the ones
+// before leave; three hold all of its bits.  A value's pieces all have its sign and
+// none is zero (2^-40 of the value, at least 2^-133, where nothing is left; an infinity
+// again): so the sum of their products with an infinity is that infinity, as the
+// value's own is, and not infinity − infinity or 0·infinity.
+template <int E>
+__device__ __forceinline__ void store_cut(bf16_t* out, int64_t stride, int pieces, float (&v)[E]) {
+    float least[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        least[e] = v[e] == 0.f ? 0.f : __builtin_copysignf(fmaxf(fabsf(v[e]) * 0x1p-40f, 0x1p-133f), v[e]);
+    for (int p = 0; p < pieces; ++p) {
+        float q[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const bool none = v[e] == 0.f;
+            q[e] = toward_zero(none ? least[e] : v[e]);
+            if (!none && fabsf(v[e]) <= 3.40282347e38f) v[e] -= q[e];
+        }
+        store_piece<E>(out + p * stride, q);
+    }
+}
+
 // [dg|du] in rows of ld elements with zeros past 2f: as fp32 (whole, the generic
-// engine's operand) and as bf16 pieces, each `stride` elements behind the one before
-// and the rounding of what that leaves.  A workgroup takes 64·E columns (E = 1, or
+// engine's operand) and as bf16 pieces, each `stride` elements behind the one before:
+// of a bf16 layer store_cut's, in fp32 the rounding of what is left.  A workgroup takes 64·E columns (E = 1, or
 // whole 16-byte chunks where all rows fit them and ld is 2f) and every gridDim.y-th
 // group of 4 rows; partial (null: no db) [gridDim.y][2f] receives its column sums of the unrounded
 // values.  Bound by memory: 8192 x 4096 bf16 with both pieces, 470 MB, 74 us (6.3 TB/s;
@@ -255,10 +282,14 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const T* __restrict__ d
 #pragma unroll
             for (int e = 0; e < E; ++e) whole[at + e] = v[e];
         }
-        for (int p = 0; p < pieces; ++p) {
-            store_piece<E>(out + p * stride + at, v);
+        if constexpr (sizeof(T) == 2) {
+            store_cut<E>(out + at, stride, pieces, v);
+        } else {
+            for (int p = 0; p < pieces; ++p) {
+                store_piece<E>(out + p * stride + at, v);
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] -= bf16_to_f32(f32_to_bf16(v[e]));
+                for (int e = 0; e < E; ++e) v[e] -= bf16_to_f32(f32_to_bf16(v[e]));
+            }
         }
     };
     if (c < f) {
@@ -328,8 +359,9 @@ struct AccStore {
         *p = accumulate ? *p + v : v;
     }
 };
-// The same, and its split-K partials, for products of pieces.
-struct PiecesStore : AccStore {
+// An epilogue, and split-K partials, for products of pieces.
+template <class EP>
+struct PiecesOf : EP {
     dma::Pieces pieces;
 };
 struct PiecesPartial : dma::PartialRowStore {
@@ -339,7 +371,8 @@ __device__ __forceinline__ PiecesPartial at_split(const PiecesPartial& ep, int z
 
 }  // namespace
 
-template <> struct nott::gemm::dma::IsPieces<PiecesStore> { static constexpr bool value = true; };
+template <class EP> struct nott::gemm::dma::IsPieces<PiecesOf<EP>> { static constexpr bool value = true; };
+template <> struct nott::gemm::dma::IsBf16RowMajor<PiecesOf<RowMajorStore<bf16_t>>> { static constexpr bool value = true; };
 template <> struct nott::gemm::dma::IsPieces<PiecesPartial> { static constexpr bool value = true; };
 
 namespace {
@@ -528,18 +561,53 @@ bool takes_rows(nott_ctx ctx, int64_t m, int64_t d, int64_t f, bool padded) {
     return weights * (m <= 32 ? 1.35 : 2.0) <= rounds * (double)ceil_div(d, 64) * 0.55 + (padded ? 2 * weights + 2 : 0);
 }
 
-// C = A·B on the generic engine; AT, BT as in gemm_dma.hpp.
+// C = A·B on the generic engine.
+template <typename T, class LA, class LB, class EP>
+int generic(nott_ctx ctx, const LA& la, const LB& lb, const EP& ep, int64_t M, int64_t N, int64_t K) {
+    return small_grid(ctx, M, N) ? run_small<T>(ctx, la, lb, ep, M, N, K) : run<T>(ctx, la, lb, ep, M, N, K);
+}
+// The same of plain operands; AT, BT as in gemm_dma.hpp.
 template <typename T, bool AT, bool BT, class EP>
 int product(nott_ctx ctx, const T* A, int64_t lda, const T* B, int64_t ldb, const EP& ep, int64_t M, int64_t N,
             int64_t K) {
-    auto go = [&](const auto& la, const auto& lb) {
-        return small_grid(ctx, M, N) ? run_small<T>(ctx, la, lb, ep, M, N, K) : run<T>(ctx, la, lb, ep, M, N, K);
-    };
     auto vec = [](const T* p, int64_t ld) { return ((uintptr_t)p % 16) == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0; };
-    if constexpr (AT) return go(ColKLoader<T>{A, lda, M, K}, ColKLoader<T>{B, ldb, N, K});
-    else if constexpr (BT) return go(RowKLoader<T>{A, lda, M, K, vec(A, lda)}, ColKLoader<T>{B, ldb, N, K});
-    else return go(RowKLoader<T>{A, lda, M, K, vec(A, lda)}, RowKLoader<T>{B, ldb, N, K, vec(B, ldb)});
+    const RowKLoader<T> row_a{A, lda, M, K, vec(A, lda)};
+    if constexpr (AT) return generic<T>(ctx, ColKLoader<T>{A, lda, M, K}, ColKLoader<T>{B, ldb, N, K}, ep, M, N, K);
+    else if constexpr (BT) return generic<T>(ctx, row_a, ColKLoader<T>{B, ldb, N, K}, ep, M, N, K);
+    else return generic<T>(ctx, row_a, RowKLoader<T>{B, ldb, N, K, vec(B, ldb)}, ep, M, N, K);
 }
+// Operands of the generic engine for products of pieces, one piece after the other along
+// k.  R(row, k) = p[stride·(k / ld) + row·ld + k % ld] for two pieces of rows of ld
+// elements, a multiple of 8: a chunk lies in one of them.
+struct TwoPieces {
+    static constexpr bool kRowFast = false;
+    static constexpr int E = 8;
+    const bf16_t* p;
+    int64_t ld, rows, stride;
+    __device__ __forceinline__ u32x4 chunk(int64_t row, int64_t k0) const {
+        if (row >= rows || k0 >= 2 * ld) return u32x4{0, 0, 0, 0};
+        return *reinterpret_cast<const u32x4*>(p + (k0 < ld ? 0 : stride - ld) + row * ld + k0);
+    }
+};
+// R(row, k) = p[(k % period)·ld + row] for k < total, at most three periods; zero where
+// k % period is K or more.
+struct Repeated {
+    static constexpr bool kRowFast = true;
+    static constexpr int E = 8;
+    const bf16_t* p;
+    int64_t ld, rows, K, period, total;
+    __device__ __forceinline__ u32x4 chunk(int64_t row, int64_t k0) const {
+        bf16_t v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            int64_t k = k0 + e;
+            if (k >= period) k -= period;
+            if (k >= period) k -= period;
+            v[e] = row < rows && k < K && k0 + e < total ? p[k * ld + row] : bf16_t(0);
+        }
+        return Pack<bf16_t>::make(v);
+    }
+};
 
 // The six products of fp32 pieces (hi 0, mid 1, lo 2), first factor and second.
 constexpr uint32_t kPairs = 6, kFirst = 0x001102, kSecond = 0x010120;
@@ -640,8 +708,8 @@ int activation_bwd(nott_ctx ctx, int64_t m, int64_t f, int64_t ld, int act, cons
 
 // ep's M×N = Σ over the pairs of pieces, K deep each, rows and columns of A and B in
 // whole chunks.
-template <bool AT, bool BT>
-int pieces_product(nott_ctx ctx, const bf16_t* A, int64_t lda, const bf16_t* B, int64_t ldb, const AccStore& ep,
+template <bool AT, bool BT, class EP>
+int pieces_product(nott_ctx ctx, const bf16_t* A, int64_t lda, const bf16_t* B, int64_t ldb, const EP& ep,
                    const dma::Pieces& pc, int64_t M, int64_t N, int64_t K) {
     const int64_t deep = pc.count * ceil_div(K, dma::BK) * dma::BK;
     dma::Plan p = dma::plan(ctx, M, N, deep, AT && BT, false, 0);
@@ -651,7 +719,7 @@ int pieces_product(nott_ctx ctx, const bf16_t* A, int64_t lda, const bf16_t* B, 
         if (!part) p = dma::plan(ctx, M, N, deep, AT && BT, false, 1);
     }
     if (!part)
-        return dma::launch_shape<AT, BT, false>(ctx, p.shape, A, lda, B, ldb, PiecesStore{ep, pc}, M, N, K, 1, deep);
+        return dma::launch_shape<AT, BT, false>(ctx, p.shape, A, lda, B, ldb, PiecesOf<EP>{ep, pc}, M, N, K, 1, deep);
     const int st = dma::launch_shape<AT, BT, false>(ctx, p.shape, A, lda, B, ldb,
                                                     PiecesPartial{{part, nullptr, M, N}, pc}, M, N, K, p.splits, p.kps);
     if (st != NOTT_OK) return st;
@@ -662,34 +730,34 @@ int pieces_product(nott_ctx ctx, const bf16_t* A, int64_t lda, const bf16_t* B, 
 int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* dh, const bf16_t* x, const bf16_t* w,
         const bf16_t* gu, bf16_t* dx, float* dw, float* db, int accumulate) {
     const int64_t dp = up8(d), fp = up8(2 * f);
+    const int pieces = dw ? 3 : dx ? 2 : 0;
     // the direct-to-LDS engine, where a product has its 128 rows and columns
     const bool dma_dx = dx && m >= 128 && d >= 128, dma_dw = dw && 2 * f >= 128 && d >= 128;
     const bool pad_x = dma_dw && !ok16(x, d), pad_w = dma_dx && (!ok16(w, d) || fp != 2 * f);
-    WorkspaceHold ws(ctx, sizeof(bf16_t) * (size_t)(m * fp * (dw ? 2 : 1) + ((pad_x ? m : 0) + (pad_w ? fp : 0)) * dp));
+    WorkspaceHold ws(ctx, sizeof(bf16_t) * (size_t)(m * fp * pieces + ((pad_x ? m : 0) + (pad_w ? fp : 0)) * dp));
     if (ws.failed()) return NOTT_ERR_ALLOC;
-    bf16_t* hi = reinterpret_cast<bf16_t*>(ws.p);
-    bf16_t* lo = hi + m * fp;
-    bf16_t* xp = hi + m * fp * (dw ? 2 : 1);
+    bf16_t* dgu = reinterpret_cast<bf16_t*>(ws.p);
+    bf16_t* xp = dgu + m * fp * pieces;
     bf16_t* wp = xp + (pad_x ? m * dp : 0);
-    int st = activation_bwd(ctx, m, f, fp, act, dh, gu, nullptr, hi, dw ? 2 : 1, db, accumulate);
+    int st = activation_bwd(ctx, m, f, fp, act, dh, gu, nullptr, dgu, pieces, db, accumulate);
     if (st != NOTT_OK) return st;
     using Job = PieceJob<bf16_t>;
     to_pieces(ctx, 1, pad_x ? Job(x, m, d, xp, m, dp) : Job(), pad_w ? Job(w, 2 * f, d, wp, fp, dp) : Job());
-    if (dx) {
+    if (dx) {   // the second piece, then the first
         const RowMajorStore<bf16_t> ep{dx, d, m, d, nullptr};
-        st = dma_dx ? dma::run<false, true>(ctx, hi, fp, pad_w ? wp : w, dp, ep, m, dp, fp)
-                    : product<bf16_t, false, true>(ctx, hi, fp, w, d, ep, m, d, 2 * f);
+        st = dma_dx ? pieces_product<false, true>(ctx, dgu, fp, pad_w ? wp : w, dp, ep, dma::pieces(2, 0x01, 0x00, m * fp, 0, fp),
+                                                  m, dp, fp)
+                    : generic<bf16_t>(ctx, TwoPieces{dgu, fp, m, m * fp}, Repeated{w, d, d, 2 * f, fp, 2 * fp}, ep, m, d, 2 * fp);
         if (st != NOTT_OK) return st;
     }
     if (!dw) return st;
-    if (!dma_dw) {
-        st = product<bf16_t, true, true>(ctx, hi, fp, x, d, AccStore{dw, 2 * f, d, accumulate}, 2 * f, d, m);
-        if (st != NOTT_OK) return st;
-        return product<bf16_t, true, true>(ctx, lo, fp, x, d, AccStore{dw, 2 * f, d, 1}, 2 * f, d, m);
-    }
-    // lo·x, then hi·x
-    return pieces_product<true, true>(ctx, hi, fp, pad_x ? xp : x, dp, AccStore{dw, 2 * f, d, accumulate},
-                                      dma::pieces(2, 0x01, 0x00, m * fp, 0, m), fp, dp, m);
+    const AccStore ep{dw, 2 * f, d, accumulate};
+    if (!dma_dw)
+        return generic<bf16_t>(ctx, ColKLoader<bf16_t>{dgu, fp, 2 * f, 3 * m}, Repeated{x, d, d, m, m, 3 * m}, ep, 2 * f, d,
+                               3 * m);
+    // third, second, first
+    return pieces_product<true, true>(ctx, dgu, fp, pad_x ? xp : x, dp, ep, dma::pieces(3, 0x012, 0x000, m * fp, 0, m), fp, dp,
+                                      m);
 }
 
 int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* dh, const float* x, const float* w,
