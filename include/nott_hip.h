@@ -391,8 +391,8 @@ int nott_qk_norm_rope_bwd(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype d
  *   [g | u] = x·wᵀ + b,  h = act(g)·u        x [m, d], h [m, f]
  * gu [m, 2·f] (dtype, nullable) receives [g | u] for the backward.  No output may
  * overlap an input.  In fp32 large products are taken from bf16 pieces of all 24 bits
- * of their operands, to fp32's accuracy (workspace: three bf16 pieces of each); an
- * operand from 3.39e38 on then gives NaN, and one below 2^-110 is taken to 2^-134. */
+ * of their operands, to fp32's accuracy (workspace: four bf16 pieces of each); an
+ * operand below 2^-110 is then taken to 2^-134. */
 enum {
     NOTT_ACT_SILU = 0,       /* g·sigmoid(g) */
     NOTT_ACT_GELU = 1,       /* g·Φ(g) */

@@ -13,10 +13,11 @@
 // fp32, the small ones first: six products, where the fp32 matrix instructions take
 // the time of sixteen, and no further from 64 bits than those (8192 rows of 1024 ->
 // 2048 408 us, 554 with fp32 instructions on tiles of the same engine; gradients 456
-// and 459 against 557 and 600).  An infinity comes out as NaN, and from 3.39e38 a value
-// counts as one; the last piece ends at bf16's least number, so that values below
-// 2^-110 keep 2^-134 rather than their own last bit (inputs of 2^-110 come out with an
-// error of 1.5e-7 in the norm as all others, of 2^-115 with 1.1e-6).
+// and 459 against 557 and 600).  A fourth piece is hi with 0 for an infinity or NaN: it
+// takes hi's place in all products but hi·hi, so that an infinity enters a sum once, as
+// its product.  The last piece ends at bf16's least number, so that values below 2^-110
+// keep 2^-134 rather than their own last bit (inputs of 2^-110 come out with an error of
+// 1.5e-7 in the norm as all others, of 2^-115 with 1.1e-6).
 #include "gemm_dma.hpp"
 
 namespace {
@@ -228,6 +229,31 @@ __device__ __forceinline__ void store_piece(bf16_t* p, const float (&v)[E]) {
     else *p = f32_to_bf16(v[0]);
 }
 
+constexpr float kLargest = 3.40282347e38f;
+// v (fp32 operands) as four bf16 pieces `stride` elements apart: the nearest, the nearest
+// of what that leaves, of what both leave; and the first again with 0 in place of an
+// infinity or NaN, which have nothing in the other two.  Finite values that round to an
+// infinity take the largest finite piece.
+constexpr int kPieces = 4;
+template <int E>
+__device__ __forceinline__ void store_nearest(bf16_t* out, int64_t stride, float (&v)[E]) {
+    float hi[E], q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const bool finite = fabsf(v[e]) <= kLargest;
+        hi[e] = finite ? bf16_to_f32(f32_to_bf16(__builtin_amdgcn_fmed3f(v[e], -0x1.fep127f, 0x1.fep127f))) : 0.f;
+        q[e] = finite ? hi[e] : v[e];
+        v[e] = finite ? v[e] - hi[e] : 0.f;
+    }
+    store_piece<E>(out, q);
+    store_piece<E>(out + 3 * stride, hi);
+#pragma unroll
+    for (int p = 1; p < 3; ++p) {
+        store_piece<E>(out + p * stride, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] -= bf16_to_f32(f32_to_bf16(v[e]));
+    }
+}
 // v cut to bf16 toward zero; NaN stays.
 __device__ __forceinline__ float toward_zero(float v) {
     return v != v ? v : __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);
@@ -249,7 +275,7 @@ __device__ __forceinline__ void store_cut(bf16_t* out, int64_t stride, int piece
         for (int e = 0; e < E; ++e) {
             const bool none = v[e] == 0.f;
             q[e] = toward_zero(none ? least[e] : v[e]);
-            if (!none && fabsf(v[e]) <= 3.40282347e38f) v[e] -= q[e];
+            if (!none && fabsf(v[e]) <= kLargest) v[e] -= q[e];
         }
         store_piece<E>(out + p * stride, q);
     }
@@ -257,7 +283,7 @@ __device__ __forceinline__ void store_cut(bf16_t* out, int64_t stride, int piece
 
 // [dg|du] in rows of ld elements with zeros past 2f: as fp32 (whole, the generic
 // engine's operand) and as bf16 pieces, each `stride` elements behind the one before:
-// of a bf16 layer store_cut's, in fp32 the rounding of what is left.  A workgroup takes 64·E columns (E = 1, or
+// of a bf16 layer store_cut's, in fp32 store_nearest's.  A workgroup takes 64·E columns (E = 1, or
 // whole 16-byte chunks where all rows fit them and ld is 2f) and every gridDim.y-th
 // group of 4 rows; partial (null: no db) [gridDim.y][2f] receives its column sums of the unrounded
 // values.  Bound by memory: 8192 x 4096 bf16 with both pieces, 470 MB, 74 us (6.3 TB/s;
@@ -284,12 +310,8 @@ __global__ __launch_bounds__(256) void gated_dact_kernel(const T* __restrict__ d
         }
         if constexpr (sizeof(T) == 2) {
             store_cut<E>(out + at, stride, pieces, v);
-        } else {
-            for (int p = 0; p < pieces; ++p) {
-                store_piece<E>(out + p * stride + at, v);
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] -= bf16_to_f32(f32_to_bf16(v[e]));
-            }
+        } else if (pieces) {
+            store_nearest<E>(out + at, stride, v);
         }
     };
     if (c < f) {
@@ -389,8 +411,8 @@ int64_t up8(int64_t n) { return (n + 7) & ~int64_t(7); }
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
-// src [rows, cols] to bf16 pieces [prows, pcols] at dst, one behind the other, zeros
-// past src's rows and columns.  No rows: nothing.
+// src [rows, cols] to bf16 [prows, pcols] at dst, of fp32 store_nearest's pieces one behind
+// the other, zeros past src's rows and columns.  No rows: nothing.
 template <typename T>
 struct PieceJob {
     const T* src = nullptr;
@@ -402,11 +424,10 @@ struct PieceJob {
     PieceJob(const T* s, int64_t r, int64_t c, bf16_t* d, int64_t prows, int64_t pcols)
         : src(s), rows(r), cols(c), dst(d), chunks(prows * pcols / 8), row((uint32_t)(pcols / 8)) {}
 };
-// Two jobs in one launch, `pieces` pieces of each, every one the rounding of what the
-// ones before leave: the copy of a bf16 tensor whose rows no 16-byte load fits, and
+// Two jobs in one launch: the copy of a bf16 tensor whose rows no 16-byte load fits, and
 // fp32 tensors for the bf16 engine.  A thread has 8 elements.
 template <typename T>
-__global__ __launch_bounds__(256) void pieces_kernel(PieceJob<T> a, PieceJob<T> b, int pieces) {
+__global__ __launch_bounds__(256) void pieces_kernel(PieceJob<T> a, PieceJob<T> b) {
     const PieceJob<T> j = blockIdx.y ? b : a;
     const bool small = j.chunks < (int64_t)1 << 32;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < j.chunks; i += (int64_t)gridDim.x * 256) {
@@ -425,19 +446,16 @@ __global__ __launch_bounds__(256) void pieces_kernel(PieceJob<T> a, PieceJob<T> 
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = r < j.rows && c + e < j.cols ? Io<T>::ld(p, e) : 0.f;
         }
-        for (int k = 0; k < pieces; ++k) {
-            Pack16<bf16_t>::st(j.dst + (k * j.chunks + i) * 8, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] -= bf16_to_f32(f32_to_bf16(v[e]));
-        }
+        if constexpr (sizeof(T) == 2) Pack16<bf16_t>::st(j.dst + i * 8, v);
+        else store_nearest<8>(j.dst + i * 8, j.chunks * 8, v);
     }
 }
 template <typename T>
-void to_pieces(nott_ctx ctx, int pieces, const PieceJob<T>& a, const PieceJob<T>& b = {}) {
+void to_pieces(nott_ctx ctx, const PieceJob<T>& a, const PieceJob<T>& b = {}) {
     const int64_t most = std::max(a.chunks, b.chunks);
     if (most == 0) return;
     const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(most, 256), 8192);
-    hipLaunchKernelGGL(pieces_kernel<T>, dim3(blocks, b.chunks ? 2 : 1), dim3(256), 0, ctx->stream, a, b, pieces);
+    hipLaunchKernelGGL(pieces_kernel<T>, dim3(blocks, b.chunks ? 2 : 1), dim3(256), 0, ctx->stream, a, b);
 }
 
 // Few rows (single tokens of some sequences): the weights are streamed once, 16
@@ -609,8 +627,9 @@ struct Repeated {
     }
 };
 
-// The six products of fp32 pieces (hi 0, mid 1, lo 2), first factor and second.
-constexpr uint32_t kPairs = 6, kFirst = 0x001102, kSecond = 0x010120;
+// The six products of fp32 pieces (hi 0, mid 1, lo 2, finite hi 3), first factor and second:
+// lo·hi, hi·lo, mid·mid, mid·hi, hi·mid, hi·hi.
+constexpr uint32_t kPairs = 6, kFirst = 0x031132, kSecond = 0x013123;
 
 // Whether an fp32 product of M×N×K, with so many elements to split into pieces, goes to
 // the direct-to-LDS engine: its plan's time and the split's against the generic engine's
@@ -638,7 +657,7 @@ int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* x,
     bf16_t* xp = reinterpret_cast<bf16_t*>(ws.p);
     bf16_t* wp = xp + (pad_x ? m * dp : 0);
     using Job = PieceJob<bf16_t>;
-    to_pieces(ctx, 1, pad_x ? Job(x, m, d, xp, m, dp) : Job(), pad_w ? Job(w, 2 * f, d, wp, 2 * f, dp) : Job());
+    to_pieces(ctx, pad_x ? Job(x, m, d, xp, m, dp) : Job(), pad_w ? Job(w, 2 * f, d, wp, 2 * f, dp) : Job());
     const bf16_t* X = pad_x ? xp : x;
     const bf16_t* W = pad_w ? wp : w;
     if (rows) return forward_rows(ctx, m, dp, f, act, X, W, b, h, gu);
@@ -664,11 +683,11 @@ int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* x, 
         });
         return launch_status(ctx, "gated_linear");
     }
-    WorkspaceHold ws(ctx, 3 * sizeof(bf16_t) * (size_t)((m + 2 * f) * dp));
+    WorkspaceHold ws(ctx, kPieces * sizeof(bf16_t) * (size_t)((m + 2 * f) * dp));
     if (ws.failed()) return NOTT_ERR_ALLOC;
     bf16_t* xp = reinterpret_cast<bf16_t*>(ws.p);
-    bf16_t* wp = xp + 3 * m * dp;
-    to_pieces(ctx, 3, PieceJob<float>(x, m, d, xp, m, dp), PieceJob<float>(w, 2 * f, d, wp, 2 * f, dp));
+    bf16_t* wp = xp + kPieces * m * dp;
+    to_pieces(ctx, PieceJob<float>(x, m, d, xp, m, dp), PieceJob<float>(w, 2 * f, d, wp, 2 * f, dp));
     const int64_t deep = kPairs * ceil_div(dp, dma::BK) * dma::BK;
     const dma::Plan p = dma::plan(ctx, m, 2 * f, deep, false, false, 1);
     const GatedPieces ep{{h, gu, b, m, f, act, ok16(h, f) && ok16(gu, f)},
@@ -742,7 +761,7 @@ int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* dh
     int st = activation_bwd(ctx, m, f, fp, act, dh, gu, nullptr, dgu, pieces, db, accumulate);
     if (st != NOTT_OK) return st;
     using Job = PieceJob<bf16_t>;
-    to_pieces(ctx, 1, pad_x ? Job(x, m, d, xp, m, dp) : Job(), pad_w ? Job(w, 2 * f, d, wp, fp, dp) : Job());
+    to_pieces(ctx, pad_x ? Job(x, m, d, xp, m, dp) : Job(), pad_w ? Job(w, 2 * f, d, wp, fp, dp) : Job());
     if (dx) {   // the second piece, then the first
         const RowMajorStore<bf16_t> ep{dx, d, m, d, nullptr};
         st = dma_dx ? pieces_product<false, true>(ctx, dgu, fp, pad_w ? wp : w, dp, ep, dma::pieces(2, 0x01, 0x00, m * fp, 0, fp),
@@ -768,16 +787,16 @@ int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* dh,
     const bool pieces = pieces_dx || pieces_dw, whole = (dx && !pieces_dx) || (dw && !pieces_dw);
     const int64_t ld = pieces ? fp : 2 * f;
     WorkspaceHold ws(ctx, sizeof(float) * (size_t)(whole ? m * ld : 0) +
-                              3 * sizeof(bf16_t) * (size_t)((pieces ? m * fp : 0) + ((pieces_dw ? m : 0) + (pieces_dx ? fp : 0)) * dp));
+                              kPieces * sizeof(bf16_t) * (size_t)((pieces ? m * fp : 0) + ((pieces_dw ? m : 0) + (pieces_dx ? fp : 0)) * dp));
     if (ws.failed()) return NOTT_ERR_ALLOC;
     bf16_t* dgu = reinterpret_cast<bf16_t*>(ws.p);
-    bf16_t* xp = dgu + (pieces ? 3 * m * fp : 0);
-    bf16_t* wp = xp + (pieces_dw ? 3 * m * dp : 0);
-    float* all = reinterpret_cast<float*>(wp + (pieces_dx ? 3 * fp * dp : 0));
-    int st = activation_bwd(ctx, m, f, ld, act, dh, gu, whole ? all : nullptr, dgu, pieces ? 3 : 0, db, accumulate);
+    bf16_t* xp = dgu + (pieces ? kPieces * m * fp : 0);
+    bf16_t* wp = xp + (pieces_dw ? kPieces * m * dp : 0);
+    float* all = reinterpret_cast<float*>(wp + (pieces_dx ? kPieces * fp * dp : 0));
+    int st = activation_bwd(ctx, m, f, ld, act, dh, gu, whole ? all : nullptr, dgu, pieces ? kPieces : 0, db, accumulate);
     if (st != NOTT_OK) return st;
     using Job = PieceJob<float>;
-    to_pieces(ctx, 3, pieces_dx ? Job(w, 2 * f, d, wp, fp, dp) : Job(), pieces_dw ? Job(x, m, d, xp, m, dp) : Job());
+    to_pieces(ctx, pieces_dx ? Job(w, 2 * f, d, wp, fp, dp) : Job(), pieces_dw ? Job(x, m, d, xp, m, dp) : Job());
     const AccStore to_dx{dx, m, d, 0}, to_dw{dw, 2 * f, d, accumulate};
     if (pieces_dx) {
         st = pieces_product<false, true>(ctx, dgu, fp, wp, dp, to_dx, dma::pieces(kPairs, kFirst, kSecond, m * fp, fp * dp, fp),
