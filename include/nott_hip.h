@@ -390,7 +390,9 @@ int nott_qk_norm_rope_bwd(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype d
  * then up rows; b [2·f] fp32 nullable:
  *   [g | u] = x·wᵀ + b,  h = act(g)·u        x [m, d], h [m, f]
  * gu [m, 2·f] (dtype, nullable) receives [g | u] for the backward.  No output may
- * overlap an input.  In fp32 large products are taken from bf16 pieces of all 24 bits
+ * overlap an input.  act and act' hold over the whole range of fp32, infinities by
+ * their limits (a gate that its bias masks with −inf or the lowest value gives 0).
+ * In fp32 large products are taken from bf16 pieces of all 24 bits
  * of their operands, to fp32's accuracy (workspace: four bf16 pieces of each); an
  * operand below 2^-110 is then taken to 2^-134. */
 enum {

@@ -27,7 +27,7 @@ using nott::ceil_div;
 using nott::launch_status;
 using nott::WorkspaceHold;
 
-// e^x, the rounding of x·log2 e taken into the result; x within ±126.
+// e^x, the rounding of x·log2 e taken into the result; x at most 88.
 __device__ __forceinline__ float exp_near(float x) {
     constexpr float kLog2e = 1.4426950408889634f;
     const float t = x * kLog2e;
@@ -36,29 +36,35 @@ __device__ __forceinline__ float exp_near(float x) {
     return fmaf(e, r * 0.69314718f, e);
 }
 // FAST (bf16 results): the exponent's rounding, |x|·2^-24 of the result, stays in;
-// no clamp is needed then (exp2 ends in 0 or infinity, 1/infinity is 0).
+// no clamp is needed then (exp2 ends in 0 or infinity, 1/infinity is 0).  Otherwise 0
+// from where it would be below fp32's least normal number (x < −87.3).
 template <bool FAST>
 __device__ __forceinline__ float sigmoid(float x) {
     if constexpr (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.4426950f));
-    const float e = exp_near(__builtin_amdgcn_fmed3f(-x, -80.f, 80.f));
-    return x != x ? x : __builtin_amdgcn_rcpf(1.f + e);
+    const float e = exp_near(__builtin_amdgcn_fmed3f(-x, -87.f, 87.3f));
+    return x != x ? x : x < -87.3f ? 0.f : __builtin_amdgcn_rcpf(1.f + e);
 }
 
-// The activation (a) and its derivative (da).
+// The activation (a) and its derivative (da).  g = ±infinity gives their limits: a
+// product of g and a factor that ends in 0 takes −kLargest for −infinity, and the
+// derivatives' terms take g within ±1e4, past which all of their exponentials are 0
+// or 1 (a NaN stays in e or cdf).
+constexpr float kLargest = 3.40282347e38f;
 template <int ACT, bool FAST>
 __device__ __forceinline__ void activate(float g, float& a, float& da) {
+    const float from = fmaxf(g, -kLargest), near = __builtin_amdgcn_fmed3f(g, -1e4f, 1e4f);
     if constexpr (ACT == NOTT_ACT_SILU) {
         const float e = sigmoid<FAST>(g);
-        a = g * e;
-        da = fmaf(a, 1.f - e, e);
+        a = from * e;
+        da = fmaf(near * e, 1.f - e, e);
     } else if constexpr (ACT == NOTT_ACT_GELU) {
         const float cdf = 0.5f * erfcf(g * -0.70710678f);
-        a = g * cdf;
-        da = fmaf(g * 0.39894228f, exp_near(fmaxf(-0.5f * g * g, -120.f)), cdf);
+        a = from * cdf;
+        da = fmaf(near * 0.39894228f, exp_near(fmaxf(-0.5f * near * near, -120.f)), cdf);
     } else if constexpr (ACT == NOTT_ACT_GELU_TANH) {
         const float e = sigmoid<FAST>(1.5957691f * fmaf(0.044715f * g, g * g, g));
-        a = g * e;
-        da = fmaf(a * (1.f - e), 1.5957691f * fmaf(0.134145f * g, g, 1.f), e);
+        a = from * e;
+        da = fmaf(near * e * (1.f - e), 1.5957691f * fmaf(0.134145f * near, near, 1.f), e);
     } else if constexpr (ACT == NOTT_ACT_RELU) {
         a = relu_out(g);
         da = g > 0.f ? 1.f : g != g ? g : 0.f;
@@ -229,7 +235,6 @@ __device__ __forceinline__ void store_piece(bf16_t* p, const float (&v)[E]) {
     else *p = f32_to_bf16(v[0]);
 }
 
-constexpr float kLargest = 3.40282347e38f;
 // v (fp32 operands) as four bf16 pieces `stride` elements apart: the nearest, the nearest
 // of what that leaves, of what both leave; and the first again with 0 in place of an
 // infinity or NaN, which have nothing in the other two.  Finite values that round to an
