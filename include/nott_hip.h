@@ -430,7 +430,8 @@ int nott_token_logprob_fwd(nott_ctx ctx, nott_dtype dtype, int64_t n, int64_t c,
                            float* lse, float* top_logprob, int64_t* top_index);
 /* dlogits = scale·(dlogprob·([j = label] − p) − dentropy·p·(log p + entropy)), from
  * the forward's lse (and entropy with dentropy, which is nullable).  dlogits may
- * be logits.  Rows with every token masked get zeros. */
+ * be logits.  Rows with every token masked get zeros.  p carries the rounding of the
+ * fp32 lse, 2^-24 of |lse|: logits with a common offset of 1e4 have gradients to 6e-4. */
 int nott_token_logprob_bwd(nott_ctx ctx, nott_dtype dtype, int64_t n, int64_t c, const void* logits,
                            const int64_t* labels, double scale, const float* lse, const float* entropy,
                            const float* dlogprob, const float* dentropy, void* dlogits);

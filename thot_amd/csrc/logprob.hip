@@ -61,10 +61,11 @@ struct Stats {
 #pragma unroll
         for (int e = 0; e < N; ++e) n = fmaxf(n, v[e]);
         raise(n, sc);
-        const float off = -n * sc.to_log2;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const float w = fmaf(v[e], sc.to_log2, off);
+            // the difference first: n·to_log2 rounded would leave 2^-24 of |n| in every
+            // exponent (rows masked with −1e9, logits with a common offset)
+            const float w = (v[e] - n) * sc.to_log2;
             const float p = __builtin_amdgcn_exp2f(w);
             s += p;
             t = fmaf(p, fmaxf(w, kLeast), t);
