@@ -164,9 +164,9 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs<T> a, int tpb) {
                         const float w = side[u] ? go[1][v] : go[0][v];
                         const float z = a.norm ? xv[u][v] * r * gm : xv[u][v];
                         const float zo = a.norm ? xo[u][v] * r * w : xo[u][v];
-                        ov[v] = fmaf(zo, s, z * c);
+                        ov[v] = pair[v] < 0 ? z : fmaf(zo, s, z * c);   // unrotated: as it is, infinities too
                     } else {
-                        const float dz = fmaf(dn[u][v], s, dv[u][v] * c), xh = xv[u][v] * r;
+                        const float dz = pair[v] < 0 ? dv[u][v] : fmaf(dn[u][v], s, dv[u][v] * c), xh = xv[u][v] * r;
                         if (base + u < items) {
                             if (side[u]) dg[1][v] = fmaf(dz, xh, dg[1][v]);
                             else dg[0][v] = fmaf(dz, xh, dg[0][v]);
@@ -253,6 +253,7 @@ __global__ __launch_bounds__(256, BWD ? 3 : 1) void rope_vec_kernel(RopeArgs<T> 
     const bool rotated = slot < hc;
     const int c0 = rotated ? slot : 2 * hc + 2 * (slot - hc), c1 = rotated ? slot + hc : c0 + 1;
     const bool has0 = c0 < nc, has1 = c1 < nc;
+    const int n0 = half - c0 * (E / 2), n1 = half - c1 * (E / 2);   // neighbours: rotated pairs from each chunk's start on
     const int e0 = has0 ? c0 * E : 0, e1 = has1 ? c1 * E : 0;
     const int ppc = inter ? E / 2 : E, chunks = inter ? nc : hc, width = ppc * chunks;   // of a token's table
     const float inv_dh = 1.f / (float)a.dh;
@@ -309,11 +310,11 @@ __global__ __launch_bounds__(256, BWD ? 3 : 1) void rope_vec_kernel(RopeArgs<T> 
                 float v0[E], v1[E];
                 const f32x4* tab = table + (int)tok[u] * (width / 2);
                 // turns the pair (a, b) by {cos, sin}, BWD: back
-                auto turn2 = [](float& a, float& b, float c, float s) {
+                auto turn2 = [](float& a, float& b, float c, float s, bool on = true) {
                     if (BWD) s = -s;
                     const float y = fmaf(-b, s, a * c);
-                    b = fmaf(a, s, b * c);
-                    a = y;
+                    b = on ? fmaf(a, s, b * c) : b;
+                    a = on ? y : a;
                 };
                 auto turn = [&](float (&p)[E], float (&q)[E]) {
                     if (half == 0) return;
@@ -330,10 +331,11 @@ __global__ __launch_bounds__(256, BWD ? 3 : 1) void rope_vec_kernel(RopeArgs<T> 
 #pragma unroll
                     for (int e = 0; e < E; e += 4) {
                         const f32x4 cs = tab[e / 4 * chunks + (has0 ? c0 : 0)], ct = tab[e / 4 * chunks + (has1 ? c1 : 0)];
-                        turn2(p[e], p[e + 1], cs.x, cs.y);
-                        turn2(p[e + 2], p[e + 3], cs.z, cs.w);
-                        turn2(q[e], q[e + 1], ct.x, ct.y);
-                        turn2(q[e + 2], q[e + 3], ct.z, ct.w);
+                        // past the rotated pairs as they are (an infinity times a sine of 0 is NaN)
+                        turn2(p[e], p[e + 1], cs.x, cs.y, e / 2 < n0);
+                        turn2(p[e + 2], p[e + 3], cs.z, cs.w, e / 2 + 1 < n0);
+                        turn2(q[e], q[e + 1], ct.x, ct.y, e / 2 < n1);
+                        turn2(q[e + 2], q[e + 3], ct.z, ct.w, e / 2 + 1 < n1);
                     }
                 };
                 float x0[E], x1[E], r = 1.f;
