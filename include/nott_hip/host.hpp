@@ -233,6 +233,12 @@ inline void* ptr(const Tensor& t) { return present(t) ? t.data_ptr() : nullptr; 
 inline float* fptr(const Tensor& t) { return present(t) ? t.data_ptr<float>() : nullptr; }
 
 inline Tensor contig(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+// An input as the kernels take it.  Whether it needs a gradient is asked here, before the
+// copy of a view: under autograd::Function's forward (grad mode off) the copy needs none.
+inline Tensor input(AutogradContext* ctx, const Tensor& x) {
+    ctx->saved_data["needs_dx"] = x.requires_grad();
+    return contig(x);
+}
 
 // Gradient buffers a fused optimizer keeps in its flat arena, by parameter.
 // A parameter whose .grad() was reset to none (Optimizer::zero_grad(true))
@@ -324,7 +330,7 @@ struct Conv2dFn : torch::autograd::Function<Conv2dFn> {
     // x: input; w: master weight (fp32, receives the gradient); wc: weight in
     // the compute dtype (== w for fp32); b: fp32 bias or undefined.
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w, Tensor wc, Tensor b, std::vector<int64_t> geom) {
-        x = contig(x);
+        x = input(ctx, x);
         const nott_conv2d_desc d = desc(x, wc, geom);
         const int64_t p = (d.h + 2 * d.pad_h - d.dil_h * (d.r - 1) - 1) / d.stride_h + 1;
         const int64_t q = (d.w + 2 * d.pad_w - d.dil_w * (d.s - 1) - 1) / d.stride_w + 1;
@@ -334,7 +340,6 @@ struct Conv2dFn : torch::autograd::Function<Conv2dFn> {
         if (!wd.defined()) check(nott_conv2d_fwd(c, &d, dtype_of(x), ptr(x), ptr(wc), fptr(b), ptr(y)), c, "conv2d forward");
         ctx->save_for_backward({x, w, wc, b, wd});
         ctx->saved_data["geom"] = geom;
-        ctx->saved_data["needs_dx"] = x.requires_grad();
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -371,7 +376,7 @@ struct Conv2dFn : torch::autograd::Function<Conv2dFn> {
 struct Conv2dReluFn : torch::autograd::Function<Conv2dReluFn> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w, Tensor wc, Tensor b, std::vector<int64_t> geom,
                           bool consumer_masks) {
-        x = contig(x);
+        x = input(ctx, x);
         const nott_conv2d_desc d = Conv2dFn::desc(x, wc, geom);
         const int64_t p = (d.h + 2 * d.pad_h - d.dil_h * (d.r - 1) - 1) / d.stride_h + 1;
         const int64_t q = (d.w + 2 * d.pad_w - d.dil_w * (d.s - 1) - 1) / d.stride_w + 1;
@@ -382,7 +387,6 @@ struct Conv2dReluFn : torch::autograd::Function<Conv2dReluFn> {
             check(nott_conv2d_fwd_act(c, &d, dtype_of(x), ptr(x), ptr(wc), fptr(b), 1, ptr(y)), c, "conv2d+relu forward");
         ctx->save_for_backward({x, w, wc, b, y, wd});
         ctx->saved_data["geom"] = geom;
-        ctx->saved_data["needs_dx"] = x.requires_grad();
         ctx->saved_data["consumer_masks"] = consumer_masks;
         return y;
     }
@@ -422,7 +426,7 @@ struct Conv2dReluFn : torch::autograd::Function<Conv2dReluFn> {
 constexpr int64_t kLinRelu = 1, kLinConsumerMasks = 2, kLinReluInput = 4;
 struct LinearFn : torch::autograd::Function<LinearFn> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w, Tensor wc, Tensor b, int64_t flags) {
-        x = contig(x);
+        x = input(ctx, x);
         const int64_t kin = x.size(-1), m = x.numel() / kin, nout = wc.size(0);
         auto shape = x.sizes().vec();
         shape.back() = nout;
@@ -432,7 +436,6 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         check(nott_linear_fwd_act(c, dtype_of(x), m, kin, nout, ptr(x), ptr(wc), fptr(b), relu ? 1 : 0, ptr(y)), c,
               "linear forward");
         ctx->save_for_backward({x, w, wc, b, relu && !(flags & kLinConsumerMasks) ? y : Tensor()});
-        ctx->saved_data["needs_dx"] = x.requires_grad();
         ctx->saved_data["flags"] = flags;
         return y;
     }
@@ -571,7 +574,7 @@ struct AvgPoolGlobalFn : torch::autograd::Function<AvgPoolGlobalFn> {
 struct BatchNorm2dFn : torch::autograd::Function<BatchNorm2dFn> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor gamma, Tensor beta, Tensor running_mean,
                           Tensor running_var, double eps, double momentum) {
-        x = contig(x);
+        x = input(ctx, x);
         const int64_t n = x.size(0), ch = x.size(1), hw = x.size(2) * x.size(3);
         Tensor y = torch::empty_like(x);
         auto fo = x.options().dtype(torch::kFloat32);
@@ -581,7 +584,6 @@ struct BatchNorm2dFn : torch::autograd::Function<BatchNorm2dFn> {
                                    fptr(running_mean), fptr(running_var), ptr(y), fptr(mean), fptr(rstd)),
               c, "batchnorm forward");
         ctx->save_for_backward({x, gamma, beta, mean, rstd});
-        ctx->saved_data["needs_dx"] = x.requires_grad();
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -605,7 +607,7 @@ struct BatchNorm2dFn : torch::autograd::Function<BatchNorm2dFn> {
 struct BatchNorm2dReluFn : torch::autograd::Function<BatchNorm2dReluFn> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor gamma, Tensor beta, Tensor running_mean,
                           Tensor running_var, double eps, double momentum) {
-        x = contig(x);
+        x = input(ctx, x);
         const int64_t n = x.size(0), ch = x.size(1), hw = x.size(2) * x.size(3);
         Tensor y = torch::empty_like(x);
         auto fo = x.options().dtype(torch::kFloat32);
@@ -616,7 +618,6 @@ struct BatchNorm2dReluFn : torch::autograd::Function<BatchNorm2dReluFn> {
                                        fptr(rstd)),
               c, "batchnorm+relu forward");
         ctx->save_for_backward({x, gamma, beta, mean, rstd});
-        ctx->saved_data["needs_dx"] = x.requires_grad();
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -643,7 +644,7 @@ struct BatchNorm2dReluFn : torch::autograd::Function<BatchNorm2dReluFn> {
 struct BatchNorm2dReluMaxPool2dFn : torch::autograd::Function<BatchNorm2dReluMaxPool2dFn> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor gamma, Tensor beta, Tensor running_mean,
                           Tensor running_var, double eps, double momentum, std::vector<int64_t> pool_geom) {
-        x = contig(x);
+        x = input(ctx, x);
         const int64_t n = x.size(0), ch = x.size(1), hw = x.size(2) * x.size(3);
         auto fo = x.options().dtype(torch::kFloat32);
         Tensor mean = torch::empty({ch}, fo), rstd = torch::empty({ch}, fo), coef = torch::empty({2 * ch}, fo);
@@ -660,7 +661,6 @@ struct BatchNorm2dReluMaxPool2dFn : torch::autograd::Function<BatchNorm2dReluMax
               c, "batchnorm+relu+maxpool forward");
         ctx->save_for_backward({x, gamma, beta, mean, rstd, tap});
         ctx->saved_data["geom"] = pool_geom;
-        ctx->saved_data["needs_dx"] = x.requires_grad();
         ctx->mark_non_differentiable({tap});
         return y;
     }
@@ -688,7 +688,7 @@ struct BatchNorm2dReluMaxPool2dFn : torch::autograd::Function<BatchNorm2dReluMax
 struct BatchNorm2dAddReluFn : torch::autograd::Function<BatchNorm2dAddReluFn> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor skip, Tensor gamma, Tensor beta,
                           Tensor running_mean, Tensor running_var, double eps, double momentum, bool consumer_masks) {
-        x = contig(x);
+        x = input(ctx, x);
         skip = contig(skip);
         const int64_t n = x.size(0), ch = x.size(1), hw = x.size(2) * x.size(3);
         Tensor y = torch::empty_like(x);
@@ -700,7 +700,6 @@ struct BatchNorm2dAddReluFn : torch::autograd::Function<BatchNorm2dAddReluFn> {
                                        fptr(rstd)),
               c, "batchnorm+add+relu forward");
         ctx->save_for_backward({x, gamma, beta, mean, rstd, consumer_masks ? Tensor() : y});
-        ctx->saved_data["needs_dx"] = x.requires_grad();
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -727,7 +726,7 @@ struct BatchNorm2dAddReluFn : torch::autograd::Function<BatchNorm2dAddReluFn> {
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor gamma, Tensor beta, Tensor gamma_c, Tensor beta_c,
                           double eps) {
-        x = contig(x);
+        x = input(ctx, x);
         const int64_t d = x.size(-1), rows = x.numel() / d;
         Tensor y = torch::empty_like(x);
         auto fo = x.options().dtype(torch::kFloat32);
@@ -737,7 +736,6 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
                                  fptr(rstd)),
               c, "layernorm forward");
         ctx->save_for_backward({x, gamma, beta, gamma_c, mean, rstd});
-        ctx->saved_data["needs_dx"] = x.requires_grad();
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -854,7 +852,7 @@ struct QkNormRopeFn : torch::autograd::Function<QkNormRopeFn> {
 // may come.
 struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w, Tensor wc, Tensor b, int64_t act, bool keep) {
-        x = contig(x);
+        x = input(ctx, x);
         if (x.dim() < 1 || wc.dim() != 2 || wc.size(0) % 2 || wc.numel() == 0 || x.size(-1) != wc.size(1) ||
             !operand(wc, x, x.scalar_type(), wc.numel()))
             throw std::invalid_argument("Nott::HIP: a gated linear layer's weight must be [2·f, d] for x [..., d], of x's type");
@@ -871,7 +869,6 @@ struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
         check(nott_gated_linear_fwd(c, dtype_of(x), m, d, f, (int)act, ptr(x), ptr(wc), fptr(b), ptr(h), ptr(gu)), c,
               "gated linear forward");
         ctx->save_for_backward({x, w, wc, b, gu});
-        ctx->saved_data["needs_dx"] = x.requires_grad();
         ctx->saved_data["act"] = act;
         return h;
     }
