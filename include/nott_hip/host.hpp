@@ -814,6 +814,7 @@ struct QkNormRopeFn : torch::autograd::Function<QkNormRopeFn> {
                                     present(inv_freq) ? positions.data_ptr<int64_t>() : nullptr,
                                     present(inv_freq) ? inv_freq.data_ptr<double>() : nullptr, ptr(yq), ptr(yk)),
               c, "norm and rotation forward");
+        ctx->set_materialize_grads(false);
         ctx->save_for_backward({q, k, gamma_q, gamma_k, gamma_qc, gamma_kc, positions, inv_freq});
         ctx->saved_data["sections"] = sections;
         ctx->saved_data["interleaved"] = interleaved;
@@ -824,6 +825,7 @@ struct QkNormRopeFn : torch::autograd::Function<QkNormRopeFn> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         auto s = ctx->get_saved_variables();
         Tensor q = s[0], k = s[1], positions = s[6], inv_freq = s[7];
+        if (!grads[0].defined() && !grads[1].defined()) return variable_list(12);
         nott_qk_rope_desc d = desc(q, k, positions, inv_freq, ctx->saved_data["sections"].toIntVector(),
                                    ctx->saved_data["interleaved"].toBool(), ctx->saved_data["norm"].toBool(),
                                    ctx->saved_data["eps"].toDouble());
@@ -1006,6 +1008,7 @@ struct TokenLogProbFn : torch::autograd::Function<TokenLogProbFn> {
         check(nott_token_logprob_fwd(h, dtype_of(logits), n, c, ptr(logits), labels.data_ptr<int64_t>(), scale, 0, fptr(lp),
                                      fptr(ent), fptr(lse), nullptr, nullptr),
               h, "token log probability");
+        ctx->set_materialize_grads(false);   // an output that a loss leaves out costs nothing
         ctx->save_for_backward({logits, labels, lse, ent});
         ctx->saved_data["scale"] = scale;
         return {lp, ent};
@@ -1013,6 +1016,7 @@ struct TokenLogProbFn : torch::autograd::Function<TokenLogProbFn> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         auto s = ctx->get_saved_variables();
         Tensor logits = s[0], labels = s[1], lse = s[2], ent = s[3];
+        if (!grads[0].defined() && !grads[1].defined()) return variable_list(3);
         Tensor dlp = grads[0].defined() ? contig(grads[0]) : torch::zeros_like(lse);
         Tensor dent = grads[1].defined() ? contig(grads[1]) : Tensor();
         Tensor out = torch::empty_like(logits);
