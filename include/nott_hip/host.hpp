@@ -229,6 +229,9 @@ inline bool operand(const Tensor& t, const Tensor& x, torch::ScalarType type, in
     return t.scalar_type() == type && t.numel() == n && t.is_contiguous() && t.device() == x.device();
 }
 
+// Whether a parameter's gradient can be accumulated (or need not be): it is fp32.
+inline bool trainable(const Tensor& t) { return !present(t) || !t.requires_grad() || t.scalar_type() == torch::kFloat32; }
+
 inline void* ptr(const Tensor& t) { return present(t) ? t.data_ptr() : nullptr; }
 inline float* fptr(const Tensor& t) { return present(t) ? t.data_ptr<float>() : nullptr; }
 
@@ -806,6 +809,8 @@ struct QkNormRopeFn : torch::autograd::Function<QkNormRopeFn> {
         for (const Tensor& g : {gamma_q, gamma_k})
             if (present(g) && !operand(g, q, g.scalar_type(), d.dh))
                 throw std::invalid_argument("Nott::HIP: a weight must be [dh] on q's device");
+        if (!trainable(gamma_q) || !trainable(gamma_k))
+            throw std::invalid_argument("Nott::HIP: a weight that needs a gradient must be fp32");
         Tensor yq = torch::empty({d.b, d.hq, d.t, d.dh}, q.options()), yk = torch::empty({d.b, d.hk, d.t, d.dh}, q.options());
         strides(d.yq_stride, yq, 2, 1);
         strides(d.yk_stride, yk, 2, 1);
@@ -860,6 +865,8 @@ struct GatedLinearFn : torch::autograd::Function<GatedLinearFn> {
             throw std::invalid_argument("Nott::HIP: a gated linear layer's weight must be [2·f, d] for x [..., d], of x's type");
         if (!operand(w, x, w.scalar_type(), wc.numel()))
             throw std::invalid_argument("Nott::HIP: a gated linear layer's weight and its working copy differ");
+        if (!trainable(w))
+            throw std::invalid_argument("Nott::HIP: a gated linear layer's weight that needs a gradient must be fp32");
         if (present(b) && !operand(b, x, torch::kFloat32, wc.size(0)))
             throw std::invalid_argument("Nott::HIP: a gated linear layer's bias must be [2·f] in fp32");
         const int64_t d = x.size(-1), m = x.numel() / d, f = wc.size(0) / 2;
