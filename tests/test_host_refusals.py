@@ -34,3 +34,17 @@ def test_trained_head_weight_that_is_not_fp32(host, which):
         host.qk_norm_rope(q, q, **{which: bf16(8)})
     with pytest.raises(ValueError, match="HIP device"):
         host.qk_norm_rope(q, q, **{which: torch.ones(8).requires_grad_(), which + "_compute": bf16(8)})
+
+
+@pytest.mark.parametrize("kw", [dict(positions=torch.zeros(1, 1, 2, dtype=torch.int64)), dict(sections=[4])])
+def test_positions_that_nothing_uses(host, kw):
+    q = torch.ones(1, 2, 3, 8)
+    with pytest.raises(ValueError, match="inv_freq"):
+        host.qk_norm_rope(q, q, **kw)
+
+
+def test_no_rotated_elements(host):
+    """Empty frequencies are frequencies: the call gets as far as the device."""
+    q = torch.ones(1, 2, 3, 8)
+    with pytest.raises(ValueError, match="HIP device"):
+        host.qk_norm_rope(q, q, torch.zeros(1, 1, 2, dtype=torch.int64), torch.ones(0, dtype=torch.float64))

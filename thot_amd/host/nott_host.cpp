@@ -574,6 +574,8 @@ PYBIND11_MODULE(_nott_host, m) {
     m.def("qk_norm_rope", [=](const Tensor& q, const Tensor& k, const OptT& positions, const OptT& inv_freq, const OptT& gq,
                               const OptT& gk, const OptT& gqc, const OptT& gkc, std::vector<int64_t> sections,
                               bool interleaved, bool norm, double eps) {
+        if (!inv_freq && (positions || !sections.empty()))
+            throw std::invalid_argument("Nott::HIP: positions and sections need inv_freq");
         auto r = NH::QkNormRopeFn::apply(q, k, NH::or_absent(given(gq), q), NH::or_absent(given(gk), q), compute(gqc, gq, q),
                                          compute(gkc, gk, q), NH::or_absent(given(positions), q),
                                          NH::or_absent(given(inv_freq), q), sections, interleaved, norm, eps);
