@@ -26,7 +26,7 @@ ROCM_LIB = "/opt/rocm/lib"
 HIP_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-mcode-object-version=5",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-Wno-unused-result",
+    "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-Wno-unused-result", "-Werror=align-mismatch",
     f"-I{INCLUDE}", f"-I{CSRC}",
 ]
 

@@ -441,7 +441,8 @@ __global__ __launch_bounds__(256) void pieces_kernel(PieceJob<T> a, PieceJob<T> 
         float v[8];
         if (r < j.rows && c + 8 <= j.cols) {
             if constexpr (sizeof(T) == 2) {
-                Pack16<bf16_t>::unpack(*reinterpret_cast<const u32x4_any*>(p), v);
+                const u32x4 raw = *reinterpret_cast<const u32x4_any*>(p);   // a copy: the reference would claim 16-byte alignment
+                Pack16<bf16_t>::unpack(raw, v);
             } else {
                 const f32x4 lo = reinterpret_cast<const f32x4_any*>(p)[0], hi = reinterpret_cast<const f32x4_any*>(p)[1];
 #pragma unroll
