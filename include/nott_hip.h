@@ -414,8 +414,8 @@ int nott_gated_linear_bwd(nott_ctx ctx, nott_dtype dtype, int64_t m, int64_t d, 
 
 /* ---- log probabilities of given tokens ----------------------------------------
  * What scoring, distillation and policy-gradient losses take from logits [n, c]
- * (dtype) beside the mean cross-entropy above.  With z = scale·logits (scale > 0,
- * an inverse temperature), per row, all outputs fp32 but the indices:
+ * (dtype) beside the mean cross-entropy above.  With z = scale·logits (an
+ * inverse temperature, 1e-30 <= scale < 1e30), per row, all outputs fp32 but the indices:
  *   lse = log Σ exp(z),  logprob = z[label] − lse,  entropy = −Σ p·log p, p = exp(z − lse)
  * and, with top > 0, the `top` largest logits, largest first (equal ones: lowest
  * column first; NaN counts as largest): top_logprob, top_index [n, top].

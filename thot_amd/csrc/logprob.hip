@@ -497,6 +497,10 @@ int backward(nott_ctx ctx, int64_t n, int64_t c, const T* logits, const int64_t*
     return nott::launch_status(ctx, "token_logprob backward");
 }
 
+// What fp32 holds, with room for a logit's product (a scale that rounds to 0 would make
+// NaN of a masked token).
+bool valid_scale(double scale) { return scale >= 1e-30 && scale < 1e30; }
+
 }  // namespace
 
 extern "C" int nott_token_logprob_fwd(nott_ctx ctx, nott_dtype dtype, int64_t n, int64_t c, const void* logits,
@@ -506,7 +510,7 @@ extern "C" int nott_token_logprob_fwd(nott_ctx ctx, nott_dtype dtype, int64_t n,
     NOTT_REQUIRE(ctx, nott::valid_dtype(dtype), "nott_token_logprob_fwd: bad dtype");
     NOTT_REQUIRE(ctx, n >= 0 && c > 0 && n < (int64_t(1) << 31) && c < (int64_t(1) << 31),
                  "nott_token_logprob_fwd: need 0 <= n and 0 < c, both below 2^31");
-    NOTT_REQUIRE(ctx, scale > 0.0 && scale < 1e30, "nott_token_logprob_fwd: scale must be positive and finite");
+    NOTT_REQUIRE(ctx, valid_scale(scale), "nott_token_logprob_fwd: scale must be 1e-30 to 1e30");
     NOTT_REQUIRE(ctx, top >= 0 && top <= kMaxTop && top <= c, "nott_token_logprob_fwd: top must be 0 to min(c, 64)");
     if (n == 0) return NOTT_OK;
     NOTT_REQUIRE(ctx, logits && labels && logprob, "nott_token_logprob_fwd: null buffer");
@@ -524,7 +528,7 @@ extern "C" int nott_token_logprob_bwd(nott_ctx ctx, nott_dtype dtype, int64_t n,
     NOTT_REQUIRE(ctx, nott::valid_dtype(dtype), "nott_token_logprob_bwd: bad dtype");
     NOTT_REQUIRE(ctx, n >= 0 && c > 0 && n < (int64_t(1) << 31) && c < (int64_t(1) << 31),
                  "nott_token_logprob_bwd: need 0 <= n and 0 < c, both below 2^31");
-    NOTT_REQUIRE(ctx, scale > 0.0 && scale < 1e30, "nott_token_logprob_bwd: scale must be positive and finite");
+    NOTT_REQUIRE(ctx, valid_scale(scale), "nott_token_logprob_bwd: scale must be 1e-30 to 1e30");
     if (n == 0) return NOTT_OK;
     NOTT_REQUIRE(ctx, logits && labels && lse && dlogprob && dlogits, "nott_token_logprob_bwd: null buffer");
     NOTT_REQUIRE(ctx, !dentropy || entropy, "nott_token_logprob_bwd: dentropy needs entropy");

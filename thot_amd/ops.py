@@ -851,8 +851,8 @@ def _logprob_shapes(logits: torch.Tensor, labels: torch.Tensor, scale: float):
         raise ValueError("logits must be [n, c] with c > 0")
     if tuple(labels.shape) != (logits.shape[0],):
         raise ValueError(f"labels has shape {tuple(labels.shape)}, expected {(logits.shape[0],)}")
-    if not 0 < scale < 1e30:
-        raise ValueError("scale must be positive and finite")
+    if not 1e-30 <= scale < 1e30:
+        raise ValueError("scale must be 1e-30 to 1e30")
     return logits.shape
 
 
