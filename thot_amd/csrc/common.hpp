@@ -251,6 +251,16 @@ __device__ __forceinline__ float lane_f32(float v) {
 // ReLU as torch::relu computes it (reference relu.hpp:13): a NaN passes.
 __device__ __forceinline__ float relu_out(float x) { return (x > 0.f || x != x) ? x : 0.f; }
 
+// e^x for x <= 88; what the rounding of x·log2 e leaves (2^-19 of the result at x = −30)
+// is taken into the result.  NaN stays.
+__device__ __forceinline__ float exp_fine(float x) {
+    constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718f;
+    const float t = x * kLog2e;
+    const float r = fmaf(x, kLog2e, -t);
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, r * kLn2, e);
+}
+
 // Σ_{z<n} p[z·stride] (n ≥ 1) as 4 floats, added in z order, with the loads
 // of 8 consecutive z in flight together (a loop over a run-time count
 // otherwise waits for each load before issuing the next).  Loads past n

@@ -7,7 +7,9 @@
 // for dx, of which the second ends at 2^-15 of a value where dx itself is rounded to
 // 2^-8 (one piece put as much into dx as its rounding: 2.3e-3 in the norm for 1.7e-3).
 //
-// fp32 layers take the bf16 matrix cores as well, wherever the products are large:
+// fp32 layers take the bf16 matrix cores as well, wherever the products are large
+// (products of bf16 pieces: Henry, Tang and Heinecke, Leveraging the bfloat16 Artificial
+// Intelligence Datatype For Higher-Precision Computations, 2019):
 // v = hi + mid + lo holds all 24 bits, and the six products of pieces that reach
 // 2^-23 of the whole (hi·hi, hi·mid, mid·hi, mid·mid, hi·lo, lo·hi) are summed in
 // fp32, the small ones first: six products, where the fp32 matrix instructions take
@@ -27,21 +29,13 @@ using nott::ceil_div;
 using nott::launch_status;
 using nott::WorkspaceHold;
 
-// e^x, the rounding of x·log2 e taken into the result; x at most 88.
-__device__ __forceinline__ float exp_near(float x) {
-    constexpr float kLog2e = 1.4426950408889634f;
-    const float t = x * kLog2e;
-    const float r = fmaf(x, kLog2e, -t);
-    const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, r * 0.69314718f, e);
-}
 // FAST (bf16 results): the exponent's rounding, |x|·2^-24 of the result, stays in;
 // no clamp is needed then (exp2 ends in 0 or infinity, 1/infinity is 0).  Otherwise 0
 // from where it would be below fp32's least normal number (x < −87.3).
 template <bool FAST>
 __device__ __forceinline__ float sigmoid(float x) {
     if constexpr (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.4426950f));
-    const float e = exp_near(__builtin_amdgcn_fmed3f(-x, -87.f, 87.3f));
+    const float e = exp_fine(__builtin_amdgcn_fmed3f(-x, -87.f, 87.3f));
     return x != x ? x : x < -87.3f ? 0.f : __builtin_amdgcn_rcpf(1.f + e);
 }
 
@@ -60,7 +54,7 @@ __device__ __forceinline__ void activate(float g, float& a, float& da) {
     } else if constexpr (ACT == NOTT_ACT_GELU) {
         const float cdf = 0.5f * erfcf(g * -0.70710678f);
         a = from * cdf;
-        da = fmaf(near * 0.39894228f, exp_near(fmaxf(-0.5f * near * near, -120.f)), cdf);
+        da = fmaf(near * 0.39894228f, exp_fine(fmaxf(-0.5f * near * near, -120.f)), cdf);
     } else if constexpr (ACT == NOTT_ACT_GELU_TANH) {
         const float e = sigmoid<FAST>(1.5957691f * fmaf(0.044715f * g, g * g, g));
         a = from * e;

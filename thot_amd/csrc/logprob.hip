@@ -20,23 +20,12 @@ constexpr int64_t kIgnoreIndex = -100;
 constexpr int kMaxTop = 64;
 constexpr int kUnroll = 4;          // 16-byte groups in flight per thread
 constexpr int kMaxSplits = 64;      // a merging wave has a lane for each
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718f;
+constexpr float kLn2 = 0.69314718f;
 // Logits of −inf or the type's lowest value mask a token: below this (times scale)
 // there is nothing.  As the maximum's first value it keeps −inf − (−inf) out.
 constexpr float kNothing = -1e30f;
 // Exponents (base 2) are not taken below this: 0·(−inf) is no part of a sum.
 constexpr float kLeast = -300.f;
-
-// e^x for x <= 0: what the rounding of x·log2 e leaves (2^-19 of the result at
-// x = −30) is taken into the result.  Below −200 (masked logits: −inf and the
-// type's lowest value) 0; NaN stays.
-__device__ __forceinline__ float exp_neg(float x) {
-    x = x < -200.f ? -200.f : x;
-    const float t = x * kLog2e;
-    const float r = fmaf(x, kLog2e, -t);
-    const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, r * kLn2, e);
-}
 
 // z = scale·logit; to_log2 = scale·log2 e; first: the maximum of no live logit.
 struct Scale {
@@ -197,7 +186,10 @@ struct Span {
 // A workgroup per row, or with splits > 1 per part of `chunk` columns, whose
 // statistics and top keys go to `stats` [row][split] and `keys` [row][split][top].
 // LDS holds `cap` candidates for the top tokens; a row in which more reach the
-// bound (many equal logits, or too few live ones for a bound) is scanned for each.
+// bound is scanned for each: many equal logits, too few live ones for a bound (fewer
+// than `top` of the 64 shares hold one), and of the one-wave rows (cap 256) with top
+// past about 60 ordinary ones too (the bound is then about the least of 64 maxima,
+// which 64·H(64) = 304 elements reach in the mean).
 // Bound by memory (one read of the logits), then by the exponential and four more
 // instructions an element.
 // 16384x32000 bf16, top 5, 187 us (5.6 TB/s; 222 in the mean of twenty in a row);
@@ -406,7 +398,8 @@ __global__ __launch_bounds__(NT) void logprob_bwd_kernel(const T* logits, const 
     const int first = (int)(sp.base - z);
     auto grad = [&](float x, int col) {
         const float lp = fmaf(x, scale, -l);
-        float g = -exp_neg(lp) * fmaf(dh, fmaxf(lp, -200.f) + h, dl);
+        // below −200 (masked logits: −inf and the type's lowest value) p is 0
+        float g = -exp_fine(lp < -200.f ? -200.f : lp) * fmaf(dh, fmaxf(lp, -200.f) + h, dl);
         if (col == (int)y) g += dl;
         return l == -INFINITY ? 0.f : g * scale;
     };
