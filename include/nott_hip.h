@@ -407,7 +407,8 @@ int nott_gated_linear_fwd(nott_ctx ctx, nott_dtype dtype, int64_t m, int64_t d, 
 /* From dh [m, f], x, w and the forward's gu:
  *   dg = dh·u·act'(g), du = dh·act(g);  dx = [dg|du]·w,  dw = [dg|du]ᵀ·x, db = Σ_rows [dg|du]
  * dx [m, d] (dtype), dw [2·f, d] and db [2·f] (fp32); each nullable (x is read
- * for dw, w for dx).  The workspace holds [dg|du]. */
+ * for dw, w for dx).  No output may overlap an input.  The workspace holds [dg|du] in
+ * bf16 pieces (three for dw, two for dx alone, four in fp32) or whole. */
 int nott_gated_linear_bwd(nott_ctx ctx, nott_dtype dtype, int64_t m, int64_t d, int64_t f, int act,
                           const void* dh, const void* x, const void* w, const void* gu,
                           void* dx, float* dw, float* db, int accumulate);

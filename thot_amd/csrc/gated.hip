@@ -14,8 +14,8 @@
 // 2^-23 of the whole (hi·hi, hi·mid, mid·hi, mid·mid, hi·lo, lo·hi) are summed in
 // fp32, the small ones first: six products, where the fp32 matrix instructions take
 // the time of sixteen, and no further from 64 bits than those (8192 rows of 1024 ->
-// 2048 408 us, 554 with fp32 instructions on tiles of the same engine; gradients 456
-// and 459 against 557 and 600).  A fourth piece is hi with 0 for an infinity or NaN: it
+// 2048 395 to 411 us, 554 with fp32 instructions on tiles of the same engine; gradients
+// 477 and 479 against 557 and 600).  A fourth piece is hi with 0 for an infinity or NaN: it
 // takes hi's place in all products but hi·hi, so that an infinity enters a sum once, as
 // its product.  The last piece ends at bf16's least number, so that values below 2^-110
 // keep 2^-134 rather than their own last bit (inputs of 2^-110 come out with an error of
@@ -85,9 +85,10 @@ __host__ __device__ __forceinline__ auto with_act(int act, F f) {
 // [row][32] and stored as whole row pieces of 64 (bf16) or 128 bytes.  bf16: the
 // 16-byte chunk at chunk ^ (row/2 % 4), its halves exchanged on rows with bit 3
 // set; fp32: at chunk ^ (row % 8).
-// Bound by the matrix cores: 8192 rows of 1024 -> 4096 bf16 146 us (940 TFLOP/s; 180 in
-// the mean of twenty in a row, as the clocks fall), 135 without [g | u]; a plain linear
-// product of the same sizes 148 to 151.
+// Bound by the matrix cores: 8192 rows of 1024 -> 4096 bf16 146 us (940 TFLOP/s, 300k
+// cycles), 135 without [g | u]; a plain linear product of the same sizes 148 to 151.  After
+// some 2 ms of such launches back to back each takes 172 to 190, the library's product
+// 141 to 145 for 109: launches with pauses between them keep 146 and the same cycles.
 template <typename T>
 struct GatedStore {
     T* h;
@@ -285,8 +286,8 @@ __device__ __forceinline__ void store_cut(bf16_t* out, int64_t stride, int piece
 // of a bf16 layer store_cut's, in fp32 store_nearest's.  A workgroup takes 64·E columns (E = 1, or
 // whole 16-byte chunks where all rows fit them and ld is 2f) and every gridDim.y-th
 // group of 4 rows; partial (null: no db) [gridDim.y][2f] receives its column sums of the unrounded
-// values.  Bound by memory: 8192 x 4096 bf16 with both pieces, 470 MB, 74 us (6.3 TB/s;
-// 94 an element at a time).
+// values.  Bound by memory: 8192 x 4096 bf16 with three pieces, 604 MB, 96 us (6.3 TB/s;
+// 108 in the mean of twenty calls in a row; two pieces an element at a time, 470 MB, 94).
 template <typename T, int ACT, int E>
 __global__ __launch_bounds__(256) void gated_dact_kernel(const T* __restrict__ dh, const T* __restrict__ gu, int64_t m,
                                                          int64_t f, int64_t ld, float* __restrict__ whole,
@@ -635,7 +636,7 @@ constexpr uint32_t kPairs = 6, kFirst = 0x031132, kSecond = 0x013123;
 // the direct-to-LDS engine: its plan's time and the split's against the generic engine's
 // 70 TFLOP/s, which spreads few tiles over the CUs by splitting k.  In us, generic and
 // pieces (forward; dx and dw with the activation gradient): 1576 rows of 768 -> 2048 162
-// and 88, 171 and 95, 140 and 102; 1024 of 768 -> 1024 43 and 57, 62 and 46, 58 and 45;
+// and 87, 171 and 99, 140 and 103; 1024 of 768 -> 1024 42 and 57, 62 and 48, 58 and 48;
 // 256 of 512 -> 1024 19 and 38, 22 and 29, 24 and 29.  On 25 sizes of 128 to 16384 rows
 // the choice costs 1.4% over the better one in the mean (most where a forward of odd
 // width has its loads element by element: 53 against 42).

@@ -190,10 +190,10 @@ struct Span {
 // than `top` of the 64 shares hold one), and of the one-wave rows (cap 256) with top
 // past about 60 ordinary ones too (the bound is then about the least of 64 maxima,
 // which 64·H(64) = 304 elements reach in the mean).
-// Bound by memory (one read of the logits), then by the exponential and four more
+// Bound by memory (one read of the logits), then by the exponential and seven more
 // instructions an element.
-// 16384x32000 bf16, top 5, 187 us (5.6 TB/s; 222 in the mean of twenty in a row);
-// 8x128256 bf16, top 8, in parts of 4096 columns and more 6.9 us and 4.7 to join them.
+// 16384x32000 bf16, top 5, 188 us (5.6 TB/s; 245 in the mean of twenty in a row);
+// 8x128256 bf16, top 8, in parts of 4096 columns and more 7.1 us and 4.6 to join them.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void logprob_kernel(const T* __restrict__ logits, const int64_t* __restrict__ labels,
                                                      int64_t c, int chunk, Scale sc, int top, int cap, FwdOut o,

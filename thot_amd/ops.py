@@ -804,8 +804,8 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w: torch.Tensor, gu: tor
                      need_dx: bool = True, need_dw: bool = True, need_db: bool = True,
                      dx: Optional[torch.Tensor] = None, dw: Optional[torch.Tensor] = None,
                      db: Optional[torch.Tensor] = None, accumulate: bool = False):
-    """(dx, dw, db) of gated_linear_fwd from dh and its gu; dw and db fp32
-    (nott_gated_linear_bwd)."""
+    """(dx, dw, db) of gated_linear_fwd from dh and its gu; dw and db fp32.  dx, dw and db
+    to write into must not overlap an input (nott_gated_linear_bwd)."""
     if accumulate and ((need_dw and dw is None) or (need_db and db is None)):
         raise ValueError("accumulate needs the gradients to add to")
     m, d, f = _gated_shapes(x, w, act)
