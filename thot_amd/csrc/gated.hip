@@ -670,7 +670,8 @@ int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* x,
 int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* x, const float* w, const float* b, float* h,
         float* gu) {
     const int64_t dp = up8(d);
-    if (!takes_pieces(ctx, m, 2 * f, dp, false, false, (m + 2 * f) * dp)) {
+    const size_t room = kPieces * sizeof(bf16_t) * (size_t)((m + 2 * f) * dp);
+    if (!takes_pieces(ctx, m, 2 * f, dp, false, false, (m + 2 * f) * dp) || !nott::optional_workspace(ctx, room)) {
         WorkspaceHold ws(ctx, sizeof(float) * (size_t)(m * 2 * f));
         if (ws.failed()) return NOTT_ERR_ALLOC;
         float* pre = reinterpret_cast<float*>(ws.p);
@@ -684,7 +685,7 @@ int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* x, 
         });
         return launch_status(ctx, "gated_linear");
     }
-    WorkspaceHold ws(ctx, kPieces * sizeof(bf16_t) * (size_t)((m + 2 * f) * dp));
+    WorkspaceHold ws(ctx, room);
     if (ws.failed()) return NOTT_ERR_ALLOC;
     bf16_t* xp = reinterpret_cast<bf16_t*>(ws.p);
     bf16_t* wp = xp + kPieces * m * dp;
@@ -696,6 +697,7 @@ int fwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* x, 
     return dma::launch_shape<false, false, false>(ctx, p.shape, xp, dp, wp, dp, ep, m, 2 * f, dp, 1, deep);
 }
 
+constexpr int64_t kMostSums = 128;   // slabs of rows that each leave sums for db
 // [dg|du] in rows of ld elements (zeros past 2·f), whole or as pieces (gated_dact_kernel); db.
 template <typename T>
 int activation_bwd(nott_ctx ctx, int64_t m, int64_t f, int64_t ld, int act, const T* dh, const T* gu, float* whole,
@@ -705,7 +707,7 @@ int activation_bwd(nott_ctx ctx, int64_t m, int64_t f, int64_t ld, int act, cons
     // about eight workgroups a CU, of at least 4 rows; fewer where each leaves sums for db
     const int64_t columns = ceil_div(f, 64 * (vec ? E : 1));
     const int64_t slabs = std::max<int64_t>(1, std::min<int64_t>({ceil_div(8 * (int64_t)ctx->num_cu, columns), ceil_div(m, 4),
-                                                                  db ? 128 : 65535}));
+                                                                  db ? kMostSums : 65535}));
     float* partial = nullptr;
     if (db) {
         partial = static_cast<float*>(nott::workspace(ctx, sizeof(float) * (size_t)(slabs * 2 * f)));
@@ -783,12 +785,20 @@ int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const bf16_t* dh
 int bwd(nott_ctx ctx, int64_t m, int64_t d, int64_t f, int act, const float* dh, const float* x, const float* w,
         const float* gu, float* dx, float* dw, float* db, int accumulate) {
     const int64_t dp = up8(d), fp = up8(2 * f);
-    const bool pieces_dx = dx && takes_pieces(ctx, m, dp, fp, false, true, fp * dp);
-    const bool pieces_dw = dw && takes_pieces(ctx, fp, dp, m, true, true, m * dp);
-    const bool pieces = pieces_dx || pieces_dw, whole = (dx && !pieces_dx) || (dw && !pieces_dw);
+    bool pieces_dx = dx && takes_pieces(ctx, m, dp, fp, false, true, fp * dp);
+    bool pieces_dw = dw && takes_pieces(ctx, fp, dp, m, true, true, m * dp);
+    auto any = [&] { return pieces_dx || pieces_dw; };
+    auto whole_too = [&] { return (dx && !pieces_dx) || (dw && !pieces_dw); };
+    auto room = [&] {
+        return sizeof(float) * (size_t)(whole_too() ? m * (any() ? fp : 2 * f) : 0) +
+               kPieces * sizeof(bf16_t) * (size_t)((any() ? m * fp : 0) + ((pieces_dw ? m : 0) + (pieces_dx ? fp : 0)) * dp);
+    };
+    // no room for them and, behind them, db's sums: the generic engine
+    if (any() && !nott::optional_workspace(ctx, room() + (db ? 256 + sizeof(float) * kMostSums * 2 * (size_t)f : 0)))
+        pieces_dx = pieces_dw = false;
+    const bool pieces = any(), whole = whole_too();
     const int64_t ld = pieces ? fp : 2 * f;
-    WorkspaceHold ws(ctx, sizeof(float) * (size_t)(whole ? m * ld : 0) +
-                              kPieces * sizeof(bf16_t) * (size_t)((pieces ? m * fp : 0) + ((pieces_dw ? m : 0) + (pieces_dx ? fp : 0)) * dp));
+    WorkspaceHold ws(ctx, room());
     if (ws.failed()) return NOTT_ERR_ALLOC;
     bf16_t* dgu = reinterpret_cast<bf16_t*>(ws.p);
     bf16_t* xp = dgu + (pieces ? kPieces * m * fp : 0);
