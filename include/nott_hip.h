@@ -475,6 +475,41 @@ int nott_adam_step_graph(nott_ctx ctx, int decoupled, int64_t n,
                          float* m, float* v, const double* hparams, nott_adam_device_state* state,
                          int weight_decay_nonzero, int zero_grad_after);
 
+/* ---- Adam / AdamW over many tensors ---------------------------------------------
+ * nott_adam_step for parameters that stay where they are (layers shared with other
+ * code, bf16 parameters, models whose moments must take less memory than fp32), any
+ * number of tensors in a launch for every 56 of one pair of types; beside the reference's
+ * torch::optim::Adam[W] (optimizer/details/adam.hpp:63-154, 159-250).
+ * m and v hold whole blocks of 256 elements, n rounded up.
+ * bits = 32: in fp32; the results are nott_adam_step's bits.
+ * bits = 8: as e4m3 codes (OCP, 448 the largest) of m and of sqrt(v), which scale
+ * [blocks][2] (fp32) multiplies.  The update takes the moments before they are
+ * rounded; zeroed buffers are moments of zero.  A nonzero sqrt(v) never gets the code of
+ * zero.  Blocks whose largest moment (or root) is below 2^-112 count as zero.  A gradient
+ * that is not finite spoils the moments of its block.
+ * copy (bf16 [n], nullable) receives the new parameters.  m and v 16-byte aligned.
+ * grad_scale (device fp32 scalar, nullable) multiplies every gradient, e.g. a clipping
+ * factor that a kernel before this one wrote.  Tensors must not overlap. */
+typedef struct nott_adam_tensor {
+    void* p;
+    void* g;
+    void* m;
+    void* v;
+    float* scale;              /* bits = 8 */
+    void* copy;
+    int64_t n;
+    int16_t p_dtype, g_dtype;  /* nott_dtype */
+    int32_t bits;              /* 8 or 32 */
+} nott_adam_tensor;
+/* tensors: host array, read during the call. */
+int nott_adam_multi_step(nott_ctx ctx, int decoupled, const nott_adam_tensor* tensors, int64_t count,
+                         double lr, double beta1, double beta2, double eps, double weight_decay,
+                         int64_t step, const float* grad_scale, int zero_grad_after);
+/* The same with its scalars taken at launch time, as nott_adam_step_graph does. */
+int nott_adam_multi_step_graph(nott_ctx ctx, int decoupled, const nott_adam_tensor* tensors, int64_t count,
+                               const double* hparams, nott_adam_device_state* state, int weight_decay_nonzero,
+                               const float* grad_scale, int zero_grad_after);
+
 /* ---- utilities used by the host modules ---------------------------------- */
 /* dst = a + b elementwise (residual gradient fan-in, block/details/blocks/residual.hpp:131). */
 int nott_add(nott_ctx ctx, nott_dtype dtype, int64_t n, const void* a, const void* b, void* dst);

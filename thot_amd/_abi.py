@@ -56,6 +56,11 @@ class QkRopeDesc(C.Structure):
                [(n, C.c_int32) for n in ("axes", "interleaved", "norm", "reserved")] + [("eps", f64)]
 
 
+class AdamTensor(C.Structure):
+    _fields_ = [(n, vp) for n in ("p", "g", "m", "v", "scale", "copy")] + \
+               [("n", i64), ("p_dtype", C.c_int16), ("g_dtype", C.c_int16), ("bits", C.c_int32)]
+
+
 NOTT_ACT_SILU, NOTT_ACT_GELU, NOTT_ACT_GELU_TANH, NOTT_ACT_RELU, NOTT_ACT_SIGMOID = range(5)
 
 
@@ -112,6 +117,8 @@ SIGNATURES: dict[str, list] = {
     "nott_token_logprob_bwd": [vp, i32, i64, i64, vp, vp, f64, fp, fp, fp, fp, vp],
     "nott_adam_step": [vp, i32, i64, vp, i32, vp, i32, fp, fp, f64, f64, f64, f64, f64, i64, i32],
     "nott_adam_step_graph": [vp, i32, i64, vp, i32, vp, i32, fp, fp, vp, vp, i32, i32],
+    "nott_adam_multi_step": [vp, i32, vp, i64, f64, f64, f64, f64, f64, i64, fp, i32],
+    "nott_adam_multi_step_graph": [vp, i32, vp, i64, vp, vp, i32, fp, i32],
     "nott_loss_accumulate": [vp, fp, f64, vp],
     "nott_add": [vp, i32, i64, vp, vp, vp],
     "nott_add_relu_bwd": [vp, i32, i64, vp, vp, vp, vp],

@@ -7,6 +7,7 @@ fallback path: a missing library or a failing launch raises.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import math
 import struct
@@ -116,6 +117,150 @@ def adam_step(p: torch.Tensor, g: torch.Tensor, m: torch.Tensor, v: torch.Tensor
     _ctx_for(p).call("nott_adam_step", int(decoupled), n, _ptr(p), nott_dtype(p.dtype), _ptr(g), nott_dtype(g.dtype),
                      _ptr(m), _ptr(v), float(lr), float(beta1), float(beta2), float(eps), float(weight_decay),
                      int(step), int(zero_grad))
+
+
+class AdamMoments:
+    """Adam's moments for parameters that stay where they are (adam_multi_step).
+
+    bits=8: `m` holds the first moment and `v` the root of the second as e4m3 codes
+    (torch.float8_e4m3fn [blocks, 256]; each parameter begins a block of its own, `first`
+    says which), `scale` (fp32 [blocks, 2]) what they are multiplied by.  bits=32: `m` and
+    `v` are the moments in fp32, laid out alike, and `scale` is None.  `copies`: a bf16
+    tensor for each parameter (or None) that every step writes the new values to.  m, v and
+    scale may be given (a loaded state); they are kept, not copied."""
+    BLOCK = 256
+
+    def __init__(self, params, *, bits: int = 8, copies=None, m: Optional[torch.Tensor] = None,
+                 v: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
+        self.params = list(params)
+        if bits not in (8, 32):
+            raise ValueError("bits must be 8 or 32")
+        if not self.params:
+            raise ValueError("params is empty")
+        self.copies = [None] * len(self.params) if copies is None else list(copies)
+        if len(self.copies) != len(self.params):
+            raise ValueError(f"{len(self.copies)} copies for {len(self.params)} parameters")
+        self.bits, self.device = bits, self.params[0].device
+        self.first, blocks = [], 0
+        for i, (p, c) in enumerate(zip(self.params, self.copies)):
+            nott_dtype(p.dtype)
+            _check(p, f"params[{i}]", device=self.device)
+            if c is not None:
+                _check(c, f"copies[{i}]", shape=p.shape, dtype=torch.bfloat16, device=self.device)
+            self.first.append(blocks)
+            blocks += -(-p.numel() // self.BLOCK)
+        spans = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in (*self.params, *self.copies)
+                       if t is not None and t.numel())
+        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+            raise ValueError("params and copies must not overlap")
+        dt = torch.float8_e4m3fn if bits == 8 else torch.float32
+        self.m, self.v = (self._held(t, nm, (blocks, self.BLOCK), dt) for t, nm in ((m, "m"), (v, "v")))
+        if bits == 32 and scale is not None:
+            raise ValueError("scale goes with bits=8")
+        self.scale = self._held(scale, "scale", (blocks, 2), torch.float32) if bits == 8 else None
+        if any(t is not None and t.data_ptr() % 16 for t in (self.m, self.v, self.scale)):
+            raise ValueError("m, v and scale must be 16-byte aligned")
+        self._meta = [(p.numel(), p.shape) for p in self.params]
+        # AdamTensor's words: what changes from step to step (p, g) is written by the step
+        row = self.BLOCK * self.m.element_size()
+        self._words = array.array("Q", bytes(64 * len(self.params)))
+        self._words[2::8] = array.array("Q", [self.m.data_ptr() + row * f for f in self.first])
+        self._words[3::8] = array.array("Q", [self.v.data_ptr() + row * f for f in self.first])
+        if bits == 8:
+            self._words[4::8] = array.array("Q", [self.scale.data_ptr() + 8 * f for f in self.first])
+        self._words[6::8] = array.array("Q", [p.numel() for p in self.params])
+
+    def _held(self, t: Optional[torch.Tensor], name: str, shape, dtype) -> torch.Tensor:
+        if t is None:
+            return torch.zeros(shape, dtype=torch.uint8 if dtype.itemsize == 1 else dtype, device=self.device).view(dtype)
+        _check(t, name, shape=shape, dtype=dtype, device=self.device)
+        return t
+
+    def _rows(self, t: torch.Tensor, i: int) -> torch.Tensor:
+        return t[self.first[i]:self.first[i] - (-self._meta[i][0] // self.BLOCK)]
+
+    def exp_avg(self, i: int) -> torch.Tensor:
+        """Parameter i's first moment in fp32."""
+        m = self._rows(self.m, i).float()
+        if self.bits == 8:
+            m = m * self._rows(self.scale, i)[:, :1]
+        return m.reshape(-1)[:self._meta[i][0]].view(self._meta[i][1])
+
+    def exp_avg_sq(self, i: int) -> torch.Tensor:
+        """Parameter i's second moment in fp32."""
+        v = self._rows(self.v, i).float()
+        if self.bits == 8:
+            v = (v * self._rows(self.scale, i)[:, 1:]).square()
+        return v.reshape(-1)[:self._meta[i][0]].view(self._meta[i][1])
+
+    def _tensors(self, grads):
+        """The words of the parameters that have a gradient."""
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
+        w, p, gp, kinds, bits, missing = self._words, [], [], [], self.bits << 32, False
+        for i, (t, g, (n, shape)) in enumerate(zip(self.params, grads, self._meta)):
+            if g is None:
+                missing = True
+                p.append(0)
+                gp.append(0)
+                kinds.append(bits)
+                continue
+            if t.shape != shape:
+                raise ValueError(f"params[{i}] has changed its shape")
+            if g.shape != shape or g.dtype not in _DTYPES or not g.is_contiguous() or g.device != self.device:
+                _check(g, f"grads[{i}]", shape=shape, device=self.device)
+                nott_dtype(g.dtype)
+            p.append(t.data_ptr())
+            gp.append(g.data_ptr())
+            kinds.append(bits | _DTYPES[g.dtype] << 16 | _DTYPES[t.dtype])
+        w[0::8] = array.array("Q", p)
+        w[1::8] = array.array("Q", gp)
+        w[5::8] = array.array("Q", [0 if c is None else c.data_ptr() for c in self.copies])
+        w[7::8] = array.array("Q", kinds)
+        if missing:
+            kept = array.array("Q")
+            for i, g in enumerate(grads):
+                if g is not None:
+                    kept.extend(w[8 * i:8 * i + 8])
+            w = kept
+        return w, len(w) // 8
+
+
+def adam_multi_step(moments: AdamMoments, grads, *, lr: float, beta1: float = 0.9, beta2: float = 0.999,
+                    eps: float = 1e-8, weight_decay: float = 0.0, step: int, decoupled: bool = True,
+                    zero_grad: bool = False, grad_scale: Optional[torch.Tensor] = None) -> None:
+    """One Adam (decoupled=False) / AdamW step over moments.params, in place; grads: a
+    gradient for each, or None to leave a parameter as it is.  grad_scale: an fp32
+    scalar on the device that multiplies the gradients (nott_adam_multi_step)."""
+    if grad_scale is not None:
+        _check(grad_scale, "grad_scale", dtype=torch.float32, device=moments.device)
+        if grad_scale.numel() != 1:
+            raise ValueError("grad_scale must be one number")
+    w, count = moments._tensors(grads)
+    context(moments.device.index).call("nott_adam_multi_step", int(decoupled), w.buffer_info()[0], count, float(lr),
+                                       float(beta1), float(beta2), float(eps), float(weight_decay), int(step),
+                                       _ptr(grad_scale), int(zero_grad))
+
+
+def adam_multi_step_graph(moments: AdamMoments, grads, hparams: torch.Tensor, state: torch.Tensor, *,
+                          decoupled: bool = True, weight_decay_nonzero: bool = True, zero_grad: bool = False,
+                          grad_scale: Optional[torch.Tensor] = None) -> None:
+    """adam_multi_step for a captured graph: hparams float64 [5] (lr, beta1, beta2, eps,
+    weight_decay) on the device or pinned, read when the kernels run; state int64 [8] on
+    the device, its first element the step count, which each launch advances
+    (nott_adam_multi_step_graph)."""
+    if hparams.dtype != torch.float64 or hparams.numel() != 5 or not hparams.is_contiguous() or \
+            not (hparams.device == moments.device or hparams.is_pinned()):
+        raise ValueError("hparams must be float64 [5] on the device or in pinned memory")
+    _check(state, "state", shape=(8,), dtype=torch.int64, device=moments.device)
+    if grad_scale is not None:
+        _check(grad_scale, "grad_scale", dtype=torch.float32, device=moments.device)
+        if grad_scale.numel() != 1:
+            raise ValueError("grad_scale must be one number")
+    w, count = moments._tensors(grads)
+    context(moments.device.index).call("nott_adam_multi_step_graph", int(decoupled), w.buffer_info()[0], count,
+                                       _ptr(hparams), _ptr(state), int(weight_decay_nonzero), _ptr(grad_scale),
+                                       int(zero_grad))
 
 
 # ---------------------------------------------------------------- elementwise
