@@ -384,6 +384,41 @@ int nott_qk_norm_rope_bwd(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype d
                           const int64_t* positions, const double* inv_freq,
                           void* dq, void* dk, float* dgamma_q, float* dgamma_k, int accumulate);
 
+/* ---- gated linear recurrence ---------------------------------------------------
+ * The state of a recurrent layer whose update is linear in it, scanned over time; each
+ * of the d channels by itself:
+ *   h_t = keep_t·h_{t−1} + take_t·x_t
+ *   a = gate, or sigmoid(gate) with sigmoid = 1;  take = 1, or 1 − a with mix = 1;
+ *   keep = a, or 0 at tokens where `reset` (bytes [b, t], nullable) is not 0: a sequence
+ *   begins there, and nothing before it reaches it, infinities and NaN included.
+ * A keep of exactly 0 forgets the state as well.  With sigmoid = 1 a gate of +infinity
+ * keeps the state (and with mix takes nothing in: padding behind a sequence leaves its
+ * state), one of −infinity forgets it.
+ * x, gate, h [b, t, d] with strides in elements for batch and token (two zeros =
+ * contiguous), channels side by side, so x and gate may be views of one projection.
+ * h0, last [b, d] fp32: the state before the first token (nullable: zeros) and after the
+ * last (nullable).  states [b, ceil(t / 256), d] fp32 (nullable): the state before every
+ * 256th token, for the backward.  The state is fp32 throughout.  h may be x or gate
+ * (same address and strides); other overlaps are not allowed.  Workspace: two fp32 [b, d] for each
+ * segment that time is cut into where the channels are few; without room for it,
+ * time is not cut. */
+typedef struct nott_scan_desc {
+    int64_t b, t, d;
+    int64_t x_stride[2], gate_stride[2];
+    int64_t h_stride[2];                   /* h, and dh in the backward */
+    int64_t dx_stride[2], dgate_stride[2]; /* backward */
+    int32_t sigmoid, mix;
+} nott_scan_desc;
+#define NOTT_SCAN_CHUNK 256                /* tokens between kept states */
+int nott_linear_scan_fwd(nott_ctx ctx, const nott_scan_desc* d, nott_dtype dtype, const void* x, const void* gate,
+                         const float* h0, const uint8_t* reset, void* h, float* last, float* states);
+/* From dh [b, t, d] and dlast [b, d] (fp32, nullable), the gradients of h and last, with
+ * the forward's inputs and states: dx, dgate [b, t, d], dh0 [b, d] (fp32, nullable).
+ * dx and dgate may each be one of dh, x, gate (same address and strides). */
+int nott_linear_scan_bwd(nott_ctx ctx, const nott_scan_desc* d, nott_dtype dtype, const void* dh, const void* x,
+                         const void* gate, const uint8_t* reset, const float* states, const float* dlast,
+                         void* dx, void* dgate, float* dh0);
+
 /* ---- gated linear (gated feed-forward) ---------------------------------------
  * A feed-forward layer's first half with a gate: both projections, the
  * activation and the product.  w [2·f, d] (dtype) is packed, gate rows first,

@@ -56,6 +56,12 @@ class QkRopeDesc(C.Structure):
                [(n, C.c_int32) for n in ("axes", "interleaved", "norm", "reserved")] + [("eps", f64)]
 
 
+class ScanDesc(C.Structure):
+    _fields_ = [(n, i64) for n in ("b", "t", "d")] + \
+               [(n, i64 * 2) for n in ("x_stride", "gate_stride", "h_stride", "dx_stride", "dgate_stride")] + \
+               [("sigmoid", C.c_int32), ("mix", C.c_int32)]
+
+
 class AdamTensor(C.Structure):
     _fields_ = [(n, vp) for n in ("p", "g", "m", "v", "scale", "copy")] + \
                [("n", i64), ("p_dtype", C.c_int16), ("g_dtype", C.c_int16), ("bits", C.c_int32)]
@@ -113,6 +119,8 @@ SIGNATURES: dict[str, list] = {
     "nott_qk_norm_rope_bwd": [vp, C.POINTER(QkRopeDesc), i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, fp, fp, i32],
     "nott_gated_linear_fwd": [vp, i32, i64, i64, i64, i32, vp, vp, fp, vp, vp],
     "nott_gated_linear_bwd": [vp, i32, i64, i64, i64, i32, vp, vp, vp, vp, vp, fp, fp, i32],
+    "nott_linear_scan_fwd": [vp, vp, i32, vp, vp, fp, vp, vp, fp, fp],
+    "nott_linear_scan_bwd": [vp, vp, i32, vp, vp, vp, vp, fp, fp, vp, vp, fp],
     "nott_token_logprob_fwd": [vp, i32, i64, i64, vp, vp, f64, i64, fp, fp, fp, fp, vp],
     "nott_token_logprob_bwd": [vp, i32, i64, i64, vp, vp, f64, fp, fp, fp, fp, vp],
     "nott_adam_step": [vp, i32, i64, vp, i32, vp, i32, fp, fp, f64, f64, f64, f64, f64, i64, i32],

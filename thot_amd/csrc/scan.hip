@@ -1,0 +1,625 @@
+// Gated linear recurrence over time, forward and backward, channel by channel:
+//
+//   h_t = keep_t·h_{t−1} + take_t·x_t
+//   a = gate or sigmoid(gate);  take = 1 or 1 − a;  keep = a, or 0 where a sequence begins
+// backward, with e_t the gradient of h_t and c_t = keep_t·e_t what it hands to t − 1:
+//   e_t = dh_t + c_{t+1},  dx = take·e,  da = e·h_{t−1} (0 where a sequence begins) [− e·x]
+//
+// Composition: a span of tokens maps the state s before it to A·s + B (A = Π keep), and
+// two spans in a row to (A₂·A₁, A₂·B₁ + B₂); c is the same recurrence in reverse with the
+// same A.  A workgroup owns 64 channels and takes 256 tokens at a time: each thread the
+// span of a few tokens of its channels in registers, one wave folds the spans' maps through
+// LDS (another wave those of the reverse scan), and the spans are gone through again
+// from the states before them.  So x and gate are read once and h is written once; the
+// backward reads x, gate and dh, forms the states again in fp32 from the one that the
+// forward kept before every 256th token (3% of h's bytes, where reading h costs a sixth
+// stream and its rounding), and writes dx and dgate.  States, maps and sums are fp32.
+//
+// Few channels (b·d of a few thousand) do not fill the chip: then the tokens are split
+// into segments, whose maps a kernel before forms (reading x and gate once more), and
+// each workgroup folds the maps before its segment, in their order.  No workgroup waits
+// for another, and results do not depend on timing.
+// A keep of exactly 0 forgets the state whatever it was, an infinity or NaN as well.
+// Bound by HBM (3 streams forward, 5 backward).
+#include "common.hpp"
+
+#include <type_traits>
+
+namespace {
+
+using nott::ceil_div;
+
+constexpr int kThreads = 512;
+constexpr int kCh = 64;             // channels of a workgroup
+constexpr int kTile = 256;          // tokens of a tile, and between kept states
+
+// VEC neighbouring channels of a token: 16 bytes, or one element where rows are not aligned.
+template <typename T, int VEC> struct Row;
+template <typename T> struct Row<T, 1> {
+    typedef T Raw;
+    static __device__ __forceinline__ Raw load(const T* p) { return *p; }
+    static __device__ __forceinline__ void floats(Raw u, float (&v)[1]) { v[0] = Io<T>::ld(&u, 0); }
+    static __device__ __forceinline__ void store(T* p, const float (&v)[1]) { Io<T>::st(p, 0, v[0]); }
+};
+template <> struct Row<float, 4> {
+    typedef f32x4 Raw;
+    static __device__ __forceinline__ Raw load(const float* p) { return Pack16<float>::raw<true>(p); }
+    static __device__ __forceinline__ void floats(const Raw& u, float (&v)[4]) { Pack16<float>::unpack(u, v); }
+    static __device__ __forceinline__ void store(float* p, const float (&v)[4]) { Pack16<float>::st<true>(p, v); }
+};
+template <> struct Row<bf16_t, 8> {
+    typedef u32x4 Raw;
+    static __device__ __forceinline__ Raw load(const bf16_t* p) { return Pack16<bf16_t>::raw<true>(p); }
+    static __device__ __forceinline__ void floats(const Raw& u, float (&v)[8]) { Pack16<bf16_t>::unpack(u, v); }
+    static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[8]) { Pack16<bf16_t>::st<true>(p, v); }
+};
+
+struct Params {
+    int64_t t, seg;                 // tokens, tokens of a segment
+    int32_t d, nblk, nseg, nchunk;  // channels, 64-channel blocks, segments, kept states
+    int64_t rows;                   // b·d
+    int64_t xb, xt, gb, gt, hb, ht, dxb, dxt, dgb, dgt;   // batch and token strides
+};
+
+// a and what multiplies the input.  From e^−|g|, so that neither overflows: infinities
+// give exactly 0 and 1.
+template <bool SIG, bool MIX>
+__device__ __forceinline__ void gates(float g, float& a, float& take) {
+    if constexpr (SIG) {
+        const float t = __builtin_amdgcn_exp2f(__builtin_fabsf(g) * -1.4426950f), big = __builtin_amdgcn_rcpf(1.f + t);
+        const float small = t * big;
+        a = g < 0.f ? small : big;
+        take = MIX ? (g < 0.f ? big : small) : 1.f;
+    } else {
+        a = g;
+        take = MIX ? 1.f - g : 1.f;
+    }
+}
+
+// A·s + B; A = 0 forgets s.
+__device__ __forceinline__ float step(float A, float s, float B) { return A == 0.f ? B : fmaf(A, s, B); }
+
+// Keeps the compiler from holding what it formed from x before (an unpacked copy, a
+// product) beside x.
+template <typename X>
+__device__ __forceinline__ void anew(X& x) { asm volatile("" : "+v"(x)); }
+
+// The place of a thread in its workgroup's tile.
+template <int VEC>
+struct Place {
+    static constexpr int L = kCh / VEC, G = kThreads / L, R = kTile / G;   // lanes of a token, spans, tokens of a span
+    int lane, span, c, cc;          // channels from c; cc: where loads go instead past the end
+    int64_t b;
+    bool in;
+    __device__ __forceinline__ explicit Place(const Params& p) {
+        lane = threadIdx.x % L;
+        span = threadIdx.x / L;
+        b = blockIdx.x / p.nblk;
+        c = (int)(blockIdx.x % p.nblk) * kCh + lane * VEC;
+        in = c < p.d;
+        cc = in ? c : 0;
+    }
+};
+
+// The maps of a tile's spans, folded in order by one wave (thread = channel): B becomes the
+// state before each span; returns the state behind them all.
+template <int G, bool REVERSE>
+__device__ __forceinline__ float fold(const float (&A)[G][kCh], float (&B)[G][kCh], int ch, float s) {
+    constexpr int U = G < 16 ? G : 16;
+#pragma unroll 1
+    for (int g0 = 0; g0 < G; g0 += U) {
+        float ta[U], tb[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int g = REVERSE ? G - 1 - g0 - u : g0 + u;
+            ta[u] = A[g][ch];
+            tb[u] = B[g][ch];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            B[REVERSE ? G - 1 - g0 - u : g0 + u][ch] = s;
+            s = step(ta[u], s, tb[u]);
+        }
+    }
+    return s;
+}
+
+// Maps of whole segments, for the segments that follow (forward) or precede (reverse):
+// agg [nseg][2][b·d].  A span is a run of the segment's tokens, gone through in registers.
+template <typename T, int VEC, bool SIG, bool MIX, bool REVERSE>
+__global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict__ x, const T* __restrict__ gate,
+                                                             const uint8_t* __restrict__ reset, float* __restrict__ agg,
+                                                             Params p) {
+    typedef Place<VEC> P;
+    __shared__ __attribute__((aligned(16))) float sA[P::G][kCh], sB[P::G][kCh];
+    const P w(p);
+    const int seg = REVERSE ? blockIdx.y + 1 : blockIdx.y;
+    const int64_t t0 = seg * p.seg, t1 = min(p.t, t0 + p.seg);
+    const int64_t run = (p.seg + P::G - 1) / P::G;
+    const int64_t r0 = min(t1, t0 + w.span * run), r1 = min(t1, r0 + run);
+    const T* px = x + w.b * (REVERSE ? p.hb : p.xb) + w.cc;      // (reverse: dh in x's place)
+    const T* pg = gate + w.b * p.gb + w.cc;
+    const int64_t xt = REVERSE ? p.ht : p.xt;
+    float A[VEC], B[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        A[v] = 1.f;
+        B[v] = 0.f;
+    }
+    constexpr int U = VEC == 1 ? 8 : 4;
+    for (int64_t q = r0; q < r1; q += U) {
+        typename Row<T, VEC>::Raw rx[U], rg[U];
+        uint8_t fresh[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = REVERSE ? max(r0, r1 - 1 - (q - r0) - u) : min(r1 - 1, q + u);
+            rx[u] = Row<T, VEC>::load(px + t * xt);
+            rg[u] = Row<T, VEC>::load(pg + t * p.gt);
+            fresh[u] = reset ? reset[w.b * p.t + t] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (q + u >= r1) break;
+            float vx[VEC], vg[VEC];
+            Row<T, VEC>::floats(rx[u], vx);
+            Row<T, VEC>::floats(rg[u], vg);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                float a, take;
+                gates<SIG, MIX>(vg[v], a, take);
+                a = fresh[u] ? 0.f : a;
+                B[v] = REVERSE ? (a == 0.f ? 0.f : a * (vx[v] + B[v])) : step(a, B[v], take * vx[v]);
+                A[v] *= a;
+            }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        sA[w.span][w.lane * VEC + v] = A[v];
+        sB[w.span][w.lane * VEC + v] = B[v];
+    }
+    __syncthreads();
+    const int ch = (int)(blockIdx.x % p.nblk) * kCh + threadIdx.x;
+    if (threadIdx.x >= kCh || ch >= p.d) return;
+    float ta = 1.f, tb = 0.f;
+    for (int g = 0; g < P::G; ++g) {
+        const int i = REVERSE ? P::G - 1 - g : g;
+        tb = step(sA[i][threadIdx.x], tb, sB[i][threadIdx.x]);
+        ta *= sA[i][threadIdx.x];
+    }
+    float* o = agg + (int64_t)seg * 2 * p.rows + w.b * p.d + ch;
+    o[0] = ta;
+    o[p.rows] = tb;
+}
+
+template <typename T, int VEC, bool SIG, bool MIX>
+__global__ __launch_bounds__(kThreads) void scan_fwd_kernel(const T* __restrict__ x, const T* __restrict__ gate,
+                                                            const float* __restrict__ h0,
+                                                            const uint8_t* __restrict__ reset,
+                                                            const float* __restrict__ agg, T* __restrict__ h,
+                                                            float* __restrict__ last, float* __restrict__ states, Params p) {
+    typedef Place<VEC> P;
+    typedef typename Row<T, VEC>::Raw Raw;
+    constexpr int R = P::R;
+    // two tiles' maps in turn: a tile's are written while another wave still reads the last one's
+    __shared__ __attribute__((aligned(16))) float sA[2][P::G][kCh], sB[2][P::G][kCh];
+    const P w(p);
+    const int seg = blockIdx.y;
+    const int64_t t0 = seg * p.seg, t1 = min(p.t, t0 + p.seg);
+    const T* px = x + w.b * p.xb + w.cc;
+    const T* pg = gate + w.b * p.gb + w.cc;
+    T* ph = h + w.b * p.hb + w.cc;
+    const int ch = (int)(blockIdx.x % p.nblk) * kCh + threadIdx.x;   // the folding wave's channel
+    const bool folds = threadIdx.x < kCh, mine = folds && ch < p.d;
+    const int64_t row = w.b * p.d + ch;
+    float s = 0.f;
+    if (mine) {
+        s = h0 ? h0[row] : 0.f;
+        for (int g = 0; g < seg; ++g) s = step(agg[(int64_t)g * 2 * p.rows + row], s, agg[((int64_t)g * 2 + 1) * p.rows + row]);
+    }
+    Raw rx[R], rg[R];
+    uint32_t fresh = 0;     // bit r: a sequence begins at token r of the span
+    auto load = [&](int64_t tile) {
+        fresh = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t t = min(p.t - 1, tile + w.span * R + r);
+            rx[r] = Row<T, VEC>::load(px + t * p.xt);
+            rg[r] = Row<T, VEC>::load(pg + t * p.gt);
+            if (reset && reset[w.b * p.t + t]) fresh |= 1u << r;
+        }
+    };
+    load(t0);
+    int buf = 0;
+    for (int64_t tile = t0; tile < t1; tile += kTile, buf ^= 1) {
+        const int64_t mt = tile + w.span * R;
+        float a[R][VEC], u[R][VEC], A[VEC], B[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            A[v] = 1.f;
+            B[v] = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float vx[VEC], vg[VEC];
+            Row<T, VEC>::floats(rx[r], vx);
+            Row<T, VEC>::floats(rg[r], vg);
+            const bool out = mt + r >= t1, begins = (fresh >> r) & 1;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                float take;
+                gates<SIG, MIX>(vg[v], a[r][v], take);
+                u[r][v] = out ? 0.f : take * vx[v];
+                a[r][v] = out ? 1.f : begins ? 0.f : a[r][v];
+                B[v] = step(a[r][v], B[v], u[r][v]);
+                A[v] *= a[r][v];
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            sA[buf][w.span][w.lane * VEC + v] = A[v];
+            sB[buf][w.span][w.lane * VEC + v] = B[v];
+        }
+        if (tile + kTile < t1) load(tile + kTile);
+        __syncthreads();
+        if (folds) {
+            if (states && mine) states[(w.b * p.nchunk + tile / kTile) * p.d + ch] = s;
+            s = fold<P::G, false>(sA[buf], sB[buf], threadIdx.x, s);
+        }
+        __syncthreads();
+        float c[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) c[v] = sB[buf][w.span][w.lane * VEC + v];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) c[v] = step(a[r][v], c[v], u[r][v]);
+            if (w.in && mt + r < t1) Row<T, VEC>::store(ph + (mt + r) * p.ht, c);
+        }
+    }
+    if (mine && last && t1 == p.t) last[row] = s;
+}
+
+template <typename T, int VEC, bool SIG, bool MIX>
+__global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict__ dh, const T* __restrict__ x,
+                                                            const T* __restrict__ gate, const uint8_t* __restrict__ reset,
+                                                            const float* __restrict__ states,
+                                                            const float* __restrict__ dlast, const float* __restrict__ agg,
+                                                            T* __restrict__ dx, T* __restrict__ dgate,
+                                                            float* __restrict__ dh0, Params p) {
+    typedef Place<VEC> P;
+    typedef typename Row<T, VEC>::Raw Raw;
+    constexpr int R = P::R;
+    // A serves both folds, which run side by side; B and C become the states before a span
+    // and the gradients from behind it
+    __shared__ __attribute__((aligned(16))) float sA[P::G][kCh], sB[P::G][kCh], sC[P::G][kCh];
+    const P w(p);
+    const int seg = blockIdx.y;
+    const int64_t t0 = seg * p.seg, t1 = min(p.t, t0 + p.seg);
+    const T* pe = dh + w.b * p.hb + w.cc;
+    const T* px = x + w.b * p.xb + w.cc;
+    const T* pg = gate + w.b * p.gb + w.cc;
+    const int fold_ch = threadIdx.x & (kCh - 1), wave = threadIdx.x / kCh;
+    const int ch = (int)(blockIdx.x % p.nblk) * kCh + fold_ch;
+    const int64_t row = w.b * p.d + ch;
+    float s = 0.f;          // wave 1: the gradient from behind the tile
+    if (wave == 1 && ch < p.d) {
+        s = dlast ? dlast[row] : 0.f;
+        for (int g = p.nseg - 1; g > seg; --g)
+            s = step(agg[(int64_t)g * 2 * p.rows + row], s, agg[((int64_t)g * 2 + 1) * p.rows + row]);
+    }
+    Raw re[R], rx[R], rg[R];
+    uint32_t fresh = 0;
+    auto load = [&](int64_t tile) {
+        fresh = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t t = min(p.t - 1, tile + w.span * R + r);
+            re[r] = Row<T, VEC>::load(pe + t * p.ht);
+            rx[r] = Row<T, VEC>::load(px + t * p.xt);
+            rg[r] = Row<T, VEC>::load(pg + t * p.gt);
+            if (reset && tile + w.span * R + r < p.t && reset[w.b * p.t + t]) fresh |= 1u << r;
+        }
+    };
+    // Loads of the next tile are in flight while a tile is computed only where both fit the
+    // registers (bf16, 16-byte rows).
+    constexpr bool AHEAD = VEC == 8;
+    const int64_t first = t0, final = t0 + (t1 - t0 - 1) / kTile * kTile;
+    if (AHEAD) load(final);
+    for (int64_t tile = final; tile >= first; tile -= kTile) {
+        if (!AHEAD) load(tile);
+        const int64_t mt = tile + w.span * R;
+        const int live = (int)min<int64_t>(R, t1 - mt);     // tokens of the span that are there
+        uint32_t begins = fresh;
+        float a[R][VEC], A[VEC], B[VEC], C[VEC];
+        float take[MIX ? R : 1][VEC];
+        Raw ex[R], ee[R];       // x and dh as loaded: half the registers in bf16
+        const float before = wave == 0 && ch < p.d ? states[(w.b * p.nchunk + tile / kTile) * p.d + ch] : 0.f;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            A[v] = 1.f;
+            B[v] = C[v] = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float vg[VEC], vx[VEC];
+            ex[r] = rx[r];
+            ee[r] = re[r];
+            Row<T, VEC>::floats(rx[r], vx);
+            Row<T, VEC>::floats(rg[r], vg);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                float tk;
+                gates<SIG, MIX>(vg[v], a[r][v], tk);
+                if constexpr (MIX) take[r][v] = tk;
+                a[r][v] = r >= live ? 1.f : a[r][v];
+                const float k = (begins >> r) & 1 ? 0.f : a[r][v];
+                B[v] = step(k, B[v], r >= live ? 0.f : tk * vx[v]);
+                A[v] *= k;
+            }
+        }
+#pragma unroll
+        for (int r = R - 1; r >= 0; --r) {
+            float ve[VEC];
+            Row<T, VEC>::floats(ee[r], ve);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float k = (begins >> r) & 1 ? 0.f : a[r][v];
+                C[v] = k == 0.f ? 0.f : k * ((r >= live ? 0.f : ve[v]) + C[v]);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            sA[w.span][w.lane * VEC + v] = A[v];
+            sB[w.span][w.lane * VEC + v] = B[v];
+            sC[w.span][w.lane * VEC + v] = C[v];
+        }
+        if (AHEAD && tile > first) load(tile - kTile);
+        __syncthreads();
+        if (wave == 0) (void)fold<P::G, false>(sA, sB, fold_ch, before);
+        else if (wave == 1) s = fold<P::G, true>(sA, sC, fold_ch, s);
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            B[v] = sB[w.span][w.lane * VEC + v];
+            C[v] = sC[w.span][w.lane * VEC + v];
+        }
+        __syncthreads();    // the next tile's maps go where these were
+        anew(begins);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            anew(ex[r]);
+            anew(ee[r]);
+        }
+        float held[R][VEC];     // what e is multiplied by in da: the state before the token [− x]
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float vx[VEC];
+            Row<T, VEC>::floats(ex[r], vx);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const bool b = (begins >> r) & 1;
+                held[r][v] = (b ? 0.f : B[v]) - (MIX ? vx[v] : 0.f);
+                B[v] = step(b ? 0.f : a[r][v], B[v], MIX ? take[r][v] * vx[v] : vx[v]);
+            }
+        }
+#pragma unroll
+        for (int r = R - 1; r >= 0; --r) {
+            float ox[VEC], og[VEC], ve[VEC];
+            Row<T, VEC>::floats(ee[r], ve);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float k = (begins >> r) & 1 ? 0.f : a[r][v];
+                const float e = (r >= live ? 0.f : ve[v]) + C[v];
+                C[v] = k == 0.f ? 0.f : k * e;
+                ox[v] = MIX ? take[r][v] * e : e;
+                float da = held[r][v];
+                if constexpr (SIG) da *= MIX ? a[r][v] * take[r][v] : a[r][v] * (1.f - a[r][v]);
+                og[v] = da * e;
+            }
+            if (w.in && r < live) {
+                Row<T, VEC>::store(dx + w.b * p.dxb + (mt + r) * p.dxt + w.c, ox);
+                Row<T, VEC>::store(dgate + w.b * p.dgb + (mt + r) * p.dgt + w.c, og);
+            }
+        }
+    }
+    if (wave == 1 && ch < p.d && dh0 && seg == 0) dh0[row] = s;
+}
+
+// Few tokens: a thread goes through them with VEC channels, no tiles (a decoding step of
+// 64 x 2048 channels is one read of each input in flight).
+template <typename T, int VEC, bool SIG, bool MIX>
+__global__ __launch_bounds__(64) void scan_steps_kernel(const T* __restrict__ x, const T* __restrict__ gate,
+                                                        const float* __restrict__ h0, const uint8_t* __restrict__ reset,
+                                                        T* __restrict__ h, float* __restrict__ last,
+                                                        float* __restrict__ states, Params p) {
+    const int per = (p.d + VEC - 1) / VEC;
+    const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    const int64_t b = i / per;
+    const int c = (int)(i - b * per) * VEC;
+    if (b * p.d >= p.rows) return;
+    const int64_t row = b * p.d + c;
+    float s[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) s[v] = h0 ? h0[row + v] : 0.f;
+    if (states) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) states[row + v] = s[v];
+    }
+    for (int64_t t = 0; t < p.t; ++t) {
+        float vx[VEC], vg[VEC];
+        Row<T, VEC>::floats(Row<T, VEC>::load(x + b * p.xb + t * p.xt + c), vx);
+        Row<T, VEC>::floats(Row<T, VEC>::load(gate + b * p.gb + t * p.gt + c), vg);
+        const bool begins = reset && reset[b * p.t + t];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            float a, take;
+            gates<SIG, MIX>(vg[v], a, take);
+            s[v] = step(begins ? 0.f : a, s[v], take * vx[v]);
+        }
+        Row<T, VEC>::store(h + b * p.hb + t * p.ht + c, s);
+    }
+    if (last) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) last[row + v] = s[v];
+    }
+}
+
+constexpr int64_t kSteps = 16;      // up to so many tokens the tiles would be nearly empty
+
+// Empty sequences: the state goes through.
+__global__ __launch_bounds__(256) void scan_pass_kernel(const float* __restrict__ from, float* __restrict__ to, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) to[i] = from ? from[i] : 0.f;
+}
+
+bool whole(const void* p, int64_t sb, int64_t st, int elem) {
+    return (uintptr_t)p % 16 == 0 && sb * elem % 16 == 0 && st * elem % 16 == 0;
+}
+
+int check(nott_ctx ctx, const nott_scan_desc* d, nott_dtype dtype, Params* p) {
+    NOTT_REQUIRE(ctx, nott::valid_dtype(dtype), "linear scan: bad dtype");
+    NOTT_REQUIRE(ctx, d != nullptr, "linear scan: null descriptor");
+    NOTT_REQUIRE(ctx, d->b >= 0 && d->t >= 0 && d->d > 0 && d->d < (int64_t(1) << 30) && d->t < (int64_t(1) << 40) &&
+                          d->b < (int64_t(1) << 31), "linear scan: bad shape");
+    NOTT_REQUIRE(ctx, (d->sigmoid | d->mix) >> 1 == 0, "linear scan: sigmoid and mix are 0 or 1");
+    p->t = d->t;
+    p->d = (int32_t)d->d;
+    p->rows = d->b * d->d;
+    p->nblk = (int32_t)ceil_div(d->d, kCh);
+    p->nchunk = 0;
+    NOTT_REQUIRE(ctx, ceil_div(d->t, kTile) < (int64_t(1) << 31) && d->b * p->nblk <= 0x7fffffff / kThreads &&
+                          p->rows < (int64_t(1) << 36), "linear scan: too many channels or tokens");
+    p->nchunk = (int32_t)ceil_div(d->t, kTile);
+    auto strides = [&](const int64_t (&s)[2], int64_t& sb, int64_t& st) {
+        const bool dense = s[0] == 0 && s[1] == 0;
+        sb = dense ? d->t * d->d : s[0];
+        st = dense ? d->d : s[1];
+    };
+    strides(d->x_stride, p->xb, p->xt);
+    strides(d->gate_stride, p->gb, p->gt);
+    strides(d->h_stride, p->hb, p->ht);
+    strides(d->dx_stride, p->dxb, p->dxt);
+    strides(d->dgate_stride, p->dgb, p->dgt);
+    return NOTT_OK;
+}
+
+// Segments: one where the channels alone give every CU a workgroup, else as many as bring
+// two for each, of at least 4 tiles.
+void segments(nott_ctx ctx, Params* p, int64_t blocks) {
+    const int64_t tiles = p->nchunk;
+    int64_t n = blocks >= ctx->num_cu / 2 ? 1 : std::min<int64_t>(ceil_div(2 * ctx->num_cu, blocks), ceil_div(tiles, 4));
+    const int64_t len = ceil_div(tiles, n);
+    p->seg = len * kTile;
+    p->nseg = (int32_t)ceil_div(tiles, len);
+}
+
+template <typename T, int VEC, bool SIG, bool MIX>
+int fwd(nott_ctx ctx, Params& p, const void* x, const void* gate, const float* h0, const uint8_t* reset, void* h,
+        float* last, float* states) {
+    const T* tx = static_cast<const T*>(x);
+    const T* tg = static_cast<const T*>(gate);
+    const int64_t batches = p.rows / p.d;
+    if (p.t <= kSteps) {
+        const int64_t n = batches * ceil_div(p.d, VEC);
+        hipLaunchKernelGGL((scan_steps_kernel<T, VEC, SIG, MIX>), dim3((unsigned)ceil_div(n, 64)), dim3(64), 0, ctx->stream, tx,
+                           tg, h0, reset, static_cast<T*>(h), last, states, p);
+        return nott::launch_status(ctx, "scan_steps_kernel");
+    }
+    const int64_t blocks = batches * p.nblk;
+    segments(ctx, &p, blocks);
+    float* agg = nullptr;
+    if (p.nseg > 1) {
+        agg = static_cast<float*>(nott::optional_workspace(ctx, (size_t)p.nseg * 2 * p.rows * sizeof(float)));
+        if (!agg) p.nseg = 1, p.seg = (int64_t)p.nchunk * kTile;
+    }
+    if (p.nseg > 1)
+        hipLaunchKernelGGL((scan_maps_kernel<T, VEC, SIG, MIX, false>), dim3((unsigned)blocks, (unsigned)(p.nseg - 1)),
+                           dim3(kThreads), 0, ctx->stream, tx, tg, reset, agg, p);
+    hipLaunchKernelGGL((scan_fwd_kernel<T, VEC, SIG, MIX>), dim3((unsigned)blocks, (unsigned)p.nseg), dim3(kThreads), 0,
+                       ctx->stream, tx, tg, h0, reset, agg, static_cast<T*>(h), last, states, p);
+    return nott::launch_status(ctx, "scan_fwd_kernel");
+}
+
+template <typename T, int VEC, bool SIG, bool MIX>
+int bwd(nott_ctx ctx, Params& p, const void* dh, const void* x, const void* gate, const uint8_t* reset, const float* states,
+        const float* dlast, void* dx, void* dgate, float* dh0) {
+    const T* te = static_cast<const T*>(dh);
+    const T* tg = static_cast<const T*>(gate);
+    const int64_t blocks = p.rows / p.d * p.nblk;
+    segments(ctx, &p, blocks);
+    float* agg = nullptr;
+    if (p.nseg > 1) {
+        agg = static_cast<float*>(nott::optional_workspace(ctx, (size_t)p.nseg * 2 * p.rows * sizeof(float)));
+        if (!agg) p.nseg = 1, p.seg = (int64_t)p.nchunk * kTile;
+    }
+    if (p.nseg > 1)
+        hipLaunchKernelGGL((scan_maps_kernel<T, VEC, SIG, false, true>), dim3((unsigned)blocks, (unsigned)(p.nseg - 1)),
+                           dim3(kThreads), 0, ctx->stream, te, tg, reset, agg, p);
+    hipLaunchKernelGGL((scan_bwd_kernel<T, VEC, SIG, MIX>), dim3((unsigned)blocks, (unsigned)p.nseg), dim3(kThreads), 0,
+                       ctx->stream, te, static_cast<const T*>(x), tg, reset, states, dlast, agg, static_cast<T*>(dx),
+                       static_cast<T*>(dgate), dh0, p);
+    return nott::launch_status(ctx, "scan_bwd_kernel");
+}
+
+// Calls f with the type, width and gate form as template arguments.
+template <typename F>
+int dispatch(nott_dtype dtype, bool wide, const nott_scan_desc* d, F&& f) {
+    auto gate = [&](auto t, auto vec) {
+        using std::bool_constant;
+        if (d->sigmoid) return d->mix ? f(t, vec, bool_constant<true>(), bool_constant<true>())
+                                      : f(t, vec, bool_constant<true>(), bool_constant<false>());
+        return d->mix ? f(t, vec, bool_constant<false>(), bool_constant<true>())
+                      : f(t, vec, bool_constant<false>(), bool_constant<false>());
+    };
+    if (dtype == NOTT_BF16)
+        return wide ? gate(bf16_t(), std::integral_constant<int, 8>()) : gate(bf16_t(), std::integral_constant<int, 1>());
+    return wide ? gate(float(), std::integral_constant<int, 4>()) : gate(float(), std::integral_constant<int, 1>());
+}
+
+}  // namespace
+
+extern "C" int nott_linear_scan_fwd(nott_ctx ctx, const nott_scan_desc* d, nott_dtype dtype, const void* x, const void* gate,
+                                    const float* h0, const uint8_t* reset, void* h, float* last, float* states) {
+    NOTT_CHECK_CTX(ctx);
+    Params p{};
+    if (const int st = check(ctx, d, dtype, &p); st != NOTT_OK) return st;
+    if (p.rows == 0) return NOTT_OK;
+    nott::DeviceScope scope(ctx->device);
+    if (p.t == 0) {
+        if (last)
+            hipLaunchKernelGGL(scan_pass_kernel, dim3((unsigned)ceil_div(p.rows, 256)), dim3(256), 0, ctx->stream, h0, last, p.rows);
+        return nott::launch_status(ctx, "scan_pass_kernel");
+    }
+    NOTT_REQUIRE(ctx, x && gate && h, "nott_linear_scan_fwd: null buffer");
+    const int elem = (int)nott::dtype_size(dtype);
+    const bool wide = whole(x, p.xb, p.xt, elem) && whole(gate, p.gb, p.gt, elem) && whole(h, p.hb, p.ht, elem) &&
+                      p.d * elem % 16 == 0;
+    return dispatch(dtype, wide, d, [&](auto t, auto vec, auto sig, auto mix) {
+        return fwd<decltype(t), decltype(vec)::value, decltype(sig)::value, decltype(mix)::value>(ctx, p, x, gate, h0, reset, h,
+                                                                                                  last, states);
+    });
+}
+
+extern "C" int nott_linear_scan_bwd(nott_ctx ctx, const nott_scan_desc* d, nott_dtype dtype, const void* dh, const void* x,
+                                    const void* gate, const uint8_t* reset, const float* states, const float* dlast, void* dx,
+                                    void* dgate, float* dh0) {
+    NOTT_CHECK_CTX(ctx);
+    Params p{};
+    if (const int st = check(ctx, d, dtype, &p); st != NOTT_OK) return st;
+    if (p.rows == 0) return NOTT_OK;
+    nott::DeviceScope scope(ctx->device);
+    if (p.t == 0) {
+        if (dh0)
+            hipLaunchKernelGGL(scan_pass_kernel, dim3((unsigned)ceil_div(p.rows, 256)), dim3(256), 0, ctx->stream, dlast, dh0, p.rows);
+        return nott::launch_status(ctx, "scan_pass_kernel");
+    }
+    NOTT_REQUIRE(ctx, dh && x && gate && states && dx && dgate, "nott_linear_scan_bwd: null buffer");
+    const int elem = (int)nott::dtype_size(dtype);
+    const bool wide = whole(x, p.xb, p.xt, elem) && whole(gate, p.gb, p.gt, elem) && whole(dh, p.hb, p.ht, elem) &&
+                      whole(dx, p.dxb, p.dxt, elem) && whole(dgate, p.dgb, p.dgt, elem) && p.d * elem % 16 == 0;
+    return dispatch(dtype, wide, d, [&](auto t, auto vec, auto sig, auto mix) {
+        return bwd<decltype(t), decltype(vec)::value, decltype(sig)::value, decltype(mix)::value>(
+            ctx, p, dh, x, gate, reset, states, dlast, dx, dgate, dh0);
+    });
+}

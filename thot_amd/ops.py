@@ -971,6 +971,96 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w: torch.Tensor, gu: tor
     return dx, dw, db
 
 
+# ------------------------------------------------------ gated linear recurrence
+SCAN_CHUNK = 256     # tokens between the states that the forward keeps
+# ScanDesc's fields in order
+_SCAN = struct.Struct("=13q2i")
+assert _SCAN.size == C.sizeof(_abi.ScanDesc)
+
+
+def _scan_strides(t: Optional[torch.Tensor], name: str, like: torch.Tensor) -> tuple:
+    """(batch, token) strides of a [b, t, d] tensor whose channels are contiguous."""
+    if not isinstance(t, torch.Tensor) or t.shape != like.shape:
+        raise ValueError(f"{name} must be a tensor of shape {tuple(like.shape)}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise TypeError(f"{name} must have the dtype and device of x")
+    sb, st, one = t.stride()
+    if one != 1 and t.shape[2] > 1:
+        raise ValueError(f"the channels of {name} must be contiguous")
+    if sb == st == 0 and t.shape[0] * t.shape[1] > 1:   # two zeros mean contiguous to the entry point
+        raise ValueError(f"{name} repeats one token (strides {t.stride()}); make it contiguous")
+    return sb, st
+
+
+def _scan_args(x: torch.Tensor, gate: torch.Tensor, reset: Optional[torch.Tensor]):
+    if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.shape[2] == 0:
+        raise ValueError("x must be [b, t, d] with d > 0")
+    nott_dtype(x.dtype)
+    xs, gs = _scan_strides(x, "x", x), _scan_strides(gate, "gate", x)
+    if not x.is_cuda:
+        raise ValueError("x must be a device tensor")
+    if reset is not None:
+        if reset.dtype not in (torch.bool, torch.uint8):
+            raise TypeError("reset must be bool or uint8")
+        _check(reset, "reset", shape=x.shape[:2], device=x.device)
+    return xs, gs
+
+
+def linear_scan_fwd(x: torch.Tensor, gate: torch.Tensor, h0: Optional[torch.Tensor] = None, *, sigmoid: bool = True,
+                    mix: bool = True, reset: Optional[torch.Tensor] = None, save: bool = False,
+                    out: Optional[torch.Tensor] = None):
+    """h_t = a_t·h_{t-1} + take_t·x_t over the tokens of x [b, t, d] (views of a
+    projection, any strides but the last), channel by channel: a = sigmoid(gate) (gate
+    itself with sigmoid=False), take = 1 - a (1 with mix=False).  h0: the state before
+    the first token, fp32 [b, d] (None: zeros); reset: bool [b, t], True where a new
+    sequence begins.  Returns (h, last, states): last, the state after the last token,
+    fp32 [b, d]; states [b, ceil(t / 256), d], what the backward needs, None unless
+    save (nott_linear_scan_fwd)."""
+    xs, gs = _scan_args(x, gate, reset)
+    b, t, d = x.shape
+    if h0 is not None:
+        _check(h0, "h0", shape=(b, d), dtype=torch.float32, device=x.device)
+    hs = (0, 0)
+    if out is None:
+        out = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
+    else:
+        hs = _scan_strides(out, "out", x)
+        _check_out(out, "out")
+    last = x.new_empty((b, d), dtype=torch.float32)
+    states = x.new_empty((b, -(-t // SCAN_CHUNK), d), dtype=torch.float32) if save else None
+    desc = _SCAN.pack(b, t, d, *xs, *gs, *hs, 0, 0, 0, 0, bool(sigmoid), bool(mix))
+    _ctx_for(x).call("nott_linear_scan_fwd", desc, _DTYPES[x.dtype], _ptr(x), _ptr(gate), _ptr(h0), _ptr(reset), _ptr(out),
+                     _ptr(last), _ptr(states))
+    return out, last, states
+
+
+def linear_scan_bwd(dh: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, states: torch.Tensor, *, sigmoid: bool = True,
+                    mix: bool = True, reset: Optional[torch.Tensor] = None, dlast: Optional[torch.Tensor] = None,
+                    out=None):
+    """(dx, dgate, dh0) of linear_scan_fwd from the gradients dh of h and dlast of last
+    (None: zeros), its inputs and its states; dh0 fp32 [b, d].  `out` = (dx, dgate) to
+    write into, e.g. views of a packed gradient (nott_linear_scan_bwd)."""
+    xs, gs = _scan_args(x, gate, reset)
+    b, t, d = x.shape
+    hs = _scan_strides(dh, "dh", x)
+    _check(states, "states", shape=(b, -(-t // SCAN_CHUNK), d), dtype=torch.float32, device=x.device)
+    if dlast is not None:
+        _check(dlast, "dlast", shape=(b, d), dtype=torch.float32, device=x.device)
+    ds = (0, 0, 0, 0)
+    if out is None:
+        dx, dgate = (torch.empty((b, t, d), dtype=x.dtype, device=x.device) for _ in range(2))
+    else:
+        dx, dgate = out
+        ds = (*_scan_strides(dx, "dx", x), *_scan_strides(dgate, "dgate", x))
+        _check_out(dx, "dx")
+        _check_out(dgate, "dgate")
+    dh0 = x.new_empty((b, d), dtype=torch.float32)
+    desc = _SCAN.pack(b, t, d, *xs, *gs, *hs, *ds, bool(sigmoid), bool(mix))
+    _ctx_for(x).call("nott_linear_scan_bwd", desc, _DTYPES[x.dtype], _ptr(dh), _ptr(x), _ptr(gate), _ptr(reset),
+                     _ptr(states), _ptr(dlast), _ptr(dx), _ptr(dgate), _ptr(dh0))
+    return dx, dgate, dh0
+
+
 # ------------------------------------------------- log probabilities of given tokens
 def token_logprob_fwd(logits: torch.Tensor, labels: torch.Tensor, *, scale: float = 1.0, top: int = 0):
     """(logprob, entropy, lse, top_logprob, top_index) of the rows of logits [n, c]
