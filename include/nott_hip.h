@@ -341,6 +341,42 @@ int nott_attention_bwd(nott_ctx ctx, const nott_attn_desc* d, nott_dtype dtype,
                        const void* q, const void* k, const void* v, const void* o,
                        const void* dO, const float* lse, void* dq, void* dk, void* dv);
 
+/* ---- differential attention ------------------------------------------------------
+ * Attention whose heads have two maps, the second subtracted with a learned weight:
+ *   z_r = q_r·k_rᵀ·scale, p_r = softmax(z_r), o_r = p_r·v for r = 1, 2;  o = o_1 − λ·o_2
+ * q [b, t, 2·h, dh] and k [b, s, 2·hk, dh]: the maps of head i are heads 2·i and 2·i + 1
+ * (of key head j = i / (h / hk): 2·j and 2·j + 1, and its values are head j of
+ * v [b, s, hk, dv]).  o, o2 [b, t, h, dv]; lse [b, 2·h, t] fp32; dv is usually 2·dh.
+ * Strides in elements for batch, token and head, columns side by side; three zeros =
+ * contiguous.  So q, k, v may be views of a packed projection, or head-major; o2 is
+ * contiguous.
+ * lam fp32: λ of each head [h], or with token_lam = 1 of each token and head [b, t, h].
+ * lengths int32 [b] (nullable: s): keys from there on are not seen (values outside [0, s]
+ * count as the nearest).  causal = 1: query i sees keys up to q_start[b] + i (q_start
+ * int32 [b], nullable: 0), so with a cache q_start = lengths − t.  A row that sees no
+ * key has o = 0 and lse = −inf.  Keys that no row of a block of rows sees are not read.
+ * scale > 0.  dh <= 128, dv <= 256 (fp32: half of both); s and t·h/hk up to 4000000.  No output may overlap an input.
+ * o2 (nullable) receives o_2 for the backward.  Workspace: fp32 parts of the output where
+ * few rows have their keys split (without room for them, they are not split). */
+typedef struct nott_diff_attn_desc {
+    int64_t b, h, hk, t, s, dh, dv;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+    int64_t do_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];   /* backward */
+    int32_t causal, token_lam;
+    double scale;                /* usually 1/sqrt(dh) */
+} nott_diff_attn_desc;
+int nott_diff_attention_fwd(nott_ctx ctx, const nott_diff_attn_desc* d, nott_dtype dtype, const void* q, const void* k,
+                            const void* v, const float* lam, const int32_t* lengths, const int32_t* q_start,
+                            void* o, float* lse, void* o2);
+/* From dO [b, t, h, dv] and the forward's arguments and results (o, o2 and lse as it left
+ * them: the sums dO·o and dO·o2 take the place of Σ p·dp): dq, dk, dv in the layouts of
+ * q, k, v (zeros for keys that no row sees), and dlam in lam's shape; accumulate = 1 adds
+ * into dlam [h].  Workspace: five fp32 [b, h, t]. */
+int nott_diff_attention_bwd(nott_ctx ctx, const nott_diff_attn_desc* d, nott_dtype dtype, const void* dO, const void* q,
+                            const void* k, const void* v, const float* lam, const int32_t* lengths,
+                            const int32_t* q_start, const void* o, const void* o2, const float* lse,
+                            void* dq, void* dk, void* dv, float* dlam, int accumulate);
+
 /* ---- queries and keys: norm of each head, rotation by position --------------
  * What decoder attention does between the packed projection and the attention
  * core, in one pass over q and k.  For head vector x of dh elements:

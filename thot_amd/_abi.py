@@ -56,6 +56,13 @@ class QkRopeDesc(C.Structure):
                [(n, C.c_int32) for n in ("axes", "interleaved", "norm", "reserved")] + [("eps", f64)]
 
 
+class DiffAttnDesc(C.Structure):
+    _fields_ = [(n, i64) for n in ("b", "h", "hk", "t", "s", "dh", "dv")] + \
+               [(n, i64 * 3) for n in ("q_stride", "k_stride", "v_stride", "o_stride", "do_stride", "dq_stride",
+                                       "dk_stride", "dv_stride")] + \
+               [("causal", C.c_int32), ("token_lam", C.c_int32), ("scale", f64)]
+
+
 class ScanDesc(C.Structure):
     _fields_ = [(n, i64) for n in ("b", "t", "d")] + \
                [(n, i64 * 2) for n in ("x_stride", "gate_stride", "h_stride", "dx_stride", "dgate_stride")] + \
@@ -115,6 +122,8 @@ SIGNATURES: dict[str, list] = {
     "nott_softmax_xent_bwd": [vp, i32, i64, i64, vp, vp, f64, f64, vp, fp],
     "nott_attention_fwd": [vp, C.POINTER(AttnDesc), i32, vp, vp, vp, vp, fp],
     "nott_attention_bwd": [vp, C.POINTER(AttnDesc), i32, vp, vp, vp, vp, vp, fp, vp, vp, vp],
+    "nott_diff_attention_fwd": [vp, vp, i32, vp, vp, vp, fp, vp, vp, vp, fp, vp],
+    "nott_diff_attention_bwd": [vp, vp, i32, vp, vp, vp, vp, fp, vp, vp, vp, vp, fp, vp, vp, vp, fp, i32],
     "nott_qk_norm_rope_fwd": [vp, C.POINTER(QkRopeDesc), i32, vp, vp, vp, vp, vp, vp, vp, vp],
     "nott_qk_norm_rope_bwd": [vp, C.POINTER(QkRopeDesc), i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, fp, fp, i32],
     "nott_gated_linear_fwd": [vp, i32, i64, i64, i64, i32, vp, vp, fp, vp, vp],

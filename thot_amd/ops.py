@@ -746,6 +746,117 @@ def attention_bwd(q, k, v, o, dO, lse, d: AttnDesc, out=None):
     return dq, dk, dv
 
 
+# ------------------------------------------------------ differential attention
+# DiffAttnDesc's fields in order
+_DIFF = struct.Struct("=31q2id")
+assert _DIFF.size == C.sizeof(_abi.DiffAttnDesc)
+
+
+def _diff_strides(t: Optional[torch.Tensor], name: str, shape: tuple, like: torch.Tensor) -> tuple:
+    """(batch, token, head) strides of a [b, rows, heads, width] tensor whose columns are contiguous."""
+    if not isinstance(t, torch.Tensor) or t.shape != shape:
+        raise ValueError(f"{name} must be a tensor of shape {tuple(shape)}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise TypeError(f"{name} must have the dtype and device of q")
+    sb, st, sh, one = t.stride()
+    if one != 1 and t.numel() and shape[3] > 1:
+        raise ValueError(f"the columns of {name} must be contiguous")
+    if sb == st == sh == 0 and t.numel() > shape[3]:   # three zeros mean contiguous to the entry point
+        raise ValueError(f"{name} repeats one row (strides {t.stride()}); make it contiguous")
+    return sb, st, sh
+
+
+def _diff_args(q, k, v, lam, scale, lengths, q_start):
+    """Checks what both directions share: (b, h, hk, t, s, dh, dv), the strides of q, k and v, scale."""
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if not isinstance(t, torch.Tensor) or t.dim() != 4:
+            raise ValueError("q must be [b, t, 2·h, dh], k [b, s, 2·hk, dh] and v [b, s, hk, dv]")
+    b, t, h, dh = q.shape
+    _, s, hk, dv = v.shape
+    if h % 2 or dh == 0 or dv == 0 or (h and (hk == 0 or h // 2 % hk)):
+        raise ValueError(f"q has {h} maps for {hk} heads of values: two for each head, heads in whole groups of v's")
+    h //= 2
+    nott_dtype(q.dtype)
+    most = 128 if q.dtype == torch.bfloat16 else 64
+    if dh > most or dv > 2 * most:
+        raise ValueError(f"head size must be 1 to {most} and that of values 1 to {2 * most} in {q.dtype}")
+    scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
+    if not 0 < scale < 1e30:
+        raise ValueError("scale must be positive")
+    st = (*_diff_strides(q, "q", q.shape, q), *_diff_strides(k, "k", (b, s, 2 * hk, dh), q),
+          *_diff_strides(v, "v", (b, s, hk, dv), q))
+    if not q.is_cuda:
+        raise ValueError("q must be a device tensor")
+    _check(lam, "lam", shape=(b, t, h) if isinstance(lam, torch.Tensor) and lam.dim() == 3 else (h,), dtype=torch.float32,
+           device=q.device)
+    for x, name in ((lengths, "lengths"), (q_start, "q_start")):
+        if x is not None:
+            _check(x, name, shape=(b,), dtype=torch.int32, device=q.device)
+    return (b, h, hk, t, s, dh, dv), st, scale
+
+
+_NONE3 = (0, 0, 0)
+
+
+def diff_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, *, causal: bool = False,
+                       scale: Optional[float] = None, lengths: Optional[torch.Tensor] = None,
+                       q_start: Optional[torch.Tensor] = None, save: bool = False, out: Optional[torch.Tensor] = None):
+    """Differential attention, o = softmax(q₁·k₁ᵀ·scale)·v − lam·softmax(q₂·k₂ᵀ·scale)·v
+    per head: q [b, t, 2·h, dh] and k [b, s, 2·hk, dh] with the two maps of a head
+    side by side, v [b, s, hk, dv], h a multiple of hk (views of a packed projection, any
+    strides but the last); lam fp32 [h], or [b, t, h].  lengths int32 [b]: the keys of each
+    sequence; causal: query i sees keys up to q_start[b] + i (int32 [b], None: 0).
+    scale None: 1/sqrt(dh).  Returns (o [b, t, h, dv], lse [b, 2·h, t], o2): o2, the second
+    map's output, is for the backward, None unless save (nott_diff_attention_fwd)."""
+    (b, h, hk, t, s, dh, dv), st, scale = _diff_args(q, k, v, lam, scale, lengths, q_start)
+    os = _NONE3
+    if out is None:
+        out = q.new_empty((b, t, h, dv))
+    else:
+        os = _diff_strides(out, "out", (b, t, h, dv), q)
+        _check_out(out, "out")
+    lse = q.new_empty((b, 2 * h, t), dtype=torch.float32)
+    o2 = q.new_empty((b, t, h, dv)) if save else None
+    desc = _DIFF.pack(b, h, hk, t, s, dh, dv, *st, *os, *_NONE3, *_NONE3, *_NONE3, *_NONE3, bool(causal), lam.dim() == 3, scale)
+    _ctx_for(q).call("nott_diff_attention_fwd", desc, _DTYPES[q.dtype], _ptr(q), _ptr(k), _ptr(v), _ptr(lam), _ptr(lengths),
+                     _ptr(q_start), _ptr(out), _ptr(lse), _ptr(o2))
+    return out, lse, o2
+
+
+def diff_attention_bwd(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
+                       o: torch.Tensor, o2: torch.Tensor, lse: torch.Tensor, *, causal: bool = False,
+                       scale: Optional[float] = None, lengths: Optional[torch.Tensor] = None,
+                       q_start: Optional[torch.Tensor] = None, dlam: Optional[torch.Tensor] = None,
+                       accumulate: bool = False, out=None):
+    """(dq, dk, dv, dlam) of diff_attention_fwd from the gradient do of its output, its
+    arguments and its o, o2 and lse; dlam in lam's shape, fp32 (accumulate: added to the
+    one given, for lam [h]).  `out` = (dq, dk, dv) to write into, e.g. views of a packed
+    gradient (nott_diff_attention_bwd)."""
+    (b, h, hk, t, s, dh, dv), st, scale = _diff_args(q, k, v, lam, scale, lengths, q_start)
+    if accumulate and (dlam is None or lam.dim() == 3):
+        raise ValueError("accumulate needs a gradient of lam [h] to add to")
+    rows = (b, t, h, dv)
+    st += (*_diff_strides(o, "o", rows, q), *_diff_strides(do, "do", rows, q))
+    _check(o2, "o2", shape=rows, dtype=q.dtype, device=q.device)
+    _check(lse, "lse", shape=(b, 2 * h, t), dtype=torch.float32, device=q.device)
+    if out is None:
+        dq, dk, dvv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
+        st += (*_NONE3, *_NONE3, *_NONE3)
+    else:
+        dq, dk, dvv = out
+        for x, name, shape in ((dq, "dq", q.shape), (dk, "dk", k.shape), (dvv, "dv", v.shape)):
+            st += _diff_strides(x, name, shape, q)
+            _check_out(x, name)
+    if dlam is None:
+        dlam = torch.empty_like(lam)
+    _check(dlam, "dlam", shape=tuple(lam.shape), dtype=torch.float32, device=q.device)
+    desc = _DIFF.pack(b, h, hk, t, s, dh, dv, *st, bool(causal), lam.dim() == 3, scale)
+    _ctx_for(q).call("nott_diff_attention_bwd", desc, _DTYPES[q.dtype], _ptr(do), _ptr(q), _ptr(k), _ptr(v), _ptr(lam),
+                     _ptr(lengths), _ptr(q_start), _ptr(o), _ptr(o2), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dvv), _ptr(dlam),
+                     int(accumulate))
+    return dq, dk, dvv, dlam
+
+
 # ------------------------------------------------- queries and keys: norm, rotation
 def rope_frequencies(rot: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
     """inv_freq[i] = theta^(-2i/rot), i < rot/2, in float64: radians per position of each rotated pair."""
