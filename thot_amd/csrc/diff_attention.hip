@@ -173,8 +173,8 @@ using nott::lds::lds_addr;
 using nott::lds::wait_vm_lgkm0;
 
 // Fills a [ROWS][32·NB] tile with the rows that `from` points to: 1 KB blocks dealt to
-// WAVES waves.
-template <int NB, int ROWS, int WAVES, typename F>
+// WAVES waves.  WHOLE: cols is 32·NB, so no chunk is padding.
+template <int NB, int ROWS, int WAVES, bool WHOLE, typename F>
 __device__ __forceinline__ void fill_rows(F&& from, int cols, char NOTT_LDS* tile, int wid, int lane) {
     constexpr int CH = 4 * NB, BLOCKS = ROWS * CH / 64;
     static_assert(BLOCKS % WAVES == 0, "blocks split evenly over the waves");
@@ -183,20 +183,67 @@ __device__ __forceinline__ void fill_rows(F&& from, int cols, char NOTT_LDS* til
         const int q = wid + WAVES * qq;
         const int i = 64 * q + lane, r = i / CH;
         const int c = swz<NB>(r, i - r * CH);   // (an involution)
-        dma16(8 * c < cols ? from(r) + 8 * c : reinterpret_cast<const bf16_t*>(&zero_chunk), lds_addr(tile) + 1024 * q);
+        const bf16_t* src = from(r) + 8 * c;
+        if constexpr (!WHOLE) {     // a select, not a branch around the address
+            uint64_t a = reinterpret_cast<uint64_t>(src), z = reinterpret_cast<uint64_t>(&zero_chunk);
+            asm volatile("" : "+v"(a));
+            src = reinterpret_cast<const bf16_t*>(8 * c < cols ? a : z);
+        }
+        dma16(src, lds_addr(tile) + 1024 * q);
     }
 }
 
 // A row as 2·NB B-operand slices: lane l holds d = 16s + 8·(l/32) + 0..7.
-template <int NB>
+template <int NB, bool WHOLE>
 __device__ __forceinline__ void load_row(const bf16_t* row, int cols, int lane, u32x4 (&r)[2 * NB]) {
 #pragma unroll
     for (int s = 0; s < 2 * NB; ++s) {
         const int d = 16 * s + 8 * (lane >> 5);
-        r[s] = *reinterpret_cast<const u32x4*>(row + (d < cols ? d : 0));
-        if (d >= cols) r[s] = u32x4{0u, 0u, 0u, 0u};
+        r[s] = *reinterpret_cast<const u32x4*>(row + (WHOLE || d < cols ? d : 0));
+        if (!WHOLE && d >= cols) r[s] = u32x4{0u, 0u, 0u, 0u};
     }
 }
+
+// Where a lane reads a tile: frag_rows' and frag_cols' places, formed once.  The swizzle
+// depends on a row's low 4 bits and permutes chunks within groups, so the places of other
+// row blocks and groups are constants away; left to itself the compiler kept a register
+// for each (61 spilled in the forward at ND = 2, 353 in the dk/dv pass at ND = 4).
+template <int NB>
+struct RowPlaces {
+    static constexpr int K = NB % 4 == 0 ? 8 : NB % 4 == 2 ? 4 : 2;      // slices of a group
+    uint32_t off[K];
+    __device__ __forceinline__ explicit RowPlaces(int lane) {
+#pragma unroll
+        for (int s = 0; s < K; ++s) off[s] = tile_off<NB>(lane & 31, 2 * s + (lane >> 5));
+    }
+    __device__ __forceinline__ bf16x8 get(const char NOTT_LDS* tile, int r0, int s) const {
+        return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 NOTT_LDS*>(tile + off[s % K] + r0 * (64 * NB) +
+                                                                                   s / K * (32 * K)));
+    }
+};
+template <int NB>
+struct ColPlaces {
+    static constexpr int K = NB % 4 == 0 ? 4 : NB % 4 == 2 ? 2 : 1;      // 32-column blocks of a group
+    uint32_t off[K][2];
+    __device__ __forceinline__ explicit ColPlaces(int lane) {
+        const int j = lane & 15, g = lane >> 4, r = 4 * (g >> 1) + (j >> 2);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int col = 32 * k + 16 * (g & 1) + 4 * (j & 3);
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi) off[k][hi] = tile_off<NB>(r + 8 * hi, col >> 3) + (col & 7) * 2;
+        }
+    }
+    // rows from rs (a multiple of 16), column block df
+    __device__ __forceinline__ bf16x8 get(const char NOTT_LDS* tile, int rs, int df) const {
+        v4i16s w[2];
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi)
+            w[hi] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (v4i16s NOTT_LDS*)(tile + off[df % K][hi] + rs * (64 * NB) + df / K * (64 * K)));
+        return __builtin_bit_cast(bf16x8, w);
+    }
+};
 
 template <int NB>
 __device__ __forceinline__ float dot_rows(const u32x4 (&a)[2 * NB], const u32x4 (&b)[2 * NB]) {
@@ -280,233 +327,207 @@ __device__ __forceinline__ void store_block(bf16_t* row, int df, int cols, int h
     }
 }
 
-// Forward: 128 rows a workgroup (32 a wave), 64 keys a stage.
-template <int ND, int RING>
-__global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_fwd32_kernel(const bf16_t* __restrict__ q,
-                                                                              const bf16_t* __restrict__ k,
-                                                                              const bf16_t* __restrict__ v,
-                                                                              bf16_t* __restrict__ o, bf16_t* __restrict__ o2,
-                                                                              float* __restrict__ lse, Params p) {
-    constexpr int NV = 2 * ND, TR = 64, KT = TR * 64 * ND, STAGE = 4 * KT;   // k1, k2, v
-    constexpr int LOADS = 4 * ND;                                            // per wave and stage
+// The tiles of 64 keys (both maps' keys, values) that a stage holds, filled by WAVES waves.
+template <int ND, int WAVES, bool WHOLE>
+struct KeyStage {
+    static constexpr int TR = 64, KT = TR * 64 * ND, BYTES = 4 * KT, LOADS = 16 * ND / WAVES;   // loads of a wave
+    const bf16_t* pk;
+    const bf16_t* pv;
+    __device__ __forceinline__ KeyStage(const Params& p, const Pair& w, const bf16_t* k, const bf16_t* v)
+        : pk(at(k, p.k, w.b, 0, 2 * w.j)), pv(at(v, p.v, w.b, 0, w.j)) {}
+    // keys past `most`, which nothing sees, are not read
+    __device__ __forceinline__ void fill(const Params& p, int tile, int most, char NOTT_LDS* st, int wid, int lane) const {
+        auto key = [&](int x) { return (int64_t)min(tile * TR + x, most - 1); };
+        fill_rows<ND, 2 * TR, WAVES, WHOLE>(
+            [&](int x) { return pk + (x >= TR ? p.k[2] : 0) + key(x >= TR ? x - TR : x) * p.k[1]; }, p.dh, st, wid, lane);
+        fill_rows<2 * ND, TR, WAVES, WHOLE>([&](int x) { return pv + key(x) * p.v[1]; }, p.dv, st + 2 * KT, wid, lane);
+    }
+};
+
+// Forward: 128 rows a workgroup, 64 keys a stage.  A wave has 32 rows of one map (8
+// waves), so that its scores and accumulator leave room for two waves a SIMD at 128 + 256
+// columns and more at 64 + 128; both maps in a wave shared the values' fragments but spilled
+// 41 and 213 registers (97.6 us for the benchmark's 8 x 1024 tokens, 8 heads of 64 + 128).
+// The second map's output goes to the first map's waves through LDS.
+template <int ND, int RING, bool WHOLE>
+__global__ __launch_bounds__(128 * NW, 2) void diff_fwd32_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k,
+                                                                 const bf16_t* __restrict__ v, bf16_t* __restrict__ o,
+                                                                 bf16_t* __restrict__ o2, float* __restrict__ lse, Params p) {
+    using Keys = KeyStage<ND, 2 * NW, WHOLE>;
+    constexpr int NV = 2 * ND, TR = Keys::TR, KT = Keys::KT;
     extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
     char NOTT_LDS* smem = (char NOTT_LDS*)smem_raw;
     const Pair w(p, blockIdx.x);
     const int nrb = (p.rows + FIXED - 1) / FIXED;
     const int r0 = (nrb - 1 - (int)blockIdx.y) * FIXED;   // heaviest (causal) blocks first
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int h = lane >> 5;
-    const int rw0 = r0 + 32 * wid, my_r = rw0 + (lane & 31);
+    const int h = lane >> 5, map = wid / NW, wr = wid % NW;
+    const int rw0 = r0 + 32 * wr, my_r = rw0 + (lane & 31);
     const RowAt r(p, w, min(my_r, p.rows - 1));
     const int vis = w.visible(p, r.i);
     const int vis_all = w.visible(p, RowAt(p, w, min(r0 + FIXED, p.rows) - 1).i);
     const int vis_lo = w.visible(p, RowAt(p, w, min(rw0, p.rows - 1)).i);
-    const int vis_hi = w.visible(p, RowAt(p, w, min(rw0 + 32, p.rows) - 1).i);
+    const int vis_hi = rw0 < p.rows ? w.visible(p, RowAt(p, w, min(rw0 + 32, p.rows) - 1).i) : 0;
     const float sl2 = p.scale * kLog2e;
-
-    u32x4 qr[2][2 * ND];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) load_row<ND>(at(q, p.q, w.b, r.i, 2 * r.head + m), p.dh, lane, qr[m]);
+    const RowPlaces<ND> rows_k(lane);
+    const ColPlaces<NV> cols_v(lane);
+    u32x4 qr[2 * ND];
+    load_row<ND, WHOLE>(at(q, p.q, w.b, r.i, 2 * r.head + map), p.dh, lane, qr);
+    const Keys keys(p, w, k, v);
     const int nk = (vis_all + TR - 1) / TR;
-    const bf16_t* pk = at(k, p.k, w.b, 0, 2 * w.j);
-    const bf16_t* pv = at(v, p.v, w.b, 0, w.j);
-    auto issue = [&](int i, int slot) {
-        char NOTT_LDS* st = smem + slot * STAGE;
-        auto key = [&](int x) { return (int64_t)min(i * TR + x, vis_all - 1); };
-        fill_rows<ND, TR, NW>([&](int x) { return pk + key(x) * p.k[1]; }, p.dh, st, wid, lane);
-        fill_rows<ND, TR, NW>([&](int x) { return pk + p.k[2] + key(x) * p.k[1]; }, p.dh, st + KT, wid, lane);
-        fill_rows<NV, TR, NW>([&](int x) { return pv + key(x) * p.v[1]; }, p.dv, st + 2 * KT, wid, lane);
-    };
 #pragma unroll
     for (int i = 0; i < RING - 1; ++i)
-        if (i < nk) issue(i, i);
+        if (i < nk) keys.fill(p, i, vis_all, smem + i * Keys::BYTES, wid, lane);
 
-    f32x16 acc[2][NV];
-    zero(acc[0]);
-    zero(acc[1]);
-    float mm[2] = {-INFINITY, -INFINITY}, ll[2] = {0.f, 0.f};   // ll: this lane's keys only
+    f32x16 acc[NV];
+    zero(acc);
+    float m = -INFINITY, l = 0.f;   // l: this lane's keys only
     int slot = 0, next = RING - 1;
     for (int i = 0; i < nk; ++i) {
-        if (i + RING - 2 < nk) wait_vm_lgkm0<(RING - 2) * LOADS>();
+        if (i + RING - 2 < nk) wait_vm_lgkm0<(RING - 2) * Keys::LOADS>();
         else wait_vm_lgkm0<0>();
         barrier();
-        if (i + RING - 1 < nk) issue(i + RING - 1, next);
-        const char NOTT_LDS* tk = smem + slot * STAGE;
-        const char NOTT_LDS* tv = tk + 2 * KT;
+        if (i + RING - 1 < nk) keys.fill(p, i + RING - 1, vis_all, smem + next * Keys::BYTES, wid, lane);
+        const char NOTT_LDS* tk = smem + slot * Keys::BYTES + map * KT;
+        const char NOTT_LDS* tv = smem + slot * Keys::BYTES + 2 * KT;
         slot = slot + 1 == RING ? 0 : slot + 1;
         next = next + 1 == RING ? 0 : next + 1;
         const int k0 = i * TR;
-        if (k0 >= vis_hi || rw0 >= p.rows) continue;   // every key of the block masked for this wave
+        if (k0 >= vis_hi) continue;   // every key of the block masked for this wave
         const bool full = k0 + TR <= vis_lo;
         const int rel = vis - k0 - 4 * h;
-        bf16x8 pb[2][4];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            f32x16 st[2];
-            zero(st);
+        for (int f = 0; f < 2; ++f) {
+            f32x16 st[1];
+            bf16x8 pb[2];
 #pragma unroll
-            for (int f = 0; f < 2; ++f)
+            for (int s = 0; s < 2 * ND; ++s)
+                st[0] = mfma(rows_k.get(tk, 32 * f, s), __builtin_bit_cast(bf16x8, qr[s]), s ? st[0] : f32x16{});
+            softmax_step<1, NV>(st, pb, acc, m, l, sl2, full, rel - 32 * f);
 #pragma unroll
-                for (int s = 0; s < 2 * ND; ++s)
-                    st[f] = mfma(frag_rows<ND>(tk + m * KT, 32 * f, s, lane), __builtin_bit_cast(bf16x8, qr[m][s]), st[f]);
-            softmax_step<2, NV>(st, pb[m], acc[m], mm[m], ll[m], sl2, full, rel);
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int df = 0; df < NV; ++df) acc[df] = mfma(cols_v.get(tv, 32 * f + 16 * s, df), pb[s], acc[df]);
         }
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int df = 0; df < NV; ++df) {
-                const bf16x8 vb = frag_cols<NV>(tv, 16 * s, 32 * df, lane);
-                acc[0][df] = mfma(vb, pb[0][s], acc[0][df]);
-                acc[1][df] = mfma(vb, pb[1][s], acc[1][df]);
-            }
     }
-#pragma unroll
-    for (int m = 0; m < 2; ++m) ll[m] += __shfl_xor(ll[m], 32, 64);
+    l += __shfl_xor(l, 32, 64);
     const bool in = my_r < p.rows;
-    const float i1 = ll[0] > 0.f ? 1.f / ll[0] : 0.f, i2 = ll[1] > 0.f ? 1.f / ll[1] : 0.f;
-    const float li2 = lambda_of(p, w.b, r) * i2;
-    bf16_t* orow = in ? at(o, p.o, w.b, r.i, r.head) : nullptr;
-    bf16_t* o2row = in && o2 ? o2 + (((int64_t)w.b * p.t + r.i) * p.h + r.head) * p.dv : nullptr;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    if (in && h == 0) *lse_at(p, lse, w.b, r, map) = log_sum(m, l);
+    float* second = reinterpret_cast<float*>(smem_raw) + (wr * NV << 10) + lane;   // [NV][16][64] of a row block
+    __syncthreads();
+    if (map) {
+        bf16_t* row = in && o2 ? o2 + (((int64_t)w.b * p.t + r.i) * p.h + r.head) * p.dv : nullptr;
 #pragma unroll
-    for (int df = 0; df < NV; ++df) {
-        store_block(orow, df, p.dv, h, [&](int e) { return acc[0][df][e] * i1 - acc[1][df][e] * li2; });
-        if (o2) store_block(o2row, df, p.dv, h, [&](int e) { return acc[1][df][e] * i2; });
+        for (int df = 0; df < NV; ++df) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) second[(df * 16 + e) << 6] = acc[df][e] * inv;
+            if (o2) store_block(row, df, p.dv, h, [&](int e) { return acc[df][e] * inv; });
+        }
     }
-    if (in) *lse_at(p, lse, w.b, r, h) = log_sum(h ? mm[1] : mm[0], h ? ll[1] : ll[0]);
+    __syncthreads();
+    if (map) return;
+    const float lam = lambda_of(p, w.b, r);
+    bf16_t* row = in ? at(o, p.o, w.b, r.i, r.head) : nullptr;
+#pragma unroll
+    for (int df = 0; df < NV; ++df)
+        store_block(row, df, p.dv, h, [&](int e) { return acc[df][e] * inv - lam * second[(df * 16 + e) << 6]; });
 }
 
-// Few rows: 32 rows a workgroup, its keys split over the grid and again over the waves,
-// each wave with 32-key tiles and a ring of its own (no barrier until the end).
-template <int ND>
-constexpr int split_waves() { return ND <= 2 ? 4 : 2; }
-
-template <int ND>
-__global__ __launch_bounds__(64 * split_waves<ND>(), 1) void diff_split32_kernel(const bf16_t* __restrict__ q,
-                                                                                 const bf16_t* __restrict__ k,
-                                                                                 const bf16_t* __restrict__ v, Parts parts,
-                                                                                 int64_t total, Params p) {
-    constexpr int NV = 2 * ND, W = split_waves<ND>(), TR = 32, KT = TR * 64 * ND, STAGE = 4 * KT;
-    constexpr int LOADS = STAGE / 1024;                  // of a wave's tile
+// Few rows: 32 rows a workgroup, its keys split over the grid; 64 keys a stage, of which a
+// wave takes half for one map (4 waves).
+template <int ND, int RING, bool WHOLE>
+__global__ __launch_bounds__(64 * NW, 1) void diff_split32_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k,
+                                                                  const bf16_t* __restrict__ v, Parts parts, int64_t total,
+                                                                  Params p) {
+    using Keys = KeyStage<ND, NW, WHOLE>;
+    constexpr int NV = 2 * ND, TR = Keys::TR, KT = Keys::KT;
     extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
     char NOTT_LDS* smem = (char NOTT_LDS*)smem_raw;
     const Pair w(p, blockIdx.x);
     const int r0 = (int)blockIdx.z * 32;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int h = lane >> 5;
+    const int h = lane >> 5, map = wid >> 1, f = wid & 1;
     const int my_r = r0 + (lane & 31);
     const RowAt r(p, w, min(my_r, p.rows - 1));
     const int vis = w.visible(p, r.i);
     const int vis_lo = w.visible(p, RowAt(p, w, min(r0, p.rows - 1)).i);
     const int vis_all = w.visible(p, RowAt(p, w, min(r0 + 32, p.rows) - 1).i);
     const float sl2 = p.scale * kLog2e;
-    u32x4 qr[2][2 * ND];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) load_row<ND>(at(q, p.q, w.b, r.i, 2 * r.head + m), p.dh, lane, qr[m]);
+    const RowPlaces<ND> rows_k(lane);
+    const ColPlaces<NV> cols_v(lane);
+    u32x4 qr[2 * ND];
+    load_row<ND, WHOLE>(at(q, p.q, w.b, r.i, 2 * r.head + map), p.dh, lane, qr);
+    const Keys keys(p, w, k, v);
     const int tiles = (vis_all + TR - 1) / TR;
     const int lo = (int)((int64_t)tiles * blockIdx.y / p.nsplit), hi = (int)((int64_t)tiles * (blockIdx.y + 1) / p.nsplit);
-    const bf16_t* pk = at(k, p.k, w.b, 0, 2 * w.j);
-    const bf16_t* pv = at(v, p.v, w.b, 0, w.j);
-    char NOTT_LDS* mine = smem + wid * 2 * STAGE;
-    auto issue = [&](int i, int slot) {
-        char NOTT_LDS* st = mine + slot * STAGE;
-        auto key = [&](int x) { return (int64_t)min(i * TR + x, vis_all - 1); };
-        fill_rows<ND, TR, 1>([&](int x) { return pk + key(x) * p.k[1]; }, p.dh, st, 0, lane);
-        fill_rows<ND, TR, 1>([&](int x) { return pk + p.k[2] + key(x) * p.k[1]; }, p.dh, st + KT, 0, lane);
-        fill_rows<NV, TR, 1>([&](int x) { return pv + key(x) * p.v[1]; }, p.dv, st + 2 * KT, 0, lane);
-    };
-    f32x16 acc[2][NV];
-    zero(acc[0]);
-    zero(acc[1]);
-    float mm[2] = {-INFINITY, -INFINITY}, ll[2] = {0.f, 0.f};
-    int i = lo + wid, slot = 0;
-    if (i < hi) issue(i, 0);
-    for (; i < hi; i += W) {
-        if (i + W < hi) {
-            issue(i + W, slot ^ 1);
-            wait_vm_lgkm0<LOADS>();
-        } else {
-            wait_vm_lgkm0<0>();
-        }
-        asm volatile("" ::: "memory");
-        const char NOTT_LDS* tk = mine + slot * STAGE;
-        const char NOTT_LDS* tv = tk + 2 * KT;
-        slot ^= 1;
-        const int k0 = i * TR;
-        const bool full = k0 + TR <= vis_lo;
-        const int rel = vis - k0 - 4 * h;
-        bf16x8 pb[2][2];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            f32x16 st[1];
-            zero(st);
+    for (int i = 0; i < RING - 1; ++i)
+        if (lo + i < hi) keys.fill(p, lo + i, vis_all, smem + i * Keys::BYTES, wid, lane);
+    f32x16 acc[NV];
+    zero(acc);
+    float m = -INFINITY, l = 0.f;
+    int slot = 0, next = RING - 1;
+    for (int i = lo; i < hi; ++i) {
+        if (i + RING - 2 < hi) wait_vm_lgkm0<(RING - 2) * Keys::LOADS>();
+        else wait_vm_lgkm0<0>();
+        barrier();
+        if (i + RING - 1 < hi) keys.fill(p, i + RING - 1, vis_all, smem + next * Keys::BYTES, wid, lane);
+        const char NOTT_LDS* tk = smem + slot * Keys::BYTES + map * KT;
+        const char NOTT_LDS* tv = smem + slot * Keys::BYTES + 2 * KT;
+        slot = slot + 1 == RING ? 0 : slot + 1;
+        next = next + 1 == RING ? 0 : next + 1;
+        const int k0 = i * TR + 32 * f;
+        f32x16 st[1];
+        bf16x8 pb[2];
 #pragma unroll
-            for (int s = 0; s < 2 * ND; ++s)
-                st[0] = mfma(frag_rows<ND>(tk + m * KT, 0, s, lane), __builtin_bit_cast(bf16x8, qr[m][s]), st[0]);
-            softmax_step<1, NV>(st, pb[m], acc[m], mm[m], ll[m], sl2, full, rel);
-        }
+        for (int s = 0; s < 2 * ND; ++s)
+            st[0] = mfma(rows_k.get(tk, 32 * f, s), __builtin_bit_cast(bf16x8, qr[s]), s ? st[0] : f32x16{});
+        softmax_step<1, NV>(st, pb, acc, m, l, sl2, k0 + 32 <= vis_lo, vis - k0 - 4 * h);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int df = 0; df < NV; ++df) {
-                const bf16x8 vb = frag_cols<NV>(tv, 16 * s, 32 * df, lane);
-                acc[0][df] = mfma(vb, pb[0][s], acc[0][df]);
-                acc[1][df] = mfma(vb, pb[1][s], acc[1][df]);
-            }
-        // this slot's reads have returned before the next turn's loads go there
-        wait_vm_lgkm0<63>();
-        asm volatile("" ::: "memory");
+            for (int df = 0; df < NV; ++df) acc[df] = mfma(cols_v.get(tv, 32 * f + 16 * s, df), pb[s], acc[df]);
     }
-    // Join the waves: their maxima and sums, then the scaled accumulators, through LDS.
-#pragma unroll
-    for (int m = 0; m < 2; ++m) ll[m] += __shfl_xor(ll[m], 32, 64);
-    float* sum = reinterpret_cast<float*>(smem_raw);                      // [W][2][NV][16][64]
-    float* ml = sum + W * 2 * NV * 16 * 64;                               // [W][2][32][2]
+    // Join the halves of a map: maxima and sums, then the scaled accumulators, through LDS.
+    l += __shfl_xor(l, 32, 64);
+    float* sum = reinterpret_cast<float*>(smem_raw);          // [map][NV][16][64], of the second halves
+    float* ml = sum + 2 * NV * 16 * 64;                       // [map][half][32][2]
     __syncthreads();
-    {
-        float* own = ml + ((wid * 2 + h) * 32 + (lane & 31)) * 2;
-        own[0] = h ? mm[1] : mm[0];
-        own[1] = h ? ll[1] : ll[0];
-    }
+    if (h == 0) *reinterpret_cast<f32x2*>(ml + ((map * 2 + f) * 32 + (lane & 31)) * 2) = f32x2{m, l};
     __syncthreads();
-    float m_all[2], l_all[2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        m_all[m] = -INFINITY;
-        for (int x = 0; x < W; ++x) m_all[m] = fmaxf(m_all[m], ml[((x * 2 + m) * 32 + (lane & 31)) * 2]);
-        l_all[m] = 0.f;
-        for (int x = 0; x < W; ++x) {
-            const float* o = ml + ((x * 2 + m) * 32 + (lane & 31)) * 2;
-            l_all[m] += o[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(o[0] - m_all[m]) * o[1];
-        }
-        const float f = mm[m] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mm[m] - m_all[m]);
+    const f32x2 other = *reinterpret_cast<const f32x2*>(ml + ((map * 2 + (f ^ 1)) * 32 + (lane & 31)) * 2);
+    const float top = fmaxf(m, other.x);
+    const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float theirs = other.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other.x - top);
+    float* half = sum + (map * NV << 10) + lane;
+    if (f) {
 #pragma unroll
         for (int df = 0; df < NV; ++df)
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                sum[((((wid * 2 + m) * NV + df) * 16 + e) << 6) + lane] = f == 0.f ? 0.f : acc[m][df][e] * f;
+            for (int e = 0; e < 16; ++e) half[(df * 16 + e) << 6] = mine == 0.f ? 0.f : acc[df][e] * mine;
     }
     __syncthreads();
-    if (my_r >= p.rows) return;
+    if (f || my_r >= p.rows) return;
     const int64_t row = blockIdx.y * total + (int64_t)blockIdx.x * p.rows + my_r;
-    if (wid == 0 && h == 0)
+    if (h == 0) *reinterpret_cast<f32x2*>(parts.ml + (row * 2 + map) * 2) = f32x2{top, l * mine + other.y * theirs};
 #pragma unroll
-        for (int m = 0; m < 2; ++m) *reinterpret_cast<f32x2*>(parts.ml + (row * 2 + m) * 2) = f32x2{m_all[m], l_all[m]};
-    for (int x = wid; x < 2 * NV; x += W) {      // (map, column block)
-        const int m = x / NV, df = x - m * NV;
+    for (int df = 0; df < NV; ++df)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            f32x4 s4 = {0.f, 0.f, 0.f, 0.f};
-            for (int y = 0; y < W; ++y)
+            f32x4 s4;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s4[e] += sum[((((y * 2 + m) * NV + df) * 16 + 4 * j + e) << 6) + lane];
+            for (int e = 0; e < 4; ++e) {
+                const int x = 4 * j + e;
+                s4[e] = (mine == 0.f ? 0.f : acc[df][x] * mine) + half[(df * 16 + x) << 6];
+            }
             const int d = 32 * df + 8 * j + 4 * h;
-            if (d < p.dv) *reinterpret_cast<f32x4*>(parts.acc + (row * 2 + m) * p.dv + d) = s4;
+            if (d < p.dv) *reinterpret_cast<f32x4*>(parts.acc + (row * 2 + map) * p.dv + d) = s4;
         }
-    }
 }
 
 // dq of both maps, and the rows' statistics: 128 rows a workgroup, 32·TF keys a stage.
-template <int ND, int TF, int RING>
+template <int ND, int TF, int RING, bool WHOLE>
 __global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_dq32_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, const bf16_t* __restrict__ o,
     const bf16_t* __restrict__ o2, const bf16_t* __restrict__ dO, const float* __restrict__ lse, float* __restrict__ stats,
@@ -529,16 +550,19 @@ __global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_dq32_kernel(
     const float sl2 = p.scale * kLog2e;
     const float lam = lambda_of(p, w.b, r);
 
+    const RowPlaces<ND> rows_k(lane);
+    const RowPlaces<NV> rows_v(lane);
+    const ColPlaces<ND> cols_k(lane);
     u32x4 qr[2][2 * ND], dr[2 * NV];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) load_row<ND>(at(q, p.q, w.b, r.i, 2 * r.head + m), p.dh, lane, qr[m]);
-    load_row<NV>(at(dO, p.od, w.b, r.i, r.head), p.dv, lane, dr);
+    for (int m = 0; m < 2; ++m) load_row<ND, WHOLE>(at(q, p.q, w.b, r.i, 2 * r.head + m), p.dh, lane, qr[m]);
+    load_row<NV, WHOLE>(at(dO, p.od, w.b, r.i, r.head), p.dv, lane, dr);
     float D[2], ls[2];
     {
         u32x4 orr[2 * NV];
-        load_row<NV>(o2 + (((int64_t)w.b * p.t + r.i) * p.h + r.head) * p.dv, p.dv, lane, orr);
+        load_row<NV, WHOLE>(o2 + (((int64_t)w.b * p.t + r.i) * p.h + r.head) * p.dv, p.dv, lane, orr);
         D[1] = dot_rows<NV>(dr, orr);
-        load_row<NV>(at(o, p.o, w.b, r.i, r.head), p.dv, lane, orr);
+        load_row<NV, WHOLE>(at(o, p.o, w.b, r.i, r.head), p.dv, lane, orr);
         D[0] = fmaf(lam, D[1], dot_rows<NV>(dr, orr));
     }
 #pragma unroll
@@ -560,9 +584,9 @@ __global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_dq32_kernel(
         char NOTT_LDS* st = smem + slot * STAGE;
         auto key = [&](int x) { return (int64_t)min(i * TR + x, vis_all - 1); };
         // (a key tile's blocks split over the waves only together with the other map's)
-        fill_rows<ND, 2 * TR, NW>([&](int x) { return pk + (x >= TR ? p.k[2] : 0) + key(x >= TR ? x - TR : x) * p.k[1]; },
+        fill_rows<ND, 2 * TR, NW, WHOLE>([&](int x) { return pk + (x >= TR ? p.k[2] : 0) + key(x >= TR ? x - TR : x) * p.k[1]; },
                                   p.dh, st, wid, lane);
-        fill_rows<NV, TR, NW>([&](int x) { return pv + key(x) * p.v[1]; }, p.dv, st + 2 * KT, wid, lane);
+        fill_rows<NV, TR, NW, WHOLE>([&](int x) { return pv + key(x) * p.v[1]; }, p.dv, st + 2 * KT, wid, lane);
     };
 #pragma unroll
     for (int i = 0; i < RING - 1; ++i)
@@ -587,15 +611,14 @@ __global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_dq32_kernel(
 #pragma unroll
         for (int f = 0; f < TF; ++f) {
             f32x16 t3[3];   // both maps' scores, dp
-            zero(t3);
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int s = 0; s < 2 * ND; ++s)
-                    t3[m] = mfma(frag_rows<ND>(tk + m * KT, 32 * f, s, lane), __builtin_bit_cast(bf16x8, qr[m][s]), t3[m]);
+                    t3[m] = mfma(rows_k.get(tk + m * KT, 32 * f, s), __builtin_bit_cast(bf16x8, qr[m][s]), s ? t3[m] : f32x16{});
 #pragma unroll
             for (int s = 0; s < 2 * NV; ++s)
-                t3[2] = mfma(frag_rows<NV>(tv, 32 * f, s, lane), __builtin_bit_cast(bf16x8, dr[s]), t3[2]);
+                t3[2] = mfma(rows_v.get(tv, 32 * f, s), __builtin_bit_cast(bf16x8, dr[s]), s ? t3[2] : f32x16{});
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -620,7 +643,7 @@ __global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_dq32_kernel(
                     const bf16x8 a = pack8(t3[m], 8 * s);
 #pragma unroll
                     for (int df = 0; df < ND; ++df)
-                        adq[m][df] = mfma(a, frag_cols<ND>(tk + m * KT, 32 * f + 16 * s, 32 * df, lane), adq[m][df]);
+                        adq[m][df] = mfma(a, cols_k.get(tk + m * KT, 32 * f + 16 * s, df), adq[m][df]);
                 }
         }
     }
@@ -642,11 +665,15 @@ __global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_dq32_kernel(
     }
 }
 
-// dk of both maps and dv: 128 keys a workgroup, 32·TF rows a stage.
-template <int ND, int TF, int RING>
-__global__ __launch_bounds__(64 * NW, 1) void diff_dkdv32_kernel(
+// dk of both maps (WHAT & 1) and dv (WHAT & 2): 128 keys a workgroup, 32·TF rows a stage,
+// one share of the rows (blockIdx.z of p.nsplit; shares leave fp32 parts
+// [nsplit][b·hk][s][2·dh + dv] for diff_join_keys_kernel).
+template <int ND, int TF, int RING, int WHAT, bool WHOLE>
+__global__ __launch_bounds__(64 * NW, WHAT == 3 || (WHAT == 1 && ND > 2) ? 1 : 2) void diff_dkdv32_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, const bf16_t* __restrict__ dO,
-    const float* __restrict__ stats, bf16_t* __restrict__ dk, bf16_t* __restrict__ dv, int64_t total, Params p) {
+    const float* __restrict__ stats, bf16_t* __restrict__ dk, bf16_t* __restrict__ dv, float* __restrict__ parts, int64_t total,
+    Params p) {
+    constexpr bool DK = WHAT & 1, DV = WHAT & 2;
     constexpr int NV = 2 * ND, TR = 32 * TF, QT = TR * 64 * ND;
     constexpr int STAGE = 4 * QT + 256 * 8;              // q1, q2, dO and the rows' statistics (64 floats each)
     constexpr int LOADS = 4 * ND * TF / 2;               // per wave and stage, beside the statistics
@@ -660,27 +687,32 @@ __global__ __launch_bounds__(64 * NW, 1) void diff_dkdv32_kernel(
     const float sl2 = p.scale * kLog2e;
     const float* st0 = stats + (int64_t)blockIdx.x * p.rows;
     const int first = k0 < w.len ? w.first_row(p, k0) : p.rows;
-    const int i0 = first / TR;
-    const int nq = first < p.rows ? (p.rows + TR - 1) / TR - i0 : 0;
+    const int all = first < p.rows ? (p.rows + TR - 1) / TR - first / TR : 0;
+    const int from = (int)((int64_t)all * blockIdx.z / p.nsplit), i0 = first / TR + from;
+    const int nq = (int)((int64_t)all * (blockIdx.z + 1) / p.nsplit) - from;
 
+    const RowPlaces<ND> rows_k(lane);
+    const RowPlaces<NV> rows_v(lane);
+    const ColPlaces<ND> cols_k(lane);
+    const ColPlaces<NV> cols_v(lane);
     u32x4 kr[2][2 * ND], vr[2 * NV];
     {
         const int key = max(0, min(my_k, w.len - 1));
 #pragma unroll
-        for (int m = 0; m < 2; ++m) load_row<ND>(at(k, p.k, w.b, key, 2 * w.j + m), p.dh, lane, kr[m]);
-        load_row<NV>(at(v, p.v, w.b, key, w.j), p.dv, lane, vr);
+        for (int m = 0; m < 2; ++m) load_row<ND, WHOLE>(at(k, p.k, w.b, key, 2 * w.j + m), p.dh, lane, kr[m]);
+        if (DK) load_row<NV, WHOLE>(at(v, p.v, w.b, key, w.j), p.dv, lane, vr);
     }
     auto issue = [&](int i, int slot) {
         char NOTT_LDS* st = smem + slot * STAGE;
         const int b0 = (i0 + i) * TR;
         auto row = [&](int x) { return RowAt(p, w, min(b0 + x, p.rows - 1)); };
-        fill_rows<ND, 2 * TR, NW>(
+        fill_rows<ND, 2 * TR, NW, WHOLE>(
             [&](int x) {
                 const RowAt y = row(x >= TR ? x - TR : x);
                 return at(q, p.q, w.b, y.i, 2 * y.head + (x >= TR));
             },
             p.dh, st, wid, lane);
-        fill_rows<NV, TR, NW>(
+        fill_rows<NV, TR, NW, WHOLE>(
             [&](int x) {
                 const RowAt y = row(x);
                 return at(dO, p.od, w.b, y.i, y.head);
@@ -717,15 +749,15 @@ __global__ __launch_bounds__(64 * NW, 1) void diff_dkdv32_kernel(
 #pragma unroll
         for (int f = 0; f < TF; ++f) {
             f32x16 t3[3];
-            zero(t3);
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int s = 0; s < 2 * ND; ++s)
-                    t3[m] = mfma(frag_rows<ND>(tq + m * QT, 32 * f, s, lane), __builtin_bit_cast(bf16x8, kr[m][s]), t3[m]);
+                    t3[m] = mfma(rows_k.get(tq + m * QT, 32 * f, s), __builtin_bit_cast(bf16x8, kr[m][s]), s ? t3[m] : f32x16{});
+            if constexpr (DK)
 #pragma unroll
-            for (int s = 0; s < 2 * NV; ++s)
-                t3[2] = mfma(frag_rows<NV>(tdo, 32 * f, s, lane), __builtin_bit_cast(bf16x8, vr[s]), t3[2]);
+                for (int s = 0; s < 2 * NV; ++s)
+                t3[2] = mfma(rows_v.get(tdo, 32 * f, s), __builtin_bit_cast(bf16x8, vr[s]), s ? t3[2] : f32x16{});
             auto stat = [&](int which, int j) {
                 return *reinterpret_cast<const f32x4 NOTT_LDS*>(ss + 64 * which + 32 * f + 8 * j + 4 * h);
             };
@@ -744,33 +776,41 @@ __global__ __launch_bounds__(64 * NW, 1) void diff_dkdv32_kernel(
                     const int c = 32 * f + 8 * (x >> 2) + (x & 3);
                     if (!((c >= lo) & (c < hi))) {
                         t3[0][x] = t3[1][x] = -INFINITY;
-                        t3[2][x] = 0.f;
+                        if (DK) t3[2][x] = 0.f;
                     }
                 }
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const f32x4 d1 = stat(2, j), d2 = stat(3, j), lm = stat(4, j);
+                f32x4 d1, d2;
+                if (DK) d1 = stat(2, j), d2 = stat(3, j);
+                const f32x4 lm = stat(4, j);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int x = 4 * j + e;
                     const float p1 = __builtin_amdgcn_exp2f(t3[0][x]), p2 = __builtin_amdgcn_exp2f(t3[1][x]) * lm[e];
-                    const float dp = t3[2][x];
-                    t3[0][x] = p1 * (dp - d1[e]);
-                    t3[1][x] = p2 * (d2[e] - dp);
-                    t3[2][x] = p1 - p2;
+                    if constexpr (DK) {
+                        const float dp = t3[2][x];
+                        t3[0][x] = p1 * (dp - d1[e]);
+                        t3[1][x] = p2 * (d2[e] - dp);
+                    }
+                    if (DV) t3[2][x] = p1 - p2;
                 }
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const bf16x8 a1 = pack8(t3[0], 8 * s), a2 = pack8(t3[1], 8 * s), aw = pack8(t3[2], 8 * s);
+                bf16x8 a1, a2, aw;
+                if (DK) a1 = pack8(t3[0], 8 * s), a2 = pack8(t3[1], 8 * s);
+                if (DV) aw = pack8(t3[2], 8 * s);
+                if constexpr (DK)
 #pragma unroll
-                for (int df = 0; df < ND; ++df) {
-                    adk[0][df] = mfma(a1, frag_cols<ND>(tq, 32 * f + 16 * s, 32 * df, lane), adk[0][df]);
-                    adk[1][df] = mfma(a2, frag_cols<ND>(tq + QT, 32 * f + 16 * s, 32 * df, lane), adk[1][df]);
+                    for (int df = 0; df < ND; ++df) {
+                    adk[0][df] = mfma(a1, cols_k.get(tq, 32 * f + 16 * s, df), adk[0][df]);
+                    adk[1][df] = mfma(a2, cols_k.get(tq + QT, 32 * f + 16 * s, df), adk[1][df]);
                 }
+                if constexpr (DV)
 #pragma unroll
-                for (int df = 0; df < NV; ++df) adv[df] = mfma(aw, frag_cols<NV>(tdo, 32 * f + 16 * s, 32 * df, lane), adv[df]);
+                    for (int df = 0; df < NV; ++df) adv[df] = mfma(aw, cols_v.get(tdo, 32 * f + 16 * s, df), adv[df]);
             }
         }
     }
@@ -778,22 +818,48 @@ __global__ __launch_bounds__(64 * NW, 1) void diff_dkdv32_kernel(
     for (int x = 0; x < 16; ++x) {
         const int key = kw0 + 8 * (x >> 2) + 4 * h + (x & 3);
         if (key >= p.s) continue;
+        float* part = parts ? parts + (((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * p.s + key) * (2 * p.dh + p.dv) : nullptr;
+        if constexpr (DK) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            bf16_t* out = at(dk, p.dk, w.b, key, 2 * w.j + m);
+            for (int m = 0; m < 2; ++m) {
+                bf16_t* out = at(dk, p.dk, w.b, key, 2 * w.j + m);
 #pragma unroll
-            for (int df = 0; df < ND; ++df) {
-                const int d = 32 * df + (lane & 31);
-                if (d < p.dh) out[d] = f32_to_bf16(adk[m][df][x] * p.scale);
+                for (int df = 0; df < ND; ++df) {
+                    const int d = 32 * df + (lane & 31);
+                    if (!WHOLE && d >= p.dh) continue;
+                    if (parts) part[m * p.dh + d] = adk[m][df][x] * p.scale;
+                    else out[d] = f32_to_bf16(adk[m][df][x] * p.scale);
+                }
             }
         }
-        bf16_t* out = at(dv, p.dv_, w.b, key, w.j);
+        if constexpr (DV) {
+            bf16_t* out = at(dv, p.dv_, w.b, key, w.j);
 #pragma unroll
-        for (int df = 0; df < NV; ++df) {
-            const int d = 32 * df + (lane & 31);
-            if (d < p.dv) out[d] = f32_to_bf16(adv[df][x]);
+            for (int df = 0; df < NV; ++df) {
+                const int d = 32 * df + (lane & 31);
+                if (!WHOLE && d >= p.dv) continue;
+                if (parts) part[2 * p.dh + d] = adv[df][x];
+                else out[d] = f32_to_bf16(adv[df][x]);
+            }
         }
     }
+}
+
+// Sums the shares of dk and dv, a thread 4 columns of a key (dh and dv are whole 8s).
+__global__ __launch_bounds__(256) void diff_join_keys_kernel(const float* __restrict__ parts, bf16_t* __restrict__ dk,
+                                                             bf16_t* __restrict__ dv, int64_t pairs, Params p) {
+    const int per = (2 * p.dh + p.dv) / 4;
+    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (n >= pairs * p.s * per) return;
+    const int64_t row = n / per;
+    const int c = (int)(n - row * per) * 4;
+    const f32x4 s = ordered_sum4(parts + 4 * n, pairs * p.s * per * 4, p.nsplit);
+    const int bk = (int)(row / p.s), key = (int)(row - (int64_t)bk * p.s);
+    const Pair w(p, bk);
+    const int m = c / p.dh;
+    bf16_t* out = m < 2 ? at(dk, p.dk, w.b, key, 2 * w.j + m) + (c - m * p.dh) : at(dv, p.dv_, w.b, key, w.j) + (c - 2 * p.dh);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = f32_to_bf16(s[e]);
 }
 
 template <typename F>
@@ -807,46 +873,79 @@ int reserve(nott_ctx ctx, F* kernel, size_t lds, bool& done) {
     return NOTT_OK;
 }
 
-template <int ND>
+template <int ND, bool WHOLE>
 int fwd(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* o, bf16_t* o2,
         float* lse) {
-    constexpr size_t lds = 2 * (size_t)4 * 64 * 64 * ND;
+    constexpr size_t lds = 2 * (size_t)KeyStage<ND, 2 * NW, WHOLE>::BYTES;
     static bool done = false;
-    auto f = &diff_fwd32_kernel<ND, 2>;
+    auto f = &diff_fwd32_kernel<ND, 2, WHOLE>;
     if (const int st = reserve(ctx, f, lds, done); st != NOTT_OK) return st;
-    hipLaunchKernelGGL(f, dim3((unsigned)pairs, (unsigned)ceil_div(p.rows, FIXED)), dim3(64 * NW), lds, ctx->stream, q, k, v, o,
-                       o2, lse, p);
+    hipLaunchKernelGGL(f, dim3((unsigned)pairs, (unsigned)ceil_div(p.rows, FIXED)), dim3(128 * NW), lds, ctx->stream, q, k, v,
+                       o, o2, lse, p);
     return launch_status(ctx, "diff_fwd32_kernel");
 }
 
-template <int ND>
+template <int ND, bool WHOLE>
 int split(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const bf16_t* k, const bf16_t* v, const Parts& parts) {
-    constexpr int W = split_waves<ND>();
-    constexpr size_t lds = (size_t)W * 2 * 4 * 32 * 64 * ND + W * 2 * 32 * 2 * sizeof(float);
+    constexpr int RING = ND <= 2 ? 4 : 2;
+    constexpr size_t lds = std::max<size_t>((size_t)RING * KeyStage<ND, NW, WHOLE>::BYTES,
+                                            (2 * 2 * ND * 16 * 64 + 2 * 2 * 32 * 2) * sizeof(float));
     static bool done = false;
-    auto f = &diff_split32_kernel<ND>;
+    auto f = &diff_split32_kernel<ND, RING, WHOLE>;
     if (const int st = reserve(ctx, f, lds, done); st != NOTT_OK) return st;
-    hipLaunchKernelGGL(f, dim3((unsigned)pairs, (unsigned)p.nsplit, (unsigned)ceil_div(p.rows, 32)), dim3(64 * W), lds,
+    hipLaunchKernelGGL(f, dim3((unsigned)pairs, (unsigned)p.nsplit, (unsigned)ceil_div(p.rows, 32)), dim3(64 * NW), lds,
                        ctx->stream, q, k, v, parts, pairs * p.rows, p);
     return launch_status(ctx, "diff_split32_kernel");
 }
 
-template <int ND, int TF, int RING, int TFK, int RINGK>
+// Whether one kernel forms dk and dv: its accumulators and operands have to fit a wave.
+template <int ND> constexpr bool kTogether = ND <= 2;
+
+template <int ND, bool WHOLE>
 int bwd(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const bf16_t* k, const bf16_t* v, const bf16_t* o,
-        const bf16_t* o2, const bf16_t* dO, const float* lse, float* stats, bf16_t* dq, bf16_t* dk, bf16_t* dv, float* dlam) {
+        const bf16_t* o2, const bf16_t* dO, const float* lse, float* stats, float* parts, bf16_t* dq, bf16_t* dk, bf16_t* dv,
+        float* dlam) {
+    // 32 rows a stage (64 where a stage is 8 KB), stages for 64 to 128 KB
+    constexpr int TF = ND == 1 ? 2 : 1, RING = ND == 1 ? 2 : ND == 3 ? 3 : 4, RINGK = ND <= 2 ? 4 : 2;
     constexpr size_t lds_q = (size_t)RING * 4 * 32 * TF * 64 * ND;
-    constexpr size_t lds_kv = (size_t)RINGK * (4 * 32 * TFK * 64 * ND + 2048);
-    static bool done[2] = {false, false};
-    auto fq = &diff_dq32_kernel<ND, TF, RING>;
-    auto fk = &diff_dkdv32_kernel<ND, TFK, RINGK>;
+    constexpr size_t lds_kv = (size_t)RINGK * (4 * 32 * 64 * ND + 2048);
+    static bool done[3] = {false, false, false};
+    auto fq = &diff_dq32_kernel<ND, TF, RING, WHOLE>;
+    auto fk = &diff_dkdv32_kernel<ND, 1, RINGK, kTogether<ND> ? 3 : 1, WHOLE>;
+    auto fv = &diff_dkdv32_kernel<ND, 1, RINGK, 2, WHOLE>;
     if (const int st = reserve(ctx, fq, lds_q, done[0]); st != NOTT_OK) return st;
     if (const int st = reserve(ctx, fk, lds_kv, done[1]); st != NOTT_OK) return st;
+    if (!kTogether<ND>)
+        if (const int st = reserve(ctx, fv, lds_kv, done[2]); st != NOTT_OK) return st;
     const int64_t total = pairs * p.rows;
     hipLaunchKernelGGL(fq, dim3((unsigned)pairs, (unsigned)ceil_div(p.rows, FIXED)), dim3(64 * NW), lds_q, ctx->stream, q, k, v,
                        o, o2, dO, lse, stats, dq, dlam, total, p);
-    hipLaunchKernelGGL(fk, dim3((unsigned)pairs, (unsigned)ceil_div(p.s, FIXED)), dim3(64 * NW), lds_kv, ctx->stream, q, k, v,
-                       dO, stats, dk, dv, total, p);
+    const dim3 grid((unsigned)pairs, (unsigned)ceil_div(p.s, FIXED), (unsigned)p.nsplit);
+    hipLaunchKernelGGL(fk, grid, dim3(64 * NW), lds_kv, ctx->stream, q, k, v, dO, stats, dk, dv, parts, total, p);
+    if (!kTogether<ND>)
+        hipLaunchKernelGGL(fv, grid, dim3(64 * NW), lds_kv, ctx->stream, q, k, v, dO, stats, dk, dv, parts, total, p);
+    if (parts)
+        hipLaunchKernelGGL(diff_join_keys_kernel, dim3((unsigned)ceil_div(pairs * p.s * ((2 * p.dh + p.dv) / 4), 256)), dim3(256),
+                           0, ctx->stream, parts, dk, dv, pairs, p);
     return launch_status(ctx, "diff_dkdv32_kernel");
+}
+
+// Blocks of 32 columns of the keys that dh and dv take (dv twice as many).
+int blocks_for(const Params& p) { return (int)std::max(ceil_div(p.dh, 32), ceil_div(p.dv, 64)); }
+
+// Calls f with that number, and whether the blocks are whole, as template arguments.
+template <typename F>
+int with_blocks(const Params& p, F&& f) {
+    const int nd = blocks_for(p);
+    auto width = [&](auto b) {
+        return p.dh == 32 * nd && p.dv == 64 * nd ? f(b, std::true_type()) : f(b, std::false_type());
+    };
+    switch (nd) {
+        case 1: return width(std::integral_constant<int, 1>());
+        case 2: return width(std::integral_constant<int, 2>());
+        case 3: return width(std::integral_constant<int, 3>());
+        default: return width(std::integral_constant<int, 4>());
+    }
 }
 
 }  // namespace mx
@@ -1367,8 +1466,6 @@ int check(nott_ctx ctx, const nott_diff_attn_desc* d, nott_dtype dtype, Params* 
     return NOTT_OK;
 }
 
-// Blocks of 32 columns of the keys that dh and dv take (dv twice as many).
-int blocks_for(const Params& p) { return (int)std::max(ceil_div(p.dh, 32), ceil_div(p.dv, 64)); }
 // 64-byte slices, a power of two.
 int slices_for(const Params& p, int sl) {
     const int need = (int)std::max(ceil_div(p.dh, sl), ceil_div(p.dv, 2 * sl));
@@ -1441,33 +1538,28 @@ extern "C" int nott_diff_attention_fwd(nott_ctx ctx, const nott_diff_attn_desc* 
     p.vec = even16(q, p.q, elem) && even16(k, p.k, elem) && even16(v, p.v, elem);
     const int64_t pairs = d->b * d->hk;
     if (dtype == NOTT_BF16 && p.vec && p.dh % 8 == 0 && p.dv % 8 == 0 && even16(o, p.o, 2) && (uintptr_t)o2 % 16 == 0) {
-        const int nd = blocks_for(p);
         const auto* tq = static_cast<const bf16_t*>(q);
         const auto* tk = static_cast<const bf16_t*>(k);
         const auto* tv = static_cast<const bf16_t*>(v);
         auto* to = static_cast<bf16_t*>(o);
         auto* to2 = static_cast<bf16_t*>(o2);
-        // Fewer workgroups than half the CUs: keys split, at least 128 of them to a wave.
+        // Fewer workgroups than half the CUs: keys split.
         if (2 * pairs * ceil_div(p.rows, mx::FIXED) <= ctx->num_cu && p.s >= 256 && ceil_div(p.rows, 32) <= 65535) {
-            const int64_t per = 32 * 4 * (nd <= 2 ? 4 : 2);
+            const int64_t per = 64 * 4;     // keys to a workgroup at the least
             const int64_t n = std::max<int64_t>(1, std::min<int64_t>(ceil_div(ctx->num_cu, pairs * ceil_div(p.rows, 32)),
                                                                      ceil_div(p.s, per)));
             const Parts parts = parts_for(ctx, p, pairs, n);
             if (parts.acc) {
                 p.nsplit = (int32_t)n;
-                const int st = nd == 1   ? mx::split<1>(ctx, p, pairs, tq, tk, tv, parts)
-                               : nd == 2 ? mx::split<2>(ctx, p, pairs, tq, tk, tv, parts)
-                               : nd == 3 ? mx::split<3>(ctx, p, pairs, tq, tk, tv, parts)
-                                         : mx::split<4>(ctx, p, pairs, tq, tk, tv, parts);
+                const int st = mx::with_blocks(p, [&](auto b, auto w) {
+                    return mx::split<decltype(b)::value, decltype(w)::value>(ctx, p, pairs, tq, tk, tv, parts);
+                });
                 return st != NOTT_OK ? st : join(ctx, p, pairs, parts, to, to2, lse);
             }
         }
-        switch (nd) {
-            case 1: return mx::fwd<1>(ctx, p, pairs, tq, tk, tv, to, to2, lse);
-            case 2: return mx::fwd<2>(ctx, p, pairs, tq, tk, tv, to, to2, lse);
-            case 3: return mx::fwd<3>(ctx, p, pairs, tq, tk, tv, to, to2, lse);
-            default: return mx::fwd<4>(ctx, p, pairs, tq, tk, tv, to, to2, lse);
-        }
+        return mx::with_blocks(p, [&](auto b, auto w) {
+            return mx::fwd<decltype(b)::value, decltype(w)::value>(ctx, p, pairs, tq, tk, tv, to, to2, lse);
+        });
     }
     auto run = [&](auto type) {
         using T = decltype(type);
@@ -1517,7 +1609,22 @@ extern "C" int nott_diff_attention_bwd(nott_ctx ctx, const nott_diff_attn_desc* 
     const int elem = (int)nott::dtype_size(dtype);
     p.vec = even16(q, p.q, elem) && even16(k, p.k, elem) && even16(v, p.v, elem) && even16(dO, p.od, elem);
     const int64_t pairs = d->b * d->hk, total = pairs * p.rows;
-    float* stats = static_cast<float*>(nott::workspace(ctx, (size_t)total * kStats * sizeof(float)));
+    // Fewer key blocks than CUs: the rows are split, if the parts find room (a share of
+    // 32·32 rows at the least).
+    const bool fast = dtype == NOTT_BF16 && p.vec && p.dh % 8 == 0 && p.dv % 8 == 0 && even16(o, p.o, 2) && (uintptr_t)o2 % 16 == 0;
+    const size_t stat_bytes = ((size_t)total * kStats * sizeof(float) + 255) & ~size_t(255);
+    const int64_t key_blocks = pairs * ceil_div(p.s, mx::FIXED);
+    float *stats = nullptr, *parts = nullptr;
+    if (fast && key_blocks < ctx->num_cu && p.rows >= 2048) {
+        const int64_t n = std::min<int64_t>(ceil_div(2 * ctx->num_cu, key_blocks), p.rows / 1024);
+        const size_t bytes = (size_t)n * pairs * p.s * (2 * p.dh + p.dv) * sizeof(float);
+        if (char* ws = static_cast<char*>(nott::optional_workspace(ctx, stat_bytes + bytes))) {
+            stats = reinterpret_cast<float*>(ws);
+            parts = reinterpret_cast<float*>(ws + stat_bytes);
+            p.nsplit = (int32_t)n;
+        }
+    }
+    if (!stats) stats = static_cast<float*>(nott::workspace(ctx, stat_bytes));
     if (!stats) return NOTT_ERR_ALLOC;
     auto run = [&](auto type) {
         using T = decltype(type);
@@ -1531,13 +1638,11 @@ extern "C" int nott_diff_attention_bwd(nott_ctx ctx, const nott_diff_attn_desc* 
         auto* tdk = static_cast<T*>(dk);
         auto* tdv = static_cast<T*>(dv);
         if constexpr (sizeof(T) == 2) {
-            if (p.vec && p.dh % 8 == 0 && p.dv % 8 == 0 && even16(o, p.o, 2) && (uintptr_t)o2 % 16 == 0) {
-                switch (blocks_for(p)) {
-                    case 1: return mx::bwd<1, 2, 2, 2, 2>(ctx, p, pairs, tq, tk, tv, to, to2, tdo, lse, stats, tdq, tdk, tdv, dlam);
-                    case 2: return mx::bwd<2, 1, 4, 2, 2>(ctx, p, pairs, tq, tk, tv, to, to2, tdo, lse, stats, tdq, tdk, tdv, dlam);
-                    case 3: return mx::bwd<3, 2, 2, 2, 2>(ctx, p, pairs, tq, tk, tv, to, to2, tdo, lse, stats, tdq, tdk, tdv, dlam);
-                    default: return mx::bwd<4, 2, 2, 2, 2>(ctx, p, pairs, tq, tk, tv, to, to2, tdo, lse, stats, tdq, tdk, tdv, dlam);
-                }
+            if (fast) {
+                return mx::with_blocks(p, [&](auto b, auto w) {
+                    return mx::bwd<decltype(b)::value, decltype(w)::value>(ctx, p, pairs, tq, tk, tv, to, to2, tdo, lse, stats, parts,
+                                                                           tdq, tdk, tdv, dlam);
+                });
             }
         }
         switch (slices_for(p, AT<T>::SL)) {
