@@ -40,6 +40,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 struct Params {
     int32_t t, s, dh, dv, h, hk, group, rows;   // rows = t·group, of a key head
     int32_t causal, token_lam, vec, nsplit;
+    int32_t near;         // 128 rows of q, k, v, dO lie within 2^31 bytes: 32-bit offsets reach a tile's
     float scale;
     FastDiv by_group;
     int64_t q[3], k[3], v[3], o[3], od[3], dq[3], dk[3], dv_[3];   // strides: batch, token, head (od: dO)
@@ -100,44 +101,68 @@ struct Parts {
     float* ml;
 };
 
-// Joins the parts: a wave a row, lane l the columns l, l + 64, ...
+// Joins the parts (at most 64): a workgroup a row.  Lane z weighs part z; a wave sums every
+// fourth part, its loads in flight beside those of the weights, and the waves' sums are
+// added in order (a wave a row, a part after the other, took 17.7 us for 128 rows in 8 parts).
+constexpr int kMostParts = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void diff_join_kernel(Parts parts, T* __restrict__ o, T* __restrict__ o2,
                                                         float* __restrict__ lse, int64_t total, Params p) {
-    const int64_t at_row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);   // (b·hk + j)·rows + row
-    const int lane = threadIdx.x & 63;
-    if (at_row >= total) return;
+    __shared__ float sum[4][2][256];
+    const int64_t at_row = blockIdx.x;      // (b·hk + j)·rows + row
+    const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int bk = (int)(at_row / p.rows), row = (int)(at_row - (int64_t)bk * p.rows);
+    const float* ml = parts.ml + at_row * 4;
+    const f32x4 mine = lane < p.nsplit ? *reinterpret_cast<const f32x4*>(ml + lane * total * 4)    // {m, l} of both maps
+                                       : f32x4{-INFINITY, 0.f, -INFINITY, 0.f};
+    constexpr int U = 4;        // parts of a wave at a time
+    float a[U][2][4];
+    auto load = [&](int z0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int z = min(z0 + 4 * u, p.nsplit - 1), d = lane + 64 * c;
+                    a[u][k][c] = d < p.dv ? parts.acc[((z * total + at_row) * 2 + k) * p.dv + d] : 0.f;
+                }
+    };
+    load(wid);
     const Pair w(p, bk);
     const RowAt r(p, w, row);
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (int z = 0; z < p.nsplit; ++z)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) m[k] = fmaxf(m[k], parts.ml[((z * total + at_row) * 2 + k) * 2]);
-    float acc[2][4] = {};
-    for (int z = 0; z < p.nsplit; ++z)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const float* ml = parts.ml + ((z * total + at_row) * 2 + k) * 2;
-            const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m[k]);
-            l[k] += f * ml[1];
-            const float* a = parts.acc + ((z * total + at_row) * 2 + k) * p.dv;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (lane + 64 * c < p.dv) acc[k][c] += f == 0.f ? 0.f : f * a[lane + 64 * c];
-        }
     const float lam = lambda_of(p, w.b, r);
-    const float i1 = l[0] > 0.f ? 1.f / l[0] : 0.f, i2 = l[1] > 0.f ? 1.f / l[1] : 0.f;
-    T* po = at(o, p.o, w.b, r.i, r.head);
+    const float m[2] = {wave_max(mine.x), wave_max(mine.z)};
+    const float f[2] = {mine.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine.x - m[0]),
+                        mine.z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine.z - m[1])};
+    const float l[2] = {wave_sum(f[0] * mine.y), wave_sum(f[1] * mine.w)};
+    float acc[2][4] = {};
+    for (int z0 = wid; z0 < p.nsplit; z0 += 4 * U) {
+        if (z0 != wid) load(z0);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const int d = lane + 64 * c;
-        if (d >= p.dv) break;
-        const float b = acc[1][c] * i2;
-        Io<T>::st(po, d, acc[0][c] * i1 - lam * b);
-        if (o2) Io<T>::st(o2, (((int64_t)w.b * p.t + r.i) * p.h + r.head) * p.dv + d, b);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float fz = __shfl(f[k], min(z0 + 4 * u, 63), 64);
+                if (z0 + 4 * u >= p.nsplit || fz == 0.f) continue;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[k][c] = fmaf(fz, a[u][k][c], acc[k][c]);
+            }
     }
-    if (lane < 2) *lse_at(p, lse, w.b, r, lane) = log_sum(m[lane], l[lane]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[wid][k][lane + 64 * c] = acc[k][c];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < p.dv) {
+        const float i1 = l[0] > 0.f ? 1.f / l[0] : 0.f, i2 = l[1] > 0.f ? 1.f / l[1] : 0.f;
+        const float first = (sum[0][0][d] + sum[1][0][d]) + (sum[2][0][d] + sum[3][0][d]);
+        const float second = ((sum[0][1][d] + sum[1][1][d]) + (sum[2][1][d] + sum[3][1][d])) * i2;
+        Io<T>::st(at(o, p.o, w.b, r.i, r.head), d, first * i1 - lam * second);
+        if (o2) Io<T>::st(o2, (((int64_t)w.b * p.t + r.i) * p.h + r.head) * p.dv + d, second);
+    }
+    if (threadIdx.x < 2) *lse_at(p, lse, w.b, r, threadIdx.x) = threadIdx.x ? log_sum(m[1], l[1]) : log_sum(m[0], l[0]);
 }
 
 // dλ of a head: −Σ D_2 over its rows, in a fixed order.
@@ -168,6 +193,7 @@ namespace mx {
 using namespace nott::attn::mx32;
 using nott::lds::barrier;
 using nott::lds::dma16;
+using nott::lds::dma16_at;
 using nott::lds::dma4;
 using nott::lds::lds_addr;
 using nott::lds::wait_vm_lgkm0;
@@ -192,6 +218,28 @@ __device__ __forceinline__ void fill_rows(F&& from, int cols, char NOTT_LDS* til
         dma16(src, lds_addr(tile) + 1024 * q);
     }
 }
+
+// The same for tiles whose rows and columns are all there: what a lane adds to the tile's
+// first row, formed once (a row's address takes some thirty cycles of vector
+// multiplications, and as long again where the row's query and head are to be divided out).
+template <int NB, int ROWS, int WAVES>
+struct TileOffsets {
+    static constexpr int CH = 4 * NB, N = ROWS * CH / 64 / WAVES;
+    uint32_t v[N];
+    // row(x): byte offset of the tile's row x
+    template <typename F>
+    __device__ __forceinline__ TileOffsets(F&& row, int wid, int lane) {
+#pragma unroll
+        for (int qq = 0; qq < N; ++qq) {
+            const int i = 64 * (wid + WAVES * qq) + lane, x = i / CH;
+            v[qq] = (uint32_t)row(x) + 16 * swz<NB>(x, i - x * CH);
+        }
+    }
+    __device__ __forceinline__ void fill(const bf16_t* first, char NOTT_LDS* tile, int wid) const {
+#pragma unroll
+        for (int qq = 0; qq < N; ++qq) dma16_at(first, v[qq], lds_addr(tile) + 1024 * (wid + WAVES * qq));
+    }
+};
 
 // A row as 2·NB B-operand slices: lane l holds d = 16s + 8·(l/32) + 0..7.
 template <int NB, bool WHOLE>
@@ -327,20 +375,81 @@ __device__ __forceinline__ void store_block(bf16_t* row, int df, int cols, int h
     }
 }
 
-// The tiles of 64 keys (both maps' keys, values) that a stage holds, filled by WAVES waves.
-template <int ND, int WAVES, bool WHOLE>
+// Stages of ROWS keys: tiles of both maps' keys, then of the values, filled by WAVES waves.
+template <int ND, int ROWS, int WAVES, bool WHOLE>
 struct KeyStage {
-    static constexpr int TR = 64, KT = TR * 64 * ND, BYTES = 4 * KT, LOADS = 16 * ND / WAVES;   // loads of a wave
+    static constexpr int TR = ROWS, KT = TR * 64 * ND, BYTES = 4 * KT, LOADS = BYTES / 1024 / WAVES;   // loads of a wave
     const bf16_t* pk;
     const bf16_t* pv;
-    __device__ __forceinline__ KeyStage(const Params& p, const Pair& w, const bf16_t* k, const bf16_t* v)
-        : pk(at(k, p.k, w.b, 0, 2 * w.j)), pv(at(v, p.v, w.b, 0, w.j)) {}
+    TileOffsets<ND, 2 * TR, WAVES> ko;
+    TileOffsets<2 * ND, TR, WAVES> vo;
+    __device__ __forceinline__ KeyStage(const Params& p, const Pair& w, const bf16_t* k, const bf16_t* v, int wid, int lane)
+        : pk(at(k, p.k, w.b, 0, 2 * w.j)), pv(at(v, p.v, w.b, 0, w.j)),
+          ko([&](int x) { return 2 * ((x >= TR ? p.k[2] : 0) + (x >= TR ? x - TR : x) * p.k[1]); }, wid, lane),
+          vo([&](int x) { return 2 * (x * p.v[1]); }, wid, lane) {}
     // keys past `most`, which nothing sees, are not read
     __device__ __forceinline__ void fill(const Params& p, int tile, int most, char NOTT_LDS* st, int wid, int lane) const {
+        if (WHOLE && p.near && (tile + 1) * TR <= most) {
+            ko.fill(pk + (int64_t)tile * TR * p.k[1], st, wid);
+            vo.fill(pv + (int64_t)tile * TR * p.v[1], st + 2 * KT, wid);
+            return;
+        }
         auto key = [&](int x) { return (int64_t)min(tile * TR + x, most - 1); };
         fill_rows<ND, 2 * TR, WAVES, WHOLE>(
             [&](int x) { return pk + (x >= TR ? p.k[2] : 0) + key(x >= TR ? x - TR : x) * p.k[1]; }, p.dh, st, wid, lane);
         fill_rows<2 * ND, TR, WAVES, WHOLE>([&](int x) { return pv + key(x) * p.v[1]; }, p.dv, st + 2 * KT, wid, lane);
+    }
+};
+
+// Stages of ROWS rows: tiles of both maps' queries, of dO, and the rows' statistics.
+template <int ND, int ROWS, int WAVES, bool WHOLE>
+struct RowStage {
+    static constexpr int TR = ROWS, QT = TR * 64 * ND, BYTES = 4 * QT + 256 * 8;   // statistics: 64 floats each
+    static constexpr int LOADS = 4 * QT / 1024 / WAVES;                            // beside the statistics
+    const bf16_t* pq;
+    const bf16_t* pd;
+    const float* stats;
+    bool even;              // a tile's rows are whole queries
+    TileOffsets<ND, 2 * TR, WAVES> qo;
+    TileOffsets<2 * ND, TR, WAVES> od;
+    __device__ __forceinline__ RowStage(const Params& p, const Pair& w, const bf16_t* q, const bf16_t* dO, const float* st,
+                                        int wid, int lane)
+        : pq(at(q, p.q, w.b, 0, 2 * w.j * p.group)), pd(at(dO, p.od, w.b, 0, w.j * p.group)), stats(st),
+          even(TR % p.group == 0),
+          qo([&](int x) {
+                 uint32_t i, g;
+                 p.by_group.divmod(x >= TR ? x - TR : x, i, g);
+                 return 2 * (i * p.q[1] + (2 * g + (x >= TR)) * p.q[2]);
+             }, wid, lane),
+          od([&](int x) {
+                 uint32_t i, g;
+                 p.by_group.divmod(x, i, g);
+                 return 2 * (i * p.od[1] + g * p.od[2]);
+             }, wid, lane) {}
+    __device__ __forceinline__ void fill(const Params& p, const Pair& w, const bf16_t* q, const bf16_t* dO, int tile, int64_t total,
+                                         char NOTT_LDS* st, int wid, int lane) const {
+        const int b0 = tile * TR;
+        if (WHOLE && p.near && even && b0 + TR <= p.rows) {
+            const int64_t i = b0 / p.group;
+            qo.fill(pq + i * p.q[1], st, wid);
+            od.fill(pd + i * p.od[1], st + 2 * QT, wid);
+        } else {
+            auto row = [&](int x) { return RowAt(p, w, min(b0 + x, p.rows - 1)); };
+            fill_rows<ND, 2 * TR, WAVES, WHOLE>(
+                [&](int x) {
+                    const RowAt y = row(x >= TR ? x - TR : x);
+                    return at(q, p.q, w.b, y.i, 2 * y.head + (x >= TR));
+                },
+                p.dh, st, wid, lane);
+            fill_rows<2 * ND, TR, WAVES, WHOLE>(
+                [&](int x) {
+                    const RowAt y = row(x);
+                    return at(dO, p.od, w.b, y.i, y.head);
+                },
+                p.dv, st + 2 * QT, wid, lane);
+        }
+        const float* src = stats + min(b0 + lane, p.rows - 1);
+        for (int x = wid; x < kStats; x += WAVES) dma4(src + x * total, lds_addr(st + 4 * QT) + 256 * x);
     }
 };
 
@@ -353,7 +462,7 @@ template <int ND, int RING, bool WHOLE>
 __global__ __launch_bounds__(128 * NW, 2) void diff_fwd32_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k,
                                                                  const bf16_t* __restrict__ v, bf16_t* __restrict__ o,
                                                                  bf16_t* __restrict__ o2, float* __restrict__ lse, Params p) {
-    using Keys = KeyStage<ND, 2 * NW, WHOLE>;
+    using Keys = KeyStage<ND, 64, 2 * NW, WHOLE>;
     constexpr int NV = 2 * ND, TR = Keys::TR, KT = Keys::KT;
     extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
     char NOTT_LDS* smem = (char NOTT_LDS*)smem_raw;
@@ -373,7 +482,7 @@ __global__ __launch_bounds__(128 * NW, 2) void diff_fwd32_kernel(const bf16_t* _
     const ColPlaces<NV> cols_v(lane);
     u32x4 qr[2 * ND];
     load_row<ND, WHOLE>(at(q, p.q, w.b, r.i, 2 * r.head + map), p.dh, lane, qr);
-    const Keys keys(p, w, k, v);
+    const Keys keys(p, w, k, v, wid, lane);
     const int nk = (vis_all + TR - 1) / TR;
 #pragma unroll
     for (int i = 0; i < RING - 1; ++i)
@@ -440,7 +549,7 @@ template <int ND, int RING, bool WHOLE>
 __global__ __launch_bounds__(64 * NW, 1) void diff_split32_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k,
                                                                   const bf16_t* __restrict__ v, Parts parts, int64_t total,
                                                                   Params p) {
-    using Keys = KeyStage<ND, NW, WHOLE>;
+    using Keys = KeyStage<ND, 64, NW, WHOLE>;
     constexpr int NV = 2 * ND, TR = Keys::TR, KT = Keys::KT;
     extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
     char NOTT_LDS* smem = (char NOTT_LDS*)smem_raw;
@@ -458,7 +567,7 @@ __global__ __launch_bounds__(64 * NW, 1) void diff_split32_kernel(const bf16_t* 
     const ColPlaces<NV> cols_v(lane);
     u32x4 qr[2 * ND];
     load_row<ND, WHOLE>(at(q, p.q, w.b, r.i, 2 * r.head + map), p.dh, lane, qr);
-    const Keys keys(p, w, k, v);
+    const Keys keys(p, w, k, v, wid, lane);
     const int tiles = (vis_all + TR - 1) / TR;
     const int lo = (int)((int64_t)tiles * blockIdx.y / p.nsplit), hi = (int)((int64_t)tiles * (blockIdx.y + 1) / p.nsplit);
 #pragma unroll
@@ -532,8 +641,8 @@ __global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_dq32_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, const bf16_t* __restrict__ o,
     const bf16_t* __restrict__ o2, const bf16_t* __restrict__ dO, const float* __restrict__ lse, float* __restrict__ stats,
     bf16_t* __restrict__ dq, float* __restrict__ dlam, int64_t total, Params p) {
-    constexpr int NV = 2 * ND, TR = 32 * TF, KT = TR * 64 * ND, STAGE = 4 * KT;
-    constexpr int LOADS = 4 * ND * TF / 2;
+    using Keys = KeyStage<ND, 32 * TF, NW, WHOLE>;
+    constexpr int NV = 2 * ND, TR = Keys::TR, KT = Keys::KT;
     extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
     char NOTT_LDS* smem = (char NOTT_LDS*)smem_raw;
     const Pair w(p, blockIdx.x);
@@ -578,29 +687,20 @@ __global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_dq32_kernel(
     }
 
     const int nk = (vis_all + TR - 1) / TR;
-    const bf16_t* pk = at(k, p.k, w.b, 0, 2 * w.j);
-    const bf16_t* pv = at(v, p.v, w.b, 0, w.j);
-    auto issue = [&](int i, int slot) {
-        char NOTT_LDS* st = smem + slot * STAGE;
-        auto key = [&](int x) { return (int64_t)min(i * TR + x, vis_all - 1); };
-        // (a key tile's blocks split over the waves only together with the other map's)
-        fill_rows<ND, 2 * TR, NW, WHOLE>([&](int x) { return pk + (x >= TR ? p.k[2] : 0) + key(x >= TR ? x - TR : x) * p.k[1]; },
-                                  p.dh, st, wid, lane);
-        fill_rows<NV, TR, NW, WHOLE>([&](int x) { return pv + key(x) * p.v[1]; }, p.dv, st + 2 * KT, wid, lane);
-    };
+    const Keys keys(p, w, k, v, wid, lane);
 #pragma unroll
     for (int i = 0; i < RING - 1; ++i)
-        if (i < nk) issue(i, i);
+        if (i < nk) keys.fill(p, i, vis_all, smem + i * Keys::BYTES, wid, lane);
     f32x16 adq[2][ND];
     zero(adq[0]);
     zero(adq[1]);
     int slot = 0, next = RING - 1;
     for (int i = 0; i < nk; ++i) {
-        if (i + RING - 2 < nk) wait_vm_lgkm0<(RING - 2) * LOADS>();
+        if (i + RING - 2 < nk) wait_vm_lgkm0<(RING - 2) * Keys::LOADS>();
         else wait_vm_lgkm0<0>();
         barrier();
-        if (i + RING - 1 < nk) issue(i + RING - 1, next);
-        const char NOTT_LDS* tk = smem + slot * STAGE;
+        if (i + RING - 1 < nk) keys.fill(p, i + RING - 1, vis_all, smem + next * Keys::BYTES, wid, lane);
+        const char NOTT_LDS* tk = smem + slot * Keys::BYTES;
         const char NOTT_LDS* tv = tk + 2 * KT;
         slot = slot + 1 == RING ? 0 : slot + 1;
         next = next + 1 == RING ? 0 : next + 1;
@@ -669,14 +769,13 @@ __global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_dq32_kernel(
 // one share of the rows (blockIdx.z of p.nsplit; shares leave fp32 parts
 // [nsplit][b·hk][s][2·dh + dv] for diff_join_keys_kernel).
 template <int ND, int TF, int RING, int WHAT, bool WHOLE>
-__global__ __launch_bounds__(64 * NW, WHAT == 3 || (WHAT == 1 && ND > 2) ? 1 : 2) void diff_dkdv32_kernel(
+__global__ __launch_bounds__(64 * NW, WHAT == 2 && ND <= 3 ? 2 : 1) void diff_dkdv32_kernel(
     const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v, const bf16_t* __restrict__ dO,
     const float* __restrict__ stats, bf16_t* __restrict__ dk, bf16_t* __restrict__ dv, float* __restrict__ parts, int64_t total,
     Params p) {
     constexpr bool DK = WHAT & 1, DV = WHAT & 2;
-    constexpr int NV = 2 * ND, TR = 32 * TF, QT = TR * 64 * ND;
-    constexpr int STAGE = 4 * QT + 256 * 8;              // q1, q2, dO and the rows' statistics (64 floats each)
-    constexpr int LOADS = 4 * ND * TF / 2;               // per wave and stage, beside the statistics
+    using Rows = RowStage<ND, 32 * TF, NW, WHOLE>;
+    constexpr int NV = 2 * ND, TR = Rows::TR, QT = Rows::QT;
     extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
     char NOTT_LDS* smem = (char NOTT_LDS*)smem_raw;
     const Pair w(p, blockIdx.x);
@@ -685,7 +784,6 @@ __global__ __launch_bounds__(64 * NW, WHAT == 3 || (WHAT == 1 && ND > 2) ? 1 : 2
     const int h = lane >> 5;
     const int kw0 = k0 + 32 * wid, my_k = kw0 + (lane & 31);
     const float sl2 = p.scale * kLog2e;
-    const float* st0 = stats + (int64_t)blockIdx.x * p.rows;
     const int first = k0 < w.len ? w.first_row(p, k0) : p.rows;
     const int all = first < p.rows ? (p.rows + TR - 1) / TR - first / TR : 0;
     const int from = (int)((int64_t)all * blockIdx.z / p.nsplit), i0 = first / TR + from;
@@ -702,25 +800,8 @@ __global__ __launch_bounds__(64 * NW, WHAT == 3 || (WHAT == 1 && ND > 2) ? 1 : 2
         for (int m = 0; m < 2; ++m) load_row<ND, WHOLE>(at(k, p.k, w.b, key, 2 * w.j + m), p.dh, lane, kr[m]);
         if (DK) load_row<NV, WHOLE>(at(v, p.v, w.b, key, w.j), p.dv, lane, vr);
     }
-    auto issue = [&](int i, int slot) {
-        char NOTT_LDS* st = smem + slot * STAGE;
-        const int b0 = (i0 + i) * TR;
-        auto row = [&](int x) { return RowAt(p, w, min(b0 + x, p.rows - 1)); };
-        fill_rows<ND, 2 * TR, NW, WHOLE>(
-            [&](int x) {
-                const RowAt y = row(x >= TR ? x - TR : x);
-                return at(q, p.q, w.b, y.i, 2 * y.head + (x >= TR));
-            },
-            p.dh, st, wid, lane);
-        fill_rows<NV, TR, NW, WHOLE>(
-            [&](int x) {
-                const RowAt y = row(x);
-                return at(dO, p.od, w.b, y.i, y.head);
-            },
-            p.dv, st + 2 * QT, wid, lane);
-        const float* src = st0 + min(b0 + lane, p.rows - 1);
-        for (int x = wid; x < kStats; x += NW) dma4(src + x * total, lds_addr(st + 4 * QT) + 256 * x);
-    };
+    const Rows rows(p, w, q, dO, stats + (int64_t)blockIdx.x * p.rows, wid, lane);
+    auto issue = [&](int i, int slot) { rows.fill(p, w, q, dO, i0 + i, total, smem + slot * Rows::BYTES, wid, lane); };
 #pragma unroll
     for (int i = 0; i < RING - 1; ++i)
         if (i < nq) issue(i, i);
@@ -733,11 +814,11 @@ __global__ __launch_bounds__(64 * NW, WHAT == 3 || (WHAT == 1 && ND > 2) ? 1 : 2
     int slot = 0, next = RING - 1;
     for (int i = 0; i < nq; ++i) {
         // (waves with statistics to load issue more; the count of the others is a safe bound)
-        if (i + RING - 2 < nq) wait_vm_lgkm0<(RING - 2) * LOADS>();
+        if (i + RING - 2 < nq) wait_vm_lgkm0<(RING - 2) * Rows::LOADS>();
         else wait_vm_lgkm0<0>();
         barrier();
         if (i + RING - 1 < nq) issue(i + RING - 1, next);
-        const char NOTT_LDS* tq = smem + slot * STAGE;
+        const char NOTT_LDS* tq = smem + slot * Rows::BYTES;
         const char NOTT_LDS* tdo = tq + 2 * QT;
         const float NOTT_LDS* ss = reinterpret_cast<const float NOTT_LDS*>(tq + 4 * QT);
         slot = slot + 1 == RING ? 0 : slot + 1;
@@ -876,7 +957,7 @@ int reserve(nott_ctx ctx, F* kernel, size_t lds, bool& done) {
 template <int ND, bool WHOLE>
 int fwd(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* o, bf16_t* o2,
         float* lse) {
-    constexpr size_t lds = 2 * (size_t)KeyStage<ND, 2 * NW, WHOLE>::BYTES;
+    constexpr size_t lds = 2 * (size_t)KeyStage<ND, 64, 2 * NW, WHOLE>::BYTES;
     static bool done = false;
     auto f = &diff_fwd32_kernel<ND, 2, WHOLE>;
     if (const int st = reserve(ctx, f, lds, done); st != NOTT_OK) return st;
@@ -887,8 +968,10 @@ int fwd(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const bf1
 
 template <int ND, bool WHOLE>
 int split(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const bf16_t* k, const bf16_t* v, const Parts& parts) {
-    constexpr int RING = ND <= 2 ? 4 : 2;
-    constexpr size_t lds = std::max<size_t>((size_t)RING * KeyStage<ND, NW, WHOLE>::BYTES,
+    // (two stages and two workgroups a CU: four stages and one took 69 us for 45 at 8 x 8192
+    // to 16384 keys of 4 heads)
+    constexpr int RING = 2;
+    constexpr size_t lds = std::max<size_t>((size_t)RING * KeyStage<ND, 64, NW, WHOLE>::BYTES,
                                             (2 * 2 * ND * 16 * 64 + 2 * 2 * 32 * 2) * sizeof(float));
     static bool done = false;
     auto f = &diff_split32_kernel<ND, RING, WHOLE>;
@@ -898,32 +981,35 @@ int split(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const b
     return launch_status(ctx, "diff_split32_kernel");
 }
 
-// Whether one kernel forms dk and dv: its accumulators and operands have to fit a wave.
-template <int ND> constexpr bool kTogether = ND <= 2;
-
 template <int ND, bool WHOLE>
 int bwd(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const bf16_t* k, const bf16_t* v, const bf16_t* o,
         const bf16_t* o2, const bf16_t* dO, const float* lse, float* stats, float* parts, bf16_t* dq, bf16_t* dk, bf16_t* dv,
         float* dlam) {
-    // 32 rows a stage (64 where a stage is 8 KB), stages for 64 to 128 KB
-    constexpr int TF = ND == 1 ? 2 : 1, RING = ND == 1 ? 2 : ND == 3 ? 3 : 4, RINGK = ND <= 2 ? 4 : 2;
-    constexpr size_t lds_q = (size_t)RING * 4 * 32 * TF * 64 * ND;
-    constexpr size_t lds_kv = (size_t)RINGK * (4 * 32 * 64 * ND + 2048);
+    // dq: 32 rows a stage (64 where a stage is 8 KB).  dk and dv: together, 64 rows a stage, as
+    // long as the accumulators and operands fit a wave (64 + 128 columns: 104 us for 8 x 1024
+    // tokens of 8 heads; apart 115, with 32 rows a stage 118), else apart.  A wave for each
+    // map, as in the forward, forms dp twice: 125 us there, and 956 for dk alone where this
+    // takes 620 (4096 tokens of 16 heads of 128 + 256).
+    constexpr int TF = ND == 1 ? 2 : 1, RING = ND == 1 ? 2 : ND == 3 ? 3 : 4;
+    constexpr int TFK = ND <= 2 ? 2 : 1, WHAT = ND <= 2 ? 3 : 1, TFV = ND == 3 ? 1 : 2;
+    constexpr size_t lds_q = (size_t)RING * KeyStage<ND, 32 * TF, NW, WHOLE>::BYTES;
+    constexpr size_t lds_kv = 2 * (size_t)RowStage<ND, 32 * TFK, NW, WHOLE>::BYTES;
+    constexpr size_t lds_v = 2 * (size_t)RowStage<ND, 32 * TFV, NW, WHOLE>::BYTES;
     static bool done[3] = {false, false, false};
     auto fq = &diff_dq32_kernel<ND, TF, RING, WHOLE>;
-    auto fk = &diff_dkdv32_kernel<ND, 1, RINGK, kTogether<ND> ? 3 : 1, WHOLE>;
-    auto fv = &diff_dkdv32_kernel<ND, 1, RINGK, 2, WHOLE>;
+    auto fk = &diff_dkdv32_kernel<ND, TFK, 2, WHAT, WHOLE>;
     if (const int st = reserve(ctx, fq, lds_q, done[0]); st != NOTT_OK) return st;
     if (const int st = reserve(ctx, fk, lds_kv, done[1]); st != NOTT_OK) return st;
-    if (!kTogether<ND>)
-        if (const int st = reserve(ctx, fv, lds_kv, done[2]); st != NOTT_OK) return st;
     const int64_t total = pairs * p.rows;
     hipLaunchKernelGGL(fq, dim3((unsigned)pairs, (unsigned)ceil_div(p.rows, FIXED)), dim3(64 * NW), lds_q, ctx->stream, q, k, v,
                        o, o2, dO, lse, stats, dq, dlam, total, p);
     const dim3 grid((unsigned)pairs, (unsigned)ceil_div(p.s, FIXED), (unsigned)p.nsplit);
     hipLaunchKernelGGL(fk, grid, dim3(64 * NW), lds_kv, ctx->stream, q, k, v, dO, stats, dk, dv, parts, total, p);
-    if (!kTogether<ND>)
-        hipLaunchKernelGGL(fv, grid, dim3(64 * NW), lds_kv, ctx->stream, q, k, v, dO, stats, dk, dv, parts, total, p);
+    if constexpr (WHAT != 3) {
+        auto fv = &diff_dkdv32_kernel<ND, TFV, 2, 2, WHOLE>;
+        if (const int st = reserve(ctx, fv, lds_v, done[2]); st != NOTT_OK) return st;
+        hipLaunchKernelGGL(fv, grid, dim3(64 * NW), lds_v, ctx->stream, q, k, v, dO, stats, dk, dv, parts, total, p);
+    }
     if (parts)
         hipLaunchKernelGGL(diff_join_keys_kernel, dim3((unsigned)ceil_div(pairs * p.s * ((2 * p.dh + p.dv) / 4), 256)), dim3(256),
                            0, ctx->stream, parts, dk, dv, pairs, p);
@@ -1463,6 +1549,9 @@ int check(nott_ctx ctx, const nott_diff_attn_desc* d, nott_dtype dtype, Params* 
     strides(d->dq_stride, p->dq, d->t, 2 * d->h, d->dh);
     strides(d->dk_stride, p->dk, d->s, 2 * d->hk, d->dh);
     strides(d->dv_stride, p->dv_, d->s, d->hk, d->dv);
+    p->near = 1;
+    for (const auto* x : {&p->q, &p->k, &p->v, &p->od})
+        p->near &= (*x)[1] >= 0 && (*x)[2] >= 0 && (*x)[1] < (int64_t(1) << 21) && (*x)[2] * 2 * (group + 1) < (int64_t(1) << 28);
     return NOTT_OK;
 }
 
@@ -1500,8 +1589,7 @@ int fill(nott_ctx ctx, nott_dtype dtype, void* dst, int64_t b, int64_t rows, int
 template <typename T>
 int join(nott_ctx ctx, const Params& p, int64_t pairs, const Parts& parts, T* o, T* o2, float* lse) {
     const int64_t total = pairs * p.rows;
-    hipLaunchKernelGGL(diff_join_kernel<T>, dim3((unsigned)ceil_div(total, 4)), dim3(256), 0, ctx->stream, parts, o, o2, lse,
-                       total, p);
+    hipLaunchKernelGGL(diff_join_kernel<T>, dim3((unsigned)total), dim3(256), 0, ctx->stream, parts, o, o2, lse, total, p);
     return launch_status(ctx, "diff_join_kernel");
 }
 
@@ -1546,8 +1634,8 @@ extern "C" int nott_diff_attention_fwd(nott_ctx ctx, const nott_diff_attn_desc* 
         // Fewer workgroups than half the CUs: keys split.
         if (2 * pairs * ceil_div(p.rows, mx::FIXED) <= ctx->num_cu && p.s >= 256 && ceil_div(p.rows, 32) <= 65535) {
             const int64_t per = 64 * 4;     // keys to a workgroup at the least
-            const int64_t n = std::max<int64_t>(1, std::min<int64_t>(ceil_div(ctx->num_cu, pairs * ceil_div(p.rows, 32)),
-                                                                     ceil_div(p.s, per)));
+            const int64_t most = std::min<int64_t>(kMostParts, ceil_div(p.s, per));
+            const int64_t n = std::min<int64_t>(most, ceil_div(2 * ctx->num_cu, pairs * ceil_div(p.rows, 32)));
             const Parts parts = parts_for(ctx, p, pairs, n);
             if (parts.acc) {
                 p.nsplit = (int32_t)n;
@@ -1571,7 +1659,8 @@ extern "C" int nott_diff_attention_fwd(nott_ctx ctx, const nott_diff_attn_desc* 
         Parts parts{};
         const int64_t groups = pairs * ceil_div(p.rows, BR);
         if (groups < ctx->num_cu && p.s >= 512) {
-            const int64_t n = std::min<int64_t>(ceil_div(2 * ctx->num_cu, groups), ceil_div(p.s, 4 * BR));
+            const int64_t most = std::min<int64_t>(kMostParts, ceil_div(p.s, 4 * BR));
+            const int64_t n = std::min<int64_t>(most, ceil_div(2 * ctx->num_cu, groups));
             parts = parts_for(ctx, p, pairs, n);
             if (parts.acc) p.nsplit = (int32_t)n;
         }

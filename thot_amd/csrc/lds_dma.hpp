@@ -55,6 +55,11 @@ __device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
 }
 
+// The same from a wave-uniform base and a byte offset per lane.
+__device__ __forceinline__ void dma16_at(const void* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+
 // global_load_lds_dword: 4 bytes per lane from `src` to LDS byte lds + 4·lane.
 __device__ __forceinline__ void dma4(const void* src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
