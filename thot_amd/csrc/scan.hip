@@ -7,10 +7,10 @@
 //
 // Composition: a span of tokens maps the state s before it to A·s + B (A = Π keep), and
 // two spans in a row to (A₂·A₁, A₂·B₁ + B₂); c is the same recurrence in reverse with the
-// same A.  A workgroup owns 64 channels and takes 256 tokens at a time: each thread the
-// span of a few tokens of its channels in registers, one wave folds the spans' maps through
-// LDS (another wave those of the reverse scan), and the spans are gone through again
-// from the states before them.  So x and gate are read once and h is written once; the
+// same A.  A workgroup owns 32 or 64 channels and takes 256 tokens at a time: each thread
+// the span of a few tokens of its channels in registers, all threads fold the spans' maps
+// through LDS (the reverse scan's beside), and the spans are gone through again from the
+// states before them.  So x and gate are read once and h is written once; the
 // backward reads x, gate and dh, forms the states again in fp32 from the one that the
 // forward kept before every 256th token (3% of h's bytes, where reading h costs a sixth
 // stream and its rounding), and writes dx and dgate.  States, maps and sums are fp32.
@@ -20,7 +20,13 @@
 // each workgroup folds the maps before its segment, in their order.  No workgroup waits
 // for another, and results do not depend on timing.
 // A keep of exactly 0 forgets the state whatever it was, an infinity or NaN as well.
-// Bound by HBM (3 streams forward, 5 backward).
+//
+// Bound by HBM (3 streams forward, 5 backward): 4 x 4096 tokens of 2048 channels in bf16
+// take 55 us forward (3.7 TB/s) and 98 backward (3.4 TB/s); a packed batch of 50001 tokens
+// of 520 channels in fp32 178 us backward (41 of them for the segments' maps; 4.0 TB/s over
+// its 7 streams).  A token's row holds 64 to 256 bytes of a workgroup, so neighbouring
+// blocks of channels share pages and lines of memory: they run on one XCD, side by side
+// (74 us without that, forward; 118 backward).
 #include "common.hpp"
 
 #include <type_traits>
@@ -29,9 +35,8 @@ namespace {
 
 using nott::ceil_div;
 
-constexpr int kThreads = 512;
-constexpr int kCh = 64;             // channels of a workgroup
 constexpr int kTile = 256;          // tokens of a tile, and between kept states
+constexpr int kThreads = 512;
 
 // VEC neighbouring channels of a token: 16 bytes, or one element where rows are not aligned.
 template <typename T, int VEC> struct Row;
@@ -43,20 +48,21 @@ template <typename T> struct Row<T, 1> {
 };
 template <> struct Row<float, 4> {
     typedef f32x4 Raw;
-    static __device__ __forceinline__ Raw load(const float* p) { return Pack16<float>::raw<true>(p); }
+    static __device__ __forceinline__ Raw load(const float* p) { return Pack16<float>::raw(p); }
     static __device__ __forceinline__ void floats(const Raw& u, float (&v)[4]) { Pack16<float>::unpack(u, v); }
+    // (a workgroup's 256 bytes of a token are whole lines: past the caches, which then keep inputs)
     static __device__ __forceinline__ void store(float* p, const float (&v)[4]) { Pack16<float>::st<true>(p, v); }
 };
 template <> struct Row<bf16_t, 8> {
     typedef u32x4 Raw;
-    static __device__ __forceinline__ Raw load(const bf16_t* p) { return Pack16<bf16_t>::raw<true>(p); }
+    static __device__ __forceinline__ Raw load(const bf16_t* p) { return Pack16<bf16_t>::raw(p); }
     static __device__ __forceinline__ void floats(const Raw& u, float (&v)[8]) { Pack16<bf16_t>::unpack(u, v); }
-    static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[8]) { Pack16<bf16_t>::st<true>(p, v); }
+    static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[8]) { Pack16<bf16_t>::st(p, v); }
 };
 
 struct Params {
     int64_t t, seg;                 // tokens, tokens of a segment
-    int32_t d, nblk, nseg, nchunk;  // channels, 64-channel blocks, segments, kept states
+    int32_t d, nblk, nseg, nchunk;  // channels, their blocks, segments, kept states
     int64_t rows;                   // b·d
     int64_t xb, xt, gb, gt, hb, ht, dxb, dxt, dgb, dgt;   // batch and token strides
 };
@@ -84,56 +90,88 @@ __device__ __forceinline__ float step(float A, float s, float B) { return A == 0
 template <typename X>
 __device__ __forceinline__ void anew(X& x) { asm volatile("" : "+v"(x)); }
 
-// The place of a thread in its workgroup's tile.
-template <int VEC>
+// The place of a thread in its workgroup's tile of 256 tokens of CH channels.
+template <int VEC, int CH>
 struct Place {
-    static constexpr int L = kCh / VEC, G = kThreads / L, R = kTile / G;   // lanes of a token, spans, tokens of a span
+    static constexpr int L = CH / VEC, G = kThreads / L, R = kTile / G;   // lanes of a token, spans, tokens of a span
+    static constexpr int E = kThreads / CH;                              // threads that fold a channel's maps
     int lane, span, c, cc;          // channels from c; cc: where loads go instead past the end
+    int block, seg;                 // of channels; of time
     int64_t b;
     bool in;
     __device__ __forceinline__ explicit Place(const Params& p) {
+        // Workgroups are dealt to the 8 XCDs in turn: each XCD takes neighbouring blocks of
+        // channels, so that its L2 meets the two halves of a line, and rows near each other.
+        const int n = (int)(gridDim.x * gridDim.y), lin = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+        const int x = lin & 7, each = n >> 3, more = n & 7;
+        int at = x * each + min(x, more) + (lin >> 3);
+        seg = at / (int)gridDim.x;
+        at -= seg * (int)gridDim.x;
         lane = threadIdx.x % L;
         span = threadIdx.x / L;
-        b = blockIdx.x / p.nblk;
-        c = (int)(blockIdx.x % p.nblk) * kCh + lane * VEC;
+        b = at / p.nblk;
+        block = at % p.nblk;
+        c = block * CH + lane * VEC;
         in = c < p.d;
         cc = in ? c : 0;
     }
 };
 
-// The maps of a tile's spans, folded in order by one wave (thread = channel): B becomes the
-// state before each span; returns the state behind them all.
-template <int G, bool REVERSE>
-__device__ __forceinline__ float fold(const float (&A)[G][kCh], float (&B)[G][kCh], int ch, float s) {
-    constexpr int U = G < 16 ? G : 16;
-#pragma unroll 1
-    for (int g0 = 0; g0 < G; g0 += U) {
-        float ta[U], tb[U];
+// Folds the maps of a tile's spans in their order (REVERSE: from the last), by all
+// threads: the q-th of E threads of a channel composes its share of the spans (compose),
+// then goes through the shares before its own and through its own spans again, and leaves
+// in B the state before each (apply): a chain of 31 or fewer steps.
+template <int G, int CH, bool REVERSE>
+struct Fold {
+    static constexpr int E = kThreads / CH, N = G / E;
+    float a[N], b[N];
+    int q, ch;
+    __device__ __forceinline__ Fold() : q(threadIdx.x / CH), ch(threadIdx.x % CH) {}
+    __device__ __forceinline__ int span(int i) const { return REVERSE ? G - 1 - (q * N + i) : q * N + i; }
+    __device__ __forceinline__ void compose(const float (&A)[G][CH], const float (&B)[G][CH], float (&M)[2][E][CH]) {
+        float ca = 1.f, cb = 0.f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int g = REVERSE ? G - 1 - g0 - u : g0 + u;
-            ta[u] = A[g][ch];
-            tb[u] = B[g][ch];
+        for (int i = 0; i < N; ++i) {
+            a[i] = A[span(i)][ch];
+            b[i] = B[span(i)][ch];
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            B[REVERSE ? G - 1 - g0 - u : g0 + u][ch] = s;
-            s = step(ta[u], s, tb[u]);
+        for (int i = 0; i < N; ++i) {
+            cb = step(a[i], cb, b[i]);
+            ca *= a[i];
         }
+        M[0][q][ch] = ca;
+        M[1][q][ch] = cb;
     }
-    return s;
-}
+    // Returns the state behind the spans (in the last share's threads).
+    __device__ __forceinline__ float apply(float (&B)[G][CH], const float (&M)[2][E][CH], float s) const {
+        float ma[E - 1], mb[E - 1];
+#pragma unroll
+        for (int j = 0; j < E - 1; ++j) {
+            ma[j] = M[0][j][ch];
+            mb[j] = M[1][j][ch];
+        }
+#pragma unroll
+        for (int j = 0; j < E - 1; ++j) s = j < q ? step(ma[j], s, mb[j]) : s;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            B[span(i)][ch] = s;
+            s = step(a[i], s, b[i]);
+        }
+        return s;
+    }
+};
 
 // Maps of whole segments, for the segments that follow (forward) or precede (reverse):
 // agg [nseg][2][b·d].  A span is a run of the segment's tokens, gone through in registers.
-template <typename T, int VEC, bool SIG, bool MIX, bool REVERSE>
+template <typename T, int VEC, int CH, bool SIG, bool MIX, bool REVERSE>
 __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict__ x, const T* __restrict__ gate,
                                                              const uint8_t* __restrict__ reset, float* __restrict__ agg,
                                                              Params p) {
-    typedef Place<VEC> P;
-    __shared__ __attribute__((aligned(16))) float sA[P::G][kCh], sB[P::G][kCh];
+    typedef Place<VEC, CH> P;
+    __shared__ __attribute__((aligned(16))) float sA[P::G][CH], sB[P::G][CH];
     const P w(p);
-    const int seg = REVERSE ? blockIdx.y + 1 : blockIdx.y;
+    const int seg = REVERSE ? w.seg + 1 : w.seg;
     const int64_t t0 = seg * p.seg, t1 = min(p.t, t0 + p.seg);
     const int64_t run = (p.seg + P::G - 1) / P::G;
     const int64_t r0 = min(t1, t0 + w.span * run), r1 = min(t1, r0 + run);
@@ -179,8 +217,8 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict
         sB[w.span][w.lane * VEC + v] = B[v];
     }
     __syncthreads();
-    const int ch = (int)(blockIdx.x % p.nblk) * kCh + threadIdx.x;
-    if (threadIdx.x >= kCh || ch >= p.d) return;
+    const int ch = w.block * CH + threadIdx.x;
+    if (threadIdx.x >= CH || ch >= p.d) return;
     float ta = 1.f, tb = 0.f;
     for (int g = 0; g < P::G; ++g) {
         const int i = REVERSE ? P::G - 1 - g : g;
@@ -192,30 +230,32 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict
     o[p.rows] = tb;
 }
 
-template <typename T, int VEC, bool SIG, bool MIX>
+template <typename T, int VEC, int CH, bool SIG, bool MIX>
 __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(const T* __restrict__ x, const T* __restrict__ gate,
                                                             const float* __restrict__ h0,
                                                             const uint8_t* __restrict__ reset,
                                                             const float* __restrict__ agg, T* __restrict__ h,
                                                             float* __restrict__ last, float* __restrict__ states, Params p) {
-    typedef Place<VEC> P;
+    typedef Place<VEC, CH> P;
     typedef typename Row<T, VEC>::Raw Raw;
     constexpr int R = P::R;
     // two tiles' maps in turn: a tile's are written while another wave still reads the last one's
-    __shared__ __attribute__((aligned(16))) float sA[2][P::G][kCh], sB[2][P::G][kCh];
+    __shared__ __attribute__((aligned(16))) float sA[2][P::G][CH], sB[2][P::G][CH];
+    __shared__ float sM[2][P::E][CH], carry[2][CH];     // (carry: the state before the tile, and the next one's)
     const P w(p);
-    const int seg = blockIdx.y;
+    const int seg = w.seg;
     const int64_t t0 = seg * p.seg, t1 = min(p.t, t0 + p.seg);
     const T* px = x + w.b * p.xb + w.cc;
     const T* pg = gate + w.b * p.gb + w.cc;
     T* ph = h + w.b * p.hb + w.cc;
-    const int ch = (int)(blockIdx.x % p.nblk) * kCh + threadIdx.x;   // the folding wave's channel
-    const bool folds = threadIdx.x < kCh, mine = folds && ch < p.d;
+    Fold<P::G, CH, false> fold;
+    const int ch = w.block * CH + fold.ch;
+    const bool mine = fold.q == 0 && ch < p.d;
     const int64_t row = w.b * p.d + ch;
-    float s = 0.f;
     if (mine) {
-        s = h0 ? h0[row] : 0.f;
+        float s = h0 ? h0[row] : 0.f;
         for (int g = 0; g < seg; ++g) s = step(agg[(int64_t)g * 2 * p.rows + row], s, agg[((int64_t)g * 2 + 1) * p.rows + row]);
+        carry[0][fold.ch] = s;
     }
     Raw rx[R], rg[R];
     uint32_t fresh = 0;     // bit r: a sequence begins at token r of the span
@@ -232,8 +272,11 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(const T* __restrict_
     load(t0);
     int buf = 0;
     for (int64_t tile = t0; tile < t1; tile += kTile, buf ^= 1) {
-        const int64_t mt = tile + w.span * R;
+        const int live = (int)max<int64_t>(0, min<int64_t>(R, t1 - tile - w.span * R));   // tokens of the span that are there
         float a[R][VEC], u[R][VEC], A[VEC], B[VEC];
+        // Where no sequence begins, no token is missing and no gate is 0 (the map's product
+        // shows it), the selects of step() and of the tile's end are left out.
+        bool careful = reset || tile + kTile > t1;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             A[v] = 1.f;
@@ -244,15 +287,39 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(const T* __restrict_
             float vx[VEC], vg[VEC];
             Row<T, VEC>::floats(rx[r], vx);
             Row<T, VEC>::floats(rg[r], vg);
-            const bool out = mt + r >= t1, begins = (fresh >> r) & 1;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 float take;
                 gates<SIG, MIX>(vg[v], a[r][v], take);
-                u[r][v] = out ? 0.f : take * vx[v];
-                a[r][v] = out ? 1.f : begins ? 0.f : a[r][v];
-                B[v] = step(a[r][v], B[v], u[r][v]);
+                u[r][v] = take * vx[v];
+            }
+        }
+        if (careful) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    u[r][v] = r >= live ? 0.f : u[r][v];
+                    a[r][v] = r >= live ? 1.f : (fresh >> r) & 1 ? 0.f : a[r][v];
+                }
+        }
+        float least = 1.f;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                B[v] = fmaf(a[r][v], B[v], u[r][v]);
                 A[v] *= a[r][v];
+            }
+            least = fminf(least, __builtin_fabsf(A[v]));
+        }
+        careful = __any(least == 0.f);
+        if (careful) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                B[v] = 0.f;
+#pragma unroll
+                for (int r = 0; r < R; ++r) B[v] = step(a[r][v], B[v], u[r][v]);
             }
         }
 #pragma unroll
@@ -262,52 +329,67 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(const T* __restrict_
         }
         if (tile + kTile < t1) load(tile + kTile);
         __syncthreads();
-        if (folds) {
+        fold.compose(sA[buf], sB[buf], sM);
+        __syncthreads();
+        {
+            const float s = carry[buf][fold.ch];
             if (states && mine) states[(w.b * p.nchunk + tile / kTile) * p.d + ch] = s;
-            s = fold<P::G, false>(sA[buf], sB[buf], threadIdx.x, s);
+            const float after = fold.apply(sB[buf], sM, s);
+            if (fold.q == P::E - 1) carry[buf ^ 1][fold.ch] = after;
         }
         __syncthreads();
         float c[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) c[v] = sB[buf][w.span][w.lane * VEC + v];
+        T* po = ph + (tile + w.span * R) * p.ht;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
+            if (careful) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) c[v] = step(a[r][v], c[v], u[r][v]);
-            if (w.in && mt + r < t1) Row<T, VEC>::store(ph + (mt + r) * p.ht, c);
+                for (int v = 0; v < VEC; ++v) c[v] = step(a[r][v], c[v], u[r][v]);
+            } else {
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) c[v] = fmaf(a[r][v], c[v], u[r][v]);
+            }
+            if (w.in && r < live) Row<T, VEC>::store(po + r * p.ht, c);
         }
     }
-    if (mine && last && t1 == p.t) last[row] = s;
+    if (mine && last && t1 == p.t) last[row] = carry[buf][fold.ch];
 }
 
-template <typename T, int VEC, bool SIG, bool MIX>
+template <typename T, int VEC, int CH, bool SIG, bool MIX>
 __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict__ dh, const T* __restrict__ x,
                                                             const T* __restrict__ gate, const uint8_t* __restrict__ reset,
                                                             const float* __restrict__ states,
                                                             const float* __restrict__ dlast, const float* __restrict__ agg,
                                                             T* __restrict__ dx, T* __restrict__ dgate,
                                                             float* __restrict__ dh0, Params p) {
-    typedef Place<VEC> P;
+    typedef Place<VEC, CH> P;
     typedef typename Row<T, VEC>::Raw Raw;
     constexpr int R = P::R;
     // A serves both folds, which run side by side; B and C become the states before a span
     // and the gradients from behind it
-    __shared__ __attribute__((aligned(16))) float sA[P::G][kCh], sB[P::G][kCh], sC[P::G][kCh];
+    __shared__ __attribute__((aligned(16))) float sA[P::G][CH], sB[P::G][CH], sC[P::G][CH];
+    __shared__ float sM[2][2][P::E][CH], carry[2][CH];      // (carry: the gradient from behind the tile)
     const P w(p);
-    const int seg = blockIdx.y;
+    const int seg = w.seg;
     const int64_t t0 = seg * p.seg, t1 = min(p.t, t0 + p.seg);
     const T* pe = dh + w.b * p.hb + w.cc;
     const T* px = x + w.b * p.xb + w.cc;
     const T* pg = gate + w.b * p.gb + w.cc;
-    const int fold_ch = threadIdx.x & (kCh - 1), wave = threadIdx.x / kCh;
-    const int ch = (int)(blockIdx.x % p.nblk) * kCh + fold_ch;
+    Fold<P::G, CH, false> states_fold;
+    Fold<P::G, CH, true> grads_fold;
+    const int fold_ch = states_fold.ch, q = states_fold.q;
+    const int ch = w.block * CH + fold_ch;
     const int64_t row = w.b * p.d + ch;
-    float s = 0.f;          // wave 1: the gradient from behind the tile
-    if (wave == 1 && ch < p.d) {
-        s = dlast ? dlast[row] : 0.f;
+    const bool mine = q == 0 && ch < p.d;
+    if (mine) {
+        float s = dlast ? dlast[row] : 0.f;
         for (int g = p.nseg - 1; g > seg; --g)
             s = step(agg[(int64_t)g * 2 * p.rows + row], s, agg[((int64_t)g * 2 + 1) * p.rows + row]);
+        carry[0][fold_ch] = s;
     }
+    int buf = 0;
     Raw re[R], rx[R], rg[R];
     uint32_t fresh = 0;
     auto load = [&](int64_t tile) {
@@ -322,52 +404,73 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
         }
     };
     // Loads of the next tile are in flight while a tile is computed only where both fit the
-    // registers (bf16, 16-byte rows).
+    // registers.
     constexpr bool AHEAD = VEC == 8;
     const int64_t first = t0, final = t0 + (t1 - t0 - 1) / kTile * kTile;
     if (AHEAD) load(final);
     for (int64_t tile = final; tile >= first; tile -= kTile) {
         if (!AHEAD) load(tile);
-        const int64_t mt = tile + w.span * R;
-        const int live = (int)min<int64_t>(R, t1 - mt);     // tokens of the span that are there
+        const int live = (int)min<int64_t>(R, t1 - tile - w.span * R);     // tokens of the span that are there
         uint32_t begins = fresh;
         float a[R][VEC], A[VEC], B[VEC], C[VEC];
         float take[MIX ? R : 1][VEC];
         Raw ex[R], ee[R];       // x and dh as loaded: half the registers in bf16
-        const float before = wave == 0 && ch < p.d ? states[(w.b * p.nchunk + tile / kTile) * p.d + ch] : 0.f;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            A[v] = 1.f;
-            B[v] = C[v] = 0.f;
-        }
+        const float before = ch < p.d ? states[(w.b * p.nchunk + tile / kTile) * p.d + ch] : 0.f;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            float vg[VEC], vx[VEC];
+            float vg[VEC];
             ex[r] = rx[r];
             ee[r] = re[r];
-            Row<T, VEC>::floats(rx[r], vx);
             Row<T, VEC>::floats(rg[r], vg);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 float tk;
                 gates<SIG, MIX>(vg[v], a[r][v], tk);
                 if constexpr (MIX) take[r][v] = tk;
-                a[r][v] = r >= live ? 1.f : a[r][v];
-                const float k = (begins >> r) & 1 ? 0.f : a[r][v];
-                B[v] = step(k, B[v], r >= live ? 0.f : tk * vx[v]);
-                A[v] *= k;
             }
         }
-#pragma unroll
-        for (int r = R - 1; r >= 0; --r) {
-            float ve[VEC];
-            Row<T, VEC>::floats(ee[r], ve);
+        // The span's maps; CAREFUL as in the forward.
+        auto maps = [&](auto which) {
+            constexpr bool CAREFUL = decltype(which)::value;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const float k = (begins >> r) & 1 ? 0.f : a[r][v];
-                C[v] = k == 0.f ? 0.f : k * ((r >= live ? 0.f : ve[v]) + C[v]);
+                A[v] = 1.f;
+                B[v] = C[v] = 0.f;
             }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float vx[VEC];
+                Row<T, VEC>::floats(ex[r], vx);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    if (CAREFUL) a[r][v] = r >= live ? 1.f : a[r][v];
+                    const float k = CAREFUL && ((begins >> r) & 1) ? 0.f : a[r][v];
+                    const float u = CAREFUL && r >= live ? 0.f : MIX ? take[r][v] * vx[v] : vx[v];
+                    B[v] = CAREFUL ? step(k, B[v], u) : fmaf(k, B[v], u);
+                    A[v] *= k;
+                }
+            }
+#pragma unroll
+            for (int r = R - 1; r >= 0; --r) {
+                float ve[VEC];
+                Row<T, VEC>::floats(ee[r], ve);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    const float k = CAREFUL && ((begins >> r) & 1) ? 0.f : a[r][v];
+                    const float e = (CAREFUL && r >= live ? 0.f : ve[v]) + C[v];
+                    C[v] = CAREFUL && k == 0.f ? 0.f : k * e;
+                }
+            }
+        };
+        bool careful = reset || tile + kTile > t1;
+        if (!careful) {
+            maps(std::false_type());
+            float least = 1.f;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) least = fminf(least, __builtin_fabsf(A[v]));
+            careful = __any(least == 0.f);
         }
+        if (careful) maps(std::true_type());
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             sA[w.span][w.lane * VEC + v] = A[v];
@@ -376,8 +479,15 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
         }
         if (AHEAD && tile > first) load(tile - kTile);
         __syncthreads();
-        if (wave == 0) (void)fold<P::G, false>(sA, sB, fold_ch, before);
-        else if (wave == 1) s = fold<P::G, true>(sA, sC, fold_ch, s);
+        states_fold.compose(sA, sB, sM[0]);
+        grads_fold.compose(sA, sC, sM[1]);
+        __syncthreads();
+        (void)states_fold.apply(sB, sM[0], before);
+        {
+            const float after = grads_fold.apply(sC, sM[1], carry[buf][fold_ch]);
+            if (q == P::E - 1) carry[buf ^ 1][fold_ch] = after;
+        }
+        buf ^= 1;
         __syncthreads();
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -391,39 +501,47 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
             anew(ex[r]);
             anew(ee[r]);
         }
-        float held[R][VEC];     // what e is multiplied by in da: the state before the token [− x]
+        const int64_t mt = tile + w.span * R;
+        auto gradients = [&](auto which) {
+            constexpr bool CAREFUL = decltype(which)::value;
+            float held[R][VEC];     // what e is multiplied by in da: the state before the token [− x]
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float vx[VEC];
-            Row<T, VEC>::floats(ex[r], vx);
+            for (int r = 0; r < R; ++r) {
+                float vx[VEC];
+                Row<T, VEC>::floats(ex[r], vx);
+                const bool b = CAREFUL && ((begins >> r) & 1);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const bool b = (begins >> r) & 1;
-                held[r][v] = (b ? 0.f : B[v]) - (MIX ? vx[v] : 0.f);
-                B[v] = step(b ? 0.f : a[r][v], B[v], MIX ? take[r][v] * vx[v] : vx[v]);
+                for (int v = 0; v < VEC; ++v) {
+                    const float u = MIX ? take[r][v] * vx[v] : vx[v];
+                    held[r][v] = (b ? 0.f : B[v]) - (MIX ? vx[v] : 0.f);
+                    B[v] = CAREFUL ? step(b ? 0.f : a[r][v], B[v], u) : fmaf(a[r][v], B[v], u);
+                }
             }
-        }
 #pragma unroll
-        for (int r = R - 1; r >= 0; --r) {
-            float ox[VEC], og[VEC], ve[VEC];
-            Row<T, VEC>::floats(ee[r], ve);
+            for (int r = R - 1; r >= 0; --r) {
+                float ox[VEC], og[VEC], ve[VEC];
+                Row<T, VEC>::floats(ee[r], ve);
+                const bool b = CAREFUL && ((begins >> r) & 1);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float k = (begins >> r) & 1 ? 0.f : a[r][v];
-                const float e = (r >= live ? 0.f : ve[v]) + C[v];
-                C[v] = k == 0.f ? 0.f : k * e;
-                ox[v] = MIX ? take[r][v] * e : e;
-                float da = held[r][v];
-                if constexpr (SIG) da *= MIX ? a[r][v] * take[r][v] : a[r][v] * (1.f - a[r][v]);
-                og[v] = da * e;
+                for (int v = 0; v < VEC; ++v) {
+                    const float k = b ? 0.f : a[r][v];
+                    const float e = (CAREFUL && r >= live ? 0.f : ve[v]) + C[v];
+                    C[v] = CAREFUL && k == 0.f ? 0.f : k * e;
+                    ox[v] = MIX ? take[r][v] * e : e;
+                    float da = held[r][v];
+                    if constexpr (SIG) da *= MIX ? a[r][v] * take[r][v] : a[r][v] * (1.f - a[r][v]);
+                    og[v] = da * e;
+                }
+                if (w.in && (!CAREFUL || r < live)) {
+                    Row<T, VEC>::store(dx + w.b * p.dxb + (mt + r) * p.dxt + w.c, ox);
+                    Row<T, VEC>::store(dgate + w.b * p.dgb + (mt + r) * p.dgt + w.c, og);
+                }
             }
-            if (w.in && r < live) {
-                Row<T, VEC>::store(dx + w.b * p.dxb + (mt + r) * p.dxt + w.c, ox);
-                Row<T, VEC>::store(dgate + w.b * p.dgb + (mt + r) * p.dgt + w.c, og);
-            }
-        }
+        };
+        if (careful) gradients(std::true_type());
+        else gradients(std::false_type());
     }
-    if (wave == 1 && ch < p.d && dh0 && seg == 0) dh0[row] = s;
+    if (mine && dh0 && seg == 0) dh0[row] = carry[buf][fold_ch];
 }
 
 // Few tokens: a thread goes through them with VEC channels, no tiles (a decoding step of
@@ -486,9 +604,8 @@ int check(nott_ctx ctx, const nott_scan_desc* d, nott_dtype dtype, Params* p) {
     p->t = d->t;
     p->d = (int32_t)d->d;
     p->rows = d->b * d->d;
-    p->nblk = (int32_t)ceil_div(d->d, kCh);
     p->nchunk = 0;
-    NOTT_REQUIRE(ctx, ceil_div(d->t, kTile) < (int64_t(1) << 31) && d->b * p->nblk <= 0x7fffffff / kThreads &&
+    NOTT_REQUIRE(ctx, ceil_div(d->t, kTile) < (int64_t(1) << 31) && d->b * ceil_div(d->d, 32) <= 0x7fffffff / 512 &&
                           p->rows < (int64_t(1) << 36), "linear scan: too many channels or tokens");
     p->nchunk = (int32_t)ceil_div(d->t, kTile);
     auto strides = [&](const int64_t (&s)[2], int64_t& sb, int64_t& st) {
@@ -504,8 +621,8 @@ int check(nott_ctx ctx, const nott_scan_desc* d, nott_dtype dtype, Params* p) {
     return NOTT_OK;
 }
 
-// Segments: one where the channels alone give every CU a workgroup, else as many as bring
-// two for each, of at least 4 tiles.
+// Segments: one where the channels alone give half of the CUs a workgroup, else as many as
+// bring two for each, of at least 4 tiles.
 void segments(nott_ctx ctx, Params* p, int64_t blocks) {
     const int64_t tiles = p->nchunk;
     int64_t n = blocks >= ctx->num_cu / 2 ? 1 : std::min<int64_t>(ceil_div(2 * ctx->num_cu, blocks), ceil_div(tiles, 4));
@@ -513,6 +630,12 @@ void segments(nott_ctx ctx, Params* p, int64_t blocks) {
     p->seg = len * kTile;
     p->nseg = (int32_t)ceil_div(tiles, len);
 }
+
+// Channels of a workgroup: 64 in fp32 rows of 16-byte groups, else 32, whose half as
+// many values a thread leave room for the next tile's loads (4 x 4096 tokens of 2048 channels in
+// bf16, forward 66 us with 64 channels and 56 with 32, backward 190 and 98; 50001 tokens of
+// 520 channels in fp32, backward 177 and 190).
+template <int VEC> constexpr int kChannels = VEC == 4 ? 64 : 32;
 
 template <typename T, int VEC, bool SIG, bool MIX>
 int fwd(nott_ctx ctx, Params& p, const void* x, const void* gate, const float* h0, const uint8_t* reset, void* h,
@@ -526,18 +649,20 @@ int fwd(nott_ctx ctx, Params& p, const void* x, const void* gate, const float* h
                            tg, h0, reset, static_cast<T*>(h), last, states, p);
         return nott::launch_status(ctx, "scan_steps_kernel");
     }
-    const int64_t blocks = batches * p.nblk;
-    segments(ctx, &p, blocks);
+    constexpr int CH = kChannels<VEC>;
+    p.nblk = (int32_t)ceil_div(p.d, CH);
+    segments(ctx, &p, batches * p.nblk);
+    const dim3 grid((unsigned)(batches * p.nblk));
     float* agg = nullptr;
     if (p.nseg > 1) {
         agg = static_cast<float*>(nott::optional_workspace(ctx, (size_t)p.nseg * 2 * p.rows * sizeof(float)));
         if (!agg) p.nseg = 1, p.seg = (int64_t)p.nchunk * kTile;
     }
     if (p.nseg > 1)
-        hipLaunchKernelGGL((scan_maps_kernel<T, VEC, SIG, MIX, false>), dim3((unsigned)blocks, (unsigned)(p.nseg - 1)),
-                           dim3(kThreads), 0, ctx->stream, tx, tg, reset, agg, p);
-    hipLaunchKernelGGL((scan_fwd_kernel<T, VEC, SIG, MIX>), dim3((unsigned)blocks, (unsigned)p.nseg), dim3(kThreads), 0,
-                       ctx->stream, tx, tg, h0, reset, agg, static_cast<T*>(h), last, states, p);
+        hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CH, SIG, MIX, false>), dim3(grid.x, (unsigned)(p.nseg - 1)), dim3(kThreads),
+                           0, ctx->stream, tx, tg, reset, agg, p);
+    hipLaunchKernelGGL((scan_fwd_kernel<T, VEC, CH, SIG, MIX>), dim3(grid.x, (unsigned)p.nseg), dim3(kThreads), 0, ctx->stream,
+                       tx, tg, h0, reset, agg, static_cast<T*>(h), last, states, p);
     return nott::launch_status(ctx, "scan_fwd_kernel");
 }
 
@@ -546,18 +671,20 @@ int bwd(nott_ctx ctx, Params& p, const void* dh, const void* x, const void* gate
         const float* dlast, void* dx, void* dgate, float* dh0) {
     const T* te = static_cast<const T*>(dh);
     const T* tg = static_cast<const T*>(gate);
-    const int64_t blocks = p.rows / p.d * p.nblk;
-    segments(ctx, &p, blocks);
+    constexpr int CH = kChannels<VEC>;
+    p.nblk = (int32_t)ceil_div(p.d, CH);
+    segments(ctx, &p, p.rows / p.d * p.nblk);
+    const dim3 grid((unsigned)(p.rows / p.d * p.nblk));
     float* agg = nullptr;
     if (p.nseg > 1) {
         agg = static_cast<float*>(nott::optional_workspace(ctx, (size_t)p.nseg * 2 * p.rows * sizeof(float)));
         if (!agg) p.nseg = 1, p.seg = (int64_t)p.nchunk * kTile;
     }
     if (p.nseg > 1)
-        hipLaunchKernelGGL((scan_maps_kernel<T, VEC, SIG, false, true>), dim3((unsigned)blocks, (unsigned)(p.nseg - 1)),
+        hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CH, SIG, false, true>), dim3(grid.x, (unsigned)(p.nseg - 1)),
                            dim3(kThreads), 0, ctx->stream, te, tg, reset, agg, p);
-    hipLaunchKernelGGL((scan_bwd_kernel<T, VEC, SIG, MIX>), dim3((unsigned)blocks, (unsigned)p.nseg), dim3(kThreads), 0,
-                       ctx->stream, te, static_cast<const T*>(x), tg, reset, states, dlast, agg, static_cast<T*>(dx),
+    hipLaunchKernelGGL((scan_bwd_kernel<T, VEC, CH, SIG, MIX>), dim3(grid.x, (unsigned)p.nseg), dim3(kThreads), 0, ctx->stream,
+                       te, static_cast<const T*>(x), tg, reset, states, dlast, agg, static_cast<T*>(dx),
                        static_cast<T*>(dgate), dh0, p);
     return nott::launch_status(ctx, "scan_bwd_kernel");
 }
