@@ -26,6 +26,7 @@
 #include <torch/torch.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <array>
 #include <cstring>
 #include <atomic>
@@ -931,6 +932,172 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     }
 };
 
+// ------------------------------------------------ differential attention
+// o = softmax(q₁·k₁ᵀ·scale)·v − λ·softmax(q₂·k₂ᵀ·scale)·v per head (nott_diff_attention_fwd / _bwd): q
+// [b, t, 2·h, dh], k [b, s, 2·hk, dh], v [b, s, hk, dv], views with any strides but the
+// last; lam fp32 [h] or [b, t, h]; lengths, q_start int32 [b] or absent.  lam's gradient:
+// a parameter [h] gets its own added to .grad, as a layer's parameters do; a lam that
+// was computed from others (or is [b, t, h]) hands it on.
+struct DiffAttentionFn : torch::autograd::Function<DiffAttentionFn> {
+    static Tensor rows(const Tensor& x) { return x.stride(-1) == 1 || x.numel() == 0 ? x : x.contiguous(); }
+    // Three zeros mean contiguous: a tensor that repeats one row is copied before.
+    static Tensor operand4(const Tensor& x) {
+        Tensor r = rows(x);
+        if (r.numel() > r.size(-1) && r.stride(0) == 0 && r.stride(1) == 0 && r.stride(2) == 0) r = r.contiguous();
+        return r;
+    }
+    static void strides(int64_t (&s)[3], const Tensor& x) {
+        for (int i = 0; i < 3; ++i) s[i] = x.numel() ? x.stride(i) : 0;
+    }
+    static nott_diff_attn_desc desc(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, bool causal,
+                                    double scale) {
+        if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || q.size(2) % 2)
+            throw std::invalid_argument("Nott::HIP: q must be [b, t, 2·h, dh], k [b, s, 2·hk, dh] and v [b, s, hk, dv]");
+        nott_diff_attn_desc d{};
+        d.b = q.size(0); d.t = q.size(1); d.h = q.size(2) / 2; d.dh = q.size(3);
+        d.s = v.size(1); d.hk = v.size(2); d.dv = v.size(3);
+        if (k.size(0) != d.b || v.size(0) != d.b || k.size(1) != d.s || k.size(2) != 2 * d.hk || k.size(3) != d.dh ||
+            (d.h && (d.hk == 0 || d.h % d.hk)))
+            throw std::invalid_argument("Nott::HIP: k and v do not go with q: two maps a head, heads in whole groups of v's");
+        for (const Tensor& t : {k, v})
+            if (t.scalar_type() != q.scalar_type() || t.device() != q.device())
+                throw std::invalid_argument("Nott::HIP: k and v must have q's type and device");
+        const bool per_head = lam.dim() == 1 && lam.size(0) == d.h;
+        const bool per_token = lam.dim() == 3 && lam.size(0) == d.b && lam.size(1) == d.t && lam.size(2) == d.h;
+        if ((!per_head && !per_token) || lam.scalar_type() != torch::kFloat32 || lam.device() != q.device())
+            throw std::invalid_argument("Nott::HIP: lam must be fp32 [h] or [b, t, h] on q's device");
+        d.causal = causal; d.token_lam = per_token; d.scale = scale;
+        strides(d.q_stride, q); strides(d.k_stride, k); strides(d.v_stride, v);
+        return d;
+    }
+    static const int32_t* counts(const Tensor& t, const Tensor& q) {
+        if (!present(t)) return nullptr;
+        if (t.dim() != 1 || !operand(t, q, torch::kInt32, q.size(0)))
+            throw std::invalid_argument("Nott::HIP: lengths and q_start must be int32 [b] on q's device");
+        return t.data_ptr<int32_t>();
+    }
+    static Tensor forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, Tensor lam, Tensor lengths, Tensor q_start,
+                          bool causal, double scale, bool keep) {
+        const bool master = lam.is_leaf() && lam.requires_grad() && lam.dim() == 1 && lam.is_contiguous();
+        q = operand4(q); k = operand4(k); v = operand4(v);
+        const nott_diff_attn_desc d = desc(q, k, v, lam, causal, scale);
+        const int32_t *len = counts(lengths, q), *start = counts(q_start, q);
+        const Tensor lc = contig(lam);
+        Tensor o = torch::empty({d.b, d.t, d.h, d.dv}, q.options());
+        Tensor o2 = keep ? torch::empty_like(o) : absent(q);
+        Tensor lse = torch::empty({d.b, 2 * d.h, d.t}, q.options().dtype(torch::kFloat32));
+        nott_ctx c = bind(q);
+        check(nott_diff_attention_fwd(c, &d, dtype_of(q), ptr(q), ptr(k), ptr(v), fptr(lc), len, start, ptr(o), fptr(lse),
+                                      ptr(o2)),
+              c, "differential attention forward");
+        ctx->save_for_backward({q, k, v, master ? lam : lc, lengths, q_start, o, o2, lse});
+        ctx->saved_data["causal"] = causal;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["master"] = master;
+        return o;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        auto s = ctx->get_saved_variables();
+        Tensor q = s[0], k = s[1], v = s[2], lam = s[3], o = s[6];
+        const bool master = ctx->saved_data["master"].toBool();
+        nott_diff_attn_desc d = desc(q, k, v, lam, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
+        Tensor dO = operand4(grads[0]);
+        strides(d.do_stride, dO);
+        Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options()),
+               dv = torch::empty(v.sizes(), v.options());
+        Tensor dlam = master ? grad_buffer(lam) : torch::empty(lam.sizes(), lam.options());
+        nott_ctx c = bind(q);
+        check(nott_diff_attention_bwd(c, &d, dtype_of(q), ptr(dO), ptr(q), ptr(k), ptr(v), fptr(lam), counts(s[4], q),
+                                      counts(s[5], q), ptr(o), ptr(s[7]), fptr(s[8]), ptr(dq), ptr(dk), ptr(dv), fptr(dlam),
+                                      master ? 1 : 0),
+              c, "differential attention backward");
+        return {dq, dk, dv, master ? Tensor() : dlam, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// ------------------------------------------------ gated linear recurrence
+// h_t = keep_t·h_{t−1} + take_t·x_t over time (nott_linear_scan_fwd / _bwd): x, gate
+// [b, t, d], views with any strides but the last; h0 fp32 [b, d] or absent; reset bool
+// [b, t] or absent.  Gives h and the fp32 state behind the last token.  A leaf h0 gets
+// its gradient added to .grad, as a layer's parameters do.
+struct LinearScanFn : torch::autograd::Function<LinearScanFn> {
+    static Tensor rows(const Tensor& x) {
+        Tensor r = x.stride(-1) == 1 || x.numel() == 0 ? x : x.contiguous();
+        // two zeros mean contiguous
+        if (r.numel() > r.size(-1) && r.stride(0) == 0 && r.stride(1) == 0) r = r.contiguous();
+        return r;
+    }
+    static void strides(int64_t (&s)[2], const Tensor& x) {
+        for (int i = 0; i < 2; ++i) s[i] = x.numel() ? x.stride(i) : 0;
+    }
+    static nott_scan_desc desc(const Tensor& x, const Tensor& gate, bool sigmoid, bool mix) {
+        nott_scan_desc d{};
+        d.b = x.size(0); d.t = x.size(1); d.d = x.size(2);
+        d.sigmoid = sigmoid; d.mix = mix;
+        strides(d.x_stride, x); strides(d.gate_stride, gate);
+        return d;
+    }
+    static const uint8_t* bytes(const Tensor& reset) {
+        return present(reset) ? static_cast<const uint8_t*>(reset.data_ptr()) : nullptr;
+    }
+    static variable_list forward(AutogradContext* ctx, Tensor x, Tensor gate, Tensor h0, Tensor reset, bool sigmoid, bool mix,
+                                 bool keep) {
+        if (x.dim() != 3 || x.size(2) == 0 || gate.sizes() != x.sizes() || gate.scalar_type() != x.scalar_type() ||
+            gate.device() != x.device())
+            throw std::invalid_argument("Nott::HIP: x must be [b, t, d] with d > 0, the gate alike in shape, type and device");
+        if (present(h0) && (h0.dim() != 2 || h0.size(0) != x.size(0) || h0.size(1) != x.size(2) ||
+                            h0.scalar_type() != torch::kFloat32 || h0.device() != x.device()))
+            throw std::invalid_argument("Nott::HIP: h0 must be fp32 [b, d] on x's device");
+        if (present(reset) && (reset.dim() != 2 || reset.size(0) != x.size(0) || reset.size(1) != x.size(1) ||
+                               (reset.scalar_type() != torch::kBool && reset.scalar_type() != torch::kUInt8) ||
+                               !reset.is_contiguous() || reset.device() != x.device()))
+            throw std::invalid_argument("Nott::HIP: reset must be bool or uint8 [b, t], contiguous, on x's device");
+        const bool master = h0.is_leaf() && h0.requires_grad();
+        x = rows(x); gate = rows(gate);
+        const nott_scan_desc d = desc(x, gate, sigmoid, mix);
+        auto f32 = x.options().dtype(torch::kFloat32);
+        Tensor h = torch::empty(x.sizes(), x.options()), last = torch::empty({d.b, d.d}, f32);
+        Tensor states = keep ? torch::empty({d.b, (d.t + NOTT_SCAN_CHUNK - 1) / NOTT_SCAN_CHUNK, d.d}, f32) : absent(x);
+        nott_ctx c = bind(x);
+        check(nott_linear_scan_fwd(c, &d, dtype_of(x), ptr(x), ptr(gate), fptr(contig(h0)), bytes(reset), ptr(h), fptr(last),
+                                   fptr(states)),
+              c, "linear scan forward");
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({x, gate, master ? h0 : Tensor(), reset, states});
+        ctx->saved_data["sigmoid"] = sigmoid;
+        ctx->saved_data["mix"] = mix;
+        ctx->saved_data["start"] = present(h0) && h0.requires_grad();
+        return {h, last};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        auto s = ctx->get_saved_variables();
+        Tensor x = s[0], gate = s[1], h0 = s[2];
+        variable_list out(7);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        nott_scan_desc d = desc(x, gate, ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["mix"].toBool());
+        // an output that nothing used has no gradient
+        Tensor dh = grads[0].defined() ? rows(grads[0]) : torch::zeros(x.sizes(), x.options());
+        Tensor dlast = grads[1].defined() ? contig(grads[1]) : Tensor();
+        strides(d.h_stride, dh);
+        out[0] = torch::empty(x.sizes(), x.options());
+        out[1] = torch::empty(x.sizes(), x.options());
+        Tensor dh0;
+        if (ctx->saved_data["start"].toBool()) dh0 = torch::empty({d.b, d.d}, x.options().dtype(torch::kFloat32));
+        nott_ctx c = bind(x);
+        check(nott_linear_scan_bwd(c, &d, dtype_of(x), ptr(dh), ptr(x), ptr(gate), bytes(s[3]), fptr(s[4]), fptr(dlast),
+                                   ptr(out[0]), ptr(out[1]), fptr(dh0)),
+              c, "linear scan backward");
+        if (h0.defined() && dh0.defined()) {
+            Tensor g = grad_buffer(h0);
+            torch::NoGradGuard ng;
+            g.add_(dh0);
+        } else {
+            out[2] = dh0;
+        }
+        return out;
+    }
+};
+
 // ---------------------------------------------------------------- Fork
 // Two uses of one tensor (residual skip): backward sums the two gradients.
 // relu_input: x is the previous block's output, a ReLU output whose backward
@@ -1277,6 +1444,27 @@ inline Tensor gated_linear(const Tensor& x, const Tensor& w, const Tensor& wc, c
     const bool keep = torch::GradMode::is_enabled() &&
                       (x.requires_grad() || w.requires_grad() || (b.defined() && b.requires_grad()));
     return GatedLinearFn::apply(x, w, wc, or_absent(b, w), act, keep);
+}
+
+// Differential attention; what its backward reads is kept only where one may come.
+// lengths and q_start may be undefined; scale 0 means 1/sqrt(dh).
+inline Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, bool causal = false,
+                             double scale = 0.0, const Tensor& lengths = {}, const Tensor& q_start = {}) {
+    if (q.dim() != 4 || q.size(3) == 0) throw std::invalid_argument("Nott::HIP: q must be [b, t, 2·h, dh]");
+    // (asked here: inside the function grad mode is off either way)
+    const bool keep = torch::GradMode::is_enabled() &&
+                      (q.requires_grad() || k.requires_grad() || v.requires_grad() || lam.requires_grad());
+    return DiffAttentionFn::apply(q, k, v, lam, or_absent(lengths, q), or_absent(q_start, q), causal,
+                                  scale == 0.0 ? 1.0 / std::sqrt((double)q.size(3)) : scale, keep);
+}
+
+// {h, last} of the gated linear recurrence; h0 and reset may be undefined.
+inline std::pair<Tensor, Tensor> linear_scan(const Tensor& x, const Tensor& gate, const Tensor& h0 = {},
+                                             const Tensor& reset = {}, bool sigmoid = true, bool mix = true) {
+    const bool keep = torch::GradMode::is_enabled() &&
+                      (x.requires_grad() || gate.requires_grad() || (h0.defined() && h0.requires_grad()));
+    auto r = LinearScanFn::apply(x, gate, or_absent(h0, x), or_absent(reset, x), sigmoid, mix, keep);
+    return {r[0], r[1]};
 }
 
 // {logprob, entropy} of each row's label under softmax(scale·logits).
@@ -1672,6 +1860,210 @@ private:
 };
 using FusedAdam = FusedAdamImpl<false>;    // Nott::Optimizer::Details::Adam
 using FusedAdamW = FusedAdamImpl<true>;    // Nott::Optimizer::Details::AdamW
+
+// Adam / AdamW over parameters that stay where they are (nott_adam_multi_step): no arena,
+// fp32 or bf16 parameters and gradients, moments in 32 bits, or in 8 (e4m3 codes with a
+// scale for every 256 elements, 2.03 bytes a parameter in place of 8).  Steps as
+// torch::optim::Adam[W] does, a parameter without a gradient left out, with one call for
+// the parameters of a group at one step count.  save / load keep the moments' own bits.
+// amsgrad is not supported.
+template <bool Decoupled>
+class MultiTensorAdamImpl : public torch::optim::Optimizer {
+public:
+    using TorchOptions = std::conditional_t<Decoupled, torch::optim::AdamWOptions, torch::optim::AdamOptions>;
+
+    MultiTensorAdamImpl(std::vector<Tensor> params, const TorchOptions& options, int bits = 32)
+        : torch::optim::Optimizer(std::move(params), std::make_unique<TorchOptions>(options)) {
+        build(bits);
+    }
+    MultiTensorAdamImpl(const std::vector<torch::optim::OptimizerParamGroup>& groups, const TorchOptions& options, int bits = 32)
+        : torch::optim::Optimizer(groups, std::make_unique<TorchOptions>(options)) {
+        build(bits);
+    }
+
+    Tensor step(LossClosure closure = nullptr) override {
+        Tensor loss;
+        if (closure) {
+            torch::AutoGradMode enable(true);
+            loss = closure();
+        }
+        if (param_groups_.size() != group_count_)
+            throw std::logic_error("MultiTensorAdam: parameter groups were added after construction");
+        if (!m_.defined()) return loss;
+        torch::NoGradGuard ng;
+        // (asked before bind, whose new contexts a capture would not survive)
+        hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+        detail::hip_ok(hipStreamIsCapturing(c10::hip::getCurrentHIPStream(m_.device().index()).stream(), &capturing),
+                       "MultiTensorAdam");
+        if (capturing != hipStreamCaptureStatusNone)   // a replay would repeat this step's bias correction
+            throw std::logic_error("MultiTensorAdam: step() is not for capture (nott_adam_multi_step_graph is)");
+        nott_ctx c = bind(m_);
+        const float* gscale = nullptr;
+        if (grad_scale_.defined()) gscale = grad_scale_.data_ptr<float>();
+        // everything is checked before the first launch
+        struct Run { size_t group; int64_t step; std::vector<nott_adam_tensor> list; };
+        std::vector<Run> runs;
+        std::vector<Slot*> moved;
+        for (size_t gi = 0; gi < param_groups_.size(); ++gi) {
+            const size_t first = runs.size();
+            for (auto& p : param_groups_[gi].params()) {
+                auto it = slots_.find(p.unsafeGetTensorImpl());
+                if (it == slots_.end() || !p.grad().defined()) continue;
+                Slot& s = it->second;
+                if (p.numel() != s.n || !p.is_contiguous() || p.device() != m_.device())
+                    throw std::logic_error("MultiTensorAdam: a parameter has changed its shape, layout or device");
+                Tensor g = p.grad();
+                if (g.layout() != torch::kStrided || g.numel() != s.n || g.device() != m_.device())
+                    throw std::invalid_argument("MultiTensorAdam: a gradient must be dense and lie where its parameter does");
+                if (!g.is_contiguous()) {
+                    g = g.contiguous();
+                    p.mutable_grad() = g;
+                }
+                nott_adam_tensor t{};
+                t.p = p.data_ptr(); t.g = g.data_ptr();
+                t.m = static_cast<char*>(m_.data_ptr()) + s.first * 256 * (bits_ / 8);
+                t.v = static_cast<char*>(v_.data_ptr()) + s.first * 256 * (bits_ / 8);
+                t.scale = bits_ == 8 ? scale_.data_ptr<float>() + 2 * s.first : nullptr;
+                t.copy = s.copy.defined() ? s.copy.data_ptr() : nullptr;
+                t.n = s.n;
+                t.p_dtype = (int16_t)dtype_of(p); t.g_dtype = (int16_t)dtype_of(g); t.bits = bits_;
+                moved.push_back(&s);
+                size_t r = first;
+                while (r < runs.size() && runs[r].step != s.step + 1) ++r;
+                if (r == runs.size()) runs.push_back({gi, s.step + 1, {}});
+                runs[r].list.push_back(t);
+            }
+        }
+        for (const Run& r : runs) {
+            const auto& o = static_cast<const TorchOptions&>(param_groups_[r.group].options());
+            check(nott_adam_multi_step(c, Decoupled ? 1 : 0, r.list.data(), (int64_t)r.list.size(), o.lr(),
+                                       std::get<0>(o.betas()), std::get<1>(o.betas()), o.eps(), o.weight_decay(), r.step,
+                                       gscale, fuse_zero_ ? 1 : 0),
+                  c, "adam step over many tensors");
+        }
+        for (Slot* s : moved) ++s->step;
+        return loss;
+    }
+
+    // step() also clears the gradients it read.
+    void set_fused_zero_grad(bool on) { fuse_zero_ = on; }
+    // A device fp32 number that multiplies every gradient of the steps to come, as it is
+    // when a step's kernels run (a clipping factor); undefined: none.
+    void set_grad_scale(const Tensor& t) {
+        if (t.defined() && m_.defined() && !operand(t, m_, torch::kFloat32, 1))
+            throw std::invalid_argument("MultiTensorAdam: the gradients' factor must be one fp32 number on their device");
+        grad_scale_ = t;
+    }
+    // A bf16 working copy of a parameter, written by every step from now on.
+    Tensor bf16_copy(const Tensor& p) {
+        Slot& s = slot(p);
+        if (!s.copy.defined()) {
+            torch::NoGradGuard ng;
+            s.copy = p.detach().to(torch::kBFloat16, false, true);
+        }
+        return s.copy;
+    }
+    int64_t step_count(const Tensor& p) const { return slot(p).step; }
+    // The moments of a parameter in fp32.
+    Tensor exp_avg(const Tensor& p) const { return moment(p, m_, 0); }
+    Tensor exp_avg_sq(const Tensor& p) const {
+        Tensor r = moment(p, v_, 1);
+        return bits_ == 8 ? r.square() : r;
+    }
+
+    void save(torch::serialize::OutputArchive& ar) const override {
+        std::vector<int64_t> steps;
+        for (const auto* impl : order_) steps.push_back(slots_.at(impl).step);
+        ar.write("step", torch::tensor(steps, torch::kInt64), true);
+        for (const auto& kv : held()) ar.write(kv.first, kv.second, true);
+    }
+    void load(torch::serialize::InputArchive& ar) override {
+        torch::NoGradGuard ng;
+        Tensor steps;
+        ar.read("step", steps, true);
+        std::vector<std::pair<Tensor, Tensor>> to;
+        for (const auto& kv : held()) {
+            Tensor t;
+            ar.read(kv.first, t, true);
+            to.emplace_back(kv.second, t);
+        }
+        bool fits = steps.scalar_type() == torch::kInt64 && steps.numel() == (int64_t)order_.size();
+        for (const auto& kv : to) fits = fits && kv.first.sizes() == kv.second.sizes() && kv.first.scalar_type() == kv.second.scalar_type();
+        if (!fits) throw std::invalid_argument("MultiTensorAdam: the saved state is of other parameters or another width");
+        steps = steps.to(torch::kCPU).contiguous();
+        for (auto& kv : to) kv.first.copy_(kv.second);
+        for (size_t i = 0; i < order_.size(); ++i) slots_.at(order_[i]).step = steps.data_ptr<int64_t>()[i];
+    }
+
+private:
+    struct Slot { int64_t first, n, step; Tensor copy; };
+
+    void build(int bits) {
+        if (bits != 8 && bits != 32) throw std::invalid_argument("MultiTensorAdam: bits must be 8 or 32");
+        bits_ = bits;
+        int64_t blocks = 0;
+        c10::optional<torch::Device> dev;
+        std::vector<std::pair<const char*, int64_t>> spans;
+        for (auto& group : param_groups_) {
+            if (static_cast<const TorchOptions&>(group.options()).amsgrad())
+                throw std::invalid_argument("MultiTensorAdam: amsgrad is not supported");
+            for (const auto& p : group.params()) {
+                if (!p.defined() || !p.requires_grad()) continue;
+                (void)dtype_of(p);
+                if (!p.is_contiguous()) throw std::invalid_argument("MultiTensorAdam: parameters must be contiguous");
+                if (!p.is_cuda()) throw std::invalid_argument("MultiTensorAdam: parameters must live on a HIP device");
+                if (dev && *dev != p.device()) throw std::invalid_argument("MultiTensorAdam: parameters on several devices");
+                dev = p.device();
+                if (!slots_.emplace(p.unsafeGetTensorImpl(), Slot{blocks, p.numel(), 0, Tensor()}).second)
+                    throw std::invalid_argument("MultiTensorAdam: a parameter is listed twice");
+                order_.push_back(p.unsafeGetTensorImpl());
+                if (p.numel()) spans.emplace_back(static_cast<const char*>(p.data_ptr()), p.numel() * (int64_t)p.element_size());
+                blocks += (p.numel() + 255) / 256;
+            }
+        }
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            if (spans[i - 1].first + spans[i - 1].second > spans[i].first)
+                throw std::invalid_argument("MultiTensorAdam: parameters must not overlap");
+        group_count_ = param_groups_.size();
+        if (!dev) return;
+        torch::NoGradGuard ng;
+        auto o = torch::TensorOptions().device(*dev).dtype(bits == 8 ? torch::kUInt8 : torch::kFloat32);
+        m_ = torch::zeros({blocks, 256}, o);
+        v_ = torch::zeros({blocks, 256}, o);
+        if (bits == 8) scale_ = torch::zeros({blocks, 2}, o.dtype(torch::kFloat32));
+    }
+    const Slot& slot(const Tensor& p) const {
+        auto it = slots_.find(p.unsafeGetTensorImpl());
+        if (it == slots_.end()) throw std::invalid_argument("MultiTensorAdam: no state for this parameter");
+        return it->second;
+    }
+    Slot& slot(const Tensor& p) { return const_cast<Slot&>(const_cast<const MultiTensorAdamImpl*>(this)->slot(p)); }
+    Tensor moment(const Tensor& p, const Tensor& of, int64_t which) const {
+        torch::NoGradGuard ng;
+        const Slot& s = slot(p);
+        Tensor r = of.narrow(0, s.first, (s.n + 255) / 256);
+        if (bits_ == 8)
+            r = r.view(torch::kFloat8_e4m3fn).to(torch::kFloat32) *
+                scale_.narrow(0, s.first, (s.n + 255) / 256).narrow(1, which, 1);
+        return r.reshape({-1}).narrow(0, 0, s.n).view(p.sizes()).clone();
+    }
+    std::vector<std::pair<std::string, Tensor>> held() const {
+        if (!m_.defined()) return {};
+        std::vector<std::pair<std::string, Tensor>> r{{"m", m_}, {"v", v_}};
+        if (bits_ == 8) r.emplace_back("scale", scale_);
+        return r;
+    }
+
+    int bits_ = 32;
+    size_t group_count_ = 0;
+    bool fuse_zero_ = false;
+    Tensor m_, v_, scale_, grad_scale_;
+    std::unordered_map<const c10::TensorImpl*, Slot> slots_;
+    std::vector<const c10::TensorImpl*> order_;
+};
+using MultiTensorAdam = MultiTensorAdamImpl<false>;
+using MultiTensorAdamW = MultiTensorAdamImpl<true>;
 
 }  // namespace HIP
 }  // namespace Nott

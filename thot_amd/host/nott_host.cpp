@@ -550,6 +550,51 @@ struct OptimizerHandle {
     }
 };
 
+namespace {
+
+// Adam[W] over parameters where they lie, by groups.
+template <bool Decoupled>
+void multi_tensor_adam(py::module_& m, const char* name) {
+    using Opt = NH::MultiTensorAdamImpl<Decoupled>;
+    using Opts = typename Opt::TorchOptions;
+    py::class_<Opt>(m, name)
+        .def(py::init([](const std::vector<std::vector<Tensor>>& groups, const std::vector<double>& lrs,
+                         const std::vector<double>& wds, double beta1, double beta2, double eps, int bits) {
+                 if (groups.size() != lrs.size() || groups.size() != wds.size())
+                     throw std::invalid_argument("one learning rate and weight decay per group");
+                 std::vector<torch::optim::OptimizerParamGroup> pg;
+                 for (size_t i = 0; i < groups.size(); ++i) {
+                     auto o = std::make_unique<Opts>(lrs[i]);
+                     o->betas(std::make_tuple(beta1, beta2)).eps(eps).weight_decay(wds[i]);
+                     pg.emplace_back(groups[i], std::move(o));
+                 }
+                 return std::make_unique<Opt>(pg, Opts(1e-3).betas(std::make_tuple(beta1, beta2)).eps(eps), bits);
+             }),
+             py::arg("groups"), py::arg("lrs"), py::arg("weight_decays"), py::arg("beta1") = 0.9, py::arg("beta2") = 0.999,
+             py::arg("eps") = 1e-8, py::arg("bits") = 32)
+        .def("step", [](Opt& o) { o.step(); }, py::call_guard<py::gil_scoped_release>())
+        .def("zero_grad", [](Opt& o, bool set_to_none) { o.zero_grad(set_to_none); }, py::arg("set_to_none") = false)
+        .def("set_lr", [](Opt& o, size_t group, double lr) { o.param_groups().at(group).options().set_lr(lr); })
+        .def("set_fused_zero_grad", &Opt::set_fused_zero_grad)
+        .def("set_grad_scale", [](Opt& o, const std::optional<Tensor>& t) { o.set_grad_scale(t ? *t : Tensor()); })
+        .def("bf16_copy", &Opt::bf16_copy)
+        .def("state_step", &Opt::step_count)
+        .def("exp_avg", &Opt::exp_avg)
+        .def("exp_avg_sq", &Opt::exp_avg_sq)
+        .def("save", [](const Opt& o, const std::string& path) {
+                 torch::serialize::OutputArchive ar;
+                 o.save(ar);
+                 ar.save_to(path);
+             }, py::arg("path"))
+        .def("load", [](Opt& o, const std::string& path) {
+                 torch::serialize::InputArchive ar;
+                 ar.load_from(path);
+                 o.load(ar);
+             }, py::arg("path"));
+}
+
+}  // namespace
+
 PYBIND11_MODULE(_nott_host, m) {
     m.doc() = "C++ host layer (Nott::HIP) over libnott_hip: configs[0] and configs[4] training steps";
     // Workspace held by the device's contexts (one per stream used).
@@ -589,6 +634,16 @@ PYBIND11_MODULE(_nott_host, m) {
     }, py::arg("x"), py::arg("w"), py::arg("b") = py::none(), py::arg("w_compute") = py::none(), py::arg("act") = 0);
     m.def("token_logprob", [](const Tensor& z, const Tensor& y, double scale) { return NH::token_logprob(z, y, scale); },
           py::arg("logits"), py::arg("labels"), py::arg("scale") = 1.0);
+    m.def("diff_attention", [=](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, bool causal,
+                                std::optional<double> scale, const OptT& lengths, const OptT& q_start) {
+        if (scale && !(*scale > 0)) throw std::invalid_argument("scale must be positive");
+        return NH::diff_attention(q, k, v, lam, causal, scale.value_or(0.0), given(lengths), given(q_start));
+    }, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("lam"), py::arg("causal") = false, py::arg("scale") = py::none(),
+          py::arg("lengths") = py::none(), py::arg("q_start") = py::none());
+    m.def("linear_scan", [=](const Tensor& x, const Tensor& gate, const OptT& h0, const OptT& reset, bool sigmoid, bool mix) {
+        return NH::linear_scan(x, gate, given(h0), given(reset), sigmoid, mix);
+    }, py::arg("x"), py::arg("gate"), py::arg("h0") = py::none(), py::arg("reset") = py::none(), py::arg("sigmoid") = true,
+          py::arg("mix") = true);
     // Whether trainers run convolution weight gradients on the side stream
     // (on by default; the switch exists so tests can compare both orders).
     m.def("set_side_stream", [](bool on) { NH::set_side_stream_enabled(on); }, py::arg("on"));
@@ -722,4 +777,6 @@ PYBIND11_MODULE(_nott_host, m) {
                  if (auto* a = dynamic_cast<torch::optim::AdamParamState*>(it->second.get())) return a->exp_avg();
                  return static_cast<torch::optim::AdamWParamState&>(*it->second).exp_avg();
              });
+    multi_tensor_adam<false>(m, "MultiTensorAdam");
+    multi_tensor_adam<true>(m, "MultiTensorAdamW");
 }
