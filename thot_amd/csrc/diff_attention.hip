@@ -101,14 +101,16 @@ struct Parts {
     float* ml;
 };
 
-// Joins the parts (at most 64): a workgroup a row.  Lane z weighs part z; a wave sums every
-// fourth part, its loads in flight beside those of the weights, and the waves' sums are
-// added in order (a wave a row, a part after the other, took 17.7 us for 128 rows in 8 parts).
+// Joins the parts (at most 64): a workgroup of WAVES waves a row.  Lane z weighs part z; a
+// wave sums every WAVES-th part, its loads in flight beside those of the weights, and the
+// waves' sums are added in order (a wave a row, a part after the other, took 17.7 us for
+// 128 rows in 8 parts; four waves 4.8).  Up to 4 parts are one wave's loads
+// (14000 rows in 3 parts 40.7 us with four waves, 15.9 with one).
 constexpr int kMostParts = 64;
-template <typename T>
-__global__ __launch_bounds__(256) void diff_join_kernel(Parts parts, T* __restrict__ o, T* __restrict__ o2,
+template <typename T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void diff_join_kernel(Parts parts, T* __restrict__ o, T* __restrict__ o2,
                                                         float* __restrict__ lse, int64_t total, Params p) {
-    __shared__ float sum[4][2][256];
+    __shared__ float sum[WAVES][2][256];
     const int64_t at_row = blockIdx.x;      // (b·hk + j)·rows + row
     const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int bk = (int)(at_row / p.rows), row = (int)(at_row - (int64_t)bk * p.rows);
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(256) void diff_join_kernel(Parts parts, T* __restri
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int z = min(z0 + 4 * u, p.nsplit - 1), d = lane + 64 * c;
+                    const int z = min(z0 + WAVES * u, p.nsplit - 1), d = lane + 64 * c;
                     a[u][k][c] = d < p.dv ? parts.acc[((z * total + at_row) * 2 + k) * p.dv + d] : 0.f;
                 }
     };
@@ -137,14 +139,14 @@ __global__ __launch_bounds__(256) void diff_join_kernel(Parts parts, T* __restri
                         mine.z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine.z - m[1])};
     const float l[2] = {wave_sum(f[0] * mine.y), wave_sum(f[1] * mine.w)};
     float acc[2][4] = {};
-    for (int z0 = wid; z0 < p.nsplit; z0 += 4 * U) {
+    for (int z0 = wid; z0 < p.nsplit; z0 += WAVES * U) {
         if (z0 != wid) load(z0);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float fz = __shfl(f[k], min(z0 + 4 * u, 63), 64);
-                if (z0 + 4 * u >= p.nsplit || fz == 0.f) continue;
+                const float fz = __shfl(f[k], min(z0 + WAVES * u, 63), 64);
+                if (z0 + WAVES * u >= p.nsplit || fz == 0.f) continue;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[k][c] = fmaf(fz, a[u][k][c], acc[k][c]);
             }
@@ -154,12 +156,17 @@ __global__ __launch_bounds__(256) void diff_join_kernel(Parts parts, T* __restri
 #pragma unroll
         for (int c = 0; c < 4; ++c) sum[wid][k][lane + 64 * c] = acc[k][c];
     __syncthreads();
-    const int d = threadIdx.x;
-    if (d < p.dv) {
-        const float i1 = l[0] > 0.f ? 1.f / l[0] : 0.f, i2 = l[1] > 0.f ? 1.f / l[1] : 0.f;
-        const float first = (sum[0][0][d] + sum[1][0][d]) + (sum[2][0][d] + sum[3][0][d]);
-        const float second = ((sum[0][1][d] + sum[1][1][d]) + (sum[2][1][d] + sum[3][1][d])) * i2;
-        Io<T>::st(at(o, p.o, w.b, r.i, r.head), d, first * i1 - lam * second);
+    const float i1 = l[0] > 0.f ? 1.f / l[0] : 0.f, i2 = l[1] > 0.f ? 1.f / l[1] : 0.f;
+    for (int d = threadIdx.x; d < p.dv; d += 64 * WAVES) {
+        float of[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            of[k] = sum[0][k][d];
+#pragma unroll
+            for (int w2 = 1; w2 < WAVES; ++w2) of[k] += sum[w2][k][d];
+        }
+        const float second = of[1] * i2;
+        Io<T>::st(at(o, p.o, w.b, r.i, r.head), d, of[0] * i1 - lam * second);
         if (o2) Io<T>::st(o2, (((int64_t)w.b * p.t + r.i) * p.h + r.head) * p.dv + d, second);
     }
     if (threadIdx.x < 2) *lse_at(p, lse, w.b, r, threadIdx.x) = threadIdx.x ? log_sum(m[1], l[1]) : log_sum(m[0], l[0]);
@@ -1589,7 +1596,10 @@ int fill(nott_ctx ctx, nott_dtype dtype, void* dst, int64_t b, int64_t rows, int
 template <typename T>
 int join(nott_ctx ctx, const Params& p, int64_t pairs, const Parts& parts, T* o, T* o2, float* lse) {
     const int64_t total = pairs * p.rows;
-    hipLaunchKernelGGL(diff_join_kernel<T>, dim3((unsigned)total), dim3(256), 0, ctx->stream, parts, o, o2, lse, total, p);
+    if (p.nsplit <= 4)
+        hipLaunchKernelGGL((diff_join_kernel<T, 1>), dim3((unsigned)total), dim3(64), 0, ctx->stream, parts, o, o2, lse, total, p);
+    else
+        hipLaunchKernelGGL((diff_join_kernel<T, 4>), dim3((unsigned)total), dim3(256), 0, ctx->stream, parts, o, o2, lse, total, p);
     return launch_status(ctx, "diff_join_kernel");
 }
 
