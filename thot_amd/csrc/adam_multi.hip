@@ -263,7 +263,8 @@ int check(nott_ctx ctx, const nott_adam_tensor* t, int64_t count) {
     NOTT_REQUIRE(ctx, count >= 0 && (count == 0 || t), "adam over tensors: bad list");
     for (int64_t i = 0; i < count; ++i) {
         const nott_adam_tensor& x = t[i];
-        NOTT_REQUIRE(ctx, x.n >= 0 && x.n < (int64_t(1) << 42), "adam over tensors: bad size");
+        // (its workgroups' threads fit a launch)
+        NOTT_REQUIRE(ctx, x.n >= 0 && x.n <= (int64_t)(0x7fffffff / kThreads) * kChunk, "adam over tensors: bad size");
         NOTT_REQUIRE(ctx, nott::valid_dtype(x.p_dtype) && nott::valid_dtype(x.g_dtype) && (x.bits == 8 || x.bits == 32),
                      "adam over tensors: bad dtype or moments that are not 8 or 32 bits");
         if (x.n == 0) continue;
@@ -298,7 +299,6 @@ int launch(nott_ctx ctx, const nott_adam_tensor* t, int64_t count, Args& a) {
         const int64_t mine = nott::ceil_div(x.n, kChunk);
         if (a.count == kTensors || chunks + mine > 0x7fffffff / kThreads)   // the launch's threads fit 31 bits
             if (const int st = flush(); st != NOTT_OK) return st;
-        NOTT_REQUIRE(ctx, mine <= 0x7fffffff / kThreads, "adam over tensors: a tensor is too large");
         a.e[a.count++] = {x.p, x.g, x.m, x.v, x.scale, static_cast<bf16_t*>(x.copy), x.n, (int32_t)chunks,
                           aligned(x.p, 4 * sizeof(TP)) && aligned(x.g, 4 * sizeof(TG)) && aligned(x.copy, 8)};
         chunks += mine;

@@ -27,6 +27,7 @@
 #include "attention_tile.hpp"
 #include "lds_dma.hpp"
 
+#include <atomic>
 #include <type_traits>
 
 namespace {
@@ -35,6 +36,7 @@ using namespace nott::attn;
 using nott::ceil_div;
 using nott::launch_status;
 
+constexpr int64_t kMostBlocks = 1 << 22;    // of 256 threads, in a launch (its threads fit 32 bits)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -950,13 +952,16 @@ __global__ __launch_bounds__(256) void diff_join_keys_kernel(const float* __rest
     for (int e = 0; e < 4; ++e) out[e] = f32_to_bf16(s[e]);
 }
 
+// LDS beyond the default is reserved once for each device (`done` a bit each, devices past
+// 64 every time).
 template <typename F>
-int reserve(nott_ctx ctx, F* kernel, size_t lds, bool& done) {
-    if (!done) {
+int reserve(nott_ctx ctx, F* kernel, size_t lds, std::atomic<uint64_t>& done) {
+    const uint64_t bit = ctx->device < 64 ? uint64_t(1) << ctx->device : 0;
+    if (!(done.load(std::memory_order_relaxed) & bit)) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return nott::hip_fail(ctx, e, "differential attention: cannot reserve LDS");
-        done = true;
+        done.fetch_or(bit, std::memory_order_relaxed);
     }
     return NOTT_OK;
 }
@@ -965,7 +970,7 @@ template <int ND, bool WHOLE>
 int fwd(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const bf16_t* k, const bf16_t* v, bf16_t* o, bf16_t* o2,
         float* lse) {
     constexpr size_t lds = 2 * (size_t)KeyStage<ND, 64, 2 * NW, WHOLE>::BYTES;
-    static bool done = false;
+    static std::atomic<uint64_t> done{0};
     auto f = &diff_fwd32_kernel<ND, 2, WHOLE>;
     if (const int st = reserve(ctx, f, lds, done); st != NOTT_OK) return st;
     hipLaunchKernelGGL(f, dim3((unsigned)pairs, (unsigned)ceil_div(p.rows, FIXED)), dim3(128 * NW), lds, ctx->stream, q, k, v,
@@ -980,7 +985,7 @@ int split(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const b
     constexpr int RING = 2;
     constexpr size_t lds = std::max<size_t>((size_t)RING * KeyStage<ND, 64, NW, WHOLE>::BYTES,
                                             (2 * 2 * ND * 16 * 64 + 2 * 2 * 32 * 2) * sizeof(float));
-    static bool done = false;
+    static std::atomic<uint64_t> done{0};
     auto f = &diff_split32_kernel<ND, RING, WHOLE>;
     if (const int st = reserve(ctx, f, lds, done); st != NOTT_OK) return st;
     hipLaunchKernelGGL(f, dim3((unsigned)pairs, (unsigned)p.nsplit, (unsigned)ceil_div(p.rows, 32)), dim3(64 * NW), lds,
@@ -1002,7 +1007,7 @@ int bwd(nott_ctx ctx, const Params& p, int64_t pairs, const bf16_t* q, const bf1
     constexpr size_t lds_q = (size_t)RING * KeyStage<ND, 32 * TF, NW, WHOLE>::BYTES;
     constexpr size_t lds_kv = 2 * (size_t)RowStage<ND, 32 * TFK, NW, WHOLE>::BYTES;
     constexpr size_t lds_v = 2 * (size_t)RowStage<ND, 32 * TFV, NW, WHOLE>::BYTES;
-    static bool done[3] = {false, false, false};
+    static std::atomic<uint64_t> done[3];
     auto fq = &diff_dq32_kernel<ND, TF, RING, WHOLE>;
     auto fk = &diff_dkdv32_kernel<ND, TFK, 2, WHAT, WHOLE>;
     if (const int st = reserve(ctx, fq, lds_q, done[0]); st != NOTT_OK) return st;
@@ -1245,31 +1250,31 @@ __global__ __launch_bounds__(256) void diff_stats_kernel(const T* __restrict__ o
                                                          const T* __restrict__ dO, const float* __restrict__ lse,
                                                          float* __restrict__ stats, float* __restrict__ dlam, int64_t total,
                                                          Params p) {
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    if (n >= total) return;
-    const int bk = (int)(n / p.rows);
-    const Pair w(p, bk);
-    const RowAt r(p, w, (int)(n - (int64_t)bk * p.rows));
-    const int64_t second = (((int64_t)w.b * p.t + r.i) * p.h + r.head) * p.dv;
-    const T* po = at(o, p.o, w.b, r.i, r.head);
-    const T* pd = at(dO, p.od, w.b, r.i, r.head);
-    float a = 0.f, b = 0.f;
-    for (int d = lane; d < p.dv; d += 64) {
-        const float g = Io<T>::ld(pd, d);
-        a = fmaf(g, Io<T>::ld(po, d), a);
-        b = fmaf(g, Io<T>::ld(o2, second + d), b);
+    for (int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); n < total; n += (int64_t)gridDim.x * 4) {
+        const int bk = (int)(n / p.rows);
+        const Pair w(p, bk);
+        const RowAt r(p, w, (int)(n - (int64_t)bk * p.rows));
+        const int64_t second = (((int64_t)w.b * p.t + r.i) * p.h + r.head) * p.dv;
+        const T* po = at(o, p.o, w.b, r.i, r.head);
+        const T* pd = at(dO, p.od, w.b, r.i, r.head);
+        float a = 0.f, b = 0.f;
+        for (int d = lane; d < p.dv; d += 64) {
+            const float g = Io<T>::ld(pd, d);
+            a = fmaf(g, Io<T>::ld(po, d), a);
+            b = fmaf(g, Io<T>::ld(o2, second + d), b);
+        }
+        a = wave_sum(a);
+        b = wave_sum(b);
+        if (lane) continue;
+        const float lam = lambda_of(p, w.b, r);
+        stats[n] = *lse_at(p, const_cast<float*>(lse), w.b, r, 0) * kLog2e;
+        stats[total + n] = *lse_at(p, const_cast<float*>(lse), w.b, r, 1) * kLog2e;
+        stats[2 * total + n] = fmaf(lam, b, a);
+        stats[3 * total + n] = b;
+        stats[4 * total + n] = lam;
+        if (p.token_lam) dlam[((int64_t)w.b * p.t + r.i) * p.h + r.head] = -b;
     }
-    a = wave_sum(a);
-    b = wave_sum(b);
-    if (lane) return;
-    const float lam = lambda_of(p, w.b, r);
-    stats[n] = *lse_at(p, const_cast<float*>(lse), w.b, r, 0) * kLog2e;
-    stats[total + n] = *lse_at(p, const_cast<float*>(lse), w.b, r, 1) * kLog2e;
-    stats[2 * total + n] = fmaf(lam, b, a);
-    stats[3 * total + n] = b;
-    stats[4 * total + n] = lam;
-    if (p.token_lam) dlam[((int64_t)w.b * p.t + r.i) * p.h + r.head] = -b;
 }
 
 template <typename T, int NS>
@@ -1488,7 +1493,7 @@ template <typename T, int NS>
 int fwd(nott_ctx ctx, const Params& p, int64_t pairs, const T* q, const T* k, const T* v, T* o, T* o2, float* lse,
         const Parts& parts) {
     constexpr size_t lds = 6 * Dim<T, NS>::X;
-    static bool done = false;
+    static std::atomic<uint64_t> done{0};
     auto f = &diff_fwd_kernel<T, NS>;
     if (const int st = mx::reserve(ctx, f, lds, done); st != NOTT_OK) return st;
     hipLaunchKernelGGL(f, dim3((unsigned)pairs, (unsigned)ceil_div(p.rows, BR), (unsigned)p.nsplit), dim3(kThreads), lds,
@@ -1500,14 +1505,14 @@ template <typename T, int NS>
 int bwd(nott_ctx ctx, const Params& p, int64_t pairs, const T* q, const T* k, const T* v, const T* o, const T* o2, const T* dO,
         const float* lse, float* stats, T* dq, T* dk, T* dv, float* dlam) {
     constexpr size_t lds_q = 8 * Dim<T, NS>::X, lds_kv = lds_q + kStats * BR * sizeof(float);
-    static bool done[2] = {false, false};
+    static std::atomic<uint64_t> done[2];
     auto fq = &diff_dq_kernel<T, NS>;
     auto fk = &diff_dkdv_kernel<T, NS>;
     if (const int st = mx::reserve(ctx, fq, lds_q, done[0]); st != NOTT_OK) return st;
     if (const int st = mx::reserve(ctx, fk, lds_kv, done[1]); st != NOTT_OK) return st;
     const int64_t total = pairs * p.rows;
-    hipLaunchKernelGGL(diff_stats_kernel<T>, dim3((unsigned)ceil_div(total, 4)), dim3(256), 0, ctx->stream, o, o2, dO, lse, stats,
-                       dlam, total, p);
+    hipLaunchKernelGGL(diff_stats_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(total, 4), kMostBlocks)), dim3(256), 0,
+                       ctx->stream, o, o2, dO, lse, stats, dlam, total, p);
     hipLaunchKernelGGL(fq, dim3((unsigned)pairs, (unsigned)ceil_div(p.rows, BR)), dim3(kThreads), lds_q, ctx->stream, q, k, v,
                        dO, stats, dq, total, p);
     hipLaunchKernelGGL(fk, dim3((unsigned)pairs, (unsigned)ceil_div(p.s, BR)), dim3(kThreads), lds_kv, ctx->stream, q, k, v, dO,
@@ -1572,22 +1577,23 @@ int slices_for(const Params& p, int sl) {
 __global__ __launch_bounds__(256) void diff_zero_kernel(uint16_t* __restrict__ p16, float* __restrict__ p32, int64_t n,
                                                         int64_t rows, int64_t heads, int64_t width, int64_t sb, int64_t st,
                                                         int64_t sh, float value) {
-    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const int64_t d = i % width;
-    i /= width;
-    const int64_t hd = i % heads;
-    i /= heads;
-    const int64_t at = i / rows * sb + i % rows * st + hd * sh + d;
-    if (p16) p16[at] = 0;
-    else p32[at] = value;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < n; x += (int64_t)gridDim.x * 256) {
+        int64_t i = x;
+        const int64_t d = i % width;
+        i /= width;
+        const int64_t hd = i % heads;
+        i /= heads;
+        const int64_t at = i / rows * sb + i % rows * st + hd * sh + d;
+        if (p16) p16[at] = 0;
+        else p32[at] = value;
+    }
 }
 int fill(nott_ctx ctx, nott_dtype dtype, void* dst, int64_t b, int64_t rows, int64_t heads, int64_t width,
          const int64_t (&st)[3], float value = 0.f) {
     const int64_t n = b * rows * heads * width;
     if (n == 0) return NOTT_OK;
     NOTT_REQUIRE(ctx, dst != nullptr, "differential attention: null buffer");
-    hipLaunchKernelGGL(diff_zero_kernel, dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, ctx->stream,
+    hipLaunchKernelGGL(diff_zero_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(n, 256), kMostBlocks)), dim3(256), 0, ctx->stream,
                        dtype == NOTT_BF16 ? static_cast<uint16_t*>(dst) : nullptr,
                        dtype == NOTT_BF16 ? nullptr : static_cast<float*>(dst), n, rows, heads, width, st[0], st[1], st[2], value);
     return launch_status(ctx, "diff_zero_kernel");
