@@ -230,8 +230,11 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict
     o[p.rows] = tb;
 }
 
+// (bf16: 128 registers, so that two workgroups share a CU where there are as many: 16 x 1024
+// tokens of 2048 channels 51.6 us for 58.4, 1 x 16384 79 for 87; in fp32 and for unaligned
+// rows that spills, 79 for 45 and 148 for 75)
 template <typename T, int VEC, int CH, bool SIG, bool MIX>
-__global__ __launch_bounds__(kThreads) void scan_fwd_kernel(const T* __restrict__ x, const T* __restrict__ gate,
+__global__ __launch_bounds__(kThreads, VEC == 8 ? 4 : 2) void scan_fwd_kernel(const T* __restrict__ x, const T* __restrict__ gate,
                                                             const float* __restrict__ h0,
                                                             const uint8_t* __restrict__ reset,
                                                             const float* __restrict__ agg, T* __restrict__ h,
