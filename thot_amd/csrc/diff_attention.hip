@@ -1714,14 +1714,19 @@ extern "C" int nott_diff_attention_bwd(nott_ctx ctx, const nott_diff_attn_desc* 
     const int elem = (int)nott::dtype_size(dtype);
     p.vec = even16(q, p.q, elem) && even16(k, p.k, elem) && even16(v, p.v, elem) && even16(dO, p.od, elem);
     const int64_t pairs = d->b * d->hk, total = pairs * p.rows;
-    // Fewer key blocks than CUs: the rows are split, if the parts find room (a share of
-    // 32·32 rows at the least).
+    // Fewer key blocks than CUs: the rows are split, if the parts find room.  One workgroup a
+    // CU with shares of 128 rows or more (3 x 105 tokens of 8 heads on 2, 128 + 256 columns 121
+    // -> 84 us; 1024 tokens of 16 heads on 4, 279 -> 219, with two a CU 248; 256 tokens of 8
+    // heads on 2, 64 + 128, 97 -> 48); causal blocks differ in length, and up to three for two CUs
+    // even that out where shares keep 2048 rows (4096 tokens 1529 us with one, 1365 with 1.5,
+    // 1416 with two).
     const bool fast = dtype == NOTT_BF16 && p.vec && p.dh % 8 == 0 && p.dv % 8 == 0 && even16(o, p.o, 2) && (uintptr_t)o2 % 16 == 0;
     const size_t stat_bytes = ((size_t)total * kStats * sizeof(float) + 255) & ~size_t(255);
     const int64_t key_blocks = pairs * ceil_div(p.s, mx::FIXED);
     float *stats = nullptr, *parts = nullptr;
-    if (fast && key_blocks < ctx->num_cu && p.rows >= 2048) {
-        const int64_t n = std::min<int64_t>(ceil_div(2 * ctx->num_cu, key_blocks), p.rows / 1024);
+    const int64_t one = std::min<int64_t>(ctx->num_cu / key_blocks, p.rows / 128);
+    const int64_t n = p.causal ? std::max<int64_t>(one, std::min<int64_t>(ctx->num_cu * 3 / 2 / key_blocks, p.rows / 2048)) : one;
+    if (fast && n > 1) {
         const size_t bytes = (size_t)n * pairs * p.s * (2 * p.dh + p.dv) * sizeof(float);
         if (char* ws = static_cast<char*>(nott::optional_workspace(ctx, stat_bytes + bytes))) {
             stats = reinterpret_cast<float*>(ws);
