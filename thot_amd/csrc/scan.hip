@@ -22,7 +22,7 @@
 // A keep of exactly 0 forgets the state whatever it was, an infinity or NaN as well.
 //
 // Bound by HBM (3 streams forward, 5 backward): 4 x 4096 tokens of 2048 channels in bf16
-// take 55 us forward (3.7 TB/s) and 98 backward (3.4 TB/s); a packed batch of 50001 tokens
+// take 56 us forward (3.6 TB/s) and 98 backward (3.4 TB/s); a packed batch of 50001 tokens
 // of 520 channels in fp32 178 us backward (41 of them for the segments' maps; 4.0 TB/s over
 // its 7 streams).  A token's row holds 64 to 256 bytes of a workgroup, so neighbouring
 // blocks of channels share pages and lines of memory: they run on one XCD, side by side
@@ -85,6 +85,9 @@ __device__ __forceinline__ void gates(float g, float& a, float& take) {
 // A·s + B; A = 0 forgets s.
 __device__ __forceinline__ float step(float A, float s, float B) { return A == 0.f ? B : fmaf(A, s, B); }
 
+// Of two maps in a row: 0 where either forgets, beside an infinity or a NaN as well.
+__device__ __forceinline__ float both(float A, float B) { return A == 0.f || B == 0.f ? 0.f : A * B; }
+
 // Keeps the compiler from holding what it formed from x before (an unpacked copy, a
 // product) beside x.
 template <typename X>
@@ -138,7 +141,7 @@ struct Fold {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             cb = step(a[i], cb, b[i]);
-            ca *= a[i];
+            ca = both(ca, a[i]);
         }
         M[0][q][ch] = ca;
         M[1][q][ch] = cb;
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict
                 gates<SIG, MIX>(vg[v], a, take);
                 a = fresh[u] ? 0.f : a;
                 B[v] = REVERSE ? (a == 0.f ? 0.f : a * (vx[v] + B[v])) : step(a, B[v], take * vx[v]);
-                A[v] *= a;
+                A[v] = both(A[v], a);
             }
         }
     }
@@ -223,7 +226,7 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict
     for (int g = 0; g < P::G; ++g) {
         const int i = REVERSE ? P::G - 1 - g : g;
         tb = step(sA[i][threadIdx.x], tb, sB[i][threadIdx.x]);
-        ta *= sA[i][threadIdx.x];
+        ta = both(ta, sA[i][threadIdx.x]);
     }
     float* o = agg + (int64_t)seg * 2 * p.rows + w.b * p.d + ch;
     o[0] = ta;
@@ -306,7 +309,7 @@ __global__ __launch_bounds__(kThreads, VEC == 8 ? 4 : 2) void scan_fwd_kernel(co
                     a[r][v] = r >= live ? 1.f : (fresh >> r) & 1 ? 0.f : a[r][v];
                 }
         }
-        float least = 1.f;
+        bool some = false;      // a product of 0, or what an infinity or a NaN made of one
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
 #pragma unroll
@@ -314,15 +317,19 @@ __global__ __launch_bounds__(kThreads, VEC == 8 ? 4 : 2) void scan_fwd_kernel(co
                 B[v] = fmaf(a[r][v], B[v], u[r][v]);
                 A[v] *= a[r][v];
             }
-            least = fminf(least, __builtin_fabsf(A[v]));
+            some |= !(__builtin_fabsf(A[v]) > 0.f);
         }
-        careful = __any(least == 0.f);
+        careful = __any(some);
         if (careful) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
+                A[v] = 1.f;
                 B[v] = 0.f;
 #pragma unroll
-                for (int r = 0; r < R; ++r) B[v] = step(a[r][v], B[v], u[r][v]);
+                for (int r = 0; r < R; ++r) {
+                    B[v] = step(a[r][v], B[v], u[r][v]);
+                    A[v] = both(A[v], a[r][v]);
+                }
             }
         }
 #pragma unroll
@@ -450,7 +457,7 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
                     const float k = CAREFUL && ((begins >> r) & 1) ? 0.f : a[r][v];
                     const float u = CAREFUL && r >= live ? 0.f : MIX ? take[r][v] * vx[v] : vx[v];
                     B[v] = CAREFUL ? step(k, B[v], u) : fmaf(k, B[v], u);
-                    A[v] *= k;
+                    A[v] = CAREFUL ? both(A[v], k) : A[v] * k;
                 }
             }
 #pragma unroll
@@ -468,10 +475,10 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
         bool careful = reset || tile + kTile > t1;
         if (!careful) {
             maps(std::false_type());
-            float least = 1.f;
+            bool some = false;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) least = fminf(least, __builtin_fabsf(A[v]));
-            careful = __any(least == 0.f);
+            for (int v = 0; v < VEC; ++v) some |= !(__builtin_fabsf(A[v]) > 0.f);
+            careful = __any(some);
         }
         if (careful) maps(std::true_type());
 #pragma unroll
