@@ -1701,10 +1701,9 @@ extern "C" int nott_diff_attention_bwd(nott_ctx ctx, const nott_diff_attn_desc* 
     NOTT_CHECK_CTX(ctx);
     Params p{};
     if (const int st = check(ctx, d, dtype, &p); st != NOTT_OK) return st;
-    if (d->b * d->h == 0) return NOTT_OK;
     nott::DeviceScope scope(ctx->device);
     NOTT_REQUIRE(ctx, !(accumulate && d->token_lam), "nott_diff_attention_bwd: accumulate goes with one lambda a head");
-    if (d->t == 0 || d->s == 0) {
+    if (d->b == 0 || d->h == 0 || d->t == 0 || d->s == 0) {     // nothing was computed; what has elements is zeros
         if (const int st = fill(ctx, dtype, dq, d->b, d->t, 2 * d->h, d->dh, p.dq); st != NOTT_OK) return st;
         if (const int st = fill(ctx, dtype, dk, d->b, d->s, 2 * d->hk, d->dh, p.dk); st != NOTT_OK) return st;
         if (const int st = fill(ctx, dtype, dv, d->b, d->s, d->hk, d->dv, p.dv_); st != NOTT_OK) return st;
