@@ -1,4 +1,5 @@
-"""Differential attention over nothing: an empty batch has a gradient of zero for lambda."""
+"""Differential attention over nothing: an empty batch has a gradient of zero for lambda, keys
+and values that no head reads gradients of zero."""
 import pytest
 import torch
 
@@ -44,3 +45,20 @@ def test_empty_batch_under_autograd(dt):
     spoil_freed_memory()
     host.diff_attention(q, k, v, 2 * base).sum().backward()
     assert not base.grad.any()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("hk", [2, 0])
+def test_no_heads(dt, hk):
+    from thot_amd import _nott_host as host
+    dt = DT[dt]
+    q, k, v, lam = rnd(2, 3, 0, 16, dt=dt), rnd(2, 5, 2 * hk, 16, dt=dt), rnd(2, 5, hk, 32, dt=dt), torch.empty(0, device="cuda")
+    o, lse, o2 = ops.diff_attention_fwd(q, k, v, lam, save=True)
+    assert o.shape == (2, 3, 0, 32) and lse.numel() == 0
+    out = (torch.empty_like(q), torch.full_like(k, 7.0), torch.full_like(v, 7.0))
+    _, dk, dv, dlam = ops.diff_attention_bwd(o, q, k, v, lam, o, o2, lse, out=out)
+    assert not dk.any() and not dv.any() and dlam.numel() == 0
+    k, v = k.requires_grad_(), v.requires_grad_()
+    spoil_freed_memory()
+    host.diff_attention(q, k, v, lam).sum().backward()
+    assert not k.grad.any() and not v.grad.any()

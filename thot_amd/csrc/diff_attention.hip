@@ -1537,7 +1537,7 @@ int check(nott_ctx ctx, const nott_diff_attn_desc* d, nott_dtype dtype, Params* 
                  "differential attention: head dim above 128 (bf16) / 64 (fp32), or values' above twice that, is not supported");
     NOTT_REQUIRE(ctx, d->scale > 0.0 && d->scale < 1e30, "differential attention: scale must be positive");
     NOTT_REQUIRE(ctx, (d->causal | d->token_lam) >> 1 == 0, "differential attention: causal and token_lam are 0 or 1");
-    const int64_t group = d->hk ? d->h / d->hk : 1;
+    const int64_t group = d->h ? d->h / d->hk : 1;      // (without heads nothing is computed, but FastDiv divides by it)
     NOTT_REQUIRE(ctx, d->b * std::max<int64_t>(d->hk, 1) < (int64_t(1) << 23) && d->h < (int64_t(1) << 20) &&
                           d->t * group <= 4000000 && d->s <= 4000000,
                  "differential attention: too many heads or too long a sequence");
