@@ -82,11 +82,32 @@ __device__ __forceinline__ void gates(float g, float& a, float& take) {
     }
 }
 
+// A sigmoid is 0 at −infinity alone: where fp32 does not hold it, it is the least number.
+template <bool SIG>
+__device__ __forceinline__ float opened(float a, float g) {
+    return SIG && a == 0.f && g > -INFINITY ? 0x1p-149f : a;
+}
+
 // A·s + B; A = 0 forgets s.
 __device__ __forceinline__ float step(float A, float s, float B) { return A == 0.f ? B : fmaf(A, s, B); }
+__device__ __forceinline__ float step(double A, float s, float B) { return A == 0.0 ? B : (float)fma(A, (double)s, (double)B); }
 
-// Of two maps in a row: 0 where either forgets, beside an infinity or a NaN as well.
-__device__ __forceinline__ float both(float A, float B) { return A == 0.f || B == 0.f ? 0.f : A * B; }
+// Of two maps in a row: 0 where either forgets, beside an infinity or a NaN as well, and only
+// there.  A product that fp32 does not hold is its least number (of the product's sign): it
+// takes 2^-149 of a state at most in, and leaves one that is infinite or NaN what it is.
+__device__ __forceinline__ float both(float A, float B) {
+    const float p = A * B;
+    const float least = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p) | 1u);
+    return A == 0.f || B == 0.f ? 0.f : p == 0.f ? least : p;
+}
+// A product over a segment also overflows fp32 (gates above 1 over a thousand tokens, before
+// which a state may be 0).  It is formed in fp64 and brought back into 2^±400 after every
+// four gates (2^±149 at most each): a state times that is 0 or infinite in fp32 all the same.
+__device__ __forceinline__ double within(double A) {
+    const double m = __builtin_fabs(A);
+    const double end = __builtin_copysign(m < 1.0 ? 0x1p-400 : 0x1p400, A);
+    return m < 0x1p-400 || (m > 0x1p400 && m < INFINITY) ? end : A;     // (an infinite gate's stays infinite, NaN NaN)
+}
 
 // Keeps the compiler from holding what it formed from x before (an unpacked copy, a
 // product) beside x.
@@ -166,13 +187,22 @@ struct Fold {
 };
 
 // Maps of whole segments, for the segments that follow (forward) or precede (reverse):
-// agg [nseg][2][b·d].  A span is a run of the segment's tokens, gone through in registers.
+// A in fp64 [nseg][b·d], then B in fp32 [nseg][b·d].  A span is a run of the segment's
+// tokens, gone through in registers.
+struct Maps {
+    double* a;
+    float* b;
+    // The state behind segment g.
+    __device__ __forceinline__ float after(int64_t g, int64_t rows, int64_t row, float s) const {
+        return step(a[g * rows + row], s, b[g * rows + row]);
+    }
+};
 template <typename T, int VEC, int CH, bool SIG, bool MIX, bool REVERSE>
 __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict__ x, const T* __restrict__ gate,
-                                                             const uint8_t* __restrict__ reset, float* __restrict__ agg,
-                                                             Params p) {
+                                                             const uint8_t* __restrict__ reset, Maps agg, Params p) {
     typedef Place<VEC, CH> P;
-    __shared__ __attribute__((aligned(16))) float sA[P::G][CH], sB[P::G][CH];
+    __shared__ __attribute__((aligned(16))) double sA[P::G][CH];
+    __shared__ __attribute__((aligned(16))) float sB[P::G][CH];
     const P w(p);
     const int seg = REVERSE ? w.seg + 1 : w.seg;
     const int64_t t0 = seg * p.seg, t1 = min(p.t, t0 + p.seg);
@@ -181,11 +211,14 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict
     const T* px = x + w.b * (REVERSE ? p.hb : p.xb) + w.cc;      // (reverse: dh in x's place)
     const T* pg = gate + w.b * p.gb + w.cc;
     const int64_t xt = REVERSE ? p.ht : p.xt;
-    float A[VEC], B[VEC];
+    double A[VEC];
+    float B[VEC];
+    bool forgot[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        A[v] = 1.f;
+        A[v] = 1.0;
         B[v] = 0.f;
+        forgot[v] = false;
     }
     constexpr int U = VEC == 1 ? 8 : 4;
     for (int64_t q = r0; q < r1; q += U) {
@@ -208,29 +241,34 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict
             for (int v = 0; v < VEC; ++v) {
                 float a, take;
                 gates<SIG, MIX>(vg[v], a, take);
-                a = fresh[u] ? 0.f : a;
+                a = fresh[u] ? 0.f : opened<SIG>(a, vg[v]);
                 B[v] = REVERSE ? (a == 0.f ? 0.f : a * (vx[v] + B[v])) : step(a, B[v], take * vx[v]);
-                A[v] = both(A[v], a);
+                A[v] *= (double)a;
+                forgot[v] |= a == 0.f;
+                if (u % 4 == 3) A[v] = within(A[v]);
             }
         }
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        sA[w.span][w.lane * VEC + v] = A[v];
+        sA[w.span][w.lane * VEC + v] = forgot[v] ? 0.0 : within(A[v]);
         sB[w.span][w.lane * VEC + v] = B[v];
     }
     __syncthreads();
     const int ch = w.block * CH + threadIdx.x;
     if (threadIdx.x >= CH || ch >= p.d) return;
-    float ta = 1.f, tb = 0.f;
+    double ta = 1.0;
+    float tb = 0.f;
+#pragma unroll 4
     for (int g = 0; g < P::G; ++g) {
         const int i = REVERSE ? P::G - 1 - g : g;
-        tb = step(sA[i][threadIdx.x], tb, sB[i][threadIdx.x]);
-        ta = both(ta, sA[i][threadIdx.x]);
+        const double a = sA[i][threadIdx.x];
+        tb = step(a, tb, sB[i][threadIdx.x]);
+        ta = ta == 0.0 || a == 0.0 ? 0.0 : within(ta * a);
     }
-    float* o = agg + (int64_t)seg * 2 * p.rows + w.b * p.d + ch;
-    o[0] = ta;
-    o[p.rows] = tb;
+    const int64_t at = (int64_t)seg * p.rows + w.b * p.d + ch;
+    agg.a[at] = ta;
+    agg.b[at] = tb;
 }
 
 // (bf16: 128 registers, so that two workgroups share a CU where there are as many: 16 x 1024
@@ -240,7 +278,7 @@ template <typename T, int VEC, int CH, bool SIG, bool MIX>
 __global__ __launch_bounds__(kThreads, VEC == 8 ? 4 : 2) void scan_fwd_kernel(const T* __restrict__ x, const T* __restrict__ gate,
                                                             const float* __restrict__ h0,
                                                             const uint8_t* __restrict__ reset,
-                                                            const float* __restrict__ agg, T* __restrict__ h,
+                                                            Maps agg, T* __restrict__ h,
                                                             float* __restrict__ last, float* __restrict__ states, Params p) {
     typedef Place<VEC, CH> P;
     typedef typename Row<T, VEC>::Raw Raw;
@@ -260,7 +298,7 @@ __global__ __launch_bounds__(kThreads, VEC == 8 ? 4 : 2) void scan_fwd_kernel(co
     const int64_t row = w.b * p.d + ch;
     if (mine) {
         float s = h0 ? h0[row] : 0.f;
-        for (int g = 0; g < seg; ++g) s = step(agg[(int64_t)g * 2 * p.rows + row], s, agg[((int64_t)g * 2 + 1) * p.rows + row]);
+        for (int g = 0; g < seg; ++g) s = agg.after(g, p.rows, row, s);
         carry[0][fold.ch] = s;
     }
     Raw rx[R], rg[R];
@@ -321,6 +359,16 @@ __global__ __launch_bounds__(kThreads, VEC == 8 ? 4 : 2) void scan_fwd_kernel(co
         }
         careful = __any(some);
         if (careful) {
+            if (SIG) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    float vg[VEC];
+                    Row<T, VEC>::floats(rg[r], vg);
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v)
+                        if (!((fresh >> r) & 1)) a[r][v] = opened<SIG>(a[r][v], vg[v]);
+                }
+            }
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 A[v] = 1.f;
@@ -371,7 +419,7 @@ template <typename T, int VEC, int CH, bool SIG, bool MIX>
 __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict__ dh, const T* __restrict__ x,
                                                             const T* __restrict__ gate, const uint8_t* __restrict__ reset,
                                                             const float* __restrict__ states,
-                                                            const float* __restrict__ dlast, const float* __restrict__ agg,
+                                                            const float* __restrict__ dlast, Maps agg,
                                                             T* __restrict__ dx, T* __restrict__ dgate,
                                                             float* __restrict__ dh0, Params p) {
     typedef Place<VEC, CH> P;
@@ -395,8 +443,7 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
     const bool mine = q == 0 && ch < p.d;
     if (mine) {
         float s = dlast ? dlast[row] : 0.f;
-        for (int g = p.nseg - 1; g > seg; --g)
-            s = step(agg[(int64_t)g * 2 * p.rows + row], s, agg[((int64_t)g * 2 + 1) * p.rows + row]);
+        for (int g = p.nseg - 1; g > seg; --g) s = agg.after(g, p.rows, row, s);
         carry[0][fold_ch] = s;
     }
     int buf = 0;
@@ -449,11 +496,12 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                float vx[VEC];
+                float vx[VEC], vg[VEC];
                 Row<T, VEC>::floats(ex[r], vx);
+                Row<T, VEC>::floats(rg[r], vg);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    if (CAREFUL) a[r][v] = r >= live ? 1.f : a[r][v];
+                    if (CAREFUL) a[r][v] = r >= live ? 1.f : opened<SIG>(a[r][v], vg[v]);
                     const float k = CAREFUL && ((begins >> r) & 1) ? 0.f : a[r][v];
                     const float u = CAREFUL && r >= live ? 0.f : MIX ? take[r][v] * vx[v] : vx[v];
                     B[v] = CAREFUL ? step(k, B[v], u) : fmaf(k, B[v], u);
@@ -583,7 +631,7 @@ __global__ __launch_bounds__(64) void scan_steps_kernel(const T* __restrict__ x,
         for (int v = 0; v < VEC; ++v) {
             float a, take;
             gates<SIG, MIX>(vg[v], a, take);
-            s[v] = step(begins ? 0.f : a, s[v], take * vx[v]);
+            s[v] = step(begins ? 0.f : opened<SIG>(a, vg[v]), s[v], take * vx[v]);
         }
         Row<T, VEC>::store(h + b * p.hb + t * p.ht + c, s);
     }
@@ -633,12 +681,19 @@ int check(nott_ctx ctx, const nott_scan_desc* d, nott_dtype dtype, Params* p) {
 
 // Segments: one where the channels alone give half of the CUs a workgroup, else as many as
 // bring two for each, of at least 4 tiles.
-void segments(nott_ctx ctx, Params* p, int64_t blocks) {
+Maps segments(nott_ctx ctx, Params* p, int64_t blocks) {
     const int64_t tiles = p->nchunk;
     int64_t n = blocks >= ctx->num_cu / 2 ? 1 : std::min<int64_t>(ceil_div(2 * ctx->num_cu, blocks), ceil_div(tiles, 4));
     const int64_t len = ceil_div(tiles, n);
     p->seg = len * kTile;
     p->nseg = (int32_t)ceil_div(tiles, len);
+    if (p->nseg == 1) return {};
+    const int64_t maps = p->nseg * p->rows;
+    if (auto* a = static_cast<double*>(nott::optional_workspace(ctx, (size_t)maps * (sizeof(double) + sizeof(float)))))
+        return {a, reinterpret_cast<float*>(a + maps)};
+    p->nseg = 1;
+    p->seg = tiles * kTile;
+    return {};
 }
 
 // Channels of a workgroup: 64 in fp32 rows of 16-byte groups, else 32, whose half as
@@ -661,13 +716,8 @@ int fwd(nott_ctx ctx, Params& p, const void* x, const void* gate, const float* h
     }
     constexpr int CH = kChannels<VEC>;
     p.nblk = (int32_t)ceil_div(p.d, CH);
-    segments(ctx, &p, batches * p.nblk);
+    const Maps agg = segments(ctx, &p, batches * p.nblk);
     const dim3 grid((unsigned)(batches * p.nblk));
-    float* agg = nullptr;
-    if (p.nseg > 1) {
-        agg = static_cast<float*>(nott::optional_workspace(ctx, (size_t)p.nseg * 2 * p.rows * sizeof(float)));
-        if (!agg) p.nseg = 1, p.seg = (int64_t)p.nchunk * kTile;
-    }
     if (p.nseg > 1)
         hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CH, SIG, MIX, false>), dim3(grid.x, (unsigned)(p.nseg - 1)), dim3(kThreads),
                            0, ctx->stream, tx, tg, reset, agg, p);
@@ -683,13 +733,8 @@ int bwd(nott_ctx ctx, Params& p, const void* dh, const void* x, const void* gate
     const T* tg = static_cast<const T*>(gate);
     constexpr int CH = kChannels<VEC>;
     p.nblk = (int32_t)ceil_div(p.d, CH);
-    segments(ctx, &p, p.rows / p.d * p.nblk);
+    const Maps agg = segments(ctx, &p, p.rows / p.d * p.nblk);
     const dim3 grid((unsigned)(p.rows / p.d * p.nblk));
-    float* agg = nullptr;
-    if (p.nseg > 1) {
-        agg = static_cast<float*>(nott::optional_workspace(ctx, (size_t)p.nseg * 2 * p.rows * sizeof(float)));
-        if (!agg) p.nseg = 1, p.seg = (int64_t)p.nchunk * kTile;
-    }
     if (p.nseg > 1)
         hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CH, SIG, false, true>), dim3(grid.x, (unsigned)(p.nseg - 1)),
                            dim3(kThreads), 0, ctx->stream, te, tg, reset, agg, p);
