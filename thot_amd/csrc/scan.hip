@@ -101,12 +101,14 @@ __device__ __forceinline__ float both(float A, float B) {
     return A == 0.f || B == 0.f ? 0.f : p == 0.f ? least : p;
 }
 // A product over a segment also overflows fp32 (gates above 1 over a thousand tokens, before
-// which a state may be 0).  It is formed in fp64 and brought back into 2^±400 after every
-// four gates (2^±149 at most each): a state times that is 0 or infinite in fp32 all the same.
+// which a state may be 0).  It is formed in fp64, its exponent brought back into ±400 after
+// every four gates (2^±149 at most each): a state times that is 0 or infinite in fp32 all the
+// same.  An infinite gate's stays infinite, NaN NaN; of a product of 0 the caller takes care.
 __device__ __forceinline__ double within(double A) {
-    const double m = __builtin_fabs(A);
-    const double end = __builtin_copysign(m < 1.0 ? 0x1p-400 : 0x1p400, A);
-    return m < 0x1p-400 || (m > 0x1p400 && m < INFINITY) ? end : A;     // (an infinite gate's stays infinite, NaN NaN)
+    uint64_t bits = __builtin_bit_cast(uint64_t, A);
+    const int e = (int)(bits >> 52) & 0x7ff, to = e == 0x7ff ? e : max(1023 - 400, min(1023 + 400, e));
+    bits = (bits & ~(uint64_t(0x7ff) << 52)) | (uint64_t)to << 52;
+    return __builtin_bit_cast(double, bits);
 }
 
 // Keeps the compiler from holding what it formed from x before (an unpacked copy, a
@@ -201,8 +203,8 @@ template <typename T, int VEC, int CH, bool SIG, bool MIX, bool REVERSE>
 __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict__ x, const T* __restrict__ gate,
                                                              const uint8_t* __restrict__ reset, Maps agg, Params p) {
     typedef Place<VEC, CH> P;
-    __shared__ __attribute__((aligned(16))) double sA[P::G][CH];
-    __shared__ __attribute__((aligned(16))) float sB[P::G][CH];
+    __shared__ __attribute__((aligned(16))) double sA[P::G][CH], mA[P::E][CH];
+    __shared__ __attribute__((aligned(16))) float sB[P::G][CH], mB[P::E][CH];
     const P w(p);
     const int seg = REVERSE ? w.seg + 1 : w.seg;
     const int64_t t0 = seg * p.seg, t1 = min(p.t, t0 + p.seg);
@@ -255,20 +257,37 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict
         sB[w.span][w.lane * VEC + v] = B[v];
     }
     __syncthreads();
-    const int ch = w.block * CH + threadIdx.x;
-    if (threadIdx.x >= CH || ch >= p.d) return;
-    double ta = 1.0;
-    float tb = 0.f;
-#pragma unroll 4
-    for (int g = 0; g < P::G; ++g) {
-        const int i = REVERSE ? P::G - 1 - g : g;
-        const double a = sA[i][threadIdx.x];
-        tb = step(a, tb, sB[i][threadIdx.x]);
-        ta = ta == 0.0 || a == 0.0 ? 0.0 : within(ta * a);
-    }
+    // Folded by all threads, as in Fold below: a thread's share of the spans, then the shares.
+    constexpr int E = P::E, N = P::G / E;
+    const int q = threadIdx.x / CH, c = threadIdx.x % CH, ch = w.block * CH + c;
+    double fa;
+    float fb;
+    auto fold = [&](const auto& a, const auto& b, int first, auto count) {
+        double ka[count];
+        float kb[count];
+#pragma unroll
+        for (int i = 0; i < count; ++i) {
+            ka[i] = a[REVERSE ? first - i : first + i][c];
+            kb[i] = b[REVERSE ? first - i : first + i][c];
+        }
+        fa = ka[0];
+        fb = kb[0];
+#pragma unroll
+        for (int i = 1; i < count; ++i) {
+            fb = step(ka[i], fb, kb[i]);
+            fa = fa == 0.0 || ka[i] == 0.0 ? 0.0 : within(fa * ka[i]);
+        }
+    };
+    fold(sA, sB, REVERSE ? P::G - 1 - q * N : q * N, std::integral_constant<int, N>());
+    const int share = REVERSE ? E - 1 - q : q;
+    mA[share][c] = fa;
+    mB[share][c] = fb;
+    __syncthreads();
+    if (q || ch >= p.d) return;
+    fold(mA, mB, REVERSE ? E - 1 : 0, std::integral_constant<int, E>());
     const int64_t at = (int64_t)seg * p.rows + w.b * p.d + ch;
-    agg.a[at] = ta;
-    agg.b[at] = tb;
+    agg.a[at] = fa;
+    agg.b[at] = fb;
 }
 
 // (bf16: 128 registers, so that two workgroups share a CU where there are as many: 16 x 1024
@@ -496,12 +515,11 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                float vx[VEC], vg[VEC];
+                float vx[VEC];
                 Row<T, VEC>::floats(ex[r], vx);
-                Row<T, VEC>::floats(rg[r], vg);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    if (CAREFUL) a[r][v] = r >= live ? 1.f : opened<SIG>(a[r][v], vg[v]);
+                    if (CAREFUL) a[r][v] = r >= live ? 1.f : a[r][v];
                     const float k = CAREFUL && ((begins >> r) & 1) ? 0.f : a[r][v];
                     const float u = CAREFUL && r >= live ? 0.f : MIX ? take[r][v] * vx[v] : vx[v];
                     B[v] = CAREFUL ? step(k, B[v], u) : fmaf(k, B[v], u);
@@ -527,6 +545,24 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
 #pragma unroll
             for (int v = 0; v < VEC; ++v) some |= !(__builtin_fabsf(A[v]) > 0.f);
             careful = __any(some);
+        }
+        if (careful && SIG) {
+            bool shut = false;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) shut |= a[r][v] == 0.f;
+            // (in fp32 the gates are read again for it, since no registers are left to keep them:
+            // 4 x 4096 tokens of 2048 channels 200 us, 222 with spills)
+            if (__any(shut)) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    float vg[VEC];
+                    Row<T, VEC>::floats(VEC == 4 ? Row<T, VEC>::load(pg + min(p.t - 1, tile + w.span * R + r) * p.gt) : rg[r], vg);
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) a[r][v] = opened<SIG>(a[r][v], vg[v]);
+                }
+            }
         }
         if (careful) maps(std::true_type());
 #pragma unroll
