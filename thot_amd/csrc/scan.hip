@@ -67,18 +67,18 @@ struct Params {
     int64_t xb, xt, gb, gt, hb, ht, dxb, dxt, dgb, dgt;   // batch and token strides
 };
 
-// a and what multiplies the input.  From e^−|g|, so that neither overflows: infinities
-// give exactly 0 and 1.
-template <bool SIG, bool MIX>
-__device__ __forceinline__ void gates(float g, float& a, float& take) {
+// a and 1 − a.  A sigmoid's both come from e^−|g|, so that neither overflows (infinities
+// give exactly 0 and 1) and each keeps its bits where it is small.
+template <bool SIG>
+__device__ __forceinline__ void gates(float g, float& a, float& rest) {
     if constexpr (SIG) {
         const float t = __builtin_amdgcn_exp2f(__builtin_fabsf(g) * -1.4426950f), big = __builtin_amdgcn_rcpf(1.f + t);
         const float small = t * big;
         a = g < 0.f ? small : big;
-        take = MIX ? (g < 0.f ? big : small) : 1.f;
+        rest = g < 0.f ? big : small;
     } else {
         a = g;
-        take = MIX ? 1.f - g : 1.f;
+        rest = 1.f - g;
     }
 }
 
@@ -241,10 +241,10 @@ __global__ __launch_bounds__(kThreads) void scan_maps_kernel(const T* __restrict
             Row<T, VEC>::floats(rg[u], vg);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                float a, take;
-                gates<SIG, MIX>(vg[v], a, take);
+                float a, rest;
+                gates<SIG>(vg[v], a, rest);
                 a = fresh[u] ? 0.f : opened<SIG>(a, vg[v]);
-                B[v] = REVERSE ? (a == 0.f ? 0.f : a * (vx[v] + B[v])) : step(a, B[v], take * vx[v]);
+                B[v] = REVERSE ? (a == 0.f ? 0.f : a * (vx[v] + B[v])) : step(a, B[v], MIX ? rest * vx[v] : vx[v]);
                 A[v] *= (double)a;
                 forgot[v] |= a == 0.f;
                 if (u % 4 == 3) A[v] = within(A[v]);
@@ -352,9 +352,9 @@ __global__ __launch_bounds__(kThreads, VEC == 8 ? 4 : 2) void scan_fwd_kernel(co
             Row<T, VEC>::floats(rg[r], vg);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                float take;
-                gates<SIG, MIX>(vg[v], a[r][v], take);
-                u[r][v] = take * vx[v];
+                float rest;
+                gates<SIG>(vg[v], a[r][v], rest);
+                u[r][v] = MIX ? rest * vx[v] : vx[v];
             }
         }
         if (careful) {
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
         const int live = (int)min<int64_t>(R, t1 - tile - w.span * R);     // tokens of the span that are there
         uint32_t begins = fresh;
         float a[R][VEC], A[VEC], B[VEC], C[VEC];
-        float take[MIX ? R : 1][VEC];
+        float rest[SIG || MIX ? R : 1][VEC];      // 1 − a
         Raw ex[R], ee[R];       // x and dh as loaded: half the registers in bf16
         const float before = ch < p.d ? states[(w.b * p.nchunk + tile / kTile) * p.d + ch] : 0.f;
 #pragma unroll
@@ -500,9 +500,9 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
             Row<T, VEC>::floats(rg[r], vg);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                float tk;
-                gates<SIG, MIX>(vg[v], a[r][v], tk);
-                if constexpr (MIX) take[r][v] = tk;
+                float rs;
+                gates<SIG>(vg[v], a[r][v], rs);
+                if constexpr (SIG || MIX) rest[r][v] = rs;
             }
         }
         // The span's maps; CAREFUL as in the forward.
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
                 for (int v = 0; v < VEC; ++v) {
                     if (CAREFUL) a[r][v] = r >= live ? 1.f : a[r][v];
                     const float k = CAREFUL && ((begins >> r) & 1) ? 0.f : a[r][v];
-                    const float u = CAREFUL && r >= live ? 0.f : MIX ? take[r][v] * vx[v] : vx[v];
+                    const float u = CAREFUL && r >= live ? 0.f : MIX ? rest[r][v] * vx[v] : vx[v];
                     B[v] = CAREFUL ? step(k, B[v], u) : fmaf(k, B[v], u);
                     A[v] = CAREFUL ? both(A[v], k) : A[v] * k;
                 }
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
         const int64_t mt = tile + w.span * R;
         auto gradients = [&](auto which) {
             constexpr bool CAREFUL = decltype(which)::value;
-            float held[R][VEC];     // what e is multiplied by in da: the state before the token [− x]
+            float held[R][VEC];     // what e is multiplied by in dgate: the state before the token [− x] [times σ′]
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 float vx[VEC];
@@ -606,8 +606,9 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
                 const bool b = CAREFUL && ((begins >> r) & 1);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    const float u = MIX ? take[r][v] * vx[v] : vx[v];
+                    const float u = MIX ? rest[r][v] * vx[v] : vx[v];
                     held[r][v] = (b ? 0.f : B[v]) - (MIX ? vx[v] : 0.f);
+                    if constexpr (SIG) held[r][v] *= a[r][v] * rest[r][v];
                     B[v] = CAREFUL ? step(b ? 0.f : a[r][v], B[v], u) : fmaf(a[r][v], B[v], u);
                 }
             }
@@ -621,10 +622,8 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(const T* __restrict_
                     const float k = b ? 0.f : a[r][v];
                     const float e = (CAREFUL && r >= live ? 0.f : ve[v]) + C[v];
                     C[v] = CAREFUL && k == 0.f ? 0.f : k * e;
-                    ox[v] = MIX ? take[r][v] * e : e;
-                    float da = held[r][v];
-                    if constexpr (SIG) da *= MIX ? a[r][v] * take[r][v] : a[r][v] * (1.f - a[r][v]);
-                    og[v] = da * e;
+                    ox[v] = MIX ? rest[r][v] * e : e;
+                    og[v] = held[r][v] * e;
                 }
                 if (w.in && (!CAREFUL || r < live)) {
                     Row<T, VEC>::store(dx + w.b * p.dxb + (mt + r) * p.dxt + w.c, ox);
@@ -665,9 +664,9 @@ __global__ __launch_bounds__(64) void scan_steps_kernel(const T* __restrict__ x,
         const bool begins = reset && reset[b * p.t + t];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            float a, take;
-            gates<SIG, MIX>(vg[v], a, take);
-            s[v] = step(begins ? 0.f : opened<SIG>(a, vg[v]), s[v], take * vx[v]);
+            float a, rest;
+            gates<SIG>(vg[v], a, rest);
+            s[v] = step(begins ? 0.f : opened<SIG>(a, vg[v]), s[v], MIX ? rest * vx[v] : vx[v]);
         }
         Row<T, VEC>::store(h + b * p.hb + t * p.ht + c, s);
     }
