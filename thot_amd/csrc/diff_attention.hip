@@ -90,7 +90,9 @@ __device__ __forceinline__ float lambda_of(const Params& p, int b, const RowAt& 
 __device__ __forceinline__ float* lse_at(const Params& p, float* lse, int b, const RowAt& r, int map) {
     return lse + ((int64_t)b * 2 * p.h + 2 * r.head + map) * p.t + r.i;
 }
-__device__ __forceinline__ float log_sum(float m, float l) { return l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY; }
+// Of a row's sum l: 0 where it sees no key; NaN (of a NaN score) stays NaN.
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // Rows' statistics that the dq pass hands to the dk/dv pass, [kStats][b·hk][rows]:
 // log2(e)·lse of both maps, D_1, D_2, λ.
@@ -158,7 +160,7 @@ __global__ __launch_bounds__(64 * WAVES) void diff_join_kernel(Parts parts, T* _
 #pragma unroll
         for (int c = 0; c < 4; ++c) sum[wid][k][lane + 64 * c] = acc[k][c];
     __syncthreads();
-    const float i1 = l[0] > 0.f ? 1.f / l[0] : 0.f, i2 = l[1] > 0.f ? 1.f / l[1] : 0.f;
+    const float i1 = inverse(l[0]), i2 = inverse(l[1]);
     for (int d = threadIdx.x; d < p.dv; d += 64 * WAVES) {
         float of[2];
 #pragma unroll
@@ -530,7 +532,7 @@ __global__ __launch_bounds__(128 * NW, 2) void diff_fwd32_kernel(const bf16_t* _
     }
     l += __shfl_xor(l, 32, 64);
     const bool in = my_r < p.rows;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = inverse(l);
     if (in && h == 0) *lse_at(p, lse, w.b, r, map) = log_sum(m, l);
     float* second = reinterpret_cast<float*>(smem_raw) + (wr * NV << 10) + lane;   // [NV][16][64] of a row block
     __syncthreads();
@@ -1222,7 +1224,7 @@ __global__ __launch_bounds__(kThreads) void diff_fwd_kernel(const T* __restrict_
         }
         return;
     }
-    const float i1 = ll[0] > 0.f ? 1.f / ll[0] : 0.f, i2 = ll[1] > 0.f ? 1.f / ll[1] : 0.f;
+    const float i1 = inverse(ll[0]), i2 = inverse(ll[1]);
     const float lam = lambda_of(p, w.b, r);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
