@@ -127,7 +127,9 @@ class AdamMoments:
     says which), `scale` (fp32 [blocks, 2]) what they are multiplied by.  bits=32: `m` and
     `v` are the moments in fp32, laid out alike, and `scale` is None.  `copies`: a bf16
     tensor for each parameter (or None) that every step writes the new values to.  m, v and
-    scale may be given (a loaded state); they are kept, not copied."""
+    scale may be given (a loaded state); they are kept, not copied.  Parameters, copies and
+    moments may get other storage, or be replaced by tensors of the same shape and type,
+    between steps: the next step checks them again."""
     BLOCK = 256
 
     def __init__(self, params, *, bits: int = 8, copies=None, m: Optional[torch.Tensor] = None,
@@ -141,40 +143,67 @@ class AdamMoments:
         if len(self.copies) != len(self.params):
             raise ValueError(f"{len(self.copies)} copies for {len(self.params)} parameters")
         self.bits, self.device = bits, self.params[0].device
-        self.first, blocks = [], 0
-        for i, (p, c) in enumerate(zip(self.params, self.copies)):
+        self.first, self._blocks = [], 0
+        for i, p in enumerate(self.params):
             nott_dtype(p.dtype)
-            _check(p, f"params[{i}]", device=self.device)
-            if c is not None:
-                _check(c, f"copies[{i}]", shape=p.shape, dtype=torch.bfloat16, device=self.device)
-            self.first.append(blocks)
-            blocks += -(-p.numel() // self.BLOCK)
-        spans = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in (*self.params, *self.copies)
-                       if t is not None and t.numel())
-        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
-            raise ValueError("params and copies must not overlap")
+            _check(p, f"params[{i}]")
+            self.first.append(self._blocks)
+            self._blocks += -(-p.numel() // self.BLOCK)
+        self._meta = [(p.numel(), p.shape) for p in self.params]
         dt = torch.float8_e4m3fn if bits == 8 else torch.float32
-        self.m, self.v = (self._held(t, nm, (blocks, self.BLOCK), dt) for t, nm in ((m, "m"), (v, "v")))
         if bits == 32 and scale is not None:
             raise ValueError("scale goes with bits=8")
-        self.scale = self._held(scale, "scale", (blocks, 2), torch.float32) if bits == 8 else None
-        if any(t is not None and t.data_ptr() % 16 for t in (self.m, self.v, self.scale)):
-            raise ValueError("m, v and scale must be 16-byte aligned")
-        self._meta = [(p.numel(), p.shape) for p in self.params]
-        # AdamTensor's words: what changes from step to step (p, g) is written by the step
-        row = self.BLOCK * self.m.element_size()
+        self.m, self.v = self._held(m, self.BLOCK, dt), self._held(v, self.BLOCK, dt)
+        self.scale = self._held(scale, 2, torch.float32) if bits == 8 else None
+        # AdamTensor's words: what changes from step to step is written by the step
         self._words = array.array("Q", bytes(64 * len(self.params)))
-        self._words[2::8] = array.array("Q", [self.m.data_ptr() + row * f for f in self.first])
-        self._words[3::8] = array.array("Q", [self.v.data_ptr() + row * f for f in self.first])
-        if bits == 8:
-            self._words[4::8] = array.array("Q", [self.scale.data_ptr() + 8 * f for f in self.first])
         self._words[6::8] = array.array("Q", [p.numel() for p in self.params])
+        self._admit(self.params)
 
-    def _held(self, t: Optional[torch.Tensor], name: str, shape, dtype) -> torch.Tensor:
-        if t is None:
-            return torch.zeros(shape, dtype=torch.uint8 if dtype.itemsize == 1 else dtype, device=self.device).view(dtype)
-        _check(t, name, shape=shape, dtype=dtype, device=self.device)
-        return t
+    def _admit(self, grads) -> None:
+        """Checks the moments and the parameters that have a gradient, and takes the addresses;
+        the step does so again when one of them has moved."""
+        spans = []
+        for i, (p, c, g, (_, shape)) in enumerate(zip(self.params, self.copies, grads, self._meta)):
+            if g is None:
+                continue
+            nott_dtype(p.dtype)
+            _check(p, f"params[{i}]", shape=shape, device=self.device)
+            if c is not None:
+                _check(c, f"copies[{i}]", shape=shape, dtype=torch.bfloat16, device=self.device)
+            spans += [(t.data_ptr(), t.numel() * t.element_size()) for t in (p, c) if t is not None and t.numel()]
+        spans.sort()
+        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+            raise ValueError("params and copies must not overlap")
+        dt = torch.float8_e4m3fn if self.bits == 8 else torch.float32
+        held = [(self.m, "m", self.BLOCK, dt), (self.v, "v", self.BLOCK, dt), (self.scale, "scale", 2, torch.float32)]
+        for t, nm, width, ty in held[:3 if self.bits == 8 else 2]:
+            _check(t, nm, shape=(self._blocks, width), dtype=ty, device=self.device)
+            if t.data_ptr() % 16:
+                raise ValueError("m, v and scale must be 16-byte aligned")
+        row = self.BLOCK * self.m.element_size()
+        w = self._words
+        w[0::8] = array.array("Q", [p.data_ptr() for p in self.params])
+        w[2::8] = array.array("Q", [self.m.data_ptr() + row * f for f in self.first])
+        w[3::8] = array.array("Q", [self.v.data_ptr() + row * f for f in self.first])
+        if self.bits == 8:
+            w[4::8] = array.array("Q", [self.scale.data_ptr() + 8 * f for f in self.first])
+        self._at = w[0::8].tolist()
+        self._rest = self._others()
+        w[5::8] = array.array("Q", [c or 0 for c in self._rest[0]])
+
+    def _others(self):
+        """Where copies (None: not what they must be) and moments lie."""
+        c = [0 if t is None else t.data_ptr() if t.numel() == n and t.dtype == torch.bfloat16 and t.is_contiguous() else None
+             for t, (n, _) in zip(self.copies, self._meta)]
+        m, v, r = self.m, self.v, self.scale
+        return (c, m.data_ptr(), m.numel(), m.dtype, m.is_contiguous(), v.data_ptr(), v.numel(), v.dtype, v.is_contiguous(),
+                r is not None and (r.data_ptr(), r.numel(), r.dtype, r.is_contiguous()))
+
+    def _held(self, t: Optional[torch.Tensor], width: int, dtype) -> torch.Tensor:
+        if t is not None:
+            return t
+        return torch.zeros((self._blocks, width), dtype=torch.uint8 if dtype.itemsize == 1 else dtype, device=self.device).view(dtype)
 
     def _rows(self, t: torch.Tensor, i: int) -> torch.Tensor:
         return t[self.first[i]:self.first[i] - (-self._meta[i][0] // self.BLOCK)]
@@ -197,25 +226,26 @@ class AdamMoments:
         """The words of the parameters that have a gradient."""
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
-        w, p, gp, kinds, bits, missing = self._words, [], [], [], self.bits << 32, False
-        for i, (t, g, (n, shape)) in enumerate(zip(self.params, grads, self._meta)):
+        w, gp, kinds, bits, missing, moved = self._words, [], [], self.bits << 32, False, False
+        known, where = _DTYPES.get, self.device.index
+        for i, (t, g, (n, shape), at) in enumerate(zip(self.params, grads, self._meta, self._at)):
             if g is None:
                 missing = True
-                p.append(0)
                 gp.append(0)
                 kinds.append(bits)
                 continue
-            if t.shape != shape:
-                raise ValueError(f"params[{i}] has changed its shape")
-            if g.shape != shape or g.dtype not in _DTYPES or not g.is_contiguous() or g.device != self.device:
+            pt, gt = known(t.dtype), known(g.dtype)
+            if pt is None or t.data_ptr() != at or t.numel() != n or not t.is_contiguous():
+                moved = True
+            if gt is None or g.shape != shape or not g.is_contiguous() or g.get_device() != where:
                 _check(g, f"grads[{i}]", shape=shape, device=self.device)
-                nott_dtype(g.dtype)
-            p.append(t.data_ptr())
+                gt = nott_dtype(g.dtype)
             gp.append(g.data_ptr())
-            kinds.append(bits | _DTYPES[g.dtype] << 16 | _DTYPES[t.dtype])
-        w[0::8] = array.array("Q", p)
+            kinds.append(bits | gt << 16 | (pt or 0))
+        rest = self._others()
+        if moved or rest != self._rest or None in rest[0]:
+            self._admit(grads)
         w[1::8] = array.array("Q", gp)
-        w[5::8] = array.array("Q", [0 if c is None else c.data_ptr() for c in self.copies])
         w[7::8] = array.array("Q", kinds)
         if missing:
             kept = array.array("Q")
