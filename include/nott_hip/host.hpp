@@ -1915,6 +1915,9 @@ public:
                 Tensor g = p.grad();
                 if (g.layout() != torch::kStrided || g.numel() != s.n || g.device() != m_.device())
                     throw std::invalid_argument("MultiTensorAdam: a gradient must be dense and lie where its parameter does");
+                if (s.copy.defined() && (s.copy.numel() != s.n || !s.copy.is_contiguous() || s.copy.device() != m_.device() ||
+                                         s.copy.scalar_type() != torch::kBFloat16))
+                    throw std::logic_error("MultiTensorAdam: a bf16 copy has changed its shape, layout, type or device");
                 if (!g.is_contiguous()) {
                     g = g.contiguous();
                     p.mutable_grad() = g;
