@@ -1613,9 +1613,9 @@ int join(nott_ctx ctx, const Params& p, int64_t pairs, const Parts& parts, T* o,
 
 // Room for nsplit parts, or none.
 Parts parts_for(nott_ctx ctx, const Params& p, int64_t pairs, int64_t nsplit) {
-    const int64_t rows = nsplit * pairs * p.rows * 2;
-    float* w = static_cast<float*>(nott::optional_workspace(ctx, (size_t)rows * (p.dv + 2) * sizeof(float)));
-    return {w, w ? w + rows * p.dv : nullptr};
+    const int64_t rows = nsplit * pairs * p.rows * 2, acc = (rows * p.dv + 3) & ~int64_t(3);   // {m, l} are read by 16 bytes
+    float* w = static_cast<float*>(nott::optional_workspace(ctx, (size_t)(acc + rows * 2) * sizeof(float)));
+    return {w, w ? w + acc : nullptr};
 }
 
 }  // namespace
