@@ -1018,8 +1018,7 @@ struct DiffAttentionFn : torch::autograd::Function<DiffAttentionFn> {
 // ------------------------------------------------ gated linear recurrence
 // h_t = keep_t·h_{t−1} + take_t·x_t over time (nott_linear_scan_fwd / _bwd): x, gate
 // [b, t, d], views with any strides but the last; h0 fp32 [b, d] or absent; reset bool
-// [b, t] or absent.  Gives h and the fp32 state behind the last token.  A leaf h0 gets
-// its gradient added to .grad, as a layer's parameters do.
+// [b, t] or absent.  Gives h and the fp32 state behind the last token.
 struct LinearScanFn : torch::autograd::Function<LinearScanFn> {
     static Tensor rows(const Tensor& x) {
         Tensor r = x.stride(-1) == 1 || x.numel() == 0 ? x : x.contiguous();
@@ -1052,7 +1051,6 @@ struct LinearScanFn : torch::autograd::Function<LinearScanFn> {
                                (reset.scalar_type() != torch::kBool && reset.scalar_type() != torch::kUInt8) ||
                                !reset.is_contiguous() || reset.device() != x.device()))
             throw std::invalid_argument("Nott::HIP: reset must be bool or uint8 [b, t], contiguous, on x's device");
-        const bool master = h0.is_leaf() && h0.requires_grad();
         x = rows(x); gate = rows(gate);
         const nott_scan_desc d = desc(x, gate, sigmoid, mix);
         auto f32 = x.options().dtype(torch::kFloat32);
@@ -1063,7 +1061,7 @@ struct LinearScanFn : torch::autograd::Function<LinearScanFn> {
                                    fptr(states)),
               c, "linear scan forward");
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({x, gate, master ? h0 : Tensor(), reset, states});
+        ctx->save_for_backward({x, gate, reset, states});
         ctx->saved_data["sigmoid"] = sigmoid;
         ctx->saved_data["mix"] = mix;
         ctx->saved_data["start"] = present(h0) && h0.requires_grad();
@@ -1071,7 +1069,7 @@ struct LinearScanFn : torch::autograd::Function<LinearScanFn> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         auto s = ctx->get_saved_variables();
-        Tensor x = s[0], gate = s[1], h0 = s[2];
+        Tensor x = s[0], gate = s[1];
         variable_list out(7);
         if (!grads[0].defined() && !grads[1].defined()) return out;
         nott_scan_desc d = desc(x, gate, ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["mix"].toBool());
@@ -1081,19 +1079,11 @@ struct LinearScanFn : torch::autograd::Function<LinearScanFn> {
         strides(d.h_stride, dh);
         out[0] = torch::empty(x.sizes(), x.options());
         out[1] = torch::empty(x.sizes(), x.options());
-        Tensor dh0;
-        if (ctx->saved_data["start"].toBool()) dh0 = torch::empty({d.b, d.d}, x.options().dtype(torch::kFloat32));
+        if (ctx->saved_data["start"].toBool()) out[2] = torch::empty({d.b, d.d}, x.options().dtype(torch::kFloat32));
         nott_ctx c = bind(x);
-        check(nott_linear_scan_bwd(c, &d, dtype_of(x), ptr(dh), ptr(x), ptr(gate), bytes(s[3]), fptr(s[4]), fptr(dlast),
-                                   ptr(out[0]), ptr(out[1]), fptr(dh0)),
+        check(nott_linear_scan_bwd(c, &d, dtype_of(x), ptr(dh), ptr(x), ptr(gate), bytes(s[2]), fptr(s[3]), fptr(dlast),
+                                   ptr(out[0]), ptr(out[1]), fptr(out[2])),
               c, "linear scan backward");
-        if (h0.defined() && dh0.defined()) {
-            Tensor g = grad_buffer(h0);
-            torch::NoGradGuard ng;
-            g.add_(dh0);
-        } else {
-            out[2] = dh0;
-        }
         return out;
     }
 };
