@@ -322,6 +322,17 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& t, int base) {
     return __builtin_bit_cast(bf16x8, w);
 }
 
+// The remainder x − bf16(x) of registers base..base+7, rounded to bf16.
+__device__ __forceinline__ bf16x8 pack8_lo(const f32x16& t, int base, const bf16x8& hi) {
+    const u32x4 h = __builtin_bit_cast(u32x4, hi);
+    auto lo2 = [&](int i, uint32_t w) {
+        return pack_bf16x2(t[base + i] - __builtin_bit_cast(float, w << 16),
+                           t[base + i + 1] - __builtin_bit_cast(float, w & 0xffff0000u));
+    };
+    const u32x4 w = {lo2(0, h.x), lo2(2, h.y), lo2(4, h.z), lo2(6, h.w)};
+    return __builtin_bit_cast(bf16x8, w);
+}
+
 __device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }

@@ -17,10 +17,16 @@
 //
 // bf16 with 16-byte aligned rows runs on 32×32×16 MFMAs (namespace mx), in the layouts of
 // attention.hip's kernels: scores are formed transposed, so that a lane owns a row.
-// Probabilities (forward), p_1 − λ·p_2 and dz enter the second products rounded to bf16:
-// each is off by at most 2^-8 of itself, which in sums of many keys puts about as much
-// into the result as the result's own rounding (see the figures beside the kernels).
 // fp32, and rows that are not aligned, take the 16×16 kernels (namespace any).
+// Probabilities (forward), p_1 − λ·p_2 and dz enter the second products as a bf16 value and
+// the bf16 value of its remainder, off by 2^-16: o_1 and λ·o_2 nearly cancel where the maps
+// resemble each other, and what one rounding (2^-8) leaves of each does not.  So the results
+// are off by their own rounding (relative error against 64 bits 1.7e-3, the least for bf16;
+// with one rounding 2.0e-3 to 2.4e-3, and up to 10 times the tolerance of tests of such
+// maps).  The second half of the products costs 8 x 1024 tokens of 8 heads of 64 + 128
+// columns 47 -> 58 us forward and 162 -> 171 backward, 4096 tokens of 16 heads on 4 of
+// 128 + 256 1396 -> 1550 backward, a step against a cache nothing.  (Times of other choices
+// beside the kernels were taken with one rounding.)
 // Few rows against many keys (a decoding step): the keys are split over workgroups and
 // waves, and a second kernel joins the parts.
 // No atomics: every result is formed in a fixed order.
@@ -322,7 +328,7 @@ __device__ __forceinline__ float dot_rows(const u32x4 (&a)[2 * NB], const u32x4 
 // probabilities (packed into pb), m, l and the accumulators follow.  rel: the lane's
 // visible keys, counted from its first of the tile; full: nothing is masked.
 template <int TF, int NV>
-__device__ __forceinline__ void softmax_step(f32x16 (&st)[TF], bf16x8 (&pb)[2 * TF], f32x16 (&acc)[NV], float& m, float& l,
+__device__ __forceinline__ void softmax_step(f32x16 (&st)[TF], bf16x8 (&pb)[2 * TF], bf16x8 (&pl)[2 * TF], f32x16 (&acc)[NV], float& m, float& l,
                                              float sl2, bool full, int rel) {
     if (!full) {
 #pragma unroll
@@ -358,6 +364,8 @@ __device__ __forceinline__ void softmax_step(f32x16 (&st)[TF], bf16x8 (&pb)[2 * 
         }
         pb[2 * f] = pack8(st[f], 0);
         pb[2 * f + 1] = pack8(st[f], 8);
+        pl[2 * f] = pack8_lo(st[f], 0, pb[2 * f]);
+        pl[2 * f + 1] = pack8_lo(st[f], 8, pb[2 * f + 1]);
     }
     l += rs;
 }
@@ -519,15 +527,19 @@ __global__ __launch_bounds__(128 * NW, 2) void diff_fwd32_kernel(const bf16_t* _
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
             f32x16 st[1];
-            bf16x8 pb[2];
+            bf16x8 pb[2], pl[2];
 #pragma unroll
             for (int s = 0; s < 2 * ND; ++s)
                 st[0] = mfma(rows_k.get(tk, 32 * f, s), __builtin_bit_cast(bf16x8, qr[s]), s ? st[0] : f32x16{});
-            softmax_step<1, NV>(st, pb, acc, m, l, sl2, full, rel - 32 * f);
+            softmax_step<1, NV>(st, pb, pl, acc, m, l, sl2, full, rel - 32 * f);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int df = 0; df < NV; ++df) acc[df] = mfma(cols_v.get(tv, 32 * f + 16 * s, df), pb[s], acc[df]);
+                for (int df = 0; df < NV; ++df) {
+                const bf16x8 c = cols_v.get(tv, 32 * f + 16 * s, df);
+                acc[df] = mfma(c, pb[s], acc[df]);
+                acc[df] = mfma(c, pl[s], acc[df]);
+            }
         }
     }
     l += __shfl_xor(l, 32, 64);
@@ -599,15 +611,19 @@ __global__ __launch_bounds__(64 * NW, 1) void diff_split32_kernel(const bf16_t* 
         next = next + 1 == RING ? 0 : next + 1;
         const int k0 = i * TR + 32 * f;
         f32x16 st[1];
-        bf16x8 pb[2];
+        bf16x8 pb[2], pl[2];
 #pragma unroll
         for (int s = 0; s < 2 * ND; ++s)
             st[0] = mfma(rows_k.get(tk, 32 * f, s), __builtin_bit_cast(bf16x8, qr[s]), s ? st[0] : f32x16{});
-        softmax_step<1, NV>(st, pb, acc, m, l, sl2, k0 + 32 <= vis_lo, vis - k0 - 4 * h);
+        softmax_step<1, NV>(st, pb, pl, acc, m, l, sl2, k0 + 32 <= vis_lo, vis - k0 - 4 * h);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int df = 0; df < NV; ++df) acc[df] = mfma(cols_v.get(tv, 32 * f + 16 * s, df), pb[s], acc[df]);
+            for (int df = 0; df < NV; ++df) {
+                const bf16x8 c = cols_v.get(tv, 32 * f + 16 * s, df);
+                acc[df] = mfma(c, pb[s], acc[df]);
+                acc[df] = mfma(c, pl[s], acc[df]);
+            }
     }
     // Join the halves of a map: maxima and sums, then the scaled accumulators, through LDS.
     l += __shfl_xor(l, 32, 64);
@@ -721,41 +737,41 @@ __global__ __launch_bounds__(64 * NW, ND <= 2 ? 2 : 1) void diff_dq32_kernel(
         const int rel = vis - k0 - 4 * h;
 #pragma unroll
         for (int f = 0; f < TF; ++f) {
-            f32x16 t3[3];   // both maps' scores, dp
+            f32x16 dp;
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int s = 0; s < 2 * NV; ++s) dp = mfma(rows_v.get(tv, 32 * f, s), __builtin_bit_cast(bf16x8, dr[s]), s ? dp : f32x16{});
+            // one map after the other (the scores of both at once spilled 10 registers at ND = 2:
+            // 8 x 1024 tokens of 8 heads 107 us, 71 so)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                f32x16 z;
 #pragma unroll
                 for (int s = 0; s < 2 * ND; ++s)
-                    t3[m] = mfma(rows_k.get(tk + m * KT, 32 * f, s), __builtin_bit_cast(bf16x8, qr[m][s]), s ? t3[m] : f32x16{});
+                    z = mfma(rows_k.get(tk + m * KT, 32 * f, s), __builtin_bit_cast(bf16x8, qr[m][s]), s ? z : f32x16{});
 #pragma unroll
-            for (int s = 0; s < 2 * NV; ++s)
-                t3[2] = mfma(rows_v.get(tv, 32 * f, s), __builtin_bit_cast(bf16x8, dr[s]), s ? t3[2] : f32x16{});
+                for (int x = 0; x < 16; ++x) z[x] = fmaf(z[x], sl2, -ls[m]);
+                if (!full) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) t3[m][x] = fmaf(t3[m][x], sl2, -ls[m]);
-            if (!full) {
+                    for (int x = 0; x < 16; ++x)
+                        if (!(32 * f + 8 * (x >> 2) + (x & 3) < rel)) {
+                            z[x] = -INFINITY;
+                            dp[x] = 0.f;
+                        }
+                }
 #pragma unroll
                 for (int x = 0; x < 16; ++x)
-                    if (!(32 * f + 8 * (x >> 2) + (x & 3) < rel)) {
-                        t3[0][x] = t3[1][x] = -INFINITY;
-                        t3[2][x] = 0.f;
-                    }
-            }
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                t3[0][x] = __builtin_amdgcn_exp2f(t3[0][x]) * (t3[2][x] - D[0]);
-                t3[1][x] = __builtin_amdgcn_exp2f(t3[1][x]) * (lam * (D[1] - t3[2][x]));
-            }
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
+                    z[x] = __builtin_amdgcn_exp2f(z[x]) * (m ? lam * (D[1] - dp[x]) : dp[x] - D[0]);
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const bf16x8 a = pack8(t3[m], 8 * s);
+                    const bf16x8 a = pack8(z, 8 * s), al = pack8_lo(z, 8 * s, a);
 #pragma unroll
-                    for (int df = 0; df < ND; ++df)
-                        adq[m][df] = mfma(a, cols_k.get(tk + m * KT, 32 * f + 16 * s, df), adq[m][df]);
+                    for (int df = 0; df < ND; ++df) {
+                        const bf16x8 c = cols_k.get(tk + m * KT, 32 * f + 16 * s, df);
+                        adq[m][df] = mfma(a, c, adq[m][df]);
+                        adq[m][df] = mfma(al, c, adq[m][df]);
+                    }
                 }
+            }
         }
     }
     // lane: column d = 32·df + l%32 of rows 8j + 4h + e of this wave's 32
@@ -891,18 +907,27 @@ __global__ __launch_bounds__(64 * NW, WHAT == 2 && ND <= 3 ? 2 : 1) void diff_dk
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                bf16x8 a1, a2, aw;
-                if (DK) a1 = pack8(t3[0], 8 * s), a2 = pack8(t3[1], 8 * s);
-                if (DV) aw = pack8(t3[2], 8 * s);
-                if constexpr (DK)
+                if constexpr (DK) {
 #pragma unroll
-                    for (int df = 0; df < ND; ++df) {
-                    adk[0][df] = mfma(a1, cols_k.get(tq, 32 * f + 16 * s, df), adk[0][df]);
-                    adk[1][df] = mfma(a2, cols_k.get(tq + QT, 32 * f + 16 * s, df), adk[1][df]);
+                    for (int m = 0; m < 2; ++m) {
+                        const bf16x8 a = pack8(t3[m], 8 * s), al = pack8_lo(t3[m], 8 * s, a);
+#pragma unroll
+                        for (int df = 0; df < ND; ++df) {
+                            const bf16x8 c = cols_k.get(tq + m * QT, 32 * f + 16 * s, df);
+                            adk[m][df] = mfma(a, c, adk[m][df]);
+                            adk[m][df] = mfma(al, c, adk[m][df]);
+                        }
+                    }
                 }
-                if constexpr (DV)
+                if constexpr (DV) {
+                    const bf16x8 a = pack8(t3[2], 8 * s), al = pack8_lo(t3[2], 8 * s, a);
 #pragma unroll
-                    for (int df = 0; df < NV; ++df) adv[df] = mfma(aw, cols_v.get(tdo, 32 * f + 16 * s, df), adv[df]);
+                    for (int df = 0; df < NV; ++df) {
+                        const bf16x8 c = cols_v.get(tdo, 32 * f + 16 * s, df);
+                        adv[df] = mfma(a, c, adv[df]);
+                        adv[df] = mfma(al, c, adv[df]);
+                    }
+                }
             }
         }
     }
@@ -1196,7 +1221,7 @@ __global__ __launch_bounds__(kThreads) void diff_fwd_kernel(const T* __restrict_
             for (int dt = 0; dt < D::DTV; ++dt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[m][dt][e] *= al[e];
-            const RegA<T, false> pa(sc);
+            const RegA<T, true> pa(sc);
 #pragma unroll
             for (int s = 0; s < D::KS; ++s)
 #pragma unroll
