@@ -7,8 +7,8 @@
 //   dz_1 = p_1∘(dp − D_1),  dz_2 = −λ·p_2∘(dp − D_2)
 //   dq_r = dz_r·k_r·scale,  dk_r = dz_rᵀ·q_r·scale,  dv = (p_1 − λ·p_2)ᵀ·dO,  dλ = −D_2
 // So a pair of query and key costs 4·dh + 4·dv operations forward and, with two passes
-// that both form the scores, 20·dh + 6·dv backward; v and dO are read, and dp and dv
-// formed, once for both maps.
+// that both form the scores and dp, 16·dh + 6·dv backward (20·dh + 6·dv where dk and dv are
+// apart, a third pass); v and dO are read, and dp and dv formed, once for both maps.
 //
 // Rows.  All queries of the heads that share a key head are one list of rows, query by
 // query (row = query·group + head of the group), so a workgroup's rows share the tiles of
@@ -1703,9 +1703,12 @@ extern "C" int nott_diff_attention_fwd(nott_ctx ctx, const nott_diff_attn_desc* 
         auto* to2 = static_cast<T*>(o2);
         Parts parts{};
         const int64_t groups = pairs * ceil_div(p.rows, BR);
-        // Fewer workgroups than CUs (causal blocks differ in length) or than three of four: keys
-        // split (1024 tokens of 8 heads in fp32, causal, 150 us whole, 93 split; 3 x 777 of 6
-        // heads on 3, all keys seen, 225 workgroups, 125 whole, 152 split).
+        // Fewer workgroups than CUs, or where all keys are seen than three of four: keys split.
+        // Split against whole, fp32 and unaligned bf16, 16 + 32 to 64 + 128 columns: causal (blocks
+        // differ in length, and parts even that out) 0.5 to 0.8 of the time at 72 to 168
+        // workgroups, 0.8 to 0.95 at 195 to 240 (at 16 + 32 columns in fp32 up to 1.1); all keys
+        // seen 0.5 to 0.8 up to 128, 0.8 to 1.1 at 144 to 168, 1.05 to 1.3 from 195 on, where
+        // the parts run in a second round.
         if (groups < (p.causal ? ctx->num_cu : ctx->num_cu * 3 / 4) && p.s >= 512) {
             const int64_t most = std::min<int64_t>(kMostParts, ceil_div(p.s, 4 * BR));
             const int64_t n = std::min<int64_t>(most, ceil_div(2 * ctx->num_cu, groups));

@@ -12,7 +12,7 @@
 // through LDS (the reverse scan's beside), and the spans are gone through again from the
 // states before them.  So x and gate are read once and h is written once; the
 // backward reads x, gate and dh, forms the states again in fp32 from the one that the
-// forward kept before every 256th token (3% of h's bytes, where reading h costs a sixth
+// forward kept before every 256th token (0.8% of h's bytes in bf16, where reading h costs a sixth
 // stream and its rounding), and writes dx and dgate.  States, maps and sums are fp32.
 //
 // Few channels (b·d of a few thousand) do not fill the chip: then the tokens are split
@@ -22,8 +22,8 @@
 // A keep of exactly 0 forgets the state whatever it was, an infinity or NaN as well.
 //
 // Bound by HBM (3 streams forward, 5 backward): 4 x 4096 tokens of 2048 channels in bf16
-// take 56 us forward (3.6 TB/s) and 98 backward (3.4 TB/s); a packed batch of 50001 tokens
-// of 520 channels in fp32 178 us backward (41 of them for the segments' maps; 4.0 TB/s over
+// take 57 us forward (3.6 TB/s) and 97 backward (3.5 TB/s); a packed batch of 50001 tokens
+// of 520 channels in fp32 182 us backward (42 of them for the segments' maps; 4.0 TB/s over
 // its 7 streams).  A token's row holds 64 to 256 bytes of a workgroup, so neighbouring
 // blocks of channels share pages and lines of memory: they run on one XCD, side by side
 // (74 us without that, forward; 118 backward).
@@ -715,7 +715,7 @@ int check(nott_ctx ctx, const nott_scan_desc* d, nott_dtype dtype, Params* p) {
 }
 
 // Segments: one where the channels alone give half of the CUs a workgroup, else as many as
-// bring two for each, of at least 4 tiles.
+// bring two for each, of about 4 tiles (n tiles make at most n/4 segments, rounded up).
 Maps segments(nott_ctx ctx, Params* p, int64_t blocks) {
     const int64_t tiles = p->nchunk;
     int64_t n = blocks >= ctx->num_cu / 2 ? 1 : std::min<int64_t>(ceil_div(2 * ctx->num_cu, blocks), ceil_div(tiles, 4));
