@@ -428,18 +428,18 @@ int nott_qk_norm_rope_bwd(nott_ctx ctx, const nott_qk_rope_desc* d, nott_dtype d
  *   keep = a, or 0 at tokens where `reset` (bytes [b, t], nullable) is not 0: a sequence
  *   begins there, and nothing before it reaches it, infinities and NaN included.
  * A keep of exactly 0 forgets the state as well; however small the product of others
- * becomes, an infinite or NaN state stays one.  (Gates above 16, with sigmoid = 0: where
- * the product over 32 tokens overflows fp32, a state of 0 before them becomes NaN.)  With sigmoid = 1 a gate of +infinity
- * keeps the state (and with mix takes nothing in: padding behind a sequence leaves its
- * state), one of −infinity forgets it.
+ * becomes, an infinite or NaN state stays one.  With sigmoid = 1 a gate of +infinity
+ * keeps the state (and with mix takes nothing of a finite x in: padding behind a sequence
+ * leaves its state), one of −infinity forgets it.  (With sigmoid = 0, where gates above 16
+ * make the product over 32 tokens overflow fp32, a state of 0 before them becomes NaN.)
  * x, gate, h [b, t, d] with strides in elements for batch and token (two zeros =
  * contiguous), channels side by side, so x and gate may be views of one projection.
  * h0, last [b, d] fp32: the state before the first token (nullable: zeros) and after the
  * last (nullable).  states [b, ceil(t / 256), d] fp32 (nullable): the state before every
  * 256th token, for the backward.  The state is fp32 throughout.  h may be x or gate
- * (same address and strides); other overlaps are not allowed.  Workspace: an fp64 and an fp32 [b, d] for each
- * segment that time is cut into where the channels are few; without room for it,
- * time is not cut. */
+ * (same address and strides); other overlaps are not allowed.
+ * Workspace: an fp64 and an fp32 [b, d] for each segment that time is cut into where the
+ * channels are few; without room for it, time is not cut. */
 typedef struct nott_scan_desc {
     int64_t b, t, d;
     int64_t x_stride[2], gate_stride[2];
